@@ -563,6 +563,94 @@ typedef struct kad_span {
 int kad_find_relocs(const void *blob, int64_t blob_bytes, const int64_t *at, int nat, const kad_span *spans, int nspans,
                     kad_reloc *relocs);
 
+/* ------------------------------------------------------------------------ */
+/* Training operators.  No reference counterpart: KAD-CNet trains with torch's */
+/* (KAD-CNet/train.py).                                                        */
+/* ------------------------------------------------------------------------ */
+
+/* Group norm with an activation on NHWC maps: with D = C / groups channels in a group,
+ *   z = weight (x - mean) rstd + bias,  rstd = 1 / sqrt(var + eps),  y = act(z),
+ * mean and (biased) var over the H W D values of an (image, group). */
+typedef struct kad_group_norm_args {
+  const void *x;          /* [N][H][W][x_cs], dtype: channels [0, C) of each pixel */
+  const void *dy;         /* backward: gradient of y, [N][H][W][dy_cs], dtype */
+  void *out;              /* forward: y, backward: dx (or NULL: not wanted); dense [N][H][W][C], dtype */
+  const void *weight;     /* [C], param_dtype, or NULL: ones */
+  const void *bias;       /* [C], param_dtype, or NULL: zeros */
+  float *mean, *rstd;     /* [N][groups]: forward writes them, backward reads them */
+  void *dweight, *dbias;  /* backward: [C], param_dtype, or NULL: not wanted */
+  float *work;            /* kad_group_norm_work_elems floats; need not be initialised, free after the call */
+  int64_t x_cs, dy_cs;    /* elements from pixel to pixel (>= C); more than C only where C is a multiple of
+                             16 bytes / sizeof(dtype) */
+  int n, c, groups, h, w; /* groups divides c */
+  float eps;
+  int act;                /* KAD_ACT_NONE, KAD_ACT_RELU or KAD_ACT_SILU */
+  int dtype, param_dtype; /* param_dtype: KAD_F32, or dtype */
+} kad_group_norm_args;
+
+/* Floats of scratch that a call on these sizes needs (sizes and types of `a` only), or KAD_EINVAL. */
+int64_t kad_group_norm_work_elems(const kad_group_norm_args *a, int backward);
+
+int kad_group_norm_fwd(const kad_group_norm_args *a, void *stream);
+
+/* dx, dweight and dbias from x, dy, the forward's mean and rstd, weight and bias. */
+int kad_group_norm_bwd(const kad_group_norm_args *a, void *stream);
+
+/* A piece of one parameter tensor: `count` consecutive values at param / grad, whose state lies
+ * `offset` values into the state buffers.  offset is a multiple of KAD_ADAMW_SEG. */
+typedef struct kad_adamw_chunk {
+  void *param;
+  const void *grad;
+  int64_t offset;
+  int count, reserved;
+} kad_adamw_chunk;
+
+#define KAD_ADAMW_SEG 256     /* a tensor's state begins at a multiple of this; an 8-bit scale holds for as many values */
+#define KAD_ADAMW_CHUNK 4096  /* values in a chunk, at most */
+
+/* Cuts n tensors (host arrays: addresses and numbers of values; tensors of 0 values are passed over) into
+ * chunks, and lays their states out one after the other; a tensor whose gradient's address is 0 has its
+ * place among the states but no chunk.  Returns the number of chunks and the length of
+ * the state buffers in *state_elems; chunks (host memory) may be NULL: count only.  Host only. */
+int64_t kad_adamw_chunks(const int64_t *params, const int64_t *grads, const int64_t *numels, int n, int elem_bytes,
+                         kad_adamw_chunk *chunks, int64_t *state_elems);
+
+/* What a step's scalars come to; kad_adamw_hyper computes them on the GPU. */
+typedef struct kad_adamw_scalars {
+  float decay;            /* 1 - lr weight_decay */
+  float rate;             /* lr / (1 - beta1^step) */
+  float inv_root;         /* 1 / sqrt(1 - beta2^step) */
+  uint32_t key;           /* of the step's random bits */
+} kad_adamw_scalars;
+
+/* One AdamW step over all chunks, with g = *grad_scale * grad (1 where grad_scale is NULL):
+ *   m <- beta1 m + (1 - beta1) g,   v <- beta2 v + (1 - beta2) g^2,
+ *   p <- decay p - rate m / (sqrt(v) inv_root + eps).
+ * state_bits 32: exp_avg and exp_avg_sq hold m and v as floats.  state_bits 8: exp_avg and exp_avg_sq hold
+ * m and sqrt(v) as e4m3 codes, times one float of exp_avg_scale / exp_avg_sq_scale for each KAD_ADAMW_SEG. */
+typedef struct kad_adamw_args {
+  const kad_adamw_chunk *chunks;  /* device memory */
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale;  /* 8-bit states only */
+  float *master;          /* fp32 parameters, laid out as the states, or NULL: param itself is updated */
+  const float *grad_scale;          /* device, or NULL */
+  const kad_adamw_scalars *scalars; /* device (kad_adamw_hyper's), or NULL: from lr .. step below */
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;           /* >= 1 */
+  int64_t nchunks;
+  uint32_t seed;          /* of the 8-bit states' stochastic rounding */
+  int dtype;              /* of param and grad */
+  int state_bits;         /* 32 or 8 */
+} kad_adamw_args;
+
+int kad_adamw_step(const kad_adamw_args *a, void *stream);
+
+/* Writes *scalars (device) for the step counted in *step (device), with *lr (device float) or, where that is
+ * NULL, a->lr: a captured step replays with a count and a rate of its own.  Uses lr, beta1, beta2,
+ * weight_decay and seed of `a`. */
+int kad_adamw_hyper(const kad_adamw_args *a, const int64_t *step, const float *lr, kad_adamw_scalars *scalars,
+                    void *stream);
+
 #ifdef __cplusplus
 }
 #endif

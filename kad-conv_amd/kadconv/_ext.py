@@ -109,6 +109,27 @@ class ScaleArgs(ctypes.Structure):
         'n', 'c', 'h', 'w', 'img_c', 'c_off', 'layout', 'dtype')]
 
 
+class GroupNormArgs(ctypes.Structure):
+    _fields_ = [(f, c_vp) for f in ('x', 'dy', 'out', 'weight', 'bias', 'mean', 'rstd', 'dweight', 'dbias', 'work')] + \
+               [('x_cs', c_i64), ('dy_cs', c_i64)] + [(f, c_int) for f in ('n', 'c', 'groups', 'h', 'w')] + \
+               [('eps', ctypes.c_float), ('act', c_int), ('dtype', c_int), ('param_dtype', c_int)]
+
+
+class AdamwChunk(ctypes.Structure):
+    _fields_ = [('param', c_vp), ('grad', c_vp), ('offset', c_i64), ('count', c_int), ('reserved', c_int)]
+
+
+class AdamwArgs(ctypes.Structure):
+    _fields_ = [(f, c_vp) for f in ('chunks', 'exp_avg', 'exp_avg_sq', 'exp_avg_scale', 'exp_avg_sq_scale', 'master',
+                                    'grad_scale', 'scalars')] + \
+               [(f, ctypes.c_double) for f in ('lr', 'beta1', 'beta2', 'eps', 'weight_decay')] + \
+               [('step', c_i64), ('nchunks', c_i64), ('seed', ctypes.c_uint32), ('dtype', c_int), ('state_bits', c_int)]
+
+
+ADAMW_SEG = 256          # KAD_ADAMW_SEG
+ADAMW_SCALARS = 4        # 4-byte words of kad_adamw_scalars
+
+
 class Call(ctypes.Structure):
     _fields_ = [('fn', c_int), ('count', c_int), ('args', c_i64), ('arg', c_int)]
 
@@ -178,6 +199,12 @@ SIGNATURES = {
     'kad_ddetect_decode': (c_int, [ctypes.POINTER(DecodeArgs), c_vp]),
     'kad_nms_mask_words': (c_i64, [c_int]),
     'kad_nms': (c_int, [c_vp, c_vp, c_vp, c_int, ctypes.c_float, c_vp]),
+    'kad_group_norm_work_elems': (c_i64, [ctypes.POINTER(GroupNormArgs), c_int]),
+    'kad_group_norm_fwd': (c_int, [ctypes.POINTER(GroupNormArgs), c_vp]),
+    'kad_group_norm_bwd': (c_int, [ctypes.POINTER(GroupNormArgs), c_vp]),
+    'kad_adamw_chunks': (c_i64, [c_vp, c_vp, c_vp, c_int, c_int, c_vp, ctypes.POINTER(c_i64)]),
+    'kad_adamw_step': (c_int, [ctypes.POINTER(AdamwArgs), c_vp]),
+    'kad_adamw_hyper': (c_int, [ctypes.POINTER(AdamwArgs), c_vp, c_vp, c_vp, c_vp]),
 }
 
 _lib = None
@@ -983,3 +1010,69 @@ def gemm1x1_nhwc(x_nhwc, cin, wpack, cout, out_nhwc, *, bias=None, act=KAD_ACT_N
     a.act, a.dtype = (1 if act == KAD_ACT_SILU else 0), kad_dtype(x_nhwc.dtype)   # kad_gemm_args.act: 1 = SiLU
     _check(load().kad_gemm1x1_fwd(ctypes.byref(a), _stream()), 'kad_gemm1x1_fwd')
     return out_nhwc
+
+
+# ---------------------------------------------------------------------------- training operators
+def _group_norm_args(x, cs, groups, weight, bias, eps, act):
+    a = GroupNormArgs()
+    a.n, a.c, a.h, a.w = x.shape
+    a.x, a.weight, a.bias, a.x_cs = _ptr(x), _ptr(weight), _ptr(bias), cs
+    a.groups, a.eps, a.act, a.dtype = groups, eps, act, kad_dtype(x.dtype)
+    p = weight if weight is not None else bias
+    a.param_dtype = kad_dtype(torch.float32 if p is None else p.dtype)
+    return a
+
+
+def _group_norm_work(a, backward, device):
+    n = load().kad_group_norm_work_elems(ctypes.byref(a), backward)
+    if n < 0:
+        _check(int(n), 'kad_group_norm_work_elems')
+    return torch.empty(n, dtype=torch.float32, device=device) if n else None
+
+
+def group_norm_fwd(x, cs, groups, weight, bias, eps, act, out, mean, rstd):
+    """x [N, C, H, W] whose pixels lie cs elements apart; out [N, C, H, W] dense channels-last; mean and
+    rstd [N, groups] fp32; weight and bias [C] of one dtype (fp32 or x's) or None."""
+    _need_gpu(x, weight, bias, out, mean, rstd)
+    a = _group_norm_args(x, cs, groups, weight, bias, eps, act)
+    a.out, a.mean, a.rstd = _ptr(out), _ptr(mean), _ptr(rstd)
+    work = _group_norm_work(a, 0, x.device)
+    a.work = _ptr(work)
+    _check(load().kad_group_norm_fwd(ctypes.byref(a), _stream()), 'kad_group_norm_fwd')
+    return out
+
+
+def group_norm_bwd(x, cs, dy, dy_cs, groups, weight, bias, eps, act, mean, rstd, dx, dweight, dbias):
+    """dx (dense channels-last or None), dweight and dbias ([C] or None) for the forward's mean and rstd."""
+    _need_gpu(x, dy, weight, bias, mean, rstd, dx, dweight, dbias)
+    a = _group_norm_args(x, cs, groups, weight, bias, eps, act)
+    a.dy, a.dy_cs, a.out, a.mean, a.rstd = _ptr(dy), dy_cs, _ptr(dx), _ptr(mean), _ptr(rstd)
+    a.dweight, a.dbias = _ptr(dweight), _ptr(dbias)
+    work = _group_norm_work(a, 1, x.device)
+    a.work = _ptr(work)
+    _check(load().kad_group_norm_bwd(ctypes.byref(a), _stream()), 'kad_group_norm_bwd')
+
+
+def adamw_chunks(params, grads, numels, elem_bytes):
+    """(chunk table, length of the state buffers) of tensors given by addresses and numbers of values
+    (lists of ints): the table as a uint8 tensor in host memory, sizeof(AdamwChunk) bytes a chunk."""
+    lib = load()
+    n = len(params)
+    cols = [array.array('q', v) for v in (params, grads, numels)]
+    at = [c.buffer_info()[0] for c in cols]
+    elems = c_i64()
+    count = lib.kad_adamw_chunks(*at, n, elem_bytes, None, ctypes.byref(elems))
+    if count < 0:
+        _check(int(count), 'kad_adamw_chunks')
+    table = torch.empty(count * ctypes.sizeof(AdamwChunk), dtype=torch.uint8)
+    if count:
+        lib.kad_adamw_chunks(*at, n, elem_bytes, table.data_ptr(), ctypes.byref(elems))
+    return table, elems.value
+
+
+def adamw_step(args):
+    _check(load().kad_adamw_step(ctypes.byref(args), _stream()), 'kad_adamw_step')
+
+
+def adamw_hyper(args, step, lr, scalars):
+    _check(load().kad_adamw_hyper(ctypes.byref(args), _ptr(step), _ptr(lr), _ptr(scalars), _stream()), 'kad_adamw_hyper')

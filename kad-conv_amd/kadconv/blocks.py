@@ -12,9 +12,12 @@
   (kad_conv.py:112-121) as
       y = sigmoid(gate) * sum_i softmax(alpha)_i * up(conv1x1_i(avgpool(x, 2^(i+1))))
   with up = bilinear (align_corners=False) to (H // 2, W // 2).
+* ``GroupNormAct`` -- group norm and an activation on channels-last maps, for
+  layers trained at a batch too small for batch statistics.
 
-Eval-mode GPU inputs run the HIP kernels (no fallback: a missing library
+The first three: eval-mode GPU inputs run the HIP kernels (no fallback: a missing library
 raises); training mode or CPU inputs run the plain torch composition.
+``GroupNormAct`` runs them in training mode too: its kernels have a backward.
 """
 import torch
 import torch.nn as nn
@@ -144,3 +147,23 @@ class KADDown(nn.Module):
         if x.is_contiguous(memory_format=torch.channels_last) and not x.is_contiguous():
             out = out.contiguous(memory_format=torch.channels_last)
         return out
+
+
+class GroupNormAct(nn.Module):
+    """act(group_norm(x)); parameters as torch.nn.GroupNorm's, so its state dicts load."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, act='silu'):
+        super().__init__()
+        if num_groups < 1 or num_channels % num_groups:
+            raise ValueError(f'{num_groups} groups do not divide {num_channels} channels')
+        if act not in (None, 'relu', 'silu'):
+            raise ValueError(f"act {act!r} is none of None, 'relu', 'silu'")
+        self.num_groups, self.num_channels, self.eps, self.act = num_groups, num_channels, eps, act
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+
+    def forward(self, x):
+        return ops.group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.act)
+
+    def extra_repr(self):
+        return f'{self.num_groups}, {self.num_channels}, eps={self.eps}, affine={self.weight is not None}, act={self.act!r}'

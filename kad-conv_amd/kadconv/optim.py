@@ -1,0 +1,337 @@
+"""AdamW over a network's tensors in one launch (kad_adamw_step).
+
+* ``AdamWPlan`` -- the step for tensors whose parameters and gradients stay where
+  they are: a table of them is laid out on the GPU once.
+* ``AdamW`` -- a ``torch.optim.Optimizer`` on such plans, which lays a table out
+  anew when gradients have moved.
+
+A detector has thousands of parameter tensors, half of them smaller than a
+wave's load (KAD-CNet-S: 2944, median 22 values), so a step a tensor is bound by
+its launches.
+
+States are kept for all tensors of a plan in flat buffers, in the order of each
+parameter's memory, each tensor's part beginning at a multiple of 256 values:
+
+  32 bits   exp_avg, exp_avg_sq                    float32
+  8 bits    exp_avg, exp_avg_sq_root               float8_e4m3fn, the numbers held
+            exp_avg_scale, exp_avg_sq_root_scale   float32, one for 256 of them
+  either    master                                 float32, with master_weights
+
+8-bit states hold m and sqrt(v) as e4m3 numbers times their segment's scale
+(its largest magnitude / 448), rounded stochastically with bits that are a hash
+of (seed, step, place): the same call gives the same result.  A segment that
+meets an infinity or NaN holds NaN from then on, as a single value does in 32 bits.
+"""
+import ctypes
+
+import torch
+
+from . import _ext
+
+_NAMES = {32: ('exp_avg', 'exp_avg_sq'),
+          8: ('exp_avg', 'exp_avg_sq_root', 'exp_avg_scale', 'exp_avg_sq_root_scale')}
+
+
+def _dense(t):
+    """Whether t's values fill its memory without gaps or overlaps, in any order of dimensions."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _same_layout(a, b):
+    return a.shape == b.shape and (a.stride() == b.stride() or all(
+        sa == sb for sa, sb, n in zip(a.stride(), b.stride(), a.shape) if n != 1))
+
+
+def _check_rates(lr, betas, eps, weight_decay):
+    if not isinstance(lr, torch.Tensor) and not lr >= 0:
+        raise ValueError(f'lr must be >= 0, got {lr}')
+    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+        raise ValueError(f'betas must lie in [0, 1), got {betas}')
+    if not (eps >= 0 and weight_decay >= 0):
+        raise ValueError(f'eps and weight_decay must be >= 0, got {eps} and {weight_decay}')
+
+
+class AdamWPlan:
+    """The AdamW step of ``params`` by ``grads``, two lists of dense GPU tensors of one dtype (fp32, fp16 or
+    bf16), equal in shapes and strides.  The plan holds their addresses: it is for tensors that keep their
+    memory from step to step, as persistent gradient buffers and captured graphs do; ``set_grads`` takes
+    others.  A gradient may be None: its parameter has a place in the state but is not stepped.
+
+    ``state_bits`` 32 or 8; ``master_weights`` (16-bit parameters): an fp32 copy of them is stepped and rounded to
+    them; ``state``: a dict of flat state buffers to use as they are, in place of new ones of zeros (and
+    masters copied from the parameters); ``seed``: of the 8-bit states' stochastic rounding.
+
+    ``plan.state`` holds the buffers, ``plan.offsets`` where each tensor's part begins."""
+
+    def __init__(self, params, grads, state_bits=32, master_weights=False, state=None, seed=0):
+        params = list(params)
+        self.params = [p.detach() for p in params]
+        # views of one tensor share its version: it stands for all of them
+        self._versioned = [p._base if p._is_view() else p for p in params]
+        if state_bits not in _NAMES:
+            raise ValueError(f'state_bits must be 32 or 8, got {state_bits}')
+        if not self.params:
+            raise ValueError('at least one parameter expected')
+        p0 = self.params[0]
+        for p in self.params:
+            if not p.is_cuda:
+                raise ValueError('kadconv.AdamWPlan needs GPU tensors')
+            if p.dtype != p0.dtype or p.device != p0.device:
+                raise TypeError('parameters must share a dtype and a device')
+            if p.is_sparse or not _dense(p):
+                raise ValueError('parameters must be dense: no gaps or overlaps in their memory')
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError('two parameters share memory')
+        _ext.kad_dtype(p0.dtype)
+        if master_weights and p0.dtype == torch.float32:
+            raise ValueError('master weights are for 16-bit parameters')
+        self.state_bits, self.master_weights, self.seed = state_bits, bool(master_weights), int(seed) & 0xFFFFFFFF
+        self._numels = [p.numel() for p in self.params]
+        seg = _ext.ADAMW_SEG
+        self.offsets, at = [], 0
+        for n in self._numels:
+            self.offsets.append(at)
+            at += -(-n // seg) * seg
+        self.state_elems = at
+        self._scalars = None
+        self.grads = None
+        self.set_grads(grads)
+        self.state = self._new_state() if state is None else self._given_state(state)
+
+    def _layout(self):
+        """{name: (values, dtype)} of the state buffers."""
+        n, seg = self.state_elems, _ext.ADAMW_SEG
+        out = {}
+        for name in _NAMES[self.state_bits]:
+            if name.endswith('_scale'):
+                out[name] = n // seg, torch.float32
+            else:
+                out[name] = n, torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
+        if self.master_weights:
+            out['master'] = n, torch.float32
+        return out
+
+    def _new_state(self):
+        device = self.params[0].device
+        state = {}
+        for name, (n, dtype) in self._layout().items():
+            state[name] = torch.zeros(n, dtype=torch.uint8 if dtype == torch.float8_e4m3fn else dtype,
+                                      device=device).view(dtype)
+        if self.master_weights:
+            for i, p in enumerate(self.params):
+                self.part(state['master'], i).copy_(p)
+        return state
+
+    def _given_state(self, state):
+        layout = self._layout()
+        if set(state) != set(layout):
+            raise ValueError(f'state must hold {sorted(layout)}, got {sorted(state)}')
+        for name, (n, dtype) in layout.items():
+            t = state[name]
+            if t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous() or t.device != self.params[0].device:
+                raise ValueError(f'{name} must be a contiguous {dtype} [{n}] on {self.params[0].device}')
+            if t.data_ptr() % 16:
+                raise ValueError(f'{name} must begin at a multiple of 16 bytes')
+        return dict(state)
+
+    def part(self, buffer, i):
+        """Parameter i's values of a state buffer (not of scales), as a view of the parameter's shape and strides."""
+        p = self.params[i]
+        return buffer[self.offsets[i]:self.offsets[i] + self._numels[i]].as_strided(
+            p.shape, p.stride(), buffer.storage_offset() + self.offsets[i])
+
+    def scales(self, buffer, i):
+        """Parameter i's scales of a buffer of them."""
+        seg = _ext.ADAMW_SEG
+        return buffer[self.offsets[i] // seg:(self.offsets[i] + self._numels[i] + seg - 1) // seg]
+
+    def check_grads(self, grads):
+        if len(grads) != len(self.params):
+            raise ValueError(f'{len(grads)} gradients for {len(self.params)} parameters')
+        for p, g in zip(self.params, grads):
+            if g is None:
+                continue
+            if g.layout != torch.strided:
+                raise ValueError('gradients must be dense tensors')
+            if g.dtype != p.dtype or g.device != p.device:
+                raise TypeError(f"a gradient is {g.dtype} on {g.device}, its parameter {p.dtype} on {p.device}")
+            if not _same_layout(p, g):
+                raise ValueError('a gradient must have the shape and strides of its parameter')
+
+    def set_grads(self, grads, keep=True):
+        """Use these gradients from the next step on.  keep=False: the plan holds their addresses alone, and the
+        caller sees to it that they live as long as it steps by them."""
+        grads = list(grads)
+        self.check_grads(grads)
+        at = [0 if g is None or not n else g.data_ptr() for g, n in zip(grads, self._numels)]
+        self._lay_out(at)
+        self.grads = [g if g is None else g.detach() for g in grads] if keep else None
+
+    def _lay_out(self, grad_at):
+        host, elems = _ext.adamw_chunks([p.data_ptr() for p in self.params], grad_at, self._numels,
+                                        self.params[0].element_size())
+        assert elems == self.state_elems
+        self._grad_at = grad_at
+        self._chunks = host.to(self.params[0].device)
+        self._nchunks = host.numel() // ctypes.sizeof(_ext.AdamwChunk)
+        self._stepped = list({id(p): p for p, g in zip(self._versioned, grad_at) if g}.values())
+
+    def step(self, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, grad_scale=None):
+        """One step, the ``step``-th (from 1).  ``grad_scale``: a float32 GPU scalar that gradients are multiplied
+        by.  For a captured graph ``step`` may be an int64 GPU scalar and ``lr`` a float32 one, whose values
+        are read when the graph runs."""
+        _check_rates(lr, betas, eps, weight_decay)
+        a = _ext.AdamwArgs()
+        st = self.state
+        if self.state_bits == 32:
+            a.exp_avg, a.exp_avg_sq = st['exp_avg'].data_ptr(), st['exp_avg_sq'].data_ptr()
+        else:
+            a.exp_avg, a.exp_avg_sq = st['exp_avg'].data_ptr(), st['exp_avg_sq_root'].data_ptr()
+            a.exp_avg_scale, a.exp_avg_sq_scale = (st[n].data_ptr() for n in _NAMES[8][2:])
+        if self.master_weights:
+            a.master = st['master'].data_ptr()
+        if grad_scale is not None:
+            self._check_scalar('grad_scale', grad_scale, torch.float32)
+            a.grad_scale = grad_scale.data_ptr()
+        a.chunks, a.nchunks = self._chunks.data_ptr(), self._nchunks
+        a.beta1, a.beta2, a.eps, a.weight_decay = betas[0], betas[1], eps, weight_decay
+        a.dtype, a.state_bits, a.seed = _ext.kad_dtype(self.params[0].dtype), self.state_bits, self.seed
+        if isinstance(step, torch.Tensor):
+            self._check_scalar('step', step, torch.int64)
+            if isinstance(lr, torch.Tensor):
+                self._check_scalar('lr', lr, torch.float32)
+            else:
+                a.lr = lr
+            if self._scalars is None:
+                self._scalars = torch.empty(_ext.ADAMW_SCALARS, dtype=torch.int32, device=step.device)
+            _ext.adamw_hyper(a, step, lr if isinstance(lr, torch.Tensor) else None, self._scalars)
+            a.scalars = self._scalars.data_ptr()
+        else:
+            if isinstance(lr, torch.Tensor):
+                raise TypeError('lr may be a GPU scalar only where step is one')
+            if step < 1:
+                raise ValueError(f'step must be at least 1, got {step}')
+            a.step, a.lr = step, lr
+        _ext.adamw_step(a)
+        # the kernel wrote them: what is kept by a parameter's version (packed weights, saved tensors) is stale
+        torch.autograd.graph.increment_version(self._stepped)
+
+    def _check_scalar(self, name, t, dtype):
+        if t.dtype != dtype or t.numel() != 1 or t.device != self.params[0].device:
+            raise ValueError(f'{name} must be one {dtype} value on {self.params[0].device}')
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay on the HIP kernel: GPU parameters in fp32, fp16 or bf16, gradients of
+    their dtype.  A group's steps are counted together: a parameter that has no gradient in a step is
+    left as it is, and the next bias correction counts that step.
+
+    ``state_bits``, ``master_weights`` (for the 16-bit parameters) and ``seed`` as in ``AdamWPlan``.  ``capturable``: the
+    count of steps is a GPU scalar, so that ``step`` can be captured into a graph (after one step outside,
+    with gradients that keep their memory); ``lr`` may be a float32 GPU scalar then.
+
+    The state dict holds each parameter's part of the flat buffers; 8-bit states load into parameters of the
+    same strides alone, as their scales follow the order in memory."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
+                 master_weights=False, seed=0, capturable=False):
+        _check_rates(lr, betas, eps, weight_decay)
+        if state_bits not in _NAMES:
+            raise ValueError(f'state_bits must be 32 or 8, got {state_bits}')
+        if isinstance(lr, torch.Tensor) and not capturable:
+            raise ValueError('lr may be a GPU scalar only with capturable=True')
+        self._plans = {}      # (group, dtype) -> plan
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=master_weights, seed=seed, capturable=capturable, step=0))
+
+    def _group_plans(self, gi):
+        """The plans of group gi, one a dtype, made of all its parameters."""
+        group = self.param_groups[gi]
+        by_dtype = {}
+        for p in group['params']:
+            by_dtype.setdefault(p.dtype, []).append(p)
+        out = []
+        for dtype, params in by_dtype.items():
+            plan = self._plans.get((gi, dtype))
+            if plan is None:
+                master = group['master_weights'] and dtype != torch.float32
+                plan = AdamWPlan(params, [None] * len(params), state_bits=group['state_bits'], master_weights=master,
+                                 seed=group['seed'] + 2 * gi + (dtype == torch.float32))
+                self._plans[gi, dtype] = plan
+                for i, p in enumerate(params):
+                    self.state[p] = {name: (plan.scales if name.endswith('_scale') else plan.part)(buf, i)
+                                     for name, buf in plan.state.items()}
+            out.append((plan, params))
+        return out
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_scale=None):
+        """One step; ``grad_scale``: a float32 GPU scalar that gradients are multiplied by (a clipping or loss
+        scale's factor)."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for gi, group in enumerate(self.param_groups):
+            if not any(p.grad is not None for p in group['params']):
+                continue
+            plans = self._group_plans(gi)
+            todo = []
+            for plan, params in plans:
+                # a parameter that moved (module.to) would be written at its old address
+                if any(p.data_ptr() != q.data_ptr() or p.stride() != q.stride() for p, q in zip(params, plan.params)):
+                    raise RuntimeError('a parameter has moved since the first step: make a new optimizer')
+                grads = [p.grad for p in params]
+                for i, (p, g) in enumerate(zip(params, grads)):
+                    if g is not None and g.layout == torch.strided and g.shape == p.shape and not _same_layout(p, g):
+                        grads[i] = torch.empty_like(p).copy_(g)
+                plan.check_grads(grads)
+                todo.append((plan, grads))
+            if group['capturable']:
+                if not isinstance(group['step'], torch.Tensor):
+                    group['step'] = torch.tensor(group['step'], dtype=torch.int64, device=plans[0][0].params[0].device)
+                group['step'].add_(1)
+            else:
+                group['step'] += 1
+            for plan, grads in todo:
+                at = [0 if g is None or not n else g.data_ptr() for g, n in zip(grads, plan._numels)]
+                if at != plan._grad_at:
+                    plan._lay_out(at)
+                plan.step(group['step'], lr=group['lr'], betas=group['betas'], eps=group['eps'],
+                          weight_decay=group['weight_decay'], grad_scale=grad_scale)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict({'state': {}, 'param_groups': state_dict['param_groups']})
+        self._plans = {}
+        saved = state_dict['state']
+        if not saved:
+            return
+        for gi, (group, old) in enumerate(zip(self.param_groups, state_dict['param_groups'])):
+            if not any(k in saved for k in old['params']):
+                continue
+            self._group_plans(gi)
+            if isinstance(group['step'], torch.Tensor):  # of the saved optimizer, or on another device
+                group['step'] = group['step'].to(device=group['params'][0].device, dtype=torch.int64, copy=True)
+            for p, k in zip(group['params'], old['params']):
+                if k not in saved:
+                    raise ValueError('the state dict holds some of a group\'s states only')
+                mine, theirs = self.state[p], saved[k]
+                if set(mine) != set(theirs):
+                    raise ValueError(f'the state dict holds {sorted(theirs)}, this optimizer {sorted(mine)}')
+                for name, t in mine.items():
+                    o = theirs[name]
+                    if o.shape != t.shape or o.dtype != t.dtype:
+                        raise ValueError(f'{name}: {tuple(o.shape)} {o.dtype} in the state dict, {tuple(t.shape)} {t.dtype} here')
+                    if group['state_bits'] == 8 and not _same_layout(o, t):
+                        raise ValueError('8-bit states load into parameters of the same strides alone')
+                for name, t in mine.items():
+                    t.copy_(theirs[name])
