@@ -1,10 +1,10 @@
-"""Builds libkadconv_hip.so (gfx950) in-tree from csrc/.
+"""Builds libkadconv_hip.so (gfx950) and the torch binding _native.so in-tree from csrc/.
 
     python kad-conv_amd/build.py            # incremental
     python kad-conv_amd/build.py --force    # rebuild everything
 
-Objects go to kad-conv_amd/_build/, the shared library to
-kad-conv_amd/kadconv/libkadconv_hip.so, where kadconv._ext loads it.
+Objects go to kad-conv_amd/_build/, the shared libraries to
+kad-conv_amd/kadconv/, where kadconv._ext loads them.
 """
 import argparse
 import concurrent.futures as cf
@@ -12,11 +12,14 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OBJ = os.path.join(HERE, '_build')
 LIB = os.path.join(HERE, 'kadconv', 'libkadconv_hip.so')
+NATIVE_SRC = os.path.join(CSRC, 'torch', 'kad_torch.cpp')
+NATIVE = os.path.join(HERE, 'kadconv', '_native.so')
 INCLUDE = os.path.join(os.path.dirname(HERE), 'include')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 ARCH = 'gfx950'
@@ -43,12 +46,41 @@ def _compile(src, force):
     return obj, None
 
 
+def _compile_native(force):
+    """The binding's object: host code only, against torch's headers."""
+    obj = os.path.join(OBJ, os.path.basename(NATIVE_SRC) + '.o')
+    newest = max(os.path.getmtime(f) for f in [NATIVE_SRC, *_deps()])
+    if not force and os.path.exists(obj) and os.path.getmtime(obj) >= newest:
+        return obj, None
+    from torch.utils import cpp_extension
+    dirs = cpp_extension.include_paths() + ['/opt/rocm/include', sysconfig.get_paths()['include']]
+    # the platform's name is what HIP's own headers ask for outside hipcc
+    cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM', '-I', INCLUDE]
+    cmd += [w for d in dirs for w in ('-isystem', d)] + ['-c', NATIVE_SRC, '-o', obj]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    return obj, f'{" ".join(cmd)}\n{r.stdout}\n{r.stderr}' if r.returncode else None
+
+
+def _link_native(obj):
+    import torch
+    libs = os.path.join(os.path.dirname(torch.__file__), 'lib')
+    tmp = NATIVE + '.tmp'
+    cmd = ['g++', '-shared', '-o', tmp, obj, '-L', os.path.dirname(LIB), '-l:' + os.path.basename(LIB), '-L', libs,
+           '-lc10', '-lc10_hip', '-ltorch_cpu', '-ltorch', '-ltorch_python', '-Wl,-rpath,$ORIGIN']
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f'link failed:\n{" ".join(cmd)}\n{r.stdout}\n{r.stderr}')
+    os.replace(tmp, NATIVE)
+
+
 def build(force=False, jobs=8, verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, '*.hip')) + glob.glob(os.path.join(CSRC, '*.cpp')))
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        native = ex.submit(_compile_native, force)
         results = list(ex.map(lambda s: _compile(s, force), srcs))
-    errs = [e for _, e in results if e]
+    native_obj, native_err = native.result()
+    errs = [e for _, e in results + [(native_obj, native_err)] if e]
     if errs:
         raise RuntimeError('HIP build failed:\n' + '\n'.join(errs))
     objs = [o for o, _ in results]
@@ -59,8 +91,10 @@ def build(force=False, jobs=8, verbose=False):
         if r.returncode != 0:
             raise RuntimeError(f'link failed:\n{" ".join(cmd)}\n{r.stdout}\n{r.stderr}')
         os.replace(tmp, LIB)
+    if force or not os.path.exists(NATIVE) or os.path.getmtime(NATIVE) < os.path.getmtime(native_obj):
+        _link_native(native_obj)
     if verbose:
-        print('built', LIB)
+        print('built', LIB, 'and', NATIVE)
     return LIB
 
 

@@ -208,6 +208,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_native = None
 
 
 def lib_path():
@@ -234,6 +235,19 @@ def load():
         raise KadExtensionError(f'ABI mismatch: library {lib.kad_abi_version()} != binding {ABI_VERSION}')
     _lib = lib
     return lib
+
+
+def native():
+    """kadconv._native: the training operators' entry points in C++ (csrc/torch), over the same library."""
+    global _native
+    if _native is None:
+        load()
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise KadExtensionError(f'kadconv._native is not built; run `python kad-conv_amd/build.py` first: {e}') from e
+        _native = module
+    return _native
 
 
 def _check(rc, what):
@@ -1013,46 +1027,6 @@ def gemm1x1_nhwc(x_nhwc, cin, wpack, cout, out_nhwc, *, bias=None, act=KAD_ACT_N
 
 
 # ---------------------------------------------------------------------------- training operators
-def _group_norm_args(x, cs, groups, weight, bias, eps, act):
-    a = GroupNormArgs()
-    a.n, a.c, a.h, a.w = x.shape
-    a.x, a.weight, a.bias, a.x_cs = _ptr(x), _ptr(weight), _ptr(bias), cs
-    a.groups, a.eps, a.act, a.dtype = groups, eps, act, kad_dtype(x.dtype)
-    p = weight if weight is not None else bias
-    a.param_dtype = kad_dtype(torch.float32 if p is None else p.dtype)
-    return a
-
-
-def _group_norm_work(a, backward, device):
-    n = load().kad_group_norm_work_elems(ctypes.byref(a), backward)
-    if n < 0:
-        _check(int(n), 'kad_group_norm_work_elems')
-    return torch.empty(n, dtype=torch.float32, device=device) if n else None
-
-
-def group_norm_fwd(x, cs, groups, weight, bias, eps, act, out, mean, rstd):
-    """x [N, C, H, W] whose pixels lie cs elements apart; out [N, C, H, W] dense channels-last; mean and
-    rstd [N, groups] fp32; weight and bias [C] of one dtype (fp32 or x's) or None."""
-    _need_gpu(x, weight, bias, out, mean, rstd)
-    a = _group_norm_args(x, cs, groups, weight, bias, eps, act)
-    a.out, a.mean, a.rstd = _ptr(out), _ptr(mean), _ptr(rstd)
-    work = _group_norm_work(a, 0, x.device)
-    a.work = _ptr(work)
-    _check(load().kad_group_norm_fwd(ctypes.byref(a), _stream()), 'kad_group_norm_fwd')
-    return out
-
-
-def group_norm_bwd(x, cs, dy, dy_cs, groups, weight, bias, eps, act, mean, rstd, dx, dweight, dbias):
-    """dx (dense channels-last or None), dweight and dbias ([C] or None) for the forward's mean and rstd."""
-    _need_gpu(x, dy, weight, bias, mean, rstd, dx, dweight, dbias)
-    a = _group_norm_args(x, cs, groups, weight, bias, eps, act)
-    a.dy, a.dy_cs, a.out, a.mean, a.rstd = _ptr(dy), dy_cs, _ptr(dx), _ptr(mean), _ptr(rstd)
-    a.dweight, a.dbias = _ptr(dweight), _ptr(dbias)
-    work = _group_norm_work(a, 1, x.device)
-    a.work = _ptr(work)
-    _check(load().kad_group_norm_bwd(ctypes.byref(a), _stream()), 'kad_group_norm_bwd')
-
-
 def adamw_chunks(params, grads, numels, elem_bytes):
     """(chunk table, length of the state buffers) of tensors given by addresses and numbers of values
     (lists of ints): the table as a uint8 tensor in host memory, sizeof(AdamwChunk) bytes a chunk."""
@@ -1068,11 +1042,3 @@ def adamw_chunks(params, grads, numels, elem_bytes):
     if count:
         lib.kad_adamw_chunks(*at, n, elem_bytes, table.data_ptr(), ctypes.byref(elems))
     return table, elems.value
-
-
-def adamw_step(args):
-    _check(load().kad_adamw_step(ctypes.byref(args), _stream()), 'kad_adamw_step')
-
-
-def adamw_hyper(args, step, lr, scalars):
-    _check(load().kad_adamw_hyper(ctypes.byref(args), _ptr(step), _ptr(lr), _ptr(scalars), _stream()), 'kad_adamw_hyper')

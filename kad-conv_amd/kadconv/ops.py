@@ -249,75 +249,16 @@ def _group_norm_act_cpu(x, num_groups, weight, bias, eps, act):
     return z.to(x.dtype)
 
 
-def _channels_last_pixels(x):
-    """(x, elements from pixel to pixel) where x [N, C, H, W] is channels-last, dense or a slice of the
-    channels of a dense map; otherwise of a dense channels-last copy.  A slice whose channels are not a
-    multiple of 16 bytes is copied too: its pieces would not tile the kernels' 16-byte vectors."""
-    N, C, H, W = x.shape
-    sn, sc, sh, sw = x.stride()
-    cs = sw if W > 1 else sh if H > 1 else sn if N > 1 else C
-    if ((sc == 1 or C == 1) and cs >= C and (H == 1 or sh == W * cs) and (N == 1 or sn == H * W * cs)
-            and (cs == C or C % (16 // x.element_size()) == 0)):
-        return x, cs
-    out = torch.empty((N, H, W, C), dtype=x.dtype, device=x.device).permute(0, 3, 1, 2)
-    return out.copy_(x), C
-
-
-def _map_like(x):
-    """A dense channels-last map of x's shape, dtype and device."""
-    N, C, H, W = x.shape
-    return torch.empty((N, H, W, C), dtype=x.dtype, device=x.device).permute(0, 3, 1, 2)
-
-
-def _param(p):
-    return None if p is None else p.detach().contiguous()
-
-
 def group_norm_act_forward(x, num_groups, weight, bias, eps, act):
     """(y, mean, rstd) of a GPU map; mean and rstd [N, num_groups] in fp32 are what the gradient needs."""
-    y = _map_like(x)
-    mean = torch.empty(x.shape[0], num_groups, dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
-    _ext.kad_dtype(x.dtype)
-    if x.numel():
-        v, cs = _channels_last_pixels(x)
-        _ext.group_norm_fwd(v, cs, num_groups, _param(weight), _param(bias), eps, _ACTS[act], y, mean, rstd)
-    return y, mean, rstd
+    return _ext.native().group_norm_act_forward(x, num_groups, weight, bias, eps, _ACTS[act])
 
 
 def group_norm_act_backward(dy, x, num_groups, weight, bias, mean, rstd, eps, act, need_x=True, need_weight=True,
                             need_bias=True):
     """(dx, dweight, dbias) of group_norm_act; None for what is not needed or has no tensor."""
-    dx = _map_like(x) if need_x else None
-    need_weight, need_bias = need_weight and weight is not None, need_bias and bias is not None
-    if not x.numel():  # sums over nothing
-        return (dx, torch.zeros_like(weight) if need_weight else None, torch.zeros_like(bias) if need_bias else None)
-    if not (need_x or need_weight or need_bias):
-        return None, None, None
-    w, b = _param(weight), _param(bias)
-    dw = torch.empty_like(w) if need_weight else None
-    db = torch.empty_like(b) if need_bias else None
-    v, cs = _channels_last_pixels(x)
-    d, dcs = _channels_last_pixels(dy)
-    _ext.group_norm_bwd(v, cs, d, dcs, num_groups, w, b, eps, _ACTS[act], mean, rstd, dx, dw, db)
-    return dx, dw, db
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, num_groups, eps, act):
-        y, mean, rstd = group_norm_act_forward(x, num_groups, weight, bias, eps, act)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.rest = num_groups, eps, act
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        num_groups, eps, act = ctx.rest
-        grads = group_norm_act_backward(dy, x, num_groups, weight, bias, mean, rstd, eps, act, *ctx.needs_input_grad[:3])
-        return (*grads, None, None, None)
+    return _ext.native().group_norm_act_backward(dy, x, num_groups, weight, bias, mean, rstd, eps, _ACTS[act], need_x,
+                                                 need_weight, need_bias)
 
 
 def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, act=None):
@@ -334,6 +275,4 @@ def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, act=None
         return _group_norm_act_cpu(input, num_groups, weight, bias, eps, act)
     if torch.compiler.is_compiling():
         return torch.ops.kadconv.group_norm_act(input, num_groups, weight, bias, eps, act)[0]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, weight, bias)):
-        return _GroupNormAct.apply(input, weight, bias, num_groups, eps, act)
-    return group_norm_act_forward(input, num_groups, weight, bias, eps, act)[0]
+    return _ext.native().group_norm_act(input, num_groups, weight, bias, eps, _ACTS[act])

@@ -22,7 +22,7 @@ parameter's memory, each tensor's part beginning at a multiple of 256 values:
 of (seed, step, place): the same call gives the same result.  A segment that
 meets an infinity or NaN holds NaN from then on, as a single value does in 32 bits.
 """
-import ctypes
+import functools
 
 import torch
 
@@ -30,18 +30,6 @@ from . import _ext
 
 _NAMES = {32: ('exp_avg', 'exp_avg_sq'),
           8: ('exp_avg', 'exp_avg_sq_root', 'exp_avg_scale', 'exp_avg_sq_root_scale')}
-
-
-def _dense(t):
-    """Whether t's values fill its memory without gaps or overlaps, in any order of dimensions."""
-    if t.is_contiguous():
-        return True
-    expect = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
-        if stride != expect:
-            return False
-        expect *= size
-    return True
 
 
 def _same_layout(a, b):
@@ -68,43 +56,36 @@ class AdamWPlan:
     them; ``state``: a dict of flat state buffers to use as they are, in place of new ones of zeros (and
     masters copied from the parameters); ``seed``: of the 8-bit states' stochastic rounding.
 
-    ``plan.state`` holds the buffers, ``plan.offsets`` where each tensor's part begins."""
+    ``plan.state`` holds the buffers."""
 
     def __init__(self, params, grads, state_bits=32, master_weights=False, state=None, seed=0):
         params = list(params)
-        self.params = [p.detach() for p in params]
-        # views of one tensor share its version: it stands for all of them
-        self._versioned = [p._base if p._is_view() else p for p in params]
         if state_bits not in _NAMES:
             raise ValueError(f'state_bits must be 32 or 8, got {state_bits}')
-        if not self.params:
-            raise ValueError('at least one parameter expected')
-        p0 = self.params[0]
-        for p in self.params:
-            if not p.is_cuda:
-                raise ValueError('kadconv.AdamWPlan needs GPU tensors')
-            if p.dtype != p0.dtype or p.device != p0.device:
-                raise TypeError('parameters must share a dtype and a device')
-            if p.is_sparse or not _dense(p):
-                raise ValueError('parameters must be dense: no gaps or overlaps in their memory')
-        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise ValueError('two parameters share memory')
-        _ext.kad_dtype(p0.dtype)
+        self._table = _ext.native().AdamWTable(params)
+        p0 = params[0]
         if master_weights and p0.dtype == torch.float32:
             raise ValueError('master weights are for 16-bit parameters')
         self.state_bits, self.master_weights, self.seed = state_bits, bool(master_weights), int(seed) & 0xFFFFFFFF
-        self._numels = [p.numel() for p in self.params]
-        seg = _ext.ADAMW_SEG
-        self.offsets, at = [], 0
-        for n in self._numels:
-            self.offsets.append(at)
-            at += -(-n // seg) * seg
-        self.state_elems = at
-        self._scalars = None
-        self.grads = None
+        self.device, self.state_elems = p0.device, self._table.elems
         self.set_grads(grads)
         self.state = self._new_state() if state is None else self._given_state(state)
+        self._table.set_state(*(self.state[n] for n in _NAMES[state_bits]), *(None, None) * (state_bits == 32),
+                              self.state.get('master'), state_bits, self.seed)
+
+    @functools.cached_property
+    def params(self):
+        """The parameters, detached."""
+        return self._table.params
+
+    @functools.cached_property
+    def offsets(self):
+        """Where each parameter's part of a state buffer begins."""
+        return self._table.offsets
+
+    @functools.cached_property
+    def _numels(self):
+        return self._table.numels
 
     def _layout(self):
         """{name: (values, dtype)} of the state buffers."""
@@ -120,11 +101,10 @@ class AdamWPlan:
         return out
 
     def _new_state(self):
-        device = self.params[0].device
         state = {}
         for name, (n, dtype) in self._layout().items():
             state[name] = torch.zeros(n, dtype=torch.uint8 if dtype == torch.float8_e4m3fn else dtype,
-                                      device=device).view(dtype)
+                                      device=self.device).view(dtype)
         if self.master_weights:
             for i, p in enumerate(self.params):
                 self.part(state['master'], i).copy_(p)
@@ -136,8 +116,8 @@ class AdamWPlan:
             raise ValueError(f'state must hold {sorted(layout)}, got {sorted(state)}')
         for name, (n, dtype) in layout.items():
             t = state[name]
-            if t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous() or t.device != self.params[0].device:
-                raise ValueError(f'{name} must be a contiguous {dtype} [{n}] on {self.params[0].device}')
+            if t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous() or t.device != self.device:
+                raise ValueError(f'{name} must be a contiguous {dtype} [{n}] on {self.device}')
             if t.data_ptr() % 16:
                 raise ValueError(f'{name} must begin at a multiple of 16 bytes')
         return dict(state)
@@ -153,80 +133,22 @@ class AdamWPlan:
         seg = _ext.ADAMW_SEG
         return buffer[self.offsets[i] // seg:(self.offsets[i] + self._numels[i] + seg - 1) // seg]
 
-    def check_grads(self, grads):
-        if len(grads) != len(self.params):
-            raise ValueError(f'{len(grads)} gradients for {len(self.params)} parameters')
-        for p, g in zip(self.params, grads):
-            if g is None:
-                continue
-            if g.layout != torch.strided:
-                raise ValueError('gradients must be dense tensors')
-            if g.dtype != p.dtype or g.device != p.device:
-                raise TypeError(f"a gradient is {g.dtype} on {g.device}, its parameter {p.dtype} on {p.device}")
-            if not _same_layout(p, g):
-                raise ValueError('a gradient must have the shape and strides of its parameter')
-
-    def set_grads(self, grads, keep=True):
-        """Use these gradients from the next step on.  keep=False: the plan holds their addresses alone, and the
-        caller sees to it that they live as long as it steps by them."""
-        grads = list(grads)
-        self.check_grads(grads)
-        at = [0 if g is None or not n else g.data_ptr() for g, n in zip(grads, self._numels)]
-        self._lay_out(at)
-        self.grads = [g if g is None else g.detach() for g in grads] if keep else None
-
-    def _lay_out(self, grad_at):
-        host, elems = _ext.adamw_chunks([p.data_ptr() for p in self.params], grad_at, self._numels,
-                                        self.params[0].element_size())
-        assert elems == self.state_elems
-        self._grad_at = grad_at
-        self._chunks = host.to(self.params[0].device)
-        self._nchunks = host.numel() // ctypes.sizeof(_ext.AdamwChunk)
-        self._stepped = list({id(p): p for p, g in zip(self._versioned, grad_at) if g}.values())
+    def set_grads(self, grads):
+        """Use these gradients from the next step on."""
+        self._table.set_grads(list(grads))
 
     def step(self, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, grad_scale=None):
         """One step, the ``step``-th (from 1).  ``grad_scale``: a float32 GPU scalar that gradients are multiplied
         by.  For a captured graph ``step`` may be an int64 GPU scalar and ``lr`` a float32 one, whose values
         are read when the graph runs."""
         _check_rates(lr, betas, eps, weight_decay)
-        a = _ext.AdamwArgs()
-        st = self.state
-        if self.state_bits == 32:
-            a.exp_avg, a.exp_avg_sq = st['exp_avg'].data_ptr(), st['exp_avg_sq'].data_ptr()
-        else:
-            a.exp_avg, a.exp_avg_sq = st['exp_avg'].data_ptr(), st['exp_avg_sq_root'].data_ptr()
-            a.exp_avg_scale, a.exp_avg_sq_scale = (st[n].data_ptr() for n in _NAMES[8][2:])
-        if self.master_weights:
-            a.master = st['master'].data_ptr()
-        if grad_scale is not None:
-            self._check_scalar('grad_scale', grad_scale, torch.float32)
-            a.grad_scale = grad_scale.data_ptr()
-        a.chunks, a.nchunks = self._chunks.data_ptr(), self._nchunks
-        a.beta1, a.beta2, a.eps, a.weight_decay = betas[0], betas[1], eps, weight_decay
-        a.dtype, a.state_bits, a.seed = _ext.kad_dtype(self.params[0].dtype), self.state_bits, self.seed
         if isinstance(step, torch.Tensor):
-            self._check_scalar('step', step, torch.int64)
-            if isinstance(lr, torch.Tensor):
-                self._check_scalar('lr', lr, torch.float32)
-            else:
-                a.lr = lr
-            if self._scalars is None:
-                self._scalars = torch.empty(_ext.ADAMW_SCALARS, dtype=torch.int32, device=step.device)
-            _ext.adamw_hyper(a, step, lr if isinstance(lr, torch.Tensor) else None, self._scalars)
-            a.scalars = self._scalars.data_ptr()
+            at, lr = (lr, 0.0) if isinstance(lr, torch.Tensor) else (None, lr)
+            self._table.step_later(step, at, lr, betas[0], betas[1], eps, weight_decay, grad_scale)
+        elif isinstance(lr, torch.Tensor):
+            raise TypeError('lr may be a GPU scalar only where step is one')
         else:
-            if isinstance(lr, torch.Tensor):
-                raise TypeError('lr may be a GPU scalar only where step is one')
-            if step < 1:
-                raise ValueError(f'step must be at least 1, got {step}')
-            a.step, a.lr = step, lr
-        _ext.adamw_step(a)
-        # the kernel wrote them: what is kept by a parameter's version (packed weights, saved tensors) is stale
-        torch.autograd.graph.increment_version(self._stepped)
-
-    def _check_scalar(self, name, t, dtype):
-        if t.dtype != dtype or t.numel() != 1 or t.device != self.params[0].device:
-            raise ValueError(f'{name} must be one {dtype} value on {self.params[0].device}')
+            self._table.step(step, lr, betas[0], betas[1], eps, weight_decay, grad_scale)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -248,28 +170,31 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f'state_bits must be 32 or 8, got {state_bits}')
         if isinstance(lr, torch.Tensor) and not capturable:
             raise ValueError('lr may be a GPU scalar only with capturable=True')
-        self._plans = {}      # (group, dtype) -> plan
+        self._plans = {}      # group -> [(plan, its parameters)]
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights, seed=seed, capturable=capturable, step=0))
 
     def _group_plans(self, gi):
-        """The plans of group gi, one a dtype, made of all its parameters."""
+        """[(plan, its parameters)] of group gi, one a dtype, made of all its parameters."""
+        if gi in self._plans:
+            return self._plans[gi]
         group = self.param_groups[gi]
         by_dtype = {}
         for p in group['params']:
             by_dtype.setdefault(p.dtype, []).append(p)
         out = []
         for dtype, params in by_dtype.items():
-            plan = self._plans.get((gi, dtype))
-            if plan is None:
-                master = group['master_weights'] and dtype != torch.float32
-                plan = AdamWPlan(params, [None] * len(params), state_bits=group['state_bits'], master_weights=master,
-                                 seed=group['seed'] + 2 * gi + (dtype == torch.float32))
-                self._plans[gi, dtype] = plan
-                for i, p in enumerate(params):
-                    self.state[p] = {name: (plan.scales if name.endswith('_scale') else plan.part)(buf, i)
-                                     for name, buf in plan.state.items()}
+            master = group['master_weights'] and dtype != torch.float32
+            plan = AdamWPlan(params, [None] * len(params), state_bits=group['state_bits'], master_weights=master,
+                             seed=group['seed'] + 2 * gi + (dtype == torch.float32))
+            for i, p in enumerate(params):
+                mine = {name: (plan.scales if name.endswith('_scale') else plan.part)(buf, i)
+                        for name, buf in plan.state.items()}
+                for name, t in self.state[p].items():  # of a copied or unpickled optimizer
+                    mine[name].copy_(t)
+                self.state[p] = mine
             out.append((plan, params))
+        self._plans[gi] = out
         return out
 
     @torch.no_grad()
@@ -284,30 +209,24 @@ class AdamW(torch.optim.Optimizer):
             if not any(p.grad is not None for p in group['params']):
                 continue
             plans = self._group_plans(gi)
-            todo = []
+            if sum(len(params) for _, params in plans) != len(group['params']):
+                raise RuntimeError('a group has gained or lost parameters since the first step: make a new optimizer')
             for plan, params in plans:
-                # a parameter that moved (module.to) would be written at its old address
-                if any(p.data_ptr() != q.data_ptr() or p.stride() != q.stride() for p, q in zip(params, plan.params)):
-                    raise RuntimeError('a parameter has moved since the first step: make a new optimizer')
-                grads = [p.grad for p in params]
-                for i, (p, g) in enumerate(zip(params, grads)):
-                    if g is not None and g.layout == torch.strided and g.shape == p.shape and not _same_layout(p, g):
-                        grads[i] = torch.empty_like(p).copy_(g)
-                plan.check_grads(grads)
-                todo.append((plan, grads))
+                plan._table.follow(params)
             if group['capturable']:
                 if not isinstance(group['step'], torch.Tensor):
-                    group['step'] = torch.tensor(group['step'], dtype=torch.int64, device=plans[0][0].params[0].device)
+                    group['step'] = torch.tensor(group['step'], dtype=torch.int64, device=plans[0][0].device)
                 group['step'].add_(1)
             else:
                 group['step'] += 1
-            for plan, grads in todo:
-                at = [0 if g is None or not n else g.data_ptr() for g, n in zip(grads, plan._numels)]
-                if at != plan._grad_at:
-                    plan._lay_out(at)
+            for plan, _ in plans:
                 plan.step(group['step'], lr=group['lr'], betas=group['betas'], eps=group['eps'],
                           weight_decay=group['weight_decay'], grad_scale=grad_scale)
         return loss
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plans = {}
 
     def load_state_dict(self, state_dict):
         super().load_state_dict({'state': {}, 'param_groups': state_dict['param_groups']})
