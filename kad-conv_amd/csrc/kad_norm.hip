@@ -5,8 +5,16 @@
 //             db = sum dz, dw = sum dz xhat        over images and pixels
 //             dx = rstd (w dz - (s1 + xhat s2) / M), s1 = sum w dz, s2 = sum w dz xhat over the group's M values
 //
-// Memory bounds it: a map is read (x; x and dy) and written (y; dx), with 20 to 25 vector operations a
-// value, a third of them the SiLU's exponential and reciprocal.
+// Memory bounds it: a map is read (x; x and dy) and written (y; dx), with 15 to 20 vector operations a
+// value, half of them the SiLU's exponential and reciprocal (quarter rate).
+//
+// Two forms.  A group of up to 32 KB stays in the registers of one block: one launch, one read.  Beyond, an
+// image is cut into tiles of whole rows: one launch leaves each tile's sums, the next joins them (every block
+// for itself, while its first rows are on their way) and writes the result, walking its rows backwards to meet
+// what the first left in its XCD's L2.  Its stores pass the caches by, which leaves x in them: a bare read and
+// a bare copy of 41 MB take 23.3 us in two launches, 19.1 us with such stores (one copy alone: 17.4, 12.5).
+// [8, 256, 100, 100] fp16 (41 MB): 26.5 us forward (statistics 9.8, result 15.5), backward 46 us (sums 23,
+// dx 22), where a bare read of x and dy, and a copy beside a read, take 13.6 and 20.
 //
 // Layout.  Threads own 16-byte vectors of V channels.  Where V does not divide C, k = V / gcd(C, V) pixels
 // are taken as one row of k C channels, which V divides: a thread's vector meets the same V channels in
@@ -44,13 +52,19 @@ __device__ __forceinline__ float act_of(float z) {
 template <int ACT>
 __device__ __forceinline__ float act_grad(float z, float dy) {
   if (ACT == KAD_ACT_SILU) {
-    const float s = logistic(z);
-    return dy * s * (1.f + z * (1.f - s));
+    const float s = logistic(z), y = z * s;
+    return dy * (s + y - y * s);
   }
   return ACT == KAD_ACT_RELU ? (z > 0.f ? dy : 0.f) : dy;
 }
 
 template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
+// 16 bytes at a T's alignment.
+typedef int intx4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef int intx4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T> struct Loose { typedef intx4_at2 type; };
+template <> struct Loose<float> { typedef intx4_at4 type; };
+template <typename T> using loose = typename Loose<T>::type;
 
 // 16 bytes at an address that need only be a T's (the memory unit takes wide accesses at any address).
 template <typename T>
@@ -69,11 +83,23 @@ __device__ __forceinline__ void unpack(intx4 r, float v[VEC<T>]) {
 // Forgets what was computed from a held vector: otherwise its unpacked values stay in registers too.
 __device__ __forceinline__ void repack(intx4& r) { asm volatile("" : "+v"(r)); }
 template <typename T>
-__device__ __forceinline__ void store_vec(T* p, const float v[VEC<T>]) {
+__device__ __forceinline__ intx4 pack(const float v[VEC<T>]) {
   T t[VEC<T>];
 #pragma unroll
   for (int i = 0; i < VEC<T>; ++i) t[i] = from_f32<T>(v[i]);
-  __builtin_memcpy(p, t, 16);
+  intx4 r;
+  __builtin_memcpy(&r, t, 16);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, const float v[VEC<T>]) {
+  const intx4 r = pack<T>(v);
+  __builtin_memcpy(p, &r, 16);
+}
+// Past the caches.
+template <typename T>
+__device__ __forceinline__ void stream_vec(T* p, const float v[VEC<T>]) {
+  __builtin_nontemporal_store(pack<T>(v), (loose<T>*)p);
 }
 template <typename T>
 __device__ __forceinline__ void load_some(const T* p, int n, float v[VEC<T>]) {
@@ -94,8 +120,7 @@ struct Geo {
   int tail;       // values of the pixels after them (fewer than k; 0 where k = 1)
   int W, q, D;
   int rows, tiles;  // split kernels: rows of a tile, tiles of an image
-  int tpg;          // threads that sum one group: a power of two, at most 64
-  int tpc;          // and one channel
+  int tpg, tpc;     // threads that join what a group, and a channel, has in a block: powers of two
   int share;        // resident kernel: consecutive sets of groups that one 128-byte line may hold
 };
 
@@ -105,47 +130,59 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// Sums over runs of D of the block's values.  Thread t < active holds val[0 .. VV), which are the places
-// t VV + v of a matrix of rows of W values; out[g] becomes the sum of columns [g D, (g + 1) D), in an order
-// that the sizes alone decide.  red: VV values a thread; out may be read by all threads afterwards.
-template <int VV>
-__device__ __forceinline__ void run_sums(const float* val, int active, int W, int q, int D, int per, float* red, float* out) {
-  const int t = threadIdx.x, T = blockDim.x;
-  if (q == 1) {
-    float s = 0.f;
-#pragma unroll
-    for (int v = 0; v < VV; ++v) s += val[v];
-    s = wave_sum(t < active ? s : 0.f);
-    __syncthreads();
-    if ((t & 63) == 0) red[t >> 6] = s;
-    __syncthreads();
-    s = 0.f;
-    for (int w = 0; w < T >> 6; ++w) s += red[w];
-    if (t == 0) out[0] = s;
-    __syncthreads();
-    return;
+// Count, mean and squares about the mean of some values.
+struct Moments {
+  float n, mean, m2;
+  __device__ __forceinline__ Moments join(const Moments& o) const {
+    const float all = n + o.n, f = all > 0.f ? o.n * __builtin_amdgcn_rcpf(all) : 0.f, d = o.mean - mean;
+    return {all, mean + d * f, m2 + o.m2 + d * d * (n * f)};
   }
-  __syncthreads();
+  __device__ __forceinline__ Moments from(int lane_mask) const {
+    return {__shfl_xor(n, lane_mask), __shfl_xor(mean, lane_mask), __shfl_xor(m2, lane_mask)};
+  }
+};
+struct Sums {
+  float a, b;
+  __device__ __forceinline__ Sums join(const Sums& o) const { return {a + o.a, b + o.b}; }
+  __device__ __forceinline__ Sums from(int lane_mask) const { return {__shfl_xor(a, lane_mask), __shfl_xor(b, lane_mask)}; }
+};
+
+// Joins over runs of D of the block's values.  Thread t < active holds val[0 .. VV), which are the places
+// t VV + v of a matrix of rows of W values; done(g, e) is called by one thread with what columns
+// [g D, (g + 1) D) come to, joined in an order that the sizes alone decide.  `per` threads (a power of two)
+// share a run.  red: VV values a thread.  Ends with a barrier.
+template <int VV, typename E, typename Done>
+__device__ __forceinline__ void join_runs(const E* val, int active, int W, int q, int D, int per, E* red, Done done) {
+  const int t = threadIdx.x, T = blockDim.x;
   if (t < active)
 #pragma unroll
     for (int v = 0; v < VV; ++v) red[t * VV + v] = val[v];
   __syncthreads();
-  const int rows = active * VV / W, l = t & (per - 1);
-  const int dp = per / D, dd = per - dp * D;
-  for (int g = t / per; g < q; g += T / per) {
-    int p = l / D, d = l - p * D;
-    float s = 0.f;
-    while (p < rows) {
-      s += red[p * W + g * D + d];
-      p += dp;
-      d += dd;
-      if (d >= D) {
-        d -= D;
-        ++p;
+  const int count = active * VV / W * D, l = t & (per - 1), wide = per < 64 ? per : 64;
+  const float inv = 1.0f / (float)D;
+  for (int base = 0; base < q; base += T / per) {
+    const int g = base + t / per;
+    E acc{};
+    if (g < q)
+      for (int i = l; i < count; i += 4 * per) {
+        E f[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int e = i + u * per, p = (int)(((float)e + 0.5f) * inv);  // e / D: e is under 2^16
+          f[u] = E{};
+          if (e < count) f[u] = red[p * (W - D) + e + g * D];
+        }
+        acc = acc.join(f[0].join(f[1]).join(f[2].join(f[3])));
       }
+    for (int m = 1; m < wide; m <<= 1) acc = acc.join(acc.from(m));
+    if (per > 64) {  // waves share a run: per is at most T / q, so this round is the only one
+      __syncthreads();
+      if ((l & 63) == 0) red[t >> 6] = acc;
+      __syncthreads();
+      if (l == 0 && g < q)
+        for (int w = 1; w < per >> 6; ++w) acc = acc.join(red[(t >> 6) + w]);
     }
-    for (int m = 1; m < per; m <<= 1) s += __shfl_xor(s, m);
-    if (l == 0) out[g] = s;
+    if (l == 0 && g < q) done(g, acc);
   }
   __syncthreads();
 }
@@ -166,20 +203,48 @@ struct Columns {
     ntail = o.tail - j * V;
     ntail = !on || r != 0 || ntail < 0 ? 0 : ntail > V ? V : ntail;
   }
-  // Channel (among the block's) of value v, and its group.
+  // Channel, among the block's, of value v.
   __device__ __forceinline__ int channel(const Geo& o, int v) const { return o.k == 1 ? j * V + v : (j * V + v) % o.W; }
-  __device__ __forceinline__ int group(const Geo& o, int v) const { return channel(o, v) / o.D; }
-  __device__ __forceinline__ void params(const Geo& o, const kad_group_norm_args& a, float w[V], float b[V]) const {
+  template <typename Q>
+  __device__ __forceinline__ void param(const Geo& o, const void* p, float none, float f[V]) const {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int c = c0 + channel(o, v);
-      w[v] = on ? load_param(a.weight, c, a.param_dtype, 1.f) : 0.f;
-      b[v] = on ? load_param(a.bias, c, a.param_dtype, 0.f) : 0.f;
+    for (int v = 0; v < V; ++v) f[v] = none;
+    if (!p || !on) return;
+    Q q[V];
+    if (o.k == 1) {
+      __builtin_memcpy(q, (const Q*)p + c0 + j * V, sizeof(q));
+    } else {
+      int c = channel(o, 0);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        q[v] = ((const Q*)p)[c];
+        c = c + 1 == o.W ? 0 : c + 1;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = to_f32(q[v]);
+  }
+  __device__ __forceinline__ void params(const Geo& o, const kad_group_norm_args& a, float w[V], float b[V]) const {
+    if (a.param_dtype == KAD_F32) {
+      param<float>(o, a.weight, 1.f, w);
+      param<float>(o, a.bias, 0.f, b);
+    } else {
+      param<T>(o, a.weight, 1.f, w);
+      param<T>(o, a.bias, 0.f, b);
     }
   }
-  __device__ __forceinline__ void of_groups(const Geo& o, const float* lds, float m[NG]) const {
+  // What p holds for the groups of its values.
+  __device__ __forceinline__ void of_groups(const Geo& o, const float* p, float m[NG]) const {
+    const int c = channel(o, 0);
+    int g = c / o.D, d = c - g * o.D;
 #pragma unroll
-    for (int v = 0; v < NG; ++v) m[v] = on ? lds[group(o, v)] : 0.f;
+    for (int v = 0; v < NG; ++v) {
+      m[v] = on ? p[g] : 0.f;
+      if (++d == o.D) {
+        d = 0;
+        g = g + 1 == o.q ? 0 : g + 1;
+      }
+    }
   }
 };
 
@@ -190,6 +255,8 @@ __device__ __forceinline__ void norm_vec(float x[VEC<T>], const float* mean, con
 }
 
 // ---------------------------------------------------------------------------- resident forward
+constexpr int MOST_RESIDENT = 4;  // vectors a thread
+
 // One block an image and set of groups, whose values stay in registers (U vectors a thread): x is read once,
 // and the variance is that of the differences to the mean.
 template <typename T, bool ONE, int U, int ACT>
@@ -214,9 +281,9 @@ __device__ __forceinline__ void resident_write(const kad_group_norm_args& a, con
   }
 }
 
-template <typename T, bool ONE, int U>
+template <typename T, bool ONE>
 __global__ __launch_bounds__(1024) void group_norm_resident_kernel(kad_group_norm_args a, Geo o) {
-  constexpr int V = VEC<T>, NG = ONE ? 1 : V;
+  constexpr int V = VEC<T>, NG = ONE ? 1 : V, U = MOST_RESIDENT;
   extern __shared__ float lds[];
   // Sets whose channels share lines run on one XCD (blocks go round the 8 of them), so its L2 fetches a line once.
   const int sets = a.groups / o.q;
@@ -224,7 +291,7 @@ __global__ __launch_bounds__(1024) void group_norm_resident_kernel(kad_group_nor
   if (id >= a.n * sets) return;
   const int n = id / sets, set = id - n * sets;
   const Columns<T, ONE> col(o, set * o.W);
-  float* mean = lds + blockDim.x * NG;
+  float* mean = lds + blockDim.x * NG * 3;
   float* rstd = mean + o.q;
   const int64_t P = (int64_t)a.h * a.w;
   const int64_t xs = o.k == 1 ? a.x_cs : (int64_t)o.k * a.c;
@@ -239,7 +306,12 @@ __global__ __launch_bounds__(1024) void group_norm_resident_kernel(kad_group_nor
     if (col.on && row < o.full) raw[u] = load_vec(x + row * xs);
   }
   load_some(x + o.full * xs, col.ntail, xt);
-  float s[NG], m[NG];
+  float w[V], b[V];
+  col.params(o, a, w, b);
+  // The thread's own values first, for each channel or for all; then the block's.
+  const int mine = col.on && col.r < o.full ? (o.full - col.r + o.R - 1) / o.R : 0;
+  Moments mo[NG];
+  float m[NG], s[NG];
 #pragma unroll
   for (int v = 0; v < NG; ++v) s[v] = 0.f;
 #pragma unroll
@@ -251,18 +323,16 @@ __global__ __launch_bounds__(1024) void group_norm_resident_kernel(kad_group_nor
 #pragma unroll
     for (int v = 0; v < V; ++v) s[ONE ? 0 : v] += f[v];
   }
-  const int active = o.R * o.S, rw = ONE ? o.S : o.W, rd = ONE ? o.D / V : o.D;
-  const float M = (float)(P * o.D);
-  run_sums<NG>(s, active, rw, o.q, rd, o.tpg, lds, mean);
-  for (int g = threadIdx.x; g < o.q; g += blockDim.x) mean[g] /= M;
+#pragma unroll
+  for (int v = 0; v < NG; ++v) {
+    mo[v].n = (float)(ONE ? mine * V + col.ntail : mine + (v < col.ntail ? 1 : 0));
+    m[v] = mo[v].mean = mo[v].n > 0.f ? s[v] / mo[v].n : 0.f;
+    s[v] = 0.f;
+  }
   if (sizeof(T) == 2) {
 #pragma unroll
     for (int u = 0; u < U; ++u) repack(raw[u]);
   }
-  __syncthreads();
-  col.of_groups(o, mean, m);
-#pragma unroll
-  for (int v = 0; v < NG; ++v) s[v] = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const float d = xt[v] - m[ONE ? 0 : v];
@@ -279,20 +349,24 @@ __global__ __launch_bounds__(1024) void group_norm_resident_kernel(kad_group_nor
         s[ONE ? 0 : v] += d * d;
       }
     }
-  run_sums<NG>(s, active, rw, o.q, rd, o.tpg, lds, rstd);
+#pragma unroll
+  for (int v = 0; v < NG; ++v) mo[v].m2 = s[v];
   if (sizeof(T) == 2) {
 #pragma unroll
     for (int u = 0; u < U; ++u) repack(raw[u]);
   }
-  for (int g = threadIdx.x; g < o.q; g += blockDim.x) {
-    rstd[g] = 1.0f / sqrtf(rstd[g] / M + a.eps);
-    a.mean[n * a.groups + set * o.q + g] = mean[g];
-    a.rstd[n * a.groups + set * o.q + g] = rstd[g];
-  }
-  __syncthreads();
+  // ONE: every thread's values are of the block's one group
+  join_runs<NG>(mo, o.R * o.S, ONE ? o.R * o.S : o.W, o.q, ONE ? o.R * o.S : o.D, o.tpg, (Moments*)lds,
+                [&](int g, const Moments& e) {
+                  const float r = 1.0f / sqrtf(e.m2 / e.n + a.eps);
+                  mean[g] = e.mean;
+                  rstd[g] = r;
+                  a.mean[n * a.groups + set * o.q + g] = e.mean;
+                  a.rstd[n * a.groups + set * o.q + g] = r;
+                });
+  col.of_groups(o, mean, m);
   if (!col.on) return;
-  float w[V], b[V], rs[NG];
-  col.params(o, a, w, b);
+  float rs[NG];
   col.of_groups(o, rstd, rs);
 #pragma unroll
   for (int v = 0; v < V; ++v) w[v] *= rs[ONE ? 0 : v];
@@ -317,11 +391,46 @@ __device__ __forceinline__ int tile_pixels(const Geo& o, int64_t P, int t) {
   return (int)((t == o.tiles - 1 ? P : next) - first);
 }
 
-// Count, mean and squares about the mean of values seen so far.
+// A thread's rows of a tile, B at a time, the next B on their way while these are worked on.  load(i) reads
+// its i-th row; use(rows, valid) takes the first `valid` of B rows.
+template <typename Raw, int B>
+struct Walk {
+  int count;
+  Raw a[B], b[B];
+  template <typename Load>
+  __device__ __forceinline__ void fetch(Raw r[B], int i, Load load) {
+    if (i < count)
+#pragma unroll
+      for (int k = 0; k < B; ++k) r[k] = load(i + k < count ? i + k : count - 1);
+  }
+  template <typename Load>
+  __device__ __forceinline__ Walk(int rows, Load load) : count(rows) {
+    fetch(a, 0, load);
+  }
+  template <typename Load, typename Use>
+  __device__ __forceinline__ void run(Load load, Use use) {
+    for (int i = 0; i < count; i += 2 * B) {
+      fetch(b, i + B, load);
+      use(i, a, count - i);
+      fetch(a, i + 2 * B, load);
+      if (i + B < count) use(i + B, b, count - i - B);
+    }
+  }
+};
+template <typename T, bool ONE>
+__device__ __forceinline__ int row_count(const Geo& o, const Columns<T, ONE>& col, const Tile& rows) {
+  const int left = rows.last - rows.first - col.r;
+  return col.on && left > 0 ? (left + o.R - 1) / o.R : 0;
+}
+struct Pair {
+  intx4 x, d;
+};
+
+// The moments of a thread's values, for each channel or for all: as many of each.
 template <int NG>
-struct Moments {
+struct Running {
   float n, mean[NG], m2[NG];
-  __device__ __forceinline__ Moments() : n(0.f) {
+  __device__ __forceinline__ Running() : n(0.f) {
 #pragma unroll
     for (int v = 0; v < NG; ++v) mean[v] = m2[v] = 0.f;
   }
@@ -339,7 +448,7 @@ struct Moments {
 
 // The moments of B rows of V values, over the rows (for each channel) or over all of them.
 template <typename T, bool ONE, int B>
-__device__ __forceinline__ void add_rows(Moments<ONE ? 1 : VEC<T>>& acc, const intx4 raw[B]) {
+__device__ __forceinline__ void add_rows(Running<ONE ? 1 : VEC<T>>& acc, const intx4 raw[B]) {
   constexpr int V = VEC<T>, NG = ONE ? 1 : V;
   float f[B][V], m[NG], q[NG];
 #pragma unroll
@@ -363,8 +472,8 @@ __device__ __forceinline__ void add_rows(Moments<ONE ? 1 : VEC<T>>& acc, const i
   acc.merge(count, m, q);
 }
 
-template <typename T, bool ONE>
-__global__ __launch_bounds__(1024) void group_norm_stats_kernel(kad_group_norm_args a, Geo o) {
+template <typename T, bool ONE, int MOST>
+__global__ __launch_bounds__(MOST) void group_norm_stats_kernel(kad_group_norm_args a, Geo o) {
   constexpr int V = VEC<T>, NG = ONE ? 1 : V, B = 4;
   extern __shared__ float lds[];
   const int n = blockIdx.y, tile = blockIdx.x;
@@ -373,74 +482,100 @@ __global__ __launch_bounds__(1024) void group_norm_stats_kernel(kad_group_norm_a
   const int64_t P = (int64_t)a.h * a.w;
   const int64_t xs = o.k == 1 ? a.x_cs : (int64_t)o.k * a.c;
   const T* x = (const T*)a.x + n * P * a.x_cs + col.j * V;
-  Moments<NG> acc;
-  if (col.on) {
-    int row = rows.first + col.r;
-    for (; row + (B - 1) * o.R < rows.last; row += B * o.R) {
-      intx4 raw[B];
+  Running<NG> acc;
+  const auto load = [&](int i) { return load_vec(x + (int64_t)(rows.first + col.r + i * o.R) * xs); };
+  Walk<intx4, B> walk(row_count(o, col, rows), load);
+  walk.run(load, [&](int, const intx4* raw, int valid) {
+    if (valid >= B) return add_rows<T, ONE, B>(acc, raw);
 #pragma unroll
-      for (int i = 0; i < B; ++i) raw[i] = load_vec(x + (row + i * o.R) * xs);
-      add_rows<T, ONE, B>(acc, raw);
-    }
-    for (; row < rows.last; row += o.R) {
-      const intx4 raw[1] = {load_vec(x + row * xs)};
-      add_rows<T, ONE, 1>(acc, raw);
-    }
-  }
-  // The short row's values: of a channel each, so counts differ from channel to channel.
-  float xt[V], s[NG];
+    for (int i = 0; i < B; ++i)
+      if (i < valid) add_rows<T, ONE, 1>(acc, raw + i);
+  });
+  // The short row's values are of a channel each, so counts differ from channel to channel.
+  Moments mo[NG];
+#pragma unroll
+  for (int v = 0; v < NG; ++v) mo[v] = Moments{acc.n, acc.mean[v], acc.m2[v]};
   const int nt = rows.tail ? col.ntail : 0;
-  load_some(x + o.full * xs, nt, xt);
+  if (nt) {
+    float xt[V];
+    load_some(x + o.full * xs, nt, xt);
 #pragma unroll
-  for (int v = 0; v < NG; ++v) s[v] = acc.n * acc.mean[v];
-#pragma unroll
-  for (int v = 0; v < V; ++v) s[ONE ? 0 : v] += xt[v];
-  const int active = o.R * o.S, rw = ONE ? o.S : o.W, rd = ONE && o.q > 1 ? o.D / V : o.D;
-  float *mean = lds + blockDim.x * NG, *m2 = mean + o.q;
-  const float count = (float)tile_pixels(o, P, tile) * (float)o.D;
-  run_sums<NG>(s, active, rw, o.q, rd, o.tpg, lds, mean);
-  for (int g = threadIdx.x; g < o.q; g += blockDim.x) mean[g] /= count;
-  __syncthreads();
-  float m[NG];
-  col.of_groups(o, mean, m);
-#pragma unroll
-  for (int v = 0; v < NG; ++v) {
-    const float d = acc.mean[v] - m[v];
-    s[v] = acc.n > 0.f ? acc.m2[v] + acc.n * d * d : 0.f;
+    for (int v = 0; v < V; ++v)
+      if (v < nt) mo[ONE ? 0 : v] = mo[ONE ? 0 : v].join(Moments{1.f, xt[v], 0.f});
   }
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const float d = xt[v] - m[ONE ? 0 : v];
-    s[ONE ? 0 : v] += v < nt ? d * d : 0.f;
-  }
-  run_sums<NG>(s, active, rw, o.q, rd, o.tpg, lds, m2);
-  float2* part = (float2*)a.work + ((int64_t)n * o.tiles + tile) * o.q;
-  for (int g = threadIdx.x; g < o.q; g += blockDim.x) part[g] = make_float2(mean[g], m2[g]);
+  const bool vectors = ONE && o.q > 1;  // a group is D / V of the threads' values; the only group is all of them
+  const int active = o.R * o.S, W = vectors ? o.S : ONE ? active : o.W, D = vectors ? o.D / V : ONE ? active : o.D;
+  Sums* part = (Sums*)a.work + ((int64_t)n * o.tiles + tile) * o.q;
+  join_runs<NG>(mo, active, W, o.q, D, o.tpg, (Moments*)lds, [&](int g, const Moments& e) { part[g] = Sums{e.mean, e.m2}; });
 }
 
-template <typename T, bool ONE, int ACT>
-__device__ __forceinline__ void apply_rows(const Geo& o, const Columns<T, ONE>& col, const Tile& rows, const T* x, int64_t xs,
-                                           T* y, int64_t ys, const float* mean, const float* w, const float* b) {
-  constexpr int V = VEC<T>, B = 4;
-  int row = rows.first + col.r;
-  for (; row + (B - 1) * o.R < rows.last; row += B * o.R) {
-    intx4 raw[B];
+// Joins what the tiles of an image left for each group: thread t takes group t mod q of every per-th tile,
+// consecutive threads consecutive groups, and halves of the block join in LDS, in an order that the sizes alone
+// decide.  The first two tiles' parts are asked for by the constructor, before the rows that a caller fetches
+// meanwhile: loads return in order.
+template <typename E>
+struct TileJoin {
+  const Sums* part;
+  int per, l, g;
+  Sums first[2];
+  __device__ __forceinline__ TileJoin(const Geo& o, const Sums* p) : part(p) {
+    const int t = threadIdx.x, most = blockDim.x / o.q;
+    per = most < 1 ? 1 : most < o.tiles ? most : o.tiles;
+    l = t / o.q;
+    g = t - l * o.q;
 #pragma unroll
-    for (int i = 0; i < B; ++i) raw[i] = load_vec(x + (row + i * o.R) * xs);
-#pragma unroll
-    for (int i = 0; i < B; ++i) {
-      float f[V];
-      unpack<T>(raw[i], f);
-      norm_vec<T, ONE, ACT>(f, mean, w, b);
-      store_vec(y + (row + i * o.R) * ys, f);
+    for (int i = 0; i < 2; ++i)
+      if (l < per && l + i * per < o.tiles) first[i] = part[(l + i * per) * o.q + g];
+  }
+  // make(tile, part) gives a tile's E.
+  template <typename Make, typename Done>
+  __device__ __forceinline__ void run(const Geo& o, E* red, Make make, Done done) {
+    const int t = threadIdx.x;
+    if (o.q > (int)blockDim.x) {  // a group a thread, over and over
+      for (int k = t; k < o.q; k += blockDim.x) {
+        E acc = make(0, part[k]);
+        for (int i = 1; i < o.tiles; ++i) acc = acc.join(make(i, part[i * o.q + k]));
+        done(k, acc);
+      }
+      __syncthreads();
+      return;
     }
+    E acc{};
+    if (l < per) {
+      acc = make(l, first[0]);
+      if (l + per < o.tiles) acc = acc.join(make(l + per, first[1]));
+      for (int i = l + 2 * per; i < o.tiles; i += per) acc = acc.join(make(i, part[i * o.q + g]));
+    }
+    red[t] = acc;
+    for (int n = per; n > 1;) {
+      const int half = (n + 1) / 2;
+      __syncthreads();
+      if (l + half < n) {
+        acc = acc.join(red[t + half * o.q]);
+        red[t] = acc;
+      }
+      n = half;
+    }
+    if (l == 0) done(g, acc);
+    __syncthreads();
   }
-  for (; row < rows.last; row += o.R) {
-    float f[V];
-    unpack<T>(load_vec(x + row * xs), f);
-    norm_vec<T, ONE, ACT>(f, mean, w, b);
-    store_vec(y + row * ys, f);
-  }
+};
+
+template <typename T, bool ONE, int ACT, int B, typename Load>
+__device__ __forceinline__ void apply_rows(const Geo& o, const Columns<T, ONE>& col, const Tile& rows, const T* x, int64_t xs,
+                                           T* y, int64_t ys, const float* mean, const float* w, const float* b,
+                                           Walk<intx4, B>& walk, Load load) {
+  constexpr int V = VEC<T>;
+  walk.run(load, [&](int at, const intx4* raw, int valid) {
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+      if (i < valid) {
+        float f[V];
+        unpack<T>(raw[i], f);
+        norm_vec<T, ONE, ACT>(f, mean, w, b);
+        stream_vec(y + (int64_t)(rows.last - 1 - col.r - (at + i) * o.R) * ys, f);
+      }
+  });
   if (rows.tail && col.ntail) {
     float f[V];
     load_some(x + o.full * xs, col.ntail, f);
@@ -449,106 +584,84 @@ __device__ __forceinline__ void apply_rows(const Geo& o, const Columns<T, ONE>& 
   }
 }
 
-template <typename T, bool ONE>
-__global__ __launch_bounds__(1024) void group_norm_apply_kernel(kad_group_norm_args a, Geo o) {
-  constexpr int V = VEC<T>, NG = ONE ? 1 : V;
+template <typename T, bool ONE, int MOST>
+__global__ __launch_bounds__(MOST) void group_norm_apply_kernel(kad_group_norm_args a, Geo o) {
+  constexpr int V = VEC<T>, NG = ONE ? 1 : V, B = 4;
   extern __shared__ float lds[];
   const int n = blockIdx.y, tile = blockIdx.x;
   const Columns<T, ONE> col(o, 0);
+  const Tile rows(o, tile);
   const int64_t P = (int64_t)a.h * a.w;
-  float *mean = lds, *rstd = lds + o.q;
-  {  // the tiles' means and squares, joined
-    const float2* part = (const float2*)a.work + (int64_t)n * o.tiles * o.q;
-    const float M = (float)P * (float)o.D;
-    const int per = o.tpg, l = threadIdx.x & (per - 1);
-    for (int g = threadIdx.x / per; g < o.q; g += blockDim.x / per) {
-      float s = 0.f;
-      for (int t = l; t < o.tiles; t += per) s += part[t * o.q + g].x * (float)tile_pixels(o, P, t);
-      for (int m = 1; m < per; m <<= 1) s += __shfl_xor(s, m);
-      const float mu = s / (float)P;
-      s = 0.f;
-      for (int t = l; t < o.tiles; t += per) {
-        const float2 p = part[t * o.q + g];
-        const float d = p.x - mu;
-        s += p.y + d * d * ((float)tile_pixels(o, P, t) * (float)o.D);
-      }
-      for (int m = 1; m < per; m <<= 1) s += __shfl_xor(s, m);
-      if (l == 0) {
-        const float rs = 1.0f / sqrtf(s / M + a.eps);
-        mean[g] = mu;
-        rstd[g] = rs;
-        if (tile == 0) {
-          a.mean[n * a.groups + g] = mu;
-          a.rstd[n * a.groups + g] = rs;
-        }
-      }
-    }
-    __syncthreads();
-  }
-  if (!col.on) return;
+  const int64_t xs = o.k == 1 ? a.x_cs : (int64_t)o.k * a.c, ys = (int64_t)o.k * a.c;
+  const T* x = (const T*)a.x + n * P * a.x_cs + col.j * V;
+  T* y = (T*)a.out + n * P * a.c + col.j * V;
   float w[V], b[V], m[NG], rs[NG];
+  TileJoin<Moments> join(o, (const Sums*)a.work + (int64_t)n * o.tiles * o.q);
   col.params(o, a, w, b);
+  // Backwards: what the statistics read last is still near.
+  const auto load = [&](int i) { return load_vec(x + (int64_t)(rows.last - 1 - col.r - i * o.R) * xs); };
+  Walk<intx4, B> walk(row_count(o, col, rows), load);
+  float *mean = lds + 3 * blockDim.x, *rstd = mean + o.q;
+  join.run(
+      o, (Moments*)lds,
+      [&](int t, const Sums& p) { return Moments{(float)tile_pixels(o, P, t) * (float)o.D, p.a, p.b}; },
+      [&](int g, const Moments& e) {
+        const float r = 1.0f / sqrtf(e.m2 / e.n + a.eps);
+        mean[g] = e.mean;
+        rstd[g] = r;
+        if (tile == 0) {
+          a.mean[n * a.groups + g] = e.mean;
+          a.rstd[n * a.groups + g] = r;
+        }
+      });
+  if (!col.on) return;
   col.of_groups(o, mean, m);
   col.of_groups(o, rstd, rs);
 #pragma unroll
   for (int v = 0; v < V; ++v) w[v] *= rs[ONE ? 0 : v];
-  const Tile rows(o, tile);
-  const int64_t xs = o.k == 1 ? a.x_cs : (int64_t)o.k * a.c, ys = (int64_t)o.k * a.c;
-  const T* x = (const T*)a.x + n * P * a.x_cs + col.j * V;
-  T* y = (T*)a.out + n * P * a.c + col.j * V;
-  if (a.act == KAD_ACT_SILU) apply_rows<T, ONE, KAD_ACT_SILU>(o, col, rows, x, xs, y, ys, m, w, b);
-  else if (a.act == KAD_ACT_RELU) apply_rows<T, ONE, KAD_ACT_RELU>(o, col, rows, x, xs, y, ys, m, w, b);
-  else apply_rows<T, ONE, KAD_ACT_NONE>(o, col, rows, x, xs, y, ys, m, w, b);
+  if (a.act == KAD_ACT_SILU) apply_rows<T, ONE, KAD_ACT_SILU, B>(o, col, rows, x, xs, y, ys, m, w, b, walk, load);
+  else if (a.act == KAD_ACT_RELU) apply_rows<T, ONE, KAD_ACT_RELU, B>(o, col, rows, x, xs, y, ys, m, w, b, walk, load);
+  else apply_rows<T, ONE, KAD_ACT_NONE, B>(o, col, rows, x, xs, y, ys, m, w, b, walk, load);
 }
 
 // ---------------------------------------------------------------------------- backward
 // Two launches: the sums of dz and dz xhat of each channel in each tile, and of w times them in each group;
 // then dx.  The last blocks of the second one sum the channels' parts to dw and db.
+// With xm = x - mean and w times rstd: z = xm w + b, and the sums of dz and dz xm.
 template <typename T, bool ONE, int ACT>
-__device__ __forceinline__ void sum_vec(const float x[VEC<T>], const float dy[VEC<T>], const float* mean, const float* rstd,
-                                        const float* w, const float* b, float* db, float* dw) {
+__device__ __forceinline__ void sum_vec(const float x[VEC<T>], const float dy[VEC<T>], const float* mean, const float* w,
+                                        const float* b, float* db, float* dw) {
 #pragma unroll
   for (int v = 0; v < VEC<T>; ++v) {
-    const float xhat = (x[v] - mean[ONE ? 0 : v]) * rstd[ONE ? 0 : v];
-    const float dz = act_grad<ACT>(xhat * w[v] + b[v], dy[v]);
+    const float xm = x[v] - mean[ONE ? 0 : v];
+    const float dz = act_grad<ACT>(xm * w[v] + b[v], dy[v]);
     db[v] += dz;
-    dw[v] += dz * xhat;
+    dw[v] += dz * xm;
   }
 }
 
-template <typename T, bool ONE, int ACT>
+template <typename T, bool ONE, int ACT, int B, typename Load>
 __device__ __forceinline__ void sum_rows(const Geo& o, const Columns<T, ONE>& col, const Tile& rows, const T* x, int64_t xs,
-                                         const T* dy, int64_t ds, const float* mean, const float* rstd, const float* w,
-                                         const float* b, float* db, float* dw) {
-  constexpr int V = VEC<T>, B = 2;
-  int row = rows.first + col.r;
-  for (; row + (B - 1) * o.R < rows.last; row += B * o.R) {
-    intx4 rx[B], rd[B];
+                                         const T* dy, int64_t ds, const float* mean, const float* w, const float* b, float* db,
+                                         float* dw, Walk<Pair, B>& walk, Load load) {
+  constexpr int V = VEC<T>;
+  walk.run(load, [&](int, const Pair* raw, int valid) {
 #pragma unroll
-    for (int i = 0; i < B; ++i) rx[i] = load_vec(x + (row + i * o.R) * xs);
-#pragma unroll
-    for (int i = 0; i < B; ++i) rd[i] = load_vec(dy + (row + i * o.R) * ds);
-#pragma unroll
-    for (int i = 0; i < B; ++i) {
-      float f[V], g[V];
-      unpack<T>(rx[i], f);
-      unpack<T>(rd[i], g);
-      sum_vec<T, ONE, ACT>(f, g, mean, rstd, w, b, db, dw);
-    }
-  }
-  for (; row < rows.last; row += o.R) {
-    float f[V], g[V];
-    unpack<T>(load_vec(x + row * xs), f);
-    unpack<T>(load_vec(dy + row * ds), g);
-    sum_vec<T, ONE, ACT>(f, g, mean, rstd, w, b, db, dw);
-  }
+    for (int i = 0; i < B; ++i)
+      if (i < valid) {
+        float f[V], g[V];
+        unpack<T>(raw[i].x, f);
+        unpack<T>(raw[i].d, g);
+        sum_vec<T, ONE, ACT>(f, g, mean, w, b, db, dw);
+      }
+  });
   if (rows.tail && col.ntail) {
     float f[V], g[V], d1[V], d2[V];
     load_some(x + o.full * xs, col.ntail, f);
     load_some(dy + o.full * ds, col.ntail, g);
 #pragma unroll
     for (int v = 0; v < V; ++v) d1[v] = d2[v] = 0.f;
-    sum_vec<T, ONE, ACT>(f, g, mean, rstd, w, b, d1, d2);
+    sum_vec<T, ONE, ACT>(f, g, mean, w, b, d1, d2);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       db[v] += v < col.ntail ? d1[v] : 0.f;
@@ -557,9 +670,9 @@ __device__ __forceinline__ void sum_rows(const Geo& o, const Columns<T, ONE>& co
   }
 }
 
-template <typename T, bool ONE>
-__global__ __launch_bounds__(1024) void group_norm_bwd_sums_kernel(kad_group_norm_args a, Geo o) {
-  constexpr int V = VEC<T>, NG = ONE ? 1 : V;
+template <typename T, bool ONE, int MOST>
+__global__ __launch_bounds__(MOST) void group_norm_bwd_sums_kernel(kad_group_norm_args a, Geo o) {
+  constexpr int V = VEC<T>, NG = ONE ? 1 : V, B = MOST > 512 ? 2 : 4;
   extern __shared__ float lds[];
   const int n = blockIdx.y, tile = blockIdx.x;
   const Columns<T, ONE> col(o, 0);
@@ -568,89 +681,90 @@ __global__ __launch_bounds__(1024) void group_norm_bwd_sums_kernel(kad_group_nor
   const int64_t xs = o.k == 1 ? a.x_cs : (int64_t)o.k * a.c, ds = o.k == 1 ? a.dy_cs : (int64_t)o.k * a.c;
   const T* x = (const T*)a.x + n * P * a.x_cs + col.j * V;
   const T* dy = (const T*)a.dy + n * P * a.dy_cs + col.j * V;
+  float w[V], b[V], m[NG], rs[NG];
+  col.params(o, a, w, b);
+  col.of_groups(o, a.mean + n * o.q, m);
+  col.of_groups(o, a.rstd + n * o.q, rs);
+  const auto load = [&](int i) {
+    const int64_t row = rows.first + col.r + i * o.R;
+    return Pair{load_vec(x + row * xs), load_vec(dy + row * ds)};
+  };
+  Walk<Pair, B> walk(row_count(o, col, rows), load);
+  // The channels' sums, and their weights, for the groups' sums.
+  Sums* red = (Sums*)lds;
+  float *cb = lds + 2 * blockDim.x * V, *cw = cb + o.W, *weight = cw + o.W;
+  if (col.on && col.r == 0) {
+    int c = col.channel(o, 0);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {  // where a row is several pixels, its threads write the same weights
+      weight[c] = w[v];
+      c = c + 1 == o.W ? 0 : c + 1;
+    }
+  }
   float db[V], dw[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) db[v] = dw[v] = 0.f;
-  if (col.on) {
-    float w[V], b[V], m[NG], rs[NG];
-    col.params(o, a, w, b);
-    col.of_groups(o, a.mean + n * o.q, m);
-    col.of_groups(o, a.rstd + n * o.q, rs);
-    if (a.act == KAD_ACT_SILU) sum_rows<T, ONE, KAD_ACT_SILU>(o, col, rows, x, xs, dy, ds, m, rs, w, b, db, dw);
-    else if (a.act == KAD_ACT_RELU) sum_rows<T, ONE, KAD_ACT_RELU>(o, col, rows, x, xs, dy, ds, m, rs, w, b, db, dw);
-    else sum_rows<T, ONE, KAD_ACT_NONE>(o, col, rows, x, xs, dy, ds, m, rs, w, b, db, dw);
+  for (int v = 0; v < V; ++v) {
+    db[v] = dw[v] = 0.f;
+    w[v] *= rs[ONE ? 0 : v];
   }
-  const int active = o.R * o.S, T_ = blockDim.x;
-  float *cb = lds + T_ * V, *cw = cb + o.W;
-  run_sums<V>(db, active, o.W, o.W, 1, o.tpc, lds, cb);
-  run_sums<V>(dw, active, o.W, o.W, 1, o.tpc, lds, cw);
+  if (a.act == KAD_ACT_SILU) sum_rows<T, ONE, KAD_ACT_SILU, B>(o, col, rows, x, xs, dy, ds, m, w, b, db, dw, walk, load);
+  else if (a.act == KAD_ACT_RELU) sum_rows<T, ONE, KAD_ACT_RELU, B>(o, col, rows, x, xs, dy, ds, m, w, b, db, dw, walk, load);
+  else sum_rows<T, ONE, KAD_ACT_NONE, B>(o, col, rows, x, xs, dy, ds, m, w, b, db, dw, walk, load);
+  Sums sums[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) sums[v] = Sums{db[v], dw[v] * rs[ONE ? 0 : v]};
   const int64_t part = (int64_t)n * o.tiles + tile;
-  float2* groups = (float2*)a.work + part * o.q;
-  const int l = threadIdx.x & (o.tpg - 1);
-  for (int g = threadIdx.x / o.tpg; g < o.q; g += T_ / o.tpg) {
-    float s1 = 0.f, s2 = 0.f;
-    for (int c = g * o.D + l; c < (g + 1) * o.D; c += o.tpg) {
-      const float w = load_param(a.weight, c, a.param_dtype, 1.f);
-      s1 += w * cb[c];
-      s2 += w * cw[c];
-    }
-    for (int m = 1; m < o.tpg; m <<= 1) {
-      s1 += __shfl_xor(s1, m);
-      s2 += __shfl_xor(s2, m);
-    }
-    if (l == 0) groups[g] = make_float2(s1, s2);
-  }
-  if (a.dweight || a.dbias) {
-    float2* chans = (float2*)a.work + (int64_t)a.n * o.tiles * o.q + part * o.W;
-    for (int c = threadIdx.x; c < o.W; c += T_) chans[c] = make_float2(cb[c], cw[c]);
+  Sums* chans = (Sums*)a.work + (int64_t)a.n * o.tiles * o.q + part * o.W;
+  const bool keep = a.dweight || a.dbias;
+  join_runs<V>(sums, o.R * o.S, o.W, o.W, 1, o.tpc, red, [&](int c, const Sums& e) {
+    cb[c] = e.a;
+    cw[c] = e.b;
+    if (keep) chans[c] = e;
+  });
+  Sums* groups = (Sums*)a.work + part * o.q;
+  const int per = o.tpg < 64 ? o.tpg : 64, l = threadIdx.x & (per - 1);
+  for (int g = threadIdx.x / per; g < o.q; g += blockDim.x / per) {
+    Sums acc{};
+    for (int c = g * o.D + l; c < (g + 1) * o.D; c += per) acc = acc.join(Sums{weight[c] * cb[c], weight[c] * cw[c]});
+    for (int k = 1; k < per; k <<= 1) acc = acc.join(acc.from(k));
+    if (l == 0) groups[g] = acc;
   }
 }
 
+// dx = rstd (w dz - s1 - xhat s2) with w times rstd, c1 = rstd s1 and c2 = rstd^2 s2.
 template <typename T, bool ONE, int ACT>
-__device__ __forceinline__ void dx_vec(float x[VEC<T>], const float dy[VEC<T>], const float* mean, const float* rstd,
-                                       const float* w, const float* b, const float* s1, const float* s2) {
+__device__ __forceinline__ void dx_vec(float x[VEC<T>], const float dy[VEC<T>], const float* mean, const float* w,
+                                       const float* b, const float* c1, const float* c2) {
 #pragma unroll
   for (int v = 0; v < VEC<T>; ++v) {
     const int g = ONE ? 0 : v;
-    const float xhat = (x[v] - mean[g]) * rstd[g];
-    const float dz = act_grad<ACT>(xhat * w[v] + b[v], dy[v]);
-    x[v] = rstd[g] * (w[v] * dz - s1[g] - xhat * s2[g]);
+    const float xm = x[v] - mean[g];
+    const float dz = act_grad<ACT>(xm * w[v] + b[v], dy[v]);
+    x[v] = w[v] * dz - (xm * c2[g] + c1[g]);
   }
 }
 
-template <typename T, bool ONE, int ACT>
+template <typename T, bool ONE, int ACT, int B, typename Load>
 __device__ __forceinline__ void dx_rows(const Geo& o, const Columns<T, ONE>& col, const Tile& rows, const T* x, int64_t xs,
-                                        const T* dy, int64_t ds, T* dx, int64_t os, const float* mean, const float* rstd,
-                                        const float* w, const float* b, const float* s1, const float* s2) {
-  constexpr int V = VEC<T>, B = 2;
-  int row = rows.first + col.r;
-  for (; row + (B - 1) * o.R < rows.last; row += B * o.R) {
-    intx4 rx[B], rd[B];
+                                        const T* dy, int64_t ds, T* dx, int64_t os, const float* mean, const float* w,
+                                        const float* b, const float* c1, const float* c2, Walk<Pair, B>& walk, Load load) {
+  constexpr int V = VEC<T>;
+  walk.run(load, [&](int at, const Pair* raw, int valid) {
 #pragma unroll
-    for (int i = 0; i < B; ++i) rx[i] = load_vec(x + (row + i * o.R) * xs);
-#pragma unroll
-    for (int i = 0; i < B; ++i) rd[i] = load_vec(dy + (row + i * o.R) * ds);
-#pragma unroll
-    for (int i = 0; i < B; ++i) {
-      float f[V], g[V];
-      unpack<T>(rx[i], f);
-      unpack<T>(rd[i], g);
-      dx_vec<T, ONE, ACT>(f, g, mean, rstd, w, b, s1, s2);
-      store_vec(dx + (row + i * o.R) * os, f);
-    }
-  }
-  for (; row < rows.last; row += o.R) {
-    float f[V], g[V];
-    unpack<T>(load_vec(x + row * xs), f);
-    unpack<T>(load_vec(dy + row * ds), g);
-    dx_vec<T, ONE, ACT>(f, g, mean, rstd, w, b, s1, s2);
-    store_vec(dx + row * os, f);
-  }
+    for (int i = 0; i < B; ++i)
+      if (i < valid) {
+        float f[V], g[V];
+        unpack<T>(raw[i].x, f);
+        unpack<T>(raw[i].d, g);
+        dx_vec<T, ONE, ACT>(f, g, mean, w, b, c1, c2);
+        stream_vec(dx + (int64_t)(rows.last - 1 - col.r - (at + i) * o.R) * os, f);
+      }
+  });
   if (rows.tail && col.ntail) {
     float f[V], g[V];
     load_some(x + o.full * xs, col.ntail, f);
     load_some(dy + o.full * ds, col.ntail, g);
-    dx_vec<T, ONE, ACT>(f, g, mean, rstd, w, b, s1, s2);
+    dx_vec<T, ONE, ACT>(f, g, mean, w, b, c1, c2);
     store_some(dx + o.full * os, col.ntail, f);
   }
 }
@@ -660,80 +774,81 @@ constexpr int PARAM_CHANNELS = 16;
 __device__ __forceinline__ void param_sums(const kad_group_norm_args& a, const Geo& o, int block, float* lds) {
   const int c = block * PARAM_CHANNELS + (threadIdx.x & (PARAM_CHANNELS - 1));
   const int parts = a.n * o.tiles, step = blockDim.x / PARAM_CHANNELS;
-  const float2* chans = (const float2*)a.work + (int64_t)parts * o.q;
+  const Sums* chans = (const Sums*)a.work + (int64_t)parts * o.q;
   float db = 0.f, dw = 0.f;
   if (c < o.W)
     for (int i = threadIdx.x / PARAM_CHANNELS; i < parts; i += step) {
-      const float2 p = chans[(int64_t)i * o.W + c];
-      db += p.x;
-      dw += p.y;
+      const Sums p = chans[(int64_t)i * o.W + c];
+      db += p.a;
+      dw += p.b;
     }
 #pragma unroll
   for (int d = PARAM_CHANNELS; d < 64; d <<= 1) {
     db += __shfl_xor(db, d);
     dw += __shfl_xor(dw, d);
   }
-  float2* waves = (float2*)lds;
-  if ((threadIdx.x & 63) < PARAM_CHANNELS) waves[(threadIdx.x >> 6) * PARAM_CHANNELS + (threadIdx.x & 63)] = make_float2(db, dw);
+  Sums* waves = (Sums*)lds;
+  if ((threadIdx.x & 63) < PARAM_CHANNELS) waves[(threadIdx.x >> 6) * PARAM_CHANNELS + (threadIdx.x & 63)] = Sums{db, dw};
   __syncthreads();
   if (threadIdx.x < PARAM_CHANNELS && c < o.W) {
     db = dw = 0.f;
     for (int w = 0; w < blockDim.x >> 6; ++w) {
-      db += waves[w * PARAM_CHANNELS + threadIdx.x].x;
-      dw += waves[w * PARAM_CHANNELS + threadIdx.x].y;
+      db += waves[w * PARAM_CHANNELS + threadIdx.x].a;
+      dw += waves[w * PARAM_CHANNELS + threadIdx.x].b;
     }
     if (a.dweight) store_param(a.dweight, c, a.param_dtype, dw);
     if (a.dbias) store_param(a.dbias, c, a.param_dtype, db);
   }
 }
 
-template <typename T, bool ONE>
-__global__ __launch_bounds__(1024) void group_norm_dx_kernel(kad_group_norm_args a, Geo o) {
-  constexpr int V = VEC<T>, NG = ONE ? 1 : V;
+template <typename T, bool ONE, int MOST>
+__global__ __launch_bounds__(MOST) void group_norm_dx_kernel(kad_group_norm_args a, Geo o) {
+  constexpr int V = VEC<T>, NG = ONE ? 1 : V, B = MOST > 512 ? 2 : 4;
   extern __shared__ float lds[];
   const int maps = a.out ? a.n * o.tiles : 0;
   if ((int)blockIdx.x >= maps) return param_sums(a, o, blockIdx.x - maps, lds);
   const int n = blockIdx.x / o.tiles, tile = blockIdx.x - n * o.tiles;
   const Columns<T, ONE> col(o, 0);
-  const int64_t P = (int64_t)a.h * a.w;
-  float *l1 = lds, *l2 = lds + o.q;
-  {
-    const float2* part = (const float2*)a.work + (int64_t)n * o.tiles * o.q;
-    const float inv = 1.0f / ((float)P * (float)o.D);
-    const int per = o.tpg, l = threadIdx.x & (per - 1);
-    for (int g = threadIdx.x / per; g < o.q; g += blockDim.x / per) {
-      float s1 = 0.f, s2 = 0.f;
-      for (int t = l; t < o.tiles; t += per) {
-        const float2 p = part[t * o.q + g];
-        s1 += p.x;
-        s2 += p.y;
-      }
-      for (int m = 1; m < per; m <<= 1) {
-        s1 += __shfl_xor(s1, m);
-        s2 += __shfl_xor(s2, m);
-      }
-      if (l == 0) {
-        l1[g] = s1 * inv;
-        l2[g] = s2 * inv;
-      }
-    }
-    __syncthreads();
-  }
-  if (!col.on) return;
-  float w[V], b[V], m[NG], rs[NG], s1[NG], s2[NG];
-  col.params(o, a, w, b);
-  col.of_groups(o, a.mean + n * o.q, m);
-  col.of_groups(o, a.rstd + n * o.q, rs);
-  col.of_groups(o, l1, s1);
-  col.of_groups(o, l2, s2);
   const Tile rows(o, tile);
+  const int64_t P = (int64_t)a.h * a.w;
   const int64_t os = (int64_t)o.k * a.c, xs = o.k == 1 ? a.x_cs : os, ds = o.k == 1 ? a.dy_cs : os;
   const T* x = (const T*)a.x + n * P * a.x_cs + col.j * V;
   const T* dy = (const T*)a.dy + n * P * a.dy_cs + col.j * V;
   T* dx = (T*)a.out + n * P * a.c + col.j * V;
-  if (a.act == KAD_ACT_SILU) dx_rows<T, ONE, KAD_ACT_SILU>(o, col, rows, x, xs, dy, ds, dx, os, m, rs, w, b, s1, s2);
-  else if (a.act == KAD_ACT_RELU) dx_rows<T, ONE, KAD_ACT_RELU>(o, col, rows, x, xs, dy, ds, dx, os, m, rs, w, b, s1, s2);
-  else dx_rows<T, ONE, KAD_ACT_NONE>(o, col, rows, x, xs, dy, ds, dx, os, m, rs, w, b, s1, s2);
+  float w[V], b[V], m[NG], rs[NG], s1[NG], s2[NG];
+  TileJoin<Sums> join(o, (const Sums*)a.work + (int64_t)n * o.tiles * o.q);
+  col.params(o, a, w, b);
+  col.of_groups(o, a.mean + n * o.q, m);
+  col.of_groups(o, a.rstd + n * o.q, rs);
+  const auto load = [&](int i) {
+    const int64_t row = rows.last - 1 - col.r - i * o.R;
+    return Pair{load_vec(x + row * xs), load_vec(dy + row * ds)};
+  };
+  Walk<Pair, B> walk(row_count(o, col, rows), load);
+  float *l1 = lds + 2 * blockDim.x, *l2 = l1 + o.q;
+  join.run(
+      o, (Sums*)lds, [](int, const Sums& p) { return p; },
+      [&](int g, const Sums& e) {
+        const float inv = 1.0f / ((float)P * (float)o.D);
+        l1[g] = e.a * inv;
+        l2[g] = e.b * inv;
+      });
+  if (!col.on) return;
+  col.of_groups(o, l1, s1);
+  col.of_groups(o, l2, s2);
+#pragma unroll
+  for (int v = 0; v < V; ++v) w[v] *= rs[ONE ? 0 : v];
+#pragma unroll
+  for (int v = 0; v < NG; ++v) {
+    s1[v] *= rs[v];
+    s2[v] *= rs[v] * rs[v];
+  }
+  if (a.act == KAD_ACT_SILU)
+    dx_rows<T, ONE, KAD_ACT_SILU, B>(o, col, rows, x, xs, dy, ds, dx, os, m, w, b, s1, s2, walk, load);
+  else if (a.act == KAD_ACT_RELU)
+    dx_rows<T, ONE, KAD_ACT_RELU, B>(o, col, rows, x, xs, dy, ds, dx, os, m, w, b, s1, s2, walk, load);
+  else
+    dx_rows<T, ONE, KAD_ACT_NONE, B>(o, col, rows, x, xs, dy, ds, dx, os, m, w, b, s1, s2, walk, load);
 }
 
 // ---------------------------------------------------------------------------- any width
@@ -838,7 +953,7 @@ __global__ __launch_bounds__(256) void group_norm_wide_param_kernel(kad_group_no
 }
 
 // ---------------------------------------------------------------------------- host
-constexpr int MOST_THREADS = 1024, MOST_GROUPS = 2048, MOST_RESIDENT = 16;
+constexpr int MOST_THREADS = 1024, MOST_GROUPS = 2048;
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 int pow2_at_most(int v, int most) {
@@ -866,39 +981,46 @@ bool lay_out(const kad_group_norm_args& a, int q, Geo& o) {
 void count_threads(Geo& o, int rows, int& threads) {
   o.R = rows < 1 ? 1 : rows;
   threads = round_up(o.R * o.S, 64);
-  o.tpg = pow2_at_most(threads / o.q, 64);
-  o.tpc = pow2_at_most(threads / o.W, 64);
+  o.tpg = pow2_at_most(threads / o.q, threads);
+  o.tpc = pow2_at_most(threads / o.W, threads);
 }
 
-// The resident kernel's layout, and the vectors a thread holds; 0: the split kernels' case.
-int resident(const kad_group_norm_args& a, Geo& o, int& threads) {
+// The resident kernel's layout; false: the split kernels' case.
+bool resident(const kad_group_norm_args& a, Geo& o, int& threads) {
   const int V = 16 / dtype_size(a.dtype), D = a.c / a.groups;
   int q = a.c % V ? a.groups : V / gcd(D, V);  // groups whose channels are whole vectors together
   if (a.groups % q) q = a.groups;
-  if (!lay_out(a, q, o)) return 0;
-  const int64_t vectors = (int64_t)o.full * o.S;
-  if (vectors > MOST_RESIDENT * MOST_THREADS) return 0;
-  const int want = (int)(vectors / 4 < 64 ? 64 : vectors / 4 < MOST_THREADS ? vectors / 4 : MOST_THREADS);
-  int rows = want / o.S;
+  if (!lay_out(a, q, o)) return false;
+  // One launch, but a block's columns of D or few channels are pieces of lines that other blocks fetch too, and
+  // one CU reads them: up to 32 KB a block this beats the split kernels ([1, 64, 20, 20] fp16: 5.5 us against 8.2,
+  // [2, 48, 13, 17] fp32: 5.3 against 7.5, [16, 512, 25, 25] in 16 groups 13 against 15), at 64 KB most of it is
+  // lost (8 blocks: 11.1 against 8.9; 256 blocks: 13.8 against 17.0), at 256 KB they take half the time.
+  if ((int64_t)o.full * o.S * 16 > 32 * 1024) return false;
+  int rows = ceil_div(o.full, MOST_RESIDENT);
+  if (rows < ceil_div(64, o.S)) rows = ceil_div(64, o.S);
   if (rows > o.full) rows = o.full;
+  if (rows * o.S > MOST_THREADS) return false;
   count_threads(o, rows, threads);
-  const int held = ceil_div(o.full, o.R);
-  if (held > MOST_RESIDENT) return 0;
-  const int64_t blocks = (int64_t)a.n * (a.groups / q), bytes = vectors * 16;
-  if (bytes > 32 * 1024 && blocks < 128) return 0;
   const int line = 128 / (o.W * dtype_size(a.dtype));
   o.share = line > 1 && (a.groups / q) % line == 0 ? line : 1;
-  return held < 1 ? 1 : held;
+  return true;
 }
 
 // The split kernels' layout; false: the any-width kernels' case.
 bool split(const kad_group_norm_args& a, Geo& o, int& threads) {
   if (!lay_out(a, a.groups, o)) return false;
-  count_threads(o, 512 / o.S < o.full ? 512 / o.S : o.full, threads);
-  // About 2048 threads a CU over all images, and 4 rows a thread at least.
-  int tiles = ceil_div(256 * 2048 / threads, a.n);
-  const int most = ceil_div(o.full, 4 * o.R);
-  if (tiles > most) tiles = most;
+  // One block of 512 threads a CU: what a block does beside its rows (places, weights, the join of what it and
+  // others left) is microseconds, so that more blocks lose more than their loads in flight gain ([8, 256, 100, 100]
+  // fp16, forward and backward: 27 and 46 us; 32 and 54 with two blocks a CU, 44 and 70 with four; 256 threads: 27
+  // and 47).  Threads of under 8 rows are halved ([3, 86, 67, 41] fp32: 9.6 and 12.0 us against 10.4 and 12.7).
+  const int most = (int64_t)a.n * o.full * o.S < 8 * 256 * 512 ? 256 : 512;
+  count_threads(o, most / o.S < o.full ? most / o.S : o.full, threads);
+  int tiles = ceil_div(256, a.n);
+  // An image of over 256 rows a thread and tile is cut finer, up to 256 tiles, whatever the batch.
+  const int64_t fine = o.full / (256 * o.R);
+  if (tiles < fine) tiles = fine < 256 ? (int)fine : 256;
+  const int least = ceil_div(o.full, 4 * o.R);  // 4 rows a thread
+  if (tiles > least) tiles = least;
   if (tiles < 1) tiles = 1;
   o.rows = round_up(ceil_div(o.full, tiles), o.R);
   if (o.rows < 1) o.rows = o.R;
@@ -930,46 +1052,47 @@ int check_call(const kad_group_norm_args* a, bool backward, const char* what) {
 }
 
 template <typename T, bool ONE>
-void launch_resident(const kad_group_norm_args& a, const Geo& o, int held, int threads, hipStream_t st) {
+void launch_resident(const kad_group_norm_args& a, const Geo& o, int threads, hipStream_t st) {
   const int64_t blocks = (int64_t)a.n * (a.groups / o.q), unit = 8 * o.share;
   const dim3 grid((unsigned)((blocks + unit - 1) / unit * unit));
-  const size_t lds = (size_t)(threads * (ONE ? 1 : VEC<T>) + 2 * o.q) * sizeof(float);
-  if (held <= 4) group_norm_resident_kernel<T, ONE, 4><<<grid, threads, lds, st>>>(a, o);
-  else if (held <= 10) group_norm_resident_kernel<T, ONE, 10><<<grid, threads, lds, st>>>(a, o);
-  else group_norm_resident_kernel<T, ONE, MOST_RESIDENT><<<grid, threads, lds, st>>>(a, o);
+  const size_t lds = threads * (ONE ? 1 : VEC<T>) * sizeof(Moments) + 2 * o.q * sizeof(float);
+  allow_lds(group_norm_resident_kernel<T, ONE>, lds);
+  group_norm_resident_kernel<T, ONE><<<grid, threads, lds, st>>>(a, o);
+}
+
+template <typename T, bool ONE, int MOST>
+void launch_split(const kad_group_norm_args& a, const Geo& o, int threads, hipStream_t st) {
+  const dim3 grid(o.tiles, a.n);
+  const size_t stats = threads * (ONE ? 1 : VEC<T>) * sizeof(Moments);
+  allow_lds(group_norm_stats_kernel<T, ONE, MOST>, stats);
+  group_norm_stats_kernel<T, ONE, MOST><<<grid, threads, stats, st>>>(a, o);
+  group_norm_apply_kernel<T, ONE, MOST><<<grid, threads, threads * sizeof(Moments) + 2 * o.q * sizeof(float), st>>>(a, o);
 }
 
 template <typename T>
 void forward(const kad_group_norm_args& a, hipStream_t st) {
   Geo o;
   int threads;
-  if (const int held = resident(a, o, threads)) {
-    if (o.q == 1) launch_resident<T, true>(a, o, held, threads, st);
-    else launch_resident<T, false>(a, o, held, threads, st);
+  if (resident(a, o, threads)) {
+    if (o.q == 1) launch_resident<T, true>(a, o, threads, st);
+    else launch_resident<T, false>(a, o, threads, st);
   } else if (split(a, o, threads)) {
-    const dim3 grid(o.tiles, a.n);
     const bool one = o.q == 1 || o.D % VEC<T> == 0;
-    const size_t own = 2 * o.q * sizeof(float), lds = threads * (one ? 1 : VEC<T>) * sizeof(float) + own;
-    if (one) {
-      group_norm_stats_kernel<T, true><<<grid, threads, lds, st>>>(a, o);
-      group_norm_apply_kernel<T, true><<<grid, threads, own, st>>>(a, o);
-    } else {
-      group_norm_stats_kernel<T, false><<<grid, threads, lds, st>>>(a, o);
-      group_norm_apply_kernel<T, false><<<grid, threads, own, st>>>(a, o);
-    }
+    if (one) threads > 512 ? launch_split<T, true, 1024>(a, o, threads, st) : launch_split<T, true, 512>(a, o, threads, st);
+    else threads > 512 ? launch_split<T, false, 1024>(a, o, threads, st) : launch_split<T, false, 512>(a, o, threads, st);
   } else {
     group_norm_wide_kernel<T><<<dim3(a.groups, a.n), 256, 0, st>>>(a);
   }
 }
 
-template <typename T, bool ONE>
+template <typename T, bool ONE, int MOST>
 void launch_backward(const kad_group_norm_args& a, const Geo& o, int threads, hipStream_t st) {
-  const size_t sums = (size_t)(threads * VEC<T> + 2 * o.W) * sizeof(float);
-  allow_lds(group_norm_bwd_sums_kernel<T, ONE>, sums);
-  group_norm_bwd_sums_kernel<T, ONE><<<dim3(o.tiles, a.n), threads, sums, st>>>(a, o);
+  const size_t sums = threads * VEC<T> * sizeof(Sums) + 3 * o.W * sizeof(float);
+  allow_lds(group_norm_bwd_sums_kernel<T, ONE, MOST>, sums);
+  group_norm_bwd_sums_kernel<T, ONE, MOST><<<dim3(o.tiles, a.n), threads, sums, st>>>(a, o);
   const int blocks = (a.out ? a.n * o.tiles : 0) + (a.dweight || a.dbias ? ceil_div(o.W, PARAM_CHANNELS) : 0);
-  const int own = 2 * o.q, waves = threads / 64 * PARAM_CHANNELS * 2;
-  group_norm_dx_kernel<T, ONE><<<dim3(blocks), threads, (own > waves ? own : waves) * sizeof(float), st>>>(a, o);
+  const int waves = threads / 64 * PARAM_CHANNELS * 2, join = 2 * threads + 2 * o.q;
+  group_norm_dx_kernel<T, ONE, MOST><<<dim3(blocks), threads, (join > waves ? join : waves) * sizeof(float), st>>>(a, o);
 }
 
 template <typename T>
@@ -978,8 +1101,9 @@ void backward(const kad_group_norm_args& a, hipStream_t st) {
   int threads;
   if (!a.out && !a.dweight && !a.dbias) return;
   if (split(a, o, threads)) {
-    if (o.q == 1 || o.D % VEC<T> == 0) launch_backward<T, true>(a, o, threads, st);
-    else launch_backward<T, false>(a, o, threads, st);
+    const bool one = o.q == 1 || o.D % VEC<T> == 0;
+    if (one) threads > 512 ? launch_backward<T, true, 1024>(a, o, threads, st) : launch_backward<T, true, 512>(a, o, threads, st);
+    else threads > 512 ? launch_backward<T, false, 1024>(a, o, threads, st) : launch_backward<T, false, 512>(a, o, threads, st);
     return;
   }
   if (a.out) group_norm_wide_dx_kernel<T><<<dim3(a.groups, a.n), 256, 0, st>>>(a);
