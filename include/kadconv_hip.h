@@ -638,6 +638,7 @@ typedef struct kad_adamw_args {
   double lr, beta1, beta2, eps, weight_decay;
   int64_t step;           /* >= 1 */
   int64_t nchunks;
+  int64_t values;         /* in all chunks together; 0: not known (it decides on speed alone) */
   uint32_t seed;          /* of the 8-bit states' stochastic rounding */
   int dtype;              /* of param and grad */
   int state_bits;         /* 32 or 8 */

@@ -405,10 +405,14 @@ class AdamWTable {
     chunks_ = host.to(params_[0].device());
     args_.chunks = (const kad_adamw_chunk*)chunks_.const_data_ptr();
     args_.nchunks = count;
+    args_.values = 0;
     stepped_.clear();
     std::unordered_set<const void*> seen;
-    for (int i = 0; i < n; ++i)
-      if (grad_at[i] && seen.insert(versioned_[i].unsafeGetTensorImpl()).second) stepped_.push_back(versioned_[i]);
+    for (int i = 0; i < n; ++i) {
+      if (!grad_at[i]) continue;
+      args_.values += numels_[i];
+      if (seen.insert(versioned_[i].unsafeGetTensorImpl()).second) stepped_.push_back(versioned_[i]);
+    }
     grad_at_ = std::move(grad_at);
   }
 
