@@ -6,6 +6,7 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 import kadconv
+from tests import _adamw_ref as R
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
@@ -145,3 +146,63 @@ def test_gradients_of_other_strides():
     kadconv.AdamW([p]).step()
     kadconv.AdamW([q]).step()
     assert torch.equal(p, q) and p.any()
+
+
+def _formula_32_bits(g, codes, scales, t, seed):
+    """One 8-bit step in 32-bit torch operations, each product and sum rounded by itself."""
+    b1, b2 = 0.9, 0.999
+    seg = 256
+    m = (codes[0].float().reshape(-1, seg) * scales[0][:, None]).reshape(-1) * b1 + g * (1 - b1)
+    u = (codes[1].float().reshape(-1, seg) * scales[1][:, None]).reshape(-1)
+    u = torch.sqrt(u * u * b2 + g * g * (1 - b2))
+    r = R.random_bits(seed, t, 0, g.numel()).to(g.device)
+    out = []
+    for v, bits, positive in ((m, r & 0xFFFF, False), (u, r >> 16, True)):
+        most = v.reshape(-1, seg).abs().amax(1, keepdim=True)
+        y = (v.reshape(-1, seg).abs() * torch.where(most > 0, 448.0 / most, torch.zeros_like(most))).clamp(max=448.0).reshape(-1)
+        near, far = (y * 2.0 ** 29).long(), y.view(torch.int32).long() - (120 << 23)
+        c = (torch.where(y < 2.0 ** -6, near, far) + (bits << 4)) >> 20
+        c = torch.where(v > 0, c.clamp(min=1), c) if positive else torch.where(v < 0, c + 128, c)
+        out.append((c.to(torch.uint8), (most * (1.0 / 448.0)).reshape(-1)))
+    return out
+
+
+def test_8_bit_codes_are_those_of_the_formula_in_32_bits():
+    """Held numbers equal, code by code, what 32-bit operations and integer arithmetic on their bits give: a
+    reciprocal that is off by a step in 1 / top * 448 may move one in a million of them to the next code."""
+    n = 256 * 4096
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    p = torch.randn(n, generator=gen, device=DEV)
+    g = torch.empty(n, device=DEV)
+    plan = kadconv.AdamWPlan([p], [g], state_bits=8, seed=11)
+    for t in (1, 2, 3):
+        size = torch.exp(3 * torch.randn(n, generator=gen, device=DEV))
+        g.copy_(torch.randn(n, generator=gen, device=DEV) * 1e-3 * size * (torch.rand(n, generator=gen, device=DEV) > 0.1))
+        st = plan.state
+        before = [st['exp_avg'].clone(), st['exp_avg_sq_root'].clone()], [st['exp_avg_scale'].clone(), st['exp_avg_sq_root_scale'].clone()]
+        want = _formula_32_bits(g, *before, t, 11)
+        plan.step(t)
+        for (c, s), name in zip(want, ('exp_avg', 'exp_avg_sq_root')):
+            got = st[name].view(torch.uint8)
+            torch.testing.assert_close(st[name + '_scale'], s, rtol=2.0 ** -22, atol=0)
+            same = (got == c) | ((got & 127) == 0) & ((c & 127) == 0)   # zeros of either sign
+            assert int((~same).sum()) <= 2, (t, name, int((~same).sum()))
+
+
+def test_steps_of_more_than_the_last_cache_holds():
+    """Over 256 MB a step: loads go past the caches; the result is that of the same values in two plans."""
+    n = 12_000_007
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    p = torch.randn(n, generator=gen, device=DEV)
+    g = torch.randn(n, generator=gen, device=DEV)
+    half = 4096 * 1400
+    q = [p[:half].clone(), p[half:].clone()]
+    whole = kadconv.AdamWPlan([p], [g])
+    parts = [kadconv.AdamWPlan([v], [w.clone()]) for v, w in zip(q, (g[:half], g[half:]))]
+    for t in (1, 2):
+        whole.step(t)
+        for plan in parts:
+            plan.step(t)
+    assert torch.equal(p, torch.cat(q))
+    for name in ('exp_avg', 'exp_avg_sq'):
+        assert torch.equal(whole.state[name][:n], torch.cat([parts[0].state[name][:half], parts[1].state[name][:n - half]]))
