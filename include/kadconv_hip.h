@@ -580,8 +580,8 @@ typedef struct kad_group_norm_args {
   float *mean, *rstd;     /* [N][groups]: forward writes them, backward reads them */
   void *dweight, *dbias;  /* backward: [C], param_dtype, or NULL: not wanted */
   float *work;            /* kad_group_norm_work_elems floats; need not be initialised, free after the call */
-  int64_t x_cs, dy_cs;    /* elements from pixel to pixel (>= C); more than C only where C is a multiple of
-                             16 bytes / sizeof(dtype) */
+  int64_t x_cs, dy_cs;    /* elements from pixel to pixel (>= C, at most 2^20); more than C only where C is a
+                             multiple of 16 bytes / sizeof(dtype) */
   int n, c, groups, h, w; /* groups divides c */
   float eps;
   int act;                /* KAD_ACT_NONE, KAD_ACT_RELU or KAD_ACT_SILU */

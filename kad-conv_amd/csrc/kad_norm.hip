@@ -13,8 +13,9 @@
 // for itself, while its first rows are on their way) and writes the result, walking its rows backwards to meet
 // what the first left in its XCD's L2.  Its stores pass the caches by, which leaves x in them: a bare read and
 // a bare copy of 41 MB take 23.3 us in two launches, 19.1 us with such stores (one copy alone: 17.4, 12.5).
-// [8, 256, 100, 100] fp16 (41 MB): 26.5 us forward (statistics 9.8, result 15.5), backward 46 us (sums 23,
-// dx 22), where a bare read of x and dy, and a copy beside a read, take 13.6 and 20.
+// [8, 256, 100, 100] fp16 (41 MB): 25.0 us forward (statistics 9, result 16), backward 44 us (sums 21,
+// dx 22), where a bare read of x and dy takes 13.6 us, and their vector operations 11 and 12: what a block does
+// beside its rows (1 us of launch, 2 of places, weights and tiles joined, 1 of sums joined) is the rest.
 //
 // Layout.  Threads own 16-byte vectors of V channels.  Where V does not divide C, k = V / gcd(C, V) pixels
 // are taken as one row of k C channels, which V divides: a thread's vector meets the same V channels in
@@ -119,10 +120,16 @@ struct Geo {
   int full;       // whole rows of an image
   int tail;       // values of the pixels after them (fewer than k; 0 where k = 1)
   int W, q, D;
-  int rows, tiles;  // split kernels: rows of a tile, tiles of an image
-  int tpg, tpc;     // threads that join what a group, and a channel, has in a block: powers of two
-  int share;        // resident kernel: consecutive sets of groups that one 128-byte line may hold
+  float inv_s, inv_w, inv_d, inv_q;  // 1 / S ...
+  int sets;       // resident kernel: sets of q groups
+  int tpg, tpc;   // threads that join what a group, and a channel, has in a block: powers of two
+  // split kernels
+  int rows, tiles;  // rows of a tile (whole R), tiles of an image
+  int whole, last, rest;  // the last tile's rows: last R + rest
+  int per;          // threads that join a group's tiles
 };
+// x / d for x in [0, 2^16), from 1 / d: an integer division is some forty instructions.
+__device__ __forceinline__ int over(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -148,27 +155,28 @@ struct Sums {
 };
 
 // Joins over runs of D of the block's values.  Thread t < active holds val[0 .. VV), which are the places
-// t VV + v of a matrix of rows of W values; done(g, e) is called by one thread with what columns
+// t VV + v of a matrix of `lines` rows of W values; done(g, e) is called by one thread with what columns
 // [g D, (g + 1) D) come to, joined in an order that the sizes alone decide.  `per` threads (a power of two)
 // share a run.  red: VV values a thread.  Ends with a barrier.
 template <int VV, typename E, typename Done>
-__device__ __forceinline__ void join_runs(const E* val, int active, int W, int q, int D, int per, E* red, Done done) {
+__device__ __forceinline__ void join_runs(const E* val, int active, int lines, int W, int q, int D, int per, E* red, Done done) {
   const int t = threadIdx.x, T = blockDim.x;
   if (t < active)
 #pragma unroll
     for (int v = 0; v < VV; ++v) red[t * VV + v] = val[v];
   __syncthreads();
-  const int count = active * VV / W * D, l = t & (per - 1), wide = per < 64 ? per : 64;
-  const float inv = 1.0f / (float)D;
-  for (int base = 0; base < q; base += T / per) {
-    const int g = base + t / per;
+  const int count = lines * D, l = t & (per - 1), wide = per < 64 ? per : 64;
+  const float inv = __builtin_amdgcn_rcpf((float)D);
+  const int shift = __builtin_ctz(per), at_once = T >> shift;
+  for (int base = 0; base < q; base += at_once) {
+    const int g = base + (t >> shift);
     E acc{};
     if (g < q)
       for (int i = l; i < count; i += 4 * per) {
         E f[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int e = i + u * per, p = (int)(((float)e + 0.5f) * inv);  // e / D: e is under 2^16
+          const int e = i + u * per, p = over(e, inv);
           f[u] = E{};
           if (e < count) f[u] = red[p * (W - D) + e + g * D];
         }
@@ -196,25 +204,26 @@ struct Columns {
   int ntail;  // values of the last, short row that are this thread's
   __device__ __forceinline__ Columns(const Geo& o, int first) {
     const int t = threadIdx.x;
-    r = t / o.S;
+    r = over(t, o.inv_s);
     j = t - r * o.S;
     on = r < o.R;
+    if (!on) r = j = 0;  // reads as the first thread does, and is told apart where it counts
     c0 = first;
     ntail = o.tail - j * V;
     ntail = !on || r != 0 || ntail < 0 ? 0 : ntail > V ? V : ntail;
   }
-  // Channel, among the block's, of value v.
-  __device__ __forceinline__ int channel(const Geo& o, int v) const { return o.k == 1 ? j * V + v : (j * V + v) % o.W; }
+  // Channel, among the block's, of its first value.
+  __device__ __forceinline__ int channel(const Geo& o) const { return o.k == 1 ? j * V : j * V - over(j * V, o.inv_w) * o.W; }
   template <typename Q>
   __device__ __forceinline__ void param(const Geo& o, const void* p, float none, float f[V]) const {
 #pragma unroll
     for (int v = 0; v < V; ++v) f[v] = none;
-    if (!p || !on) return;
+    if (!p) return;
     Q q[V];
     if (o.k == 1) {
       __builtin_memcpy(q, (const Q*)p + c0 + j * V, sizeof(q));
     } else {
-      int c = channel(o, 0);
+      int c = channel(o);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         q[v] = ((const Q*)p)[c];
@@ -235,11 +244,11 @@ struct Columns {
   }
   // What p holds for the groups of its values.
   __device__ __forceinline__ void of_groups(const Geo& o, const float* p, float m[NG]) const {
-    const int c = channel(o, 0);
-    int g = c / o.D, d = c - g * o.D;
+    const int c = channel(o);
+    int g = over(c, o.inv_d), d = c - g * o.D;
 #pragma unroll
     for (int v = 0; v < NG; ++v) {
-      m[v] = on ? p[g] : 0.f;
+      m[v] = p[g];
       if (++d == o.D) {
         d = 0;
         g = g + 1 == o.q ? 0 : g + 1;
@@ -285,9 +294,7 @@ template <typename T, bool ONE>
 __global__ __launch_bounds__(1024) void group_norm_resident_kernel(kad_group_norm_args a, Geo o) {
   constexpr int V = VEC<T>, NG = ONE ? 1 : V, U = MOST_RESIDENT;
   extern __shared__ float lds[];
-  // Sets whose channels share lines run on one XCD (blocks go round the 8 of them), so its L2 fetches a line once.
-  const int sets = a.groups / o.q;
-  const int id = (blockIdx.x / (8 * o.share) * 8 + (blockIdx.x & 7)) * o.share + (blockIdx.x >> 3) % o.share;
+  const int sets = o.sets, id = (blockIdx.z * 8 + blockIdx.x) * gridDim.y + blockIdx.y;
   if (id >= a.n * sets) return;
   const int n = id / sets, set = id - n * sets;
   const Columns<T, ONE> col(o, set * o.W);
@@ -309,7 +316,9 @@ __global__ __launch_bounds__(1024) void group_norm_resident_kernel(kad_group_nor
   float w[V], b[V];
   col.params(o, a, w, b);
   // The thread's own values first, for each channel or for all; then the block's.
-  const int mine = col.on && col.r < o.full ? (o.full - col.r + o.R - 1) / o.R : 0;
+  int mine = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) mine += col.on && col.r + u * o.R < o.full ? 1 : 0;
   Moments mo[NG];
   float m[NG], s[NG];
 #pragma unroll
@@ -356,7 +365,7 @@ __global__ __launch_bounds__(1024) void group_norm_resident_kernel(kad_group_nor
     for (int u = 0; u < U; ++u) repack(raw[u]);
   }
   // ONE: every thread's values are of the block's one group
-  join_runs<NG>(mo, o.R * o.S, ONE ? o.R * o.S : o.W, o.q, ONE ? o.R * o.S : o.D, o.tpg, (Moments*)lds,
+  join_runs<NG>(mo, o.R * o.S, ONE ? 1 : o.R * o.k, ONE ? o.R * o.S : o.W, o.q, ONE ? o.R * o.S : o.D, o.tpg, (Moments*)lds,
                 [&](int g, const Moments& e) {
                   const float r = 1.0f / sqrtf(e.m2 / e.n + a.eps);
                   mean[g] = e.mean;
@@ -376,52 +385,75 @@ __global__ __launch_bounds__(1024) void group_norm_resident_kernel(kad_group_nor
 }
 
 // ---------------------------------------------------------------------------- split forward
-// Rows of tile t of an image, and how many pixels it holds.
+// A tile's rows, R at a time: `whole` times all of them, then `rest` threads' rows, in `count` rounds.
 struct Tile {
-  int first, last;
+  int64_t first;
+  int whole, rest, count;
   bool tail;
   __device__ __forceinline__ Tile(const Geo& o, int t) {
-    first = t * o.rows;
-    last = first + o.rows < o.full ? first + o.rows : o.full;
     tail = t == o.tiles - 1;
+    first = (int64_t)t * o.rows;
+    whole = tail ? o.last : o.whole;
+    rest = tail ? o.rest : 0;
+    count = whole + (rest ? 1 : 0);
   }
+  // The i-th round of a walk from the end: the whole ones backwards, then the partial one.
+  __device__ __forceinline__ int back(int i) const { return i < whole ? whole - 1 - i : i; }
 };
 __device__ __forceinline__ int tile_pixels(const Geo& o, int64_t P, int t) {
   const int64_t first = (int64_t)t * o.rows * o.k, next = first + (int64_t)o.rows * o.k;
   return (int)((t == o.tiles - 1 ? P : next) - first);
 }
 
-// A thread's rows of a tile, B at a time, the next B on their way while these are worked on.  load(i) reads
-// its i-th row; use(rows, valid) takes the first `valid` of B rows.
+// A map's rows as a thread meets them in a tile: an address that all threads share moves from round to round, the
+// thread's own offset stays (32 bits of bytes: 512 rows of at most 2^20 elements apart).
+template <typename T>
+struct Lane {
+  T* base;
+  int64_t step;
+  uint32_t off, edge;  // edge: in the last, partial round, where a thread may have no row
+  template <typename C>
+  __device__ __forceinline__ Lane(const Geo& o, const C& col, const Tile& rows, T* image, int64_t stride)
+      : base(image + rows.first * stride), step(o.R * stride) {
+    off = ((uint32_t)col.r * (uint32_t)stride + col.j * C::V) * (uint32_t)sizeof(T);
+    edge = col.r < rows.rest ? off : 0;
+  }
+  __device__ __forceinline__ T* at(const Tile& rows, int round) const {
+    return (T*)((char*)(base + round * step) + (round < rows.whole ? off : edge));
+  }
+};
+
+// A tile's rounds, B at a time, the next B on their way while these are worked on.  load(i) reads the i-th;
+// all(i, rows) takes B whole ones from the i-th on, some(i, rows, n) the n that are left, the partial one among them.
+// Loads and stores stand outside of branches (past the end the last round is read again): with a branch around
+// one, the compiler no longer knows how many are in flight and waits for all ([16, 128, 200, 200] bf16 forward
+// and backward: 136 and 176 us).
 template <typename Raw, int B>
 struct Walk {
   int count;
-  Raw a[B], b[B];
+  Raw next[B];
   template <typename Load>
-  __device__ __forceinline__ void fetch(Raw r[B], int i, Load load) {
-    if (i < count)
+  __device__ __forceinline__ void fetch(int i, Load load) {
 #pragma unroll
-      for (int k = 0; k < B; ++k) r[k] = load(i + k < count ? i + k : count - 1);
+    for (int k = 0; k < B; ++k) next[k] = load(i + k < count ? i + k : count - 1);
   }
   template <typename Load>
-  __device__ __forceinline__ Walk(int rows, Load load) : count(rows) {
-    fetch(a, 0, load);
+  __device__ __forceinline__ Walk(int rounds, Load load) : count(rounds) {
+    if (count) fetch(0, load);
   }
-  template <typename Load, typename Use>
-  __device__ __forceinline__ void run(Load load, Use use) {
-    for (int i = 0; i < count; i += 2 * B) {
-      fetch(b, i + B, load);
-      use(i, a, count - i);
-      fetch(a, i + 2 * B, load);
-      if (i + B < count) use(i + B, b, count - i - B);
+  template <typename Load, typename All, typename Some>
+  __device__ __forceinline__ void run(int whole, Load load, All all, Some some) {
+    int i = 0;
+    for (; i + B <= whole; i += B) {
+      Raw now[B];
+#pragma unroll
+      for (int k = 0; k < B; ++k) now[k] = next[k];
+      fetch(i + B, load);
+      all(i, now);
     }
+    if (i < count) some(i, next, count - i);
   }
 };
-template <typename T, bool ONE>
-__device__ __forceinline__ int row_count(const Geo& o, const Columns<T, ONE>& col, const Tile& rows) {
-  const int left = rows.last - rows.first - col.r;
-  return col.on && left > 0 ? (left + o.R - 1) / o.R : 0;
-}
 struct Pair {
   intx4 x, d;
 };
@@ -481,16 +513,18 @@ __global__ __launch_bounds__(MOST) void group_norm_stats_kernel(kad_group_norm_a
   const Tile rows(o, tile);
   const int64_t P = (int64_t)a.h * a.w;
   const int64_t xs = o.k == 1 ? a.x_cs : (int64_t)o.k * a.c;
-  const T* x = (const T*)a.x + n * P * a.x_cs + col.j * V;
+  const T* x = (const T*)a.x + n * P * a.x_cs;
+  const Lane<const T> lane(o, col, rows, x, xs);
   Running<NG> acc;
-  const auto load = [&](int i) { return load_vec(x + (int64_t)(rows.first + col.r + i * o.R) * xs); };
-  Walk<intx4, B> walk(row_count(o, col, rows), load);
-  walk.run(load, [&](int, const intx4* raw, int valid) {
-    if (valid >= B) return add_rows<T, ONE, B>(acc, raw);
+  const auto load = [&](int i) { return load_vec(lane.at(rows, i)); };
+  Walk<intx4, B> walk(rows.count, load);
+  walk.run(
+      rows.whole, load, [&](int, const intx4* raw) { add_rows<T, ONE, B>(acc, raw); },
+      [&](int at, const intx4* raw, int left) {
 #pragma unroll
-    for (int i = 0; i < B; ++i)
-      if (i < valid) add_rows<T, ONE, 1>(acc, raw + i);
-  });
+        for (int i = 0; i < B; ++i)
+          if (i < left && (at + i < rows.whole || col.r < rows.rest)) add_rows<T, ONE, 1>(acc, raw + i);
+      });
   // The short row's values are of a channel each, so counts differ from channel to channel.
   Moments mo[NG];
 #pragma unroll
@@ -498,19 +532,20 @@ __global__ __launch_bounds__(MOST) void group_norm_stats_kernel(kad_group_norm_a
   const int nt = rows.tail ? col.ntail : 0;
   if (nt) {
     float xt[V];
-    load_some(x + o.full * xs, nt, xt);
+    load_some(x + o.full * xs + col.j * V, nt, xt);
 #pragma unroll
     for (int v = 0; v < V; ++v)
       if (v < nt) mo[ONE ? 0 : v] = mo[ONE ? 0 : v].join(Moments{1.f, xt[v], 0.f});
   }
   const bool vectors = ONE && o.q > 1;  // a group is D / V of the threads' values; the only group is all of them
   const int active = o.R * o.S, W = vectors ? o.S : ONE ? active : o.W, D = vectors ? o.D / V : ONE ? active : o.D;
+  const int lines = vectors ? o.R : ONE ? 1 : o.R * o.k;
   Sums* part = (Sums*)a.work + ((int64_t)n * o.tiles + tile) * o.q;
-  join_runs<NG>(mo, active, W, o.q, D, o.tpg, (Moments*)lds, [&](int g, const Moments& e) { part[g] = Sums{e.mean, e.m2}; });
+  join_runs<NG>(mo, active, lines, W, o.q, D, o.tpg, (Moments*)lds, [&](int g, const Moments& e) { part[g] = Sums{e.mean, e.m2}; });
 }
 
 // Joins what the tiles of an image left for each group: thread t takes group t mod q of every per-th tile,
-// consecutive threads consecutive groups, and halves of the block join in LDS, in an order that the sizes alone
+// consecutive threads consecutive groups, and quarters of the block join in LDS, in an order that the sizes alone
 // decide.  The first two tiles' parts are asked for by the constructor, before the rows that a caller fetches
 // meanwhile: loads return in order.
 template <typename E>
@@ -519,9 +554,9 @@ struct TileJoin {
   int per, l, g;
   Sums first[2];
   __device__ __forceinline__ TileJoin(const Geo& o, const Sums* p) : part(p) {
-    const int t = threadIdx.x, most = blockDim.x / o.q;
-    per = most < 1 ? 1 : most < o.tiles ? most : o.tiles;
-    l = t / o.q;
+    const int t = threadIdx.x;
+    per = o.per;
+    l = over(t, o.inv_q);
     g = t - l * o.q;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -547,14 +582,21 @@ struct TileJoin {
       for (int i = l + 2 * per; i < o.tiles; i += per) acc = acc.join(make(i, part[i * o.q + g]));
     }
     red[t] = acc;
-    for (int n = per; n > 1;) {
-      const int half = (n + 1) / 2;
+    for (int n = per; n > 1;) {  // quarters join
+      const int part = (n + 3) / 4;
       __syncthreads();
-      if (l + half < n) {
-        acc = acc.join(red[t + half * o.q]);
-        red[t] = acc;
+      if (l < part) {
+        E more[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const int from = l + (i + 1) * part;
+          more[i] = E{};
+          if (from < n) more[i] = red[t + (i + 1) * part * o.q];
+        }
+        acc = acc.join(more[0]).join(more[1].join(more[2]));
+        if (part > 1) red[t] = acc;
       }
-      n = half;
+      n = part;
     }
     if (l == 0) done(g, acc);
     __syncthreads();
@@ -562,25 +604,31 @@ struct TileJoin {
 };
 
 template <typename T, bool ONE, int ACT, int B, typename Load>
-__device__ __forceinline__ void apply_rows(const Geo& o, const Columns<T, ONE>& col, const Tile& rows, const T* x, int64_t xs,
-                                           T* y, int64_t ys, const float* mean, const float* w, const float* b,
-                                           Walk<intx4, B>& walk, Load load) {
+__device__ __forceinline__ void apply_rows(const Columns<T, ONE>& col, const Tile& rows, const Lane<T>& out, const T* xt, T* yt,
+                                           const float* mean, const float* w, const float* b, Walk<intx4, B>& walk, Load load) {
   constexpr int V = VEC<T>;
-  walk.run(load, [&](int at, const intx4* raw, int valid) {
+  const auto write = [&](int round, intx4 raw) {
+    float f[V];
+    unpack<T>(raw, f);
+    norm_vec<T, ONE, ACT>(f, mean, w, b);
+    stream_vec(out.at(rows, round), f);
+  };
+  walk.run(
+      rows.whole, load,
+      [&](int at, const intx4* raw) {
 #pragma unroll
-    for (int i = 0; i < B; ++i)
-      if (i < valid) {
-        float f[V];
-        unpack<T>(raw[i], f);
-        norm_vec<T, ONE, ACT>(f, mean, w, b);
-        stream_vec(y + (int64_t)(rows.last - 1 - col.r - (at + i) * o.R) * ys, f);
-      }
-  });
+        for (int i = 0; i < B; ++i) write(rows.back(at + i), raw[i]);
+      },
+      [&](int at, const intx4* raw, int left) {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+          if (i < left && (at + i < rows.whole || col.r < rows.rest)) write(rows.back(at + i), raw[i]);
+      });
   if (rows.tail && col.ntail) {
     float f[V];
-    load_some(x + o.full * xs, col.ntail, f);
+    load_some(xt, col.ntail, f);
     norm_vec<T, ONE, ACT>(f, mean, w, b);
-    store_some(y + o.full * ys, col.ntail, f);
+    store_some(yt, col.ntail, f);
   }
 }
 
@@ -593,14 +641,16 @@ __global__ __launch_bounds__(MOST) void group_norm_apply_kernel(kad_group_norm_a
   const Tile rows(o, tile);
   const int64_t P = (int64_t)a.h * a.w;
   const int64_t xs = o.k == 1 ? a.x_cs : (int64_t)o.k * a.c, ys = (int64_t)o.k * a.c;
-  const T* x = (const T*)a.x + n * P * a.x_cs + col.j * V;
-  T* y = (T*)a.out + n * P * a.c + col.j * V;
+  const T* x = (const T*)a.x + n * P * a.x_cs;
+  T* y = (T*)a.out + n * P * a.c;
+  const Lane<const T> lane(o, col, rows, x, xs);
+  const Lane<T> out(o, col, rows, y, ys);
   float w[V], b[V], m[NG], rs[NG];
   TileJoin<Moments> join(o, (const Sums*)a.work + (int64_t)n * o.tiles * o.q);
   col.params(o, a, w, b);
   // Backwards: what the statistics read last is still near.
-  const auto load = [&](int i) { return load_vec(x + (int64_t)(rows.last - 1 - col.r - i * o.R) * xs); };
-  Walk<intx4, B> walk(row_count(o, col, rows), load);
+  const auto load = [&](int i) { return load_vec(lane.at(rows, rows.back(i))); };
+  Walk<intx4, B> walk(rows.count, load);
   float *mean = lds + 3 * blockDim.x, *rstd = mean + o.q;
   join.run(
       o, (Moments*)lds,
@@ -619,9 +669,11 @@ __global__ __launch_bounds__(MOST) void group_norm_apply_kernel(kad_group_norm_a
   col.of_groups(o, rstd, rs);
 #pragma unroll
   for (int v = 0; v < V; ++v) w[v] *= rs[ONE ? 0 : v];
-  if (a.act == KAD_ACT_SILU) apply_rows<T, ONE, KAD_ACT_SILU, B>(o, col, rows, x, xs, y, ys, m, w, b, walk, load);
-  else if (a.act == KAD_ACT_RELU) apply_rows<T, ONE, KAD_ACT_RELU, B>(o, col, rows, x, xs, y, ys, m, w, b, walk, load);
-  else apply_rows<T, ONE, KAD_ACT_NONE, B>(o, col, rows, x, xs, y, ys, m, w, b, walk, load);
+  const T* xt = x + o.full * xs + col.j * V;
+  T* yt = y + o.full * ys + col.j * V;
+  if (a.act == KAD_ACT_SILU) apply_rows<T, ONE, KAD_ACT_SILU, B>(col, rows, out, xt, yt, m, w, b, walk, load);
+  else if (a.act == KAD_ACT_RELU) apply_rows<T, ONE, KAD_ACT_RELU, B>(col, rows, out, xt, yt, m, w, b, walk, load);
+  else apply_rows<T, ONE, KAD_ACT_NONE, B>(col, rows, out, xt, yt, m, w, b, walk, load);
 }
 
 // ---------------------------------------------------------------------------- backward
@@ -641,24 +693,30 @@ __device__ __forceinline__ void sum_vec(const float x[VEC<T>], const float dy[VE
 }
 
 template <typename T, bool ONE, int ACT, int B, typename Load>
-__device__ __forceinline__ void sum_rows(const Geo& o, const Columns<T, ONE>& col, const Tile& rows, const T* x, int64_t xs,
-                                         const T* dy, int64_t ds, const float* mean, const float* w, const float* b, float* db,
-                                         float* dw, Walk<Pair, B>& walk, Load load) {
+__device__ __forceinline__ void sum_rows(const Columns<T, ONE>& col, const Tile& rows, const T* xt, const T* dt, const float* mean,
+                                         const float* w, const float* b, float* db, float* dw, Walk<Pair, B>& walk, Load load) {
   constexpr int V = VEC<T>;
-  walk.run(load, [&](int, const Pair* raw, int valid) {
+  const auto add = [&](const Pair& raw) {
+    float f[V], g[V];
+    unpack<T>(raw.x, f);
+    unpack<T>(raw.d, g);
+    sum_vec<T, ONE, ACT>(f, g, mean, w, b, db, dw);
+  };
+  walk.run(
+      rows.whole, load,
+      [&](int, const Pair* raw) {
 #pragma unroll
-    for (int i = 0; i < B; ++i)
-      if (i < valid) {
-        float f[V], g[V];
-        unpack<T>(raw[i].x, f);
-        unpack<T>(raw[i].d, g);
-        sum_vec<T, ONE, ACT>(f, g, mean, w, b, db, dw);
-      }
-  });
+        for (int i = 0; i < B; ++i) add(raw[i]);
+      },
+      [&](int at, const Pair* raw, int left) {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+          if (i < left && (at + i < rows.whole || col.r < rows.rest)) add(raw[i]);
+      });
   if (rows.tail && col.ntail) {
     float f[V], g[V], d1[V], d2[V];
-    load_some(x + o.full * xs, col.ntail, f);
-    load_some(dy + o.full * ds, col.ntail, g);
+    load_some(xt, col.ntail, f);
+    load_some(dt, col.ntail, g);
 #pragma unroll
     for (int v = 0; v < V; ++v) d1[v] = d2[v] = 0.f;
     sum_vec<T, ONE, ACT>(f, g, mean, w, b, d1, d2);
@@ -679,22 +737,20 @@ __global__ __launch_bounds__(MOST) void group_norm_bwd_sums_kernel(kad_group_nor
   const Tile rows(o, tile);
   const int64_t P = (int64_t)a.h * a.w;
   const int64_t xs = o.k == 1 ? a.x_cs : (int64_t)o.k * a.c, ds = o.k == 1 ? a.dy_cs : (int64_t)o.k * a.c;
-  const T* x = (const T*)a.x + n * P * a.x_cs + col.j * V;
-  const T* dy = (const T*)a.dy + n * P * a.dy_cs + col.j * V;
+  const T* x = (const T*)a.x + n * P * a.x_cs;
+  const T* dy = (const T*)a.dy + n * P * a.dy_cs;
+  const Lane<const T> lx(o, col, rows, x, xs), ld(o, col, rows, dy, ds);
   float w[V], b[V], m[NG], rs[NG];
   col.params(o, a, w, b);
   col.of_groups(o, a.mean + n * o.q, m);
   col.of_groups(o, a.rstd + n * o.q, rs);
-  const auto load = [&](int i) {
-    const int64_t row = rows.first + col.r + i * o.R;
-    return Pair{load_vec(x + row * xs), load_vec(dy + row * ds)};
-  };
-  Walk<Pair, B> walk(row_count(o, col, rows), load);
+  const auto load = [&](int i) { return Pair{load_vec(lx.at(rows, i)), load_vec(ld.at(rows, i))}; };
+  Walk<Pair, B> walk(rows.count, load);
   // The channels' sums, and their weights, for the groups' sums.
   Sums* red = (Sums*)lds;
   float *cb = lds + 2 * blockDim.x * V, *cw = cb + o.W, *weight = cw + o.W;
   if (col.on && col.r == 0) {
-    int c = col.channel(o, 0);
+    int c = col.channel(o);
 #pragma unroll
     for (int v = 0; v < V; ++v) {  // where a row is several pixels, its threads write the same weights
       weight[c] = w[v];
@@ -707,16 +763,17 @@ __global__ __launch_bounds__(MOST) void group_norm_bwd_sums_kernel(kad_group_nor
     db[v] = dw[v] = 0.f;
     w[v] *= rs[ONE ? 0 : v];
   }
-  if (a.act == KAD_ACT_SILU) sum_rows<T, ONE, KAD_ACT_SILU, B>(o, col, rows, x, xs, dy, ds, m, w, b, db, dw, walk, load);
-  else if (a.act == KAD_ACT_RELU) sum_rows<T, ONE, KAD_ACT_RELU, B>(o, col, rows, x, xs, dy, ds, m, w, b, db, dw, walk, load);
-  else sum_rows<T, ONE, KAD_ACT_NONE, B>(o, col, rows, x, xs, dy, ds, m, w, b, db, dw, walk, load);
+  const T *xt = x + o.full * xs + col.j * V, *dt = dy + o.full * ds + col.j * V;
+  if (a.act == KAD_ACT_SILU) sum_rows<T, ONE, KAD_ACT_SILU, B>(col, rows, xt, dt, m, w, b, db, dw, walk, load);
+  else if (a.act == KAD_ACT_RELU) sum_rows<T, ONE, KAD_ACT_RELU, B>(col, rows, xt, dt, m, w, b, db, dw, walk, load);
+  else sum_rows<T, ONE, KAD_ACT_NONE, B>(col, rows, xt, dt, m, w, b, db, dw, walk, load);
   Sums sums[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) sums[v] = Sums{db[v], dw[v] * rs[ONE ? 0 : v]};
   const int64_t part = (int64_t)n * o.tiles + tile;
   Sums* chans = (Sums*)a.work + (int64_t)a.n * o.tiles * o.q + part * o.W;
   const bool keep = a.dweight || a.dbias;
-  join_runs<V>(sums, o.R * o.S, o.W, o.W, 1, o.tpc, red, [&](int c, const Sums& e) {
+  join_runs<V>(sums, o.R * o.S, o.R * o.k, o.W, o.W, 1, o.tpc, red, [&](int c, const Sums& e) {
     cb[c] = e.a;
     cw[c] = e.b;
     if (keep) chans[c] = e;
@@ -745,27 +802,34 @@ __device__ __forceinline__ void dx_vec(float x[VEC<T>], const float dy[VEC<T>], 
 }
 
 template <typename T, bool ONE, int ACT, int B, typename Load>
-__device__ __forceinline__ void dx_rows(const Geo& o, const Columns<T, ONE>& col, const Tile& rows, const T* x, int64_t xs,
-                                        const T* dy, int64_t ds, T* dx, int64_t os, const float* mean, const float* w,
-                                        const float* b, const float* c1, const float* c2, Walk<Pair, B>& walk, Load load) {
+__device__ __forceinline__ void dx_rows(const Columns<T, ONE>& col, const Tile& rows, const Lane<T>& out, const T* xt, const T* dt,
+                                        T* ot, const float* mean, const float* w, const float* b, const float* c1, const float* c2,
+                                        Walk<Pair, B>& walk, Load load) {
   constexpr int V = VEC<T>;
-  walk.run(load, [&](int at, const Pair* raw, int valid) {
+  const auto write = [&](int round, const Pair& raw) {
+    float f[V], g[V];
+    unpack<T>(raw.x, f);
+    unpack<T>(raw.d, g);
+    dx_vec<T, ONE, ACT>(f, g, mean, w, b, c1, c2);
+    stream_vec(out.at(rows, round), f);
+  };
+  walk.run(
+      rows.whole, load,
+      [&](int at, const Pair* raw) {
 #pragma unroll
-    for (int i = 0; i < B; ++i)
-      if (i < valid) {
-        float f[V], g[V];
-        unpack<T>(raw[i].x, f);
-        unpack<T>(raw[i].d, g);
-        dx_vec<T, ONE, ACT>(f, g, mean, w, b, c1, c2);
-        stream_vec(dx + (int64_t)(rows.last - 1 - col.r - (at + i) * o.R) * os, f);
-      }
-  });
+        for (int i = 0; i < B; ++i) write(rows.back(at + i), raw[i]);
+      },
+      [&](int at, const Pair* raw, int left) {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+          if (i < left && (at + i < rows.whole || col.r < rows.rest)) write(rows.back(at + i), raw[i]);
+      });
   if (rows.tail && col.ntail) {
     float f[V], g[V];
-    load_some(x + o.full * xs, col.ntail, f);
-    load_some(dy + o.full * ds, col.ntail, g);
+    load_some(xt, col.ntail, f);
+    load_some(dt, col.ntail, g);
     dx_vec<T, ONE, ACT>(f, g, mean, w, b, c1, c2);
-    store_some(dx + o.full * os, col.ntail, f);
+    store_some(ot, col.ntail, f);
   }
 }
 
@@ -803,28 +867,29 @@ __device__ __forceinline__ void param_sums(const kad_group_norm_args& a, const G
 
 template <typename T, bool ONE, int MOST>
 __global__ __launch_bounds__(MOST) void group_norm_dx_kernel(kad_group_norm_args a, Geo o) {
-  constexpr int V = VEC<T>, NG = ONE ? 1 : V, B = MOST > 512 ? 2 : 4;
+  constexpr int V = VEC<T>, NG = ONE ? 1 : V, B = 2;
   extern __shared__ float lds[];
-  const int maps = a.out ? a.n * o.tiles : 0;
-  if ((int)blockIdx.x >= maps) return param_sums(a, o, blockIdx.x - maps, lds);
-  const int n = blockIdx.x / o.tiles, tile = blockIdx.x - n * o.tiles;
+  const int maps = a.out ? a.n : 0;  // the rows of blocks after the images' are the parameters'
+  if ((int)blockIdx.y >= maps) return param_sums(a, o, (blockIdx.y - maps) * gridDim.x + blockIdx.x, lds);
+  const int n = blockIdx.y, tile = blockIdx.x;
   const Columns<T, ONE> col(o, 0);
   const Tile rows(o, tile);
   const int64_t P = (int64_t)a.h * a.w;
   const int64_t os = (int64_t)o.k * a.c, xs = o.k == 1 ? a.x_cs : os, ds = o.k == 1 ? a.dy_cs : os;
-  const T* x = (const T*)a.x + n * P * a.x_cs + col.j * V;
-  const T* dy = (const T*)a.dy + n * P * a.dy_cs + col.j * V;
-  T* dx = (T*)a.out + n * P * a.c + col.j * V;
+  const T* x = (const T*)a.x + n * P * a.x_cs;
+  const T* dy = (const T*)a.dy + n * P * a.dy_cs;
+  T* dx = (T*)a.out + n * P * a.c;
+  const Lane<const T> lx(o, col, rows, x, xs), ld(o, col, rows, dy, ds);
+  const Lane<T> out(o, col, rows, dx, os);
   float w[V], b[V], m[NG], rs[NG], s1[NG], s2[NG];
   TileJoin<Sums> join(o, (const Sums*)a.work + (int64_t)n * o.tiles * o.q);
   col.params(o, a, w, b);
   col.of_groups(o, a.mean + n * o.q, m);
   col.of_groups(o, a.rstd + n * o.q, rs);
   const auto load = [&](int i) {
-    const int64_t row = rows.last - 1 - col.r - i * o.R;
-    return Pair{load_vec(x + row * xs), load_vec(dy + row * ds)};
+    return Pair{load_vec(lx.at(rows, rows.back(i))), load_vec(ld.at(rows, rows.back(i)))};
   };
-  Walk<Pair, B> walk(row_count(o, col, rows), load);
+  Walk<Pair, B> walk(rows.count, load);
   float *l1 = lds + 2 * blockDim.x, *l2 = l1 + o.q;
   join.run(
       o, (Sums*)lds, [](int, const Sums& p) { return p; },
@@ -843,12 +908,14 @@ __global__ __launch_bounds__(MOST) void group_norm_dx_kernel(kad_group_norm_args
     s1[v] *= rs[v];
     s2[v] *= rs[v] * rs[v];
   }
+  const T *xt = x + o.full * xs + col.j * V, *dt = dy + o.full * ds + col.j * V;
+  T* ot = dx + o.full * os + col.j * V;
   if (a.act == KAD_ACT_SILU)
-    dx_rows<T, ONE, KAD_ACT_SILU, B>(o, col, rows, x, xs, dy, ds, dx, os, m, w, b, s1, s2, walk, load);
+    dx_rows<T, ONE, KAD_ACT_SILU, B>(col, rows, out, xt, dt, ot, m, w, b, s1, s2, walk, load);
   else if (a.act == KAD_ACT_RELU)
-    dx_rows<T, ONE, KAD_ACT_RELU, B>(o, col, rows, x, xs, dy, ds, dx, os, m, w, b, s1, s2, walk, load);
+    dx_rows<T, ONE, KAD_ACT_RELU, B>(col, rows, out, xt, dt, ot, m, w, b, s1, s2, walk, load);
   else
-    dx_rows<T, ONE, KAD_ACT_NONE, B>(o, col, rows, x, xs, dy, ds, dx, os, m, w, b, s1, s2, walk, load);
+    dx_rows<T, ONE, KAD_ACT_NONE, B>(col, rows, out, xt, dt, ot, m, w, b, s1, s2, walk, load);
 }
 
 // ---------------------------------------------------------------------------- any width
@@ -974,6 +1041,10 @@ bool lay_out(const kad_group_norm_args& a, int q, Geo& o) {
   if (P / o.k > INT32_MAX - 8 * MOST_THREADS) return false;  // row numbers and the steps past them are 32-bit
   if (o.W > MOST_THREADS * V || o.k * o.W / V > MOST_THREADS || q > MOST_GROUPS) return false;
   o.S = o.k * o.W / V;
+  o.inv_s = 1.0f / (float)o.S;
+  o.inv_w = 1.0f / (float)o.W;
+  o.inv_d = 1.0f / (float)o.D;
+  o.inv_q = 1.0f / (float)o.q;
   o.full = (int)(P / o.k);
   o.tail = (int)(P % o.k) * o.W;
   return true;
@@ -992,8 +1063,8 @@ bool resident(const kad_group_norm_args& a, Geo& o, int& threads) {
   if (a.groups % q) q = a.groups;
   if (!lay_out(a, q, o)) return false;
   // One launch, but a block's columns of D or few channels are pieces of lines that other blocks fetch too, and
-  // one CU reads them: up to 32 KB a block this beats the split kernels ([1, 64, 20, 20] fp16: 5.5 us against 8.2,
-  // [2, 48, 13, 17] fp32: 5.3 against 7.5, [16, 512, 25, 25] in 16 groups 13 against 15), at 64 KB most of it is
+  // one CU reads them: up to 32 KB a block this beats the split kernels ([1, 64, 20, 20] fp16: 4.8 us against 8.1,
+  // [2, 48, 13, 17] fp32: 4.5 against 7.4, [16, 512, 25, 25] in 16 groups 13 against 15), at 64 KB most of it is
   // lost (8 blocks: 11.1 against 8.9; 256 blocks: 13.8 against 17.0), at 256 KB they take half the time.
   if ((int64_t)o.full * o.S * 16 > 32 * 1024) return false;
   int rows = ceil_div(o.full, MOST_RESIDENT);
@@ -1001,8 +1072,7 @@ bool resident(const kad_group_norm_args& a, Geo& o, int& threads) {
   if (rows > o.full) rows = o.full;
   if (rows * o.S > MOST_THREADS) return false;
   count_threads(o, rows, threads);
-  const int line = 128 / (o.W * dtype_size(a.dtype));
-  o.share = line > 1 && (a.groups / q) % line == 0 ? line : 1;
+  o.sets = a.groups / q;
   return true;
 }
 
@@ -1011,8 +1081,8 @@ bool split(const kad_group_norm_args& a, Geo& o, int& threads) {
   if (!lay_out(a, a.groups, o)) return false;
   // One block of 512 threads a CU: what a block does beside its rows (places, weights, the join of what it and
   // others left) is microseconds, so that more blocks lose more than their loads in flight gain ([8, 256, 100, 100]
-  // fp16, forward and backward: 27 and 46 us; 32 and 54 with two blocks a CU, 44 and 70 with four; 256 threads: 27
-  // and 47).  Threads of under 8 rows are halved ([3, 86, 67, 41] fp32: 9.6 and 12.0 us against 10.4 and 12.7).
+  // fp16, forward and backward: 27 and 46 us where this was tried; 32 and 54 with two blocks a CU, 44 and 70 with
+  // four; 27 and 47 with 256 threads).  Threads of under 8 rows are halved ([3, 86, 67, 41] fp32: 9.6 and 12.0 us against 10.4 and 12.7).
   const int most = (int64_t)a.n * o.full * o.S < 8 * 256 * 512 ? 256 : 512;
   count_threads(o, most / o.S < o.full ? most / o.S : o.full, threads);
   int tiles = ceil_div(256, a.n);
@@ -1025,6 +1095,10 @@ bool split(const kad_group_norm_args& a, Geo& o, int& threads) {
   o.rows = round_up(ceil_div(o.full, tiles), o.R);
   if (o.rows < 1) o.rows = o.R;
   o.tiles = o.full ? ceil_div(o.full, o.rows) : 1;
+  o.whole = o.rows / o.R;
+  o.last = (o.full - (o.tiles - 1) * o.rows) / o.R;
+  o.rest = (o.full - (o.tiles - 1) * o.rows) % o.R;
+  o.per = threads / o.q < 1 ? 1 : threads / o.q < o.tiles ? threads / o.q : o.tiles;
   return true;
 }
 
@@ -1045,6 +1119,7 @@ int check_call(const kad_group_norm_args* a, bool backward, const char* what) {
   if (int rc = check_args(a, what)) return rc;
   KAD_CHECK_ARG(a->x && a->mean && a->rstd && (backward ? a->dy : a->out), "%s: null pointer", what);
   const int v = 16 / dtype_size(a->dtype);
+  KAD_CHECK_ARG(a->x_cs <= (1 << 20) && (!backward || a->dy_cs <= (1 << 20)), "%s: pixels lie at most 2^20 elements apart", what);
   KAD_CHECK_ARG(a->x_cs == a->c || (a->x_cs > a->c && a->c % v == 0), "%s: x_cs does not fit c", what);
   KAD_CHECK_ARG(!backward || a->dy_cs == a->c || (a->dy_cs > a->c && a->c % v == 0), "%s: dy_cs does not fit c", what);
   KAD_CHECK_ARG(a->work || kad_group_norm_work_elems(a, backward) == 0, "%s: work is missing", what);
@@ -1053,8 +1128,10 @@ int check_call(const kad_group_norm_args* a, bool backward, const char* what) {
 
 template <typename T, bool ONE>
 void launch_resident(const kad_group_norm_args& a, const Geo& o, int threads, hipStream_t st) {
-  const int64_t blocks = (int64_t)a.n * (a.groups / o.q), unit = 8 * o.share;
-  const dim3 grid((unsigned)((blocks + unit - 1) / unit * unit));
+  // Blocks go round the 8 XCDs by their number: those whose sets share 128-byte lines of a pixel are kept on one.
+  const int line = 128 / (o.W * (int)sizeof(T)), share = line > 1 && o.sets % line == 0 ? line : 1;
+  const int64_t blocks = (int64_t)a.n * o.sets;
+  const dim3 grid(8, share, (unsigned)((blocks + 8 * share - 1) / (8 * share)));
   const size_t lds = threads * (ONE ? 1 : VEC<T>) * sizeof(Moments) + 2 * o.q * sizeof(float);
   allow_lds(group_norm_resident_kernel<T, ONE>, lds);
   group_norm_resident_kernel<T, ONE><<<grid, threads, lds, st>>>(a, o);
@@ -1090,9 +1167,16 @@ void launch_backward(const kad_group_norm_args& a, const Geo& o, int threads, hi
   const size_t sums = threads * VEC<T> * sizeof(Sums) + 3 * o.W * sizeof(float);
   allow_lds(group_norm_bwd_sums_kernel<T, ONE, MOST>, sums);
   group_norm_bwd_sums_kernel<T, ONE, MOST><<<dim3(o.tiles, a.n), threads, sums, st>>>(a, o);
-  const int blocks = (a.out ? a.n * o.tiles : 0) + (a.dweight || a.dbias ? ceil_div(o.W, PARAM_CHANNELS) : 0);
+  const int params = a.dweight || a.dbias ? ceil_div(ceil_div(o.W, PARAM_CHANNELS), o.tiles) : 0;
   const int waves = threads / 64 * PARAM_CHANNELS * 2, join = 2 * threads + 2 * o.q;
-  group_norm_dx_kernel<T, ONE, MOST><<<dim3(blocks), threads, (join > waves ? join : waves) * sizeof(float), st>>>(a, o);
+  if (a.out && a.n + params > 65535) {  // more rows of blocks than a grid has
+    kad_group_norm_args only = a;
+    only.out = nullptr;
+    group_norm_dx_kernel<T, ONE, MOST><<<dim3(o.tiles, params), threads, (join > waves ? join : waves) * sizeof(float), st>>>(only, o);
+    group_norm_dx_kernel<T, ONE, MOST><<<dim3(o.tiles, a.n), threads, (join > waves ? join : waves) * sizeof(float), st>>>(a, o);
+    return;
+  }
+  group_norm_dx_kernel<T, ONE, MOST><<<dim3(o.tiles, (a.out ? a.n : 0) + params), threads, (join > waves ? join : waves) * sizeof(float), st>>>(a, o);
 }
 
 template <typename T>

@@ -63,7 +63,7 @@ Tensor channels_last_pixels(const Tensor& x, int64_t& cs) {
   const int64_t n = x.size(0), c = x.size(1), h = x.size(2), w = x.size(3);
   cs = w > 1 ? x.stride(3) : h > 1 ? x.stride(2) : n > 1 ? x.stride(0) : c;
   if ((c == 1 || x.stride(1) == 1) && cs >= c && (h == 1 || x.stride(2) == w * cs) && (n == 1 || x.stride(0) == h * w * cs) &&
-      (cs == c || c % (16 / (int64_t)x.element_size()) == 0))
+      (cs == c || (c % (16 / (int64_t)x.element_size()) == 0 && cs <= 1 << 20)))
     return x;
   cs = c;
   Tensor out = map_like(x);
