@@ -66,7 +66,7 @@ def _link_native(obj):
     libs = os.path.join(os.path.dirname(torch.__file__), 'lib')
     tmp = NATIVE + '.tmp'
     cmd = ['g++', '-shared', '-o', tmp, obj, '-L', os.path.dirname(LIB), '-l:' + os.path.basename(LIB), '-L', libs,
-           '-lc10', '-lc10_hip', '-ltorch_cpu', '-ltorch', '-ltorch_python', '-Wl,-rpath,$ORIGIN']
+           '-lc10', '-lc10_hip', '-ltorch_cpu', '-ltorch_hip', '-ltorch', '-ltorch_python', '-Wl,-rpath,$ORIGIN']
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f'link failed:\n{" ".join(cmd)}\n{r.stdout}\n{r.stderr}')

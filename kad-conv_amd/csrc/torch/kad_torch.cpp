@@ -5,9 +5,9 @@
 // threads moves the interpreter's state from core to core); as an autograd node of C++ it does without the
 // interpreter.  Arguments are checked by the Python entry points, sizes by the kernels' own entry points.
 #include <ATen/core/Tensor.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
-#include <ATen/ops/empty_strided.h>
 #include <ATen/ops/zeros_like.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
@@ -53,7 +53,7 @@ void* mutable_pointer(const Tensor& t) { return t.defined() ? t.mutable_data_ptr
 // A dense channels-last map of x's shape, dtype and device.
 Tensor map_like(const Tensor& x) {
   const int64_t n = x.size(0), c = x.size(1), h = x.size(2), w = x.size(3);
-  return at::empty_strided({n, c, h, w}, {h * w * c, 1, w * c, c}, x.options().memory_format(std::nullopt));
+  return at::detail::empty_strided_cuda({n, c, h, w}, {h * w * c, 1, w * c, c}, x.scalar_type(), x.device());
 }
 
 // x [N, C, H, W] where it is channels-last, dense or a slice of the channels of a dense map; otherwise a dense
@@ -96,7 +96,7 @@ kad_group_norm_args norm_args(const Tensor& x, int64_t cs, const Tensor& weight,
 }
 
 Tensor floats(const Tensor& x, at::IntArrayRef sizes) {
-  return at::empty(sizes, x.options().dtype(at::kFloat).memory_format(std::nullopt));
+  return at::detail::empty_cuda(sizes, at::kFloat, x.device(), std::nullopt);
 }
 
 Tensor scratch(const kad_group_norm_args& a, int backward, const Tensor& x) {
@@ -136,8 +136,8 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& dy, const Tensor&
     return {dx, need.weight ? at::zeros_like(weight) : Tensor(), need.bias ? at::zeros_like(bias) : Tensor()};
   if (!(need.x || need.weight || need.bias)) return {};
   const Tensor w = dense(weight), b = dense(bias);
-  Tensor dw = need.weight ? at::empty({x.size(1)}, w.options()) : Tensor();
-  Tensor db = need.bias ? at::empty({x.size(1)}, b.options()) : Tensor();
+  Tensor dw = need.weight ? at::detail::empty_cuda({x.size(1)}, w.scalar_type(), w.device(), std::nullopt) : Tensor();
+  Tensor db = need.bias ? at::detail::empty_cuda({x.size(1)}, b.scalar_type(), b.device(), std::nullopt) : Tensor();
   int64_t cs, dcs;
   const Tensor v = channels_last_pixels(x, cs), d = channels_last_pixels(dy, dcs);
   kad_group_norm_args a = norm_args(v, cs, w, b, o);
