@@ -126,7 +126,8 @@ struct Geo {
   // split kernels
   int rows, tiles;  // rows of a tile (whole R), tiles of an image
   int whole, last, rest;  // the last tile's rows: last R + rest
-  int per;          // threads that join a group's tiles
+  int parts, part_rows;   // tiles and their rows in the launch whose sums are joined
+  int per;          // threads that join a group's parts
 };
 // x / d for x in [0, 2^16), from 1 / d: an integer division is some forty instructions.
 __device__ __forceinline__ int over(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
@@ -400,9 +401,10 @@ struct Tile {
   // The i-th round of a walk from the end: the whole ones backwards, then the partial one.
   __device__ __forceinline__ int back(int i) const { return i < whole ? whole - 1 - i : i; }
 };
-__device__ __forceinline__ int tile_pixels(const Geo& o, int64_t P, int t) {
-  const int64_t first = (int64_t)t * o.rows * o.k, next = first + (int64_t)o.rows * o.k;
-  return (int)((t == o.tiles - 1 ? P : next) - first);
+// Pixels of the t-th tile of the first launch.
+__device__ __forceinline__ int part_pixels(const Geo& o, int64_t P, int t) {
+  const int64_t first = (int64_t)t * o.part_rows * o.k, next = first + (int64_t)o.part_rows * o.k;
+  return (int)((t == o.parts - 1 ? P : next) - first);
 }
 
 // A map's rows as a thread meets them in a tile: an address that all threads share moves from round to round, the
@@ -560,7 +562,7 @@ struct TileJoin {
     g = t - l * o.q;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (l < per && l + i * per < o.tiles) first[i] = part[(l + i * per) * o.q + g];
+      if (l < per && l + i * per < o.parts) first[i] = part[(l + i * per) * o.q + g];
   }
   // make(tile, part) gives a tile's E.
   template <typename Make, typename Done>
@@ -569,7 +571,7 @@ struct TileJoin {
     if (o.q > (int)blockDim.x) {  // a group a thread, over and over
       for (int k = t; k < o.q; k += blockDim.x) {
         E acc = make(0, part[k]);
-        for (int i = 1; i < o.tiles; ++i) acc = acc.join(make(i, part[i * o.q + k]));
+        for (int i = 1; i < o.parts; ++i) acc = acc.join(make(i, part[i * o.q + k]));
         done(k, acc);
       }
       __syncthreads();
@@ -578,8 +580,8 @@ struct TileJoin {
     E acc{};
     if (l < per) {
       acc = make(l, first[0]);
-      if (l + per < o.tiles) acc = acc.join(make(l + per, first[1]));
-      for (int i = l + 2 * per; i < o.tiles; i += per) acc = acc.join(make(i, part[i * o.q + g]));
+      if (l + per < o.parts) acc = acc.join(make(l + per, first[1]));
+      for (int i = l + 2 * per; i < o.parts; i += per) acc = acc.join(make(i, part[i * o.q + g]));
     }
     red[t] = acc;
     for (int n = per; n > 1;) {  // quarters join
@@ -646,7 +648,7 @@ __global__ __launch_bounds__(MOST) void group_norm_apply_kernel(kad_group_norm_a
   const Lane<const T> lane(o, col, rows, x, xs);
   const Lane<T> out(o, col, rows, y, ys);
   float w[V], b[V], m[NG], rs[NG];
-  TileJoin<Moments> join(o, (const Sums*)a.work + (int64_t)n * o.tiles * o.q);
+  TileJoin<Moments> join(o, (const Sums*)a.work + (int64_t)n * o.parts * o.q);
   col.params(o, a, w, b);
   // Backwards: what the statistics read last is still near.
   const auto load = [&](int i) { return load_vec(lane.at(rows, rows.back(i))); };
@@ -654,7 +656,7 @@ __global__ __launch_bounds__(MOST) void group_norm_apply_kernel(kad_group_norm_a
   float *mean = lds + 3 * blockDim.x, *rstd = mean + o.q;
   join.run(
       o, (Moments*)lds,
-      [&](int t, const Sums& p) { return Moments{(float)tile_pixels(o, P, t) * (float)o.D, p.a, p.b}; },
+      [&](int t, const Sums& p) { return Moments{(float)part_pixels(o, P, t) * (float)o.D, p.a, p.b}; },
       [&](int g, const Moments& e) {
         const float r = 1.0f / sqrtf(e.m2 / e.n + a.eps);
         mean[g] = e.mean;
@@ -837,7 +839,7 @@ __device__ __forceinline__ void dx_rows(const Columns<T, ONE>& col, const Tile& 
 constexpr int PARAM_CHANNELS = 16;
 __device__ __forceinline__ void param_sums(const kad_group_norm_args& a, const Geo& o, int block, float* lds) {
   const int c = block * PARAM_CHANNELS + (threadIdx.x & (PARAM_CHANNELS - 1));
-  const int parts = a.n * o.tiles, step = blockDim.x / PARAM_CHANNELS;
+  const int parts = a.n * o.parts, step = blockDim.x / PARAM_CHANNELS;
   const Sums* chans = (const Sums*)a.work + (int64_t)parts * o.q;
   float db = 0.f, dw = 0.f;
   if (c < o.W)
@@ -882,7 +884,7 @@ __global__ __launch_bounds__(MOST) void group_norm_dx_kernel(kad_group_norm_args
   const Lane<const T> lx(o, col, rows, x, xs), ld(o, col, rows, dy, ds);
   const Lane<T> out(o, col, rows, dx, os);
   float w[V], b[V], m[NG], rs[NG], s1[NG], s2[NG];
-  TileJoin<Sums> join(o, (const Sums*)a.work + (int64_t)n * o.tiles * o.q);
+  TileJoin<Sums> join(o, (const Sums*)a.work + (int64_t)n * o.parts * o.q);
   col.params(o, a, w, b);
   col.of_groups(o, a.mean + n * o.q, m);
   col.of_groups(o, a.rstd + n * o.q, rs);
@@ -1076,29 +1078,47 @@ bool resident(const kad_group_norm_args& a, Geo& o, int& threads) {
   return true;
 }
 
-// The split kernels' layout; false: the any-width kernels' case.
-bool split(const kad_group_norm_args& a, Geo& o, int& threads) {
-  if (!lay_out(a, a.groups, o)) return false;
-  // One block of 512 threads a CU: what a block does beside its rows (places, weights, the join of what it and
-  // others left) is microseconds, so that more blocks lose more than their loads in flight gain ([8, 256, 100, 100]
-  // fp16, forward and backward: 27 and 46 us where this was tried; 32 and 54 with two blocks a CU, 44 and 70 with
-  // four; 27 and 47 with 256 threads).  Threads of under 8 rows are halved ([3, 86, 67, 41] fp32: 9.6 and 12.0 us against 10.4 and 12.7).
-  const int most = (int64_t)a.n * o.full * o.S < 8 * 256 * 512 ? 256 : 512;
-  count_threads(o, most / o.S < o.full ? most / o.S : o.full, threads);
-  int tiles = ceil_div(256, a.n);
-  // An image of over 256 rows a thread and tile is cut finer, up to 256 tiles, whatever the batch.
-  const int64_t fine = o.full / (256 * o.R);
-  if (tiles < fine) tiles = fine < 256 ? (int)fine : 256;
-  const int least = ceil_div(o.full, 4 * o.R);  // 4 rows a thread
-  if (tiles > least) tiles = least;
-  if (tiles < 1) tiles = 1;
+// Cuts an image's rows into about `tiles` tiles.
+void cut(Geo& o, int tiles) {
   o.rows = round_up(ceil_div(o.full, tiles), o.R);
   if (o.rows < 1) o.rows = o.R;
   o.tiles = o.full ? ceil_div(o.full, o.rows) : 1;
   o.whole = o.rows / o.R;
   o.last = (o.full - (o.tiles - 1) * o.rows) / o.R;
   o.rest = (o.full - (o.tiles - 1) * o.rows) % o.R;
-  o.per = threads / o.q < 1 ? 1 : threads / o.q < o.tiles ? threads / o.q : o.tiles;
+}
+
+// The split kernels' layouts, of the launch that sums and of the one that writes; false: the any-width kernels' case.
+bool split(const kad_group_norm_args& a, bool backward, Geo& sums, Geo& writes, int& threads) {
+  Geo o;
+  if (!lay_out(a, a.groups, o)) return false;
+  // One block of 512 threads a CU: what a block does beside its rows (places, weights, the join of what it and
+  // others left) is microseconds, so that more blocks lose more than their loads in flight gain ([8, 256, 100, 100]
+  // fp16, forward and backward: 27 and 46 us where this was tried; 32 and 54 with two blocks a CU, 44 and 70 with
+  // four; 27 and 47 with 256 threads).  Threads of under 8 rows are halved ([3, 86, 67, 41] fp32: 9.6 and 12.0 us
+  // against 10.4 and 12.7).
+  const int most = (int64_t)a.n * o.full * o.S < 8 * 256 * 512 ? 256 : 512;
+  count_threads(o, most / o.S < o.full ? most / o.S : o.full, threads);
+  int tiles = a.n < 256 ? 256 / a.n : 1;
+  // An image of over 256 rows a thread and tile is cut finer, up to 256 tiles, whatever the batch.
+  const int64_t fine = o.full / (256 * o.R);
+  if (tiles < fine) tiles = fine < 256 ? (int)fine : 256;
+  const int least = ceil_div(o.full, 4 * o.R);  // 4 rows a thread
+  if (tiles > least) tiles = least;
+  if (tiles < 1) tiles = 1;
+  sums = writes = o;
+  cut(writes, tiles);
+  // Every block of the second launch joins all parts of its image: few images with many groups are summed in fewer
+  // tiles than they are written in, 8 parts a thread to join forward and 16 backward, where the sums take longer
+  // ([1, 384, 18, 166] fp32 in 32 groups: 12.4 and 16.3 us, 19.0 and 21.0 with as many parts as tiles, 14.3 and 22.8
+  // with 64 rows a thread; [1, 128, 100, 100] fp16: 13.4 and 19.1, 15.4 and 19.2, 18.5 and 33.7).
+  int parts = (backward ? 16 : 8) * threads / o.q;
+  const int busy = ceil_div(o.full, 32 * o.R);
+  if (parts < busy) parts = busy;
+  cut(sums, parts < tiles ? parts : tiles);
+  sums.parts = writes.parts = sums.tiles;
+  sums.part_rows = writes.part_rows = sums.rows;
+  writes.per = threads / o.q < 1 ? 1 : threads / o.q < writes.parts ? threads / o.q : writes.parts;
   return true;
 }
 
@@ -1138,35 +1158,34 @@ void launch_resident(const kad_group_norm_args& a, const Geo& o, int threads, hi
 }
 
 template <typename T, bool ONE, int MOST>
-void launch_split(const kad_group_norm_args& a, const Geo& o, int threads, hipStream_t st) {
-  const dim3 grid(o.tiles, a.n);
+void launch_split(const kad_group_norm_args& a, const Geo& first, const Geo& o, int threads, hipStream_t st) {
   const size_t stats = threads * (ONE ? 1 : VEC<T>) * sizeof(Moments);
   allow_lds(group_norm_stats_kernel<T, ONE, MOST>, stats);
-  group_norm_stats_kernel<T, ONE, MOST><<<grid, threads, stats, st>>>(a, o);
-  group_norm_apply_kernel<T, ONE, MOST><<<grid, threads, threads * sizeof(Moments) + 2 * o.q * sizeof(float), st>>>(a, o);
+  group_norm_stats_kernel<T, ONE, MOST><<<dim3(first.tiles, a.n), threads, stats, st>>>(a, first);
+  group_norm_apply_kernel<T, ONE, MOST><<<dim3(o.tiles, a.n), threads, threads * sizeof(Moments) + 2 * o.q * sizeof(float), st>>>(a, o);
 }
 
 template <typename T>
 void forward(const kad_group_norm_args& a, hipStream_t st) {
-  Geo o;
+  Geo o, first;
   int threads;
   if (resident(a, o, threads)) {
     if (o.q == 1) launch_resident<T, true>(a, o, threads, st);
     else launch_resident<T, false>(a, o, threads, st);
-  } else if (split(a, o, threads)) {
+  } else if (split(a, false, first, o, threads)) {
     const bool one = o.q == 1 || o.D % VEC<T> == 0;
-    if (one) threads > 512 ? launch_split<T, true, 1024>(a, o, threads, st) : launch_split<T, true, 512>(a, o, threads, st);
-    else threads > 512 ? launch_split<T, false, 1024>(a, o, threads, st) : launch_split<T, false, 512>(a, o, threads, st);
+    if (one) threads > 512 ? launch_split<T, true, 1024>(a, first, o, threads, st) : launch_split<T, true, 512>(a, first, o, threads, st);
+    else threads > 512 ? launch_split<T, false, 1024>(a, first, o, threads, st) : launch_split<T, false, 512>(a, first, o, threads, st);
   } else {
     group_norm_wide_kernel<T><<<dim3(a.groups, a.n), 256, 0, st>>>(a);
   }
 }
 
 template <typename T, bool ONE, int MOST>
-void launch_backward(const kad_group_norm_args& a, const Geo& o, int threads, hipStream_t st) {
+void launch_backward(const kad_group_norm_args& a, const Geo& first, const Geo& o, int threads, hipStream_t st) {
   const size_t sums = threads * VEC<T> * sizeof(Sums) + 3 * o.W * sizeof(float);
   allow_lds(group_norm_bwd_sums_kernel<T, ONE, MOST>, sums);
-  group_norm_bwd_sums_kernel<T, ONE, MOST><<<dim3(o.tiles, a.n), threads, sums, st>>>(a, o);
+  group_norm_bwd_sums_kernel<T, ONE, MOST><<<dim3(first.tiles, a.n), threads, sums, st>>>(a, first);
   const int params = a.dweight || a.dbias ? ceil_div(ceil_div(o.W, PARAM_CHANNELS), o.tiles) : 0;
   const int waves = threads / 64 * PARAM_CHANNELS * 2, join = 2 * threads + 2 * o.q;
   if (a.out && a.n + params > 65535) {  // more rows of blocks than a grid has
@@ -1181,13 +1200,13 @@ void launch_backward(const kad_group_norm_args& a, const Geo& o, int threads, hi
 
 template <typename T>
 void backward(const kad_group_norm_args& a, hipStream_t st) {
-  Geo o;
+  Geo o, first;
   int threads;
   if (!a.out && !a.dweight && !a.dbias) return;
-  if (split(a, o, threads)) {
+  if (split(a, true, first, o, threads)) {
     const bool one = o.q == 1 || o.D % VEC<T> == 0;
-    if (one) threads > 512 ? launch_backward<T, true, 1024>(a, o, threads, st) : launch_backward<T, true, 512>(a, o, threads, st);
-    else threads > 512 ? launch_backward<T, false, 1024>(a, o, threads, st) : launch_backward<T, false, 512>(a, o, threads, st);
+    if (one) threads > 512 ? launch_backward<T, true, 1024>(a, first, o, threads, st) : launch_backward<T, true, 512>(a, first, o, threads, st);
+    else threads > 512 ? launch_backward<T, false, 1024>(a, first, o, threads, st) : launch_backward<T, false, 512>(a, first, o, threads, st);
     return;
   }
   if (a.out) group_norm_wide_dx_kernel<T><<<dim3(a.groups, a.n), 256, 0, st>>>(a);
@@ -1201,11 +1220,11 @@ using namespace kad;
 
 extern "C" int64_t kad_group_norm_work_elems(const kad_group_norm_args* a, int backward) {
   if (int rc = check_args(a, "kad_group_norm_work_elems")) return rc;
-  Geo o;
+  Geo o, first;
   int threads;
   if (!backward && resident(*a, o, threads)) return 0;
-  if (!split(*a, o, threads)) return 0;
-  return (int64_t)a->n * o.tiles * 2 * (o.q + (backward ? o.W : 0));
+  if (!split(*a, backward, first, o, threads)) return 0;
+  return (int64_t)a->n * o.parts * 2 * (o.q + (backward ? o.W : 0));
 }
 
 extern "C" int kad_group_norm_fwd(const kad_group_norm_args* a, void* stream) {
