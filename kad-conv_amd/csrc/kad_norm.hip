@@ -11,8 +11,10 @@
 // Two forms.  A group of up to 32 KB stays in the registers of one block: one launch, one read.  Beyond, an
 // image is cut into tiles of whole rows: one launch leaves each tile's sums, the next joins them (every block
 // for itself, while its first rows are on their way) and writes the result, walking its rows backwards to meet
-// what the first left in its XCD's L2.  Its stores pass the caches by, which leaves x in them: a bare read and
-// a bare copy of 41 MB take 23.3 us in two launches, 19.1 us with such stores (one copy alone: 17.4, 12.5).
+// what the first left in the cache before memory (an XCD's L2 is emptied between launches; forwards: 5 % more at
+// 41 MB, [16, 256, 200, 200] bf16 205 and 331 us against 174 and 303).  Its stores pass the caches by, which leaves
+// x in them: a bare read and a bare copy of 41 MB take 23.3 us in two launches, 19.1 us with such stores (one copy
+// alone: 17.4, 12.5).
 // [8, 256, 100, 100] fp16 (41 MB): 25.0 us forward (statistics 9, result 16), backward 44 us (sums 21,
 // dx 22), where a bare read of x and dy takes 13.6 us, and their vector operations 11 and 12: what a block does
 // beside its rows (1 us of launch, 2 of places, weights and tiles joined, 1 of sums joined) is the rest.
@@ -42,18 +44,22 @@ __device__ __forceinline__ void store_param(void* p, int i, int dtype, float v) 
   else ((bf16_t*)p)[i] = (bf16_t)v;
 }
 
-// 1 / (1 + e^-z) with the hardware's reciprocal (off by one step of 32 bits at most): 0 where e^-z overflows.
-__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+// 1 / (1 + e^-z): 0 where e^-z overflows.  For 16-bit maps with the hardware's reciprocal alone (off by one step of
+// 32 bits at most, 2^-12 of a step of theirs); for fp32 ones the quotient rounded.
+template <typename T>
+__device__ __forceinline__ float logistic(float z) {
+  return sizeof(T) == 2 ? __builtin_amdgcn_rcpf(1.0f + __expf(-z)) : sigmoidf_(z);
+}
 
 // act(z), and act'(z) times dy.
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ float act_of(float z) {
-  return ACT == KAD_ACT_SILU ? z * logistic(z) : ACT == KAD_ACT_RELU ? (z > 0.f ? z : z != z ? z : 0.f) : z;
+  return ACT == KAD_ACT_SILU ? z * logistic<T>(z) : ACT == KAD_ACT_RELU ? (z > 0.f ? z : z != z ? z : 0.f) : z;
 }
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ float act_grad(float z, float dy) {
   if (ACT == KAD_ACT_SILU) {
-    const float s = logistic(z), y = z * s;
+    const float s = logistic<T>(z), y = z * s;
     return dy * (s + y - y * s);
   }
   return ACT == KAD_ACT_RELU ? (z > 0.f ? dy : 0.f) : dy;
@@ -261,7 +267,7 @@ struct Columns {
 template <typename T, bool ONE, int ACT>
 __device__ __forceinline__ void norm_vec(float x[VEC<T>], const float* mean, const float* w, const float* b) {
 #pragma unroll
-  for (int v = 0; v < VEC<T>; ++v) x[v] = act_of<ACT>((x[v] - mean[ONE ? 0 : v]) * w[v] + b[v]);
+  for (int v = 0; v < VEC<T>; ++v) x[v] = act_of<T, ACT>((x[v] - mean[ONE ? 0 : v]) * w[v] + b[v]);
 }
 
 // ---------------------------------------------------------------------------- resident forward
@@ -650,7 +656,7 @@ __global__ __launch_bounds__(MOST) void group_norm_apply_kernel(kad_group_norm_a
   float w[V], b[V], m[NG], rs[NG];
   TileJoin<Moments> join(o, (const Sums*)a.work + (int64_t)n * o.parts * o.q);
   col.params(o, a, w, b);
-  // Backwards: what the statistics read last is still near.
+  // Backwards: what the statistics read last is in the cache before memory still.
   const auto load = [&](int i) { return load_vec(lane.at(rows, rows.back(i))); };
   Walk<intx4, B> walk(rows.count, load);
   float *mean = lds + 3 * blockDim.x, *rstd = mean + o.q;
@@ -688,7 +694,7 @@ __device__ __forceinline__ void sum_vec(const float x[VEC<T>], const float dy[VE
 #pragma unroll
   for (int v = 0; v < VEC<T>; ++v) {
     const float xm = x[v] - mean[ONE ? 0 : v];
-    const float dz = act_grad<ACT>(xm * w[v] + b[v], dy[v]);
+    const float dz = act_grad<T, ACT>(xm * w[v] + b[v], dy[v]);
     db[v] += dz;
     dw[v] += dz * xm;
   }
@@ -798,7 +804,7 @@ __device__ __forceinline__ void dx_vec(float x[VEC<T>], const float dy[VEC<T>], 
   for (int v = 0; v < VEC<T>; ++v) {
     const int g = ONE ? 0 : v;
     const float xm = x[v] - mean[g];
-    const float dz = act_grad<ACT>(xm * w[v] + b[v], dy[v]);
+    const float dz = act_grad<T, ACT>(xm * w[v] + b[v], dy[v]);
     x[v] = w[v] * dz - (xm * c2[g] + c1[g]);
   }
 }
@@ -921,104 +927,176 @@ __global__ __launch_bounds__(MOST) void group_norm_dx_kernel(kad_group_norm_args
 }
 
 // ---------------------------------------------------------------------------- any width
-// Rows of more than 1024 vectors (C over 8192, or over 1024 and odd, for 16-bit types): one block an (image,
-// group), a value at a time, the group read again for each sum.
+// Rows of more than 1024 vectors (C over 8192, or over 1024 and odd, for 16-bit types): a block takes a group's
+// columns of a tile of pixels, a value a thread at a time: L threads beside each other on a pixel's D channels,
+// 256 / L pixels at once.  Sums and joins as above, an (image, group) for itself.  Loads of single values bound it:
+// [2, 9000, 40, 40] fp16 in 30 groups takes 138 us forward and 196 backward, 0.8 and 0.9 TB/s.
+struct Wide {
+  int L, at_once;     // min(D, 256), 256 / L
+  float inv;          // 1 / L
+  int rows, tiles;    // pixels of a tile, tiles of an image
+};
+struct WidePlace {
+  int r, l;
+  bool on;
+  int64_t first, last;  // the tile's pixels
+  __device__ __forceinline__ WidePlace(const Wide& o, int64_t P) {
+    r = over(threadIdx.x, o.inv);
+    l = threadIdx.x - r * o.L;
+    on = r < o.at_once;
+    first = (int64_t)blockIdx.z * o.rows;
+    last = first + o.rows < P ? first + o.rows : P;
+  }
+};
+template <typename T>
 __device__ __forceinline__ float wide_act(float z, int act) {
-  return act == KAD_ACT_SILU ? act_of<KAD_ACT_SILU>(z) : act == KAD_ACT_RELU ? act_of<KAD_ACT_RELU>(z) : z;
+  return act == KAD_ACT_SILU ? act_of<T, KAD_ACT_SILU>(z) : act == KAD_ACT_RELU ? act_of<T, KAD_ACT_RELU>(z) : z;
 }
+template <typename T>
 __device__ __forceinline__ float wide_grad(float z, float dy, int act) {
-  return act == KAD_ACT_SILU ? act_grad<KAD_ACT_SILU>(z, dy) : act == KAD_ACT_RELU ? act_grad<KAD_ACT_RELU>(z, dy) : dy;
+  return act == KAD_ACT_SILU ? act_grad<T, KAD_ACT_SILU>(z, dy) : act == KAD_ACT_RELU ? act_grad<T, KAD_ACT_RELU>(z, dy) : dy;
 }
 
-// Sum over the block's 256 threads, for all of them.
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-  v = wave_sum(v);
+// What the block's 256 threads have, joined, for all of them.
+template <typename E>
+__device__ __forceinline__ E block_join(E e) {
+  __shared__ E waves[4];
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) e = e.join(e.from(m));
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = e;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  e = waves[0].join(waves[1]).join(waves[2].join(waves[3]));
   __syncthreads();
-  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  return e;
+}
+// The parts that the tiles of an (image, group) left, joined, for all threads.
+template <typename E, typename Make>
+__device__ __forceinline__ E wide_join(const kad_group_norm_args& a, const Wide& o, int n, int g, Make make) {
+  E e{};
+  for (int t = threadIdx.x; t < o.tiles; t += 256) e = e.join(make(t, ((const Sums*)a.work)[((int64_t)n * o.tiles + t) * a.groups + g]));
+  return block_join(e);
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void group_norm_wide_kernel(kad_group_norm_args a) {
-  __shared__ float lds[4];
+__global__ __launch_bounds__(256) void group_norm_wide_stats_kernel(kad_group_norm_args a, Wide o) {
   const int g = blockIdx.x, n = blockIdx.y, D = a.c / a.groups;
-  const int64_t P = (int64_t)a.h * a.w, M = P * D;
-  const T* x = (const T*)a.x + (int64_t)n * P * a.x_cs + g * D;
-  T* y = (T*)a.out + (int64_t)n * P * a.c + g * D;
-  float s = 0.f;
-  for (int64_t i = threadIdx.x; i < M; i += 256) s += to_f32(x[i / D * a.x_cs + i % D]);
-  const float mean = block_sum(s, lds) / (float)M;
-  s = 0.f;
-  for (int64_t i = threadIdx.x; i < M; i += 256) {
-    const float d = to_f32(x[i / D * a.x_cs + i % D]) - mean;
-    s += d * d;
-  }
-  const float rstd = 1.0f / sqrtf(block_sum(s, lds) / (float)M + a.eps);
-  if (threadIdx.x == 0) {
+  const int64_t P = (int64_t)a.h * a.w;
+  const WidePlace at(o, P);
+  const T* x = (const T*)a.x + n * P * a.x_cs + (int64_t)g * D;
+  Moments acc{};
+  if (at.on)
+    for (int64_t p = at.first + at.r; p < at.last; p += o.at_once)
+      for (int d = at.l; d < D; d += 4 * o.L) {
+        float v[4], n4 = 0.f, s = 0.f, q = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = d + i * o.L < D;
+          v[i] = to_f32(x[p * a.x_cs + (in ? d + i * o.L : d)]);
+          n4 += in ? 1.f : 0.f;
+          s += in ? v[i] : 0.f;
+        }
+        s /= n4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q += d + i * o.L < D ? (v[i] - s) * (v[i] - s) : 0.f;
+        acc = acc.join(Moments{n4, s, q});
+      }
+  acc = block_join(acc);
+  if (threadIdx.x == 0) ((Sums*)a.work)[((int64_t)n * o.tiles + blockIdx.z) * a.groups + g] = Sums{acc.mean, acc.m2};
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void group_norm_wide_apply_kernel(kad_group_norm_args a, Wide o) {
+  const int g = blockIdx.x, n = blockIdx.y, D = a.c / a.groups;
+  const int64_t P = (int64_t)a.h * a.w;
+  const WidePlace at(o, P);
+  const Moments e = wide_join<Moments>(a, o, n, g, [&](int t, const Sums& p) {
+    const int64_t left = P - (int64_t)t * o.rows;
+    return Moments{(float)(left < o.rows ? left : o.rows) * (float)D, p.a, p.b};
+  });
+  const float mean = e.mean, rstd = 1.0f / sqrtf(e.m2 / e.n + a.eps);
+  if (blockIdx.z == 0 && threadIdx.x == 0) {
     a.mean[n * a.groups + g] = mean;
     a.rstd[n * a.groups + g] = rstd;
   }
-  for (int64_t i = threadIdx.x; i < M; i += 256) {
-    const int c = (int)(i % D);
-    const float w = load_param(a.weight, g * D + c, a.param_dtype, 1.f);
-    const float b = load_param(a.bias, g * D + c, a.param_dtype, 0.f);
-    y[i / D * a.c + c] = from_f32<T>(wide_act((to_f32(x[i / D * a.x_cs + c]) - mean) * rstd * w + b, a.act));
+  if (!at.on) return;
+  const T* x = (const T*)a.x + n * P * a.x_cs + (int64_t)g * D;
+  T* y = (T*)a.out + n * P * a.c + (int64_t)g * D;
+  for (int d = at.l; d < D; d += o.L) {
+    const float w = load_param(a.weight, g * D + d, a.param_dtype, 1.f) * rstd;
+    const float b = load_param(a.bias, g * D + d, a.param_dtype, 0.f);
+#pragma unroll 4
+    for (int64_t p = at.first + at.r; p < at.last; p += o.at_once)
+      y[p * a.c + d] = from_f32<T>(wide_act<T>((to_f32(x[p * a.x_cs + d]) - mean) * w + b, a.act));
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void group_norm_wide_dx_kernel(kad_group_norm_args a) {
-  __shared__ float lds[4];
+__global__ __launch_bounds__(256) void group_norm_wide_sums_kernel(kad_group_norm_args a, Wide o) {
+  __shared__ Sums red[256];
   const int g = blockIdx.x, n = blockIdx.y, D = a.c / a.groups;
-  const int64_t P = (int64_t)a.h * a.w, M = P * D;
-  const T* x = (const T*)a.x + (int64_t)n * P * a.x_cs + g * D;
-  const T* dy = (const T*)a.dy + (int64_t)n * P * a.dy_cs + g * D;
-  T* dx = (T*)a.out + (int64_t)n * P * a.c + g * D;
+  const int64_t P = (int64_t)a.h * a.w, part = (int64_t)n * o.tiles + blockIdx.z;
+  const WidePlace at(o, P);
   const float mean = a.mean[n * a.groups + g], rstd = a.rstd[n * a.groups + g];
-  float s1 = 0.f, s2 = 0.f;
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int64_t i = threadIdx.x; i < M; i += 256) {
-      const int c = (int)(i % D);
-      const int64_t p = i / D;
-      const float w = load_param(a.weight, g * D + c, a.param_dtype, 1.f);
-      const float b = load_param(a.bias, g * D + c, a.param_dtype, 0.f);
-      const float xhat = (to_f32(x[p * a.x_cs + c]) - mean) * rstd;
-      const float wdz = w * wide_grad(xhat * w + b, to_f32(dy[p * a.dy_cs + c]), a.act);
-      if (pass == 0) {
-        s1 += wdz;
-        s2 += wdz * xhat;
-      } else {
-        dx[p * a.c + c] = from_f32<T>(rstd * (wdz - s1 - xhat * s2));
+  const T* x = (const T*)a.x + n * P * a.x_cs + (int64_t)g * D;
+  const T* dy = (const T*)a.dy + n * P * a.dy_cs + (int64_t)g * D;
+  Sums* chans = (Sums*)a.work + (int64_t)a.n * o.tiles * a.groups + part * a.c + (int64_t)g * D;
+  const bool keep = a.dweight || a.dbias;
+  Sums group{};
+  for (int d0 = 0; d0 < D; d0 += o.L) {  // L channels at a time, their pixels shared by 256 / L threads
+    const int d = d0 + at.l;
+    Sums s{};
+    float w = 0.f;
+    if (at.on && d < D) {
+      w = load_param(a.weight, g * D + d, a.param_dtype, 1.f);
+      const float b = load_param(a.bias, g * D + d, a.param_dtype, 0.f);
+#pragma unroll 4
+      for (int64_t p = at.first + at.r; p < at.last; p += o.at_once) {
+        const float xhat = (to_f32(x[p * a.x_cs + d]) - mean) * rstd;
+        const float dz = wide_grad<T>(xhat * w + b, to_f32(dy[p * a.dy_cs + d]), a.act);
+        s.a += dz;
+        s.b += dz * xhat;
       }
     }
-    if (pass == 0) {
-      s1 = block_sum(s1, lds) / (float)M;
-      s2 = block_sum(s2, lds) / (float)M;
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (at.on && at.r == 0 && d < D) {
+      for (int r = 1; r < o.at_once; ++r) s = s.join(red[threadIdx.x + r * o.L]);
+      if (keep) chans[d] = s;
+      group = group.join(Sums{w * s.a, w * s.b});
+    }
+    __syncthreads();
+  }
+  group = block_join(group);
+  if (threadIdx.x == 0) ((Sums*)a.work)[part * a.groups + g] = group;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void group_norm_wide_dx_kernel(kad_group_norm_args a, Wide o) {
+  const int g = blockIdx.x, n = blockIdx.y, D = a.c / a.groups;
+  const int64_t P = (int64_t)a.h * a.w;
+  const WidePlace at(o, P);
+  const Sums e = wide_join<Sums>(a, o, n, g, [](int, const Sums& p) { return p; });
+  const float mean = a.mean[n * a.groups + g], rstd = a.rstd[n * a.groups + g], inv = 1.0f / ((float)P * (float)D);
+  const float s1 = e.a * inv, s2 = e.b * inv;
+  if (!at.on) return;
+  const T* x = (const T*)a.x + n * P * a.x_cs + (int64_t)g * D;
+  const T* dy = (const T*)a.dy + n * P * a.dy_cs + (int64_t)g * D;
+  T* dx = (T*)a.out + n * P * a.c + (int64_t)g * D;
+  for (int d = at.l; d < D; d += o.L) {
+    const float w = load_param(a.weight, g * D + d, a.param_dtype, 1.f);
+    const float b = load_param(a.bias, g * D + d, a.param_dtype, 0.f);
+#pragma unroll 4
+    for (int64_t p = at.first + at.r; p < at.last; p += o.at_once) {
+      const float xhat = (to_f32(x[p * a.x_cs + d]) - mean) * rstd;
+      const float dz = wide_grad<T>(xhat * w + b, to_f32(dy[p * a.dy_cs + d]), a.act);
+      dx[p * a.c + d] = from_f32<T>(rstd * (w * dz - s1 - xhat * s2));
     }
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void group_norm_wide_param_kernel(kad_group_norm_args a) {
-  __shared__ float lds[4];
-  const int c = blockIdx.x, g = c / (a.c / a.groups);
-  const int64_t P = (int64_t)a.h * a.w, rows = P * a.n;
-  const float w = load_param(a.weight, c, a.param_dtype, 1.f), b = load_param(a.bias, c, a.param_dtype, 0.f);
-  float dw = 0.f, db = 0.f;
-  for (int64_t r = threadIdx.x; r < rows; r += 256) {
-    const int k = (int)(r / P) * a.groups + g;
-    const float xhat = (to_f32(((const T*)a.x)[r * a.x_cs + c]) - a.mean[k]) * a.rstd[k];
-    const float dz = wide_grad(xhat * w + b, to_f32(((const T*)a.dy)[r * a.dy_cs + c]), a.act);
-    dw += dz * xhat;
-    db += dz;
-  }
-  dw = block_sum(dw, lds);
-  db = block_sum(db, lds);
-  if (threadIdx.x == 0) {
-    if (a.dweight) store_param(a.dweight, c, a.param_dtype, dw);
-    if (a.dbias) store_param(a.dbias, c, a.param_dtype, db);
-  }
+__global__ __launch_bounds__(256) void group_norm_wide_param_kernel(kad_group_norm_args a, Geo o) {
+  __shared__ float lds[4 * PARAM_CHANNELS * 2];
+  param_sums(a, o, blockIdx.x, lds);
 }
 
 // ---------------------------------------------------------------------------- host
@@ -1122,6 +1200,22 @@ bool split(const kad_group_norm_args& a, bool backward, Geo& sums, Geo& writes, 
   return true;
 }
 
+// The any-width kernels' layout: four blocks a CU over all images and groups, 16 pixels a thread at least.
+Wide wide(const kad_group_norm_args& a) {
+  const int D = a.c / a.groups;
+  const int64_t P = (int64_t)a.h * a.w;
+  Wide o;
+  o.L = D < 256 ? D : 256;
+  o.at_once = 256 / o.L;
+  o.inv = 1.0f / (float)o.L;
+  const int64_t cells = (int64_t)a.n * a.groups, least = 16 * o.at_once;
+  int64_t tiles = cells < 1024 ? 1024 / cells : 1;
+  if (tiles * least > P) tiles = (P + least - 1) / least;
+  o.rows = (int)((P + tiles - 1) / tiles);
+  o.tiles = (int)((P + o.rows - 1) / o.rows);
+  return o;
+}
+
 int check_args(const kad_group_norm_args* a, const char* what) {
   KAD_CHECK_ARG(a, "%s: null pointer", what);
   KAD_CHECK_ARG(a->dtype == KAD_F32 || a->dtype == KAD_F16 || a->dtype == KAD_BF16, "%s: bad dtype", what);
@@ -1177,7 +1271,9 @@ void forward(const kad_group_norm_args& a, hipStream_t st) {
     if (one) threads > 512 ? launch_split<T, true, 1024>(a, first, o, threads, st) : launch_split<T, true, 512>(a, first, o, threads, st);
     else threads > 512 ? launch_split<T, false, 1024>(a, first, o, threads, st) : launch_split<T, false, 512>(a, first, o, threads, st);
   } else {
-    group_norm_wide_kernel<T><<<dim3(a.groups, a.n), 256, 0, st>>>(a);
+    const Wide v = wide(a);
+    group_norm_wide_stats_kernel<T><<<dim3(a.groups, a.n, v.tiles), 256, 0, st>>>(a, v);
+    group_norm_wide_apply_kernel<T><<<dim3(a.groups, a.n, v.tiles), 256, 0, st>>>(a, v);
   }
 }
 
@@ -1209,8 +1305,17 @@ void backward(const kad_group_norm_args& a, hipStream_t st) {
     else threads > 512 ? launch_backward<T, false, 1024>(a, first, o, threads, st) : launch_backward<T, false, 512>(a, first, o, threads, st);
     return;
   }
-  if (a.out) group_norm_wide_dx_kernel<T><<<dim3(a.groups, a.n), 256, 0, st>>>(a);
-  if (a.dweight || a.dbias) group_norm_wide_param_kernel<T><<<dim3(a.c), 256, 0, st>>>(a);
+  const Wide v = wide(a);
+  const dim3 grid(a.groups, a.n, v.tiles);
+  group_norm_wide_sums_kernel<T><<<grid, 256, 0, st>>>(a, v);
+  if (a.out) group_norm_wide_dx_kernel<T><<<grid, 256, 0, st>>>(a, v);
+  if (a.dweight || a.dbias) {
+    o = Geo{};
+    o.q = a.groups;
+    o.W = a.c;
+    o.parts = v.tiles;
+    group_norm_wide_param_kernel<<<dim3(ceil_div(a.c, PARAM_CHANNELS)), 256, 0, st>>>(a, o);
+  }
 }
 
 }  // namespace
@@ -1223,7 +1328,7 @@ extern "C" int64_t kad_group_norm_work_elems(const kad_group_norm_args* a, int b
   Geo o, first;
   int threads;
   if (!backward && resident(*a, o, threads)) return 0;
-  if (!split(*a, backward, first, o, threads)) return 0;
+  if (!split(*a, backward, first, o, threads)) return (int64_t)a->n * wide(*a).tiles * 2 * (a->groups + (backward ? a->c : 0));
   return (int64_t)a->n * o.parts * 2 * (o.q + (backward ? o.W : 0));
 }
 
