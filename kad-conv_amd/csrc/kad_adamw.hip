@@ -2,13 +2,13 @@
 //
 //   m <- b1 m + (1 - b1) g     v <- b2 v + (1 - b2) g^2     p <- decay p - rate m / (sqrt(v) inv_root + eps)
 //
-// Every value is read and written once, so bytes bound it: 28 a value for fp32 with 32-bit states, 12 with 8-bit
-// ones, where its 60 vector operations take as long.  What a network of thousands of small tensors costs beside that
+// Every value is read and written once, so bytes bound it: 28 a value for fp32 with 32-bit states, 16 with 8-bit
+// ones (bf16: 10, where 65 vector operations a value take as long).  What a network of thousands of small tensors costs beside that
 // is launches; a table of chunks in device memory makes it one.  A block takes a chunk (at most 4096 values of one
 // tensor), a wave 1024 values of it, all of whose loads are on their way at once (blocks that walk over chunks,
 // with the next one's entry fetched ahead, take a tenth longer, and a wave a chunk a fifth).
-//   64 M values, bf16 with masters, 32 bits: 312 us (5.7 TB/s); 8 bits, no masters: 123 us (5.2 TB/s);
-//   2944 tensors of 7 M values, fp32: 37 us and 27 us; 12 tensors of 150 000: 5 us.
+//   64 M values, bf16 with masters, 32 bits: 312 us (5.7 TB/s); 8 bits, no masters: 122 us (5.3 TB/s);
+//   2944 tensors of 7 M values, fp32: 37 us and 26 us; 12 tensors of 150 000: 4.6 us.
 // A copy of 1 GiB runs at 5.1 TB/s here.
 //
 // 8-bit states: 256 values are a segment with one scale.  A lane has 16 of them, so 16 lanes (a row, that DPP
