@@ -11,6 +11,8 @@
 #include <ATen/ops/zeros_like.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/hip/HIPCachingAllocator.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/FunctionsManual.h>
 #include <torch/csrc/autograd/function.h>
@@ -403,6 +405,7 @@ class AdamWTable {
     if (count)
       kad_adamw_chunks(at_.data(), grad_at.data(), numels_.data(), n, bytes, (kad_adamw_chunk*)host.mutable_data_ptr(), &elems);
     chunks_ = host.to(params_[0].device());
+    chunks_stream_ = c10::hip::getCurrentHIPStream(params_[0].device().index());
     args_.chunks = (const kad_adamw_chunk*)chunks_.const_data_ptr();
     args_.nchunks = count;
     args_.values = 0;
@@ -424,7 +427,14 @@ class AdamWTable {
     args_.eps = eps;
     args_.weight_decay = weight_decay;
     const c10::DeviceGuard guard(params_[0].device());
-    check(kad_adamw_step(&args_, stream_of(params_[0])), "kad_adamw_step");
+    const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream(params_[0].device().index());
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+      // a graph reads the table whenever it is replayed, also after another one has been laid out
+      if (captured_.empty() || !captured_.back().is_same(chunks_)) captured_.push_back(chunks_);
+    } else if (stream != chunks_stream_) {
+      c10::hip::HIPCachingAllocator::recordStream(chunks_.storage().data_ptr(), stream);
+    }
+    check(kad_adamw_step(&args_, (void*)stream.stream()), "kad_adamw_step");
     // the kernel wrote them: what is kept by a parameter's version (packed weights, saved tensors) is stale
     for (const Tensor& t : stepped_)
       if (!t.is_inference()) torch::autograd::impl::bump_version(t);
@@ -434,6 +444,8 @@ class AdamWTable {
   std::vector<int64_t> at_, numels_, offsets_, grad_at_;
   int64_t elems_ = 0;
   Tensor chunks_, scalars_;
+  std::vector<Tensor> captured_;
+  std::optional<c10::hip::HIPStream> chunks_stream_;
   kad_adamw_args args_{};
 };
 

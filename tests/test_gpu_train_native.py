@@ -206,3 +206,49 @@ def test_steps_of_more_than_the_last_cache_holds():
     assert torch.equal(p, torch.cat(q))
     for name in ('exp_avg', 'exp_avg_sq'):
         assert torch.equal(whole.state[name][:n], torch.cat([parts[0].state[name][:half], parts[1].state[name][:n - half]]))
+
+
+def test_captured_step_outlives_its_table():
+    """A step captured, an eager step by gradients elsewhere (which lays another table out), then replays."""
+    n = 5000
+    p, q = torch.nn.Parameter(torch.zeros(n, device=DEV)), torch.nn.Parameter(torch.zeros(n, device=DEV))
+    g = torch.randn(n, device=DEV)
+    opt, ref = kadconv.AdamW([p], lr=1e-2, capturable=True), kadconv.AdamW([q], lr=1e-2, capturable=True)
+    p.grad, q.grad = g, g
+    opt.step(), ref.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for k in range(3):
+        other = torch.randn(n, device=DEV)
+        p.grad, q.grad = other.clone(), other.clone()
+        opt.step(), ref.step()
+        junk = [torch.full((64,), -1, dtype=torch.int32, device=DEV) for _ in range(50)]   # of the size of a table
+        g.normal_()
+        q.grad = g
+        graph.replay()
+        ref.step()
+        torch.cuda.synchronize()
+        del junk
+        assert torch.equal(p, q), k
+
+
+def test_steps_on_another_stream():
+    """A plan made on one stream and stepped on another, its gradients changed at once."""
+    n = 3_000_000
+    p, q = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+    grads = [torch.randn(n, device=DEV) for _ in range(4)]
+    plan, ref = kadconv.AdamWPlan([p], [grads[0]]), kadconv.AdamWPlan([q], [grads[0]])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for t, g in enumerate(grads, 1):
+        plan.set_grads([g])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            plan.step(t, lr=1e-2)
+    torch.cuda.current_stream().wait_stream(side)
+    for t, g in enumerate(grads, 1):
+        ref.set_grads([g])
+        ref.step(t, lr=1e-2)
+    assert torch.equal(p, q)
