@@ -3,7 +3,7 @@
 // A group norm's forward and backward are a few microseconds on the GPU.  As a Python autograd function the
 // pair took 160 us of host time (its backward runs on the engine's thread, and each switch between the two
 // threads moves the interpreter's state from core to core); as an autograd node of C++ it does without the
-// interpreter.  Arguments are checked by the Python entry points, sizes by the kernels' own entry points.
+// interpreter.
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/ops/empty.h>
@@ -23,6 +23,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <string_view>
 #include <tuple>
 #include <unordered_set>
 #include <vector>
@@ -196,9 +197,30 @@ struct GroupNormActBackward : torch::autograd::Node {
   }
 };
 
-Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps, int act) {
+// The checks of kadconv.ops._group_norm_check, and the activation's number.
+int checked_act(const Tensor& x, int64_t groups, const Tensor& weight, const Tensor& bias, double eps,
+                const std::optional<std::string_view>& act) {
+  TORCH_CHECK_VALUE(x.dim() == 4, "input [N, C, H, W] expected");
+  const int64_t c = x.size(1);
+  TORCH_CHECK_VALUE(groups >= 1 && c >= 1 && c % groups == 0, groups, " groups do not divide ", c, " channels");
+  TORCH_CHECK_VALUE(!act || *act == "relu" || *act == "silu", "act '", act.value_or(""), "' is none of None, 'relu', 'silu'");
+  TORCH_CHECK_VALUE(eps >= 0, "eps must be >= 0");
+  for (const Tensor* p : {&weight, &bias}) {
+    if (!p->defined()) continue;
+    TORCH_CHECK_VALUE(p->dim() == 1 && p->size(0) == c, "weight and bias must have shape (", c, ",), got ", p->sizes());
+    TORCH_CHECK_VALUE(p->device() == x.device(), "input, weight and bias must be on one device");
+    TORCH_CHECK_TYPE(p->scalar_type() == at::kFloat || p->scalar_type() == x.scalar_type(), "weight and bias must be float32 or ",
+                     x.scalar_type(), ", got ", p->scalar_type());
+  }
+  TORCH_CHECK_TYPE(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(),
+                   "weight and bias must share a dtype");
+  return !act ? KAD_ACT_NONE : *act == "relu" ? KAD_ACT_RELU : KAD_ACT_SILU;
+}
+
+Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps,
+                      const std::optional<std::string_view>& act) {
   const Tensor w = defined(weight), b = defined(bias);
-  const Norm norm{groups, eps, act};
+  const Norm norm{groups, eps, checked_act(x, groups, w, b, eps, act)};
   std::shared_ptr<GroupNormActBackward> node;
   TORCH_CHECK_NOT_IMPLEMENTED(!(torch::autograd::isFwGradDefined(x) || torch::autograd::isFwGradDefined(w) ||
                                 torch::autograd::isFwGradDefined(b)),

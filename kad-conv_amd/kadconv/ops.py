@@ -270,9 +270,9 @@ def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, act=None
     GPU maps (fp32, fp16, bf16) run the gfx950 HIP kernels, forward and backward (once differentiable).
     They compute on channels-last maps, dense or a slice of a wider map's channels; another layout is
     copied to it first.  The result is dense channels-last.  CPU maps run the plain composition."""
+    if input.is_cuda and not torch.compiler.is_compiling():
+        return _ext.native().group_norm_act(input, num_groups, weight, bias, eps, act)  # with the same checks
     _group_norm_check(input, num_groups, weight, bias, eps, act)
-    if not input.is_cuda:
-        return _group_norm_act_cpu(input, num_groups, weight, bias, eps, act)
-    if torch.compiler.is_compiling():
+    if input.is_cuda:
         return torch.ops.kadconv.group_norm_act(input, num_groups, weight, bias, eps, act)[0]
-    return _ext.native().group_norm_act(input, num_groups, weight, bias, eps, _ACTS[act])
+    return _group_norm_act_cpu(input, num_groups, weight, bias, eps, act)

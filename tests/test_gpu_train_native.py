@@ -252,3 +252,20 @@ def test_steps_on_another_stream():
         ref.set_grads([g])
         ref.step(t, lr=1e-2)
     assert torch.equal(p, q)
+
+
+def test_group_norm_refusals_on_the_gpu():
+    """The GPU path's checks are those of the CPU path: the same errors for the same arguments."""
+    x = torch.randn(2, 12, 3, 3, device=DEV)
+    w = torch.ones(12, device=DEV)
+    cases = [((x[0], 3), ValueError, 'N, C, H, W'), ((x, 5), ValueError, 'divide'), ((x, 0), ValueError, 'divide'),
+             ((x, 3, None, None, 1e-5, 'gelu'), ValueError, 'act'), ((x, 3, torch.ones(11, device=DEV)), ValueError, 'shape'),
+             ((x, 3, torch.ones(1, 12, device=DEV)), ValueError, 'shape'), ((x, 3, w, None, -1.0), ValueError, 'eps'),
+             ((x, 3, w, None, float('nan')), ValueError, 'eps'), ((x, 3, w.half()), TypeError, 'float32'),
+             ((x.half(), 3, w.half(), w), TypeError, 'share'), ((x, 3, None, w.cpu()), ValueError, 'one device')]
+    for args, error, words in cases:
+        with pytest.raises(error, match=words):
+            kadconv.group_norm_act(*args)
+        if words != 'one device':
+            with pytest.raises(error, match=words):
+                kadconv.group_norm_act(*(a.cpu() if isinstance(a, torch.Tensor) else a for a in args))
