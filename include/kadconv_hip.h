@@ -630,7 +630,7 @@ typedef struct kad_adamw_scalars {
  * m and sqrt(v) as e4m3 codes, times one float of exp_avg_scale / exp_avg_sq_scale for each KAD_ADAMW_SEG. */
 typedef struct kad_adamw_args {
   const kad_adamw_chunk *chunks;  /* device memory */
-  void *exp_avg, *exp_avg_sq;
+  void *exp_avg, *exp_avg_sq;     /* 16-byte aligned, as master */
   float *exp_avg_scale, *exp_avg_sq_scale;  /* 8-bit states only */
   float *master;          /* fp32 parameters, laid out as the states, or NULL: param itself is updated */
   const float *grad_scale;          /* device, or NULL */

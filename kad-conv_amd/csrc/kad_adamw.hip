@@ -354,6 +354,8 @@ extern "C" int kad_adamw_step(const kad_adamw_args* a, void* stream) {
   if (a->nchunks == 0) return KAD_OK;
   KAD_CHECK_ARG(a->chunks && a->exp_avg && a->exp_avg_sq, "kad_adamw_step: null pointer");
   KAD_CHECK_ARG(a->state_bits == 32 || (a->exp_avg_scale && a->exp_avg_sq_scale), "kad_adamw_step: 8-bit states need scales");
+  KAD_CHECK_ARG((((uintptr_t)a->exp_avg | (uintptr_t)a->exp_avg_sq | (uintptr_t)a->master) & 15) == 0,
+                "kad_adamw_step: state buffers must begin at multiples of 16 bytes");
   KAD_CHECK_ARG(!a->master || a->dtype != KAD_F32, "kad_adamw_step: masters are for 16-bit parameters");
   KAD_CHECK_ARG(a->scalars || a->step >= 1, "kad_adamw_step: step must be at least 1");
   if (int rc = check_rates(a, "kad_adamw_step")) return rc;

@@ -190,7 +190,7 @@ __device__ __forceinline__ void join_runs(const E* val, int active, int lines, i
         acc = acc.join(f[0].join(f[1]).join(f[2].join(f[3])));
       }
     for (int m = 1; m < wide; m <<= 1) acc = acc.join(acc.from(m));
-    if (per > 64) {  // waves share a run: per is at most T / q, so this round is the only one
+    if (per > 64) {  // waves share a run: per is at most T / q, so one pass meets all runs
       __syncthreads();
       if ((l & 63) == 0) red[t >> 6] = acc;
       __syncthreads();

@@ -222,3 +222,19 @@ def test_structs_match_header(tmp_path):
     subprocess.run(['gcc', '-std=c11', '-I', os.path.join(ROOT, 'include'), str(src), '-o', str(exe)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
     assert got == expect
+
+
+@pytest.mark.parametrize('name', ['exp_avg', 'exp_avg_sq', 'master'])
+def test_adamw_c_alignment(name):
+    lib = _ext.load()
+    a = _ext.AdamwArgs()
+    a.chunks = a.exp_avg = a.exp_avg_sq = a.master = 256   # never dereferenced: rejected first
+    a.beta1, a.beta2, a.step, a.nchunks, a.dtype, a.state_bits = 0.9, 0.99, 1, 1, _ext.KAD_F16, 32
+    setattr(a, name, 264)
+    assert lib.kad_adamw_step(ctypes.byref(a), None) == -1 and b'16 bytes' in lib.kad_last_error()
+
+
+def test_group_norm_c_refuses_far_pixels():
+    lib = _ext.load()
+    for kw in (dict(x_cs=(1 << 20) + 8), dict(dy_cs=(1 << 20) + 8)):
+        assert lib.kad_group_norm_bwd(ctypes.byref(_gn_args(**kw)), None) == -1
