@@ -582,7 +582,7 @@ typedef struct kad_group_norm_args {
   float *work;            /* kad_group_norm_work_elems floats; need not be initialised, free after the call */
   int64_t x_cs, dy_cs;    /* elements from pixel to pixel (>= C, at most 2^20); more than C only where C is a
                              multiple of 16 bytes / sizeof(dtype) */
-  int n, c, groups, h, w; /* groups divides c */
+  int n, c, groups, h, w; /* groups divides c; n <= 65535, c <= 2^20, h w < 2^31, n groups <= 2^30 */
   float eps;
   int act;                /* KAD_ACT_NONE, KAD_ACT_RELU or KAD_ACT_SILU */
   int dtype, param_dtype; /* param_dtype: KAD_F32, or dtype */

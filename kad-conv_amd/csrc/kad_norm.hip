@@ -1224,6 +1224,8 @@ int check_args(const kad_group_norm_args* a, const char* what) {
                 "%s: sizes must be positive and groups divide c", what);
   KAD_CHECK_ARG(a->n <= 65535 && a->c <= (1 << 20) && (int64_t)a->h * a->w <= INT32_MAX,
                 "%s: at most 65535 images, 2^20 channels and 2^31 - 1 pixels", what);
+  // (image, group) pairs are numbered in 32 bits, up to 64 blocks past the last
+  KAD_CHECK_ARG((int64_t)a->n * a->groups <= (1 << 30), "%s: at most 2^30 groups in all images together", what);
   KAD_CHECK_ARG(a->act == KAD_ACT_NONE || a->act == KAD_ACT_RELU || a->act == KAD_ACT_SILU, "%s: unknown activation", what);
   KAD_CHECK_ARG(a->eps >= 0.f, "%s: eps must be >= 0", what);
   return KAD_OK;

@@ -124,6 +124,15 @@ def test_group_norm_c_refusals_of_one_direction():
         assert lib.kad_group_norm_bwd(ctypes.byref(big), None) == -1
 
 
+def test_group_norm_groups_are_numbered_in_32_bits():
+    lib = _ext.load()
+    for backward in (0, 1):
+        most = _gn_args(n=1 << 10, c=1 << 20, groups=1 << 20, h=1, w=1)
+        assert lib.kad_group_norm_work_elems(ctypes.byref(most), backward) >= 0
+        most.n += 1
+        assert lib.kad_group_norm_work_elems(ctypes.byref(most), backward) == -1
+
+
 def _table(host):
     n = host.numel() // ctypes.sizeof(_ext.AdamwChunk)
     return list((_ext.AdamwChunk * n).from_buffer_copy(bytes(host.numpy().tobytes())))
