@@ -1136,6 +1136,13 @@ void count_threads(Geo& o, int rows, int& threads) {
   o.tpc = pow2_at_most(threads / o.W, threads);
 }
 
+// Blocks go round the 8 XCDs by their number: those whose sets share 128-byte lines of a pixel are kept on one.
+dim3 resident_grid(const kad_group_norm_args& a, const Geo& o) {
+  const int line = 128 / (o.W * dtype_size(a.dtype)), share = line > 1 && o.sets % line == 0 ? line : 1;
+  const int64_t blocks = (int64_t)a.n * o.sets;
+  return dim3(8, share, (unsigned)((blocks + 8 * share - 1) / (8 * share)));
+}
+
 // The resident kernel's layout; false: the split kernels' case.
 bool resident(const kad_group_norm_args& a, Geo& o, int& threads) {
   const int V = 16 / dtype_size(a.dtype), D = a.c / a.groups;
@@ -1153,7 +1160,7 @@ bool resident(const kad_group_norm_args& a, Geo& o, int& threads) {
   if (rows * o.S > MOST_THREADS) return false;
   count_threads(o, rows, threads);
   o.sets = a.groups / q;
-  return true;
+  return resident_grid(a, o).z <= 65535;  // a grid's layers
 }
 
 // Cuts an image's rows into about `tiles` tiles.
@@ -1244,13 +1251,9 @@ int check_call(const kad_group_norm_args* a, bool backward, const char* what) {
 
 template <typename T, bool ONE>
 void launch_resident(const kad_group_norm_args& a, const Geo& o, int threads, hipStream_t st) {
-  // Blocks go round the 8 XCDs by their number: those whose sets share 128-byte lines of a pixel are kept on one.
-  const int line = 128 / (o.W * (int)sizeof(T)), share = line > 1 && o.sets % line == 0 ? line : 1;
-  const int64_t blocks = (int64_t)a.n * o.sets;
-  const dim3 grid(8, share, (unsigned)((blocks + 8 * share - 1) / (8 * share)));
   const size_t lds = threads * (ONE ? 1 : VEC<T>) * sizeof(Moments) + 2 * o.q * sizeof(float);
   allow_lds(group_norm_resident_kernel<T, ONE>, lds);
-  group_norm_resident_kernel<T, ONE><<<grid, threads, lds, st>>>(a, o);
+  group_norm_resident_kernel<T, ONE><<<resident_grid(a, o), threads, lds, st>>>(a, o);
 }
 
 template <typename T, bool ONE, int MOST>

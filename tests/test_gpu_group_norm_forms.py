@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from kadconv import ops
+from tests._norm_ref import EPS32, assert_within, reference
 from tests.test_gpu_group_norm import BF16, DEV, F16, F32, check, make, params
 
 pytestmark = pytest.mark.gpu
@@ -94,3 +95,23 @@ def test_values_past_a_slice_stay_out():
     grads = ops.group_norm_act_backward(x, x, 4, wt, bs, mean, rstd, 1e-5, 'silu')
     assert all(torch.isfinite(t).all() for t in (y, mean, rstd, *grads))
     assert torch.equal(wide.view(torch.int16), keep.view(torch.int16))
+
+
+def test_more_images_and_groups_than_a_grid_has_layers():
+    """65535 images of 128 groups: the first and the last images' results, their gradients the only ones."""
+    n, c, g, h, w = 65535, 1024, 128, 1, 2
+    wt, bs = params(c)
+    x, dy = make(6, c, h, w, F16, 11), make(6, c, h, w, F16, 12)
+    ends = torch.tensor([0, 1, 2, n - 3, n - 2, n - 1], device=DEV)
+
+    def among_many(t):
+        many = torch.zeros(n, h, w, c, dtype=F16, device=DEV).permute(0, 3, 1, 2)
+        many[ends] = t
+        return many
+
+    xs, dys = among_many(x), among_many(dy)
+    y, mean, rstd = ops.group_norm_act_forward(xs, g, wt, bs, 1e-5, 'silu')
+    dx, dw, db = ops.group_norm_act_backward(dys, xs, g, wt, bs, mean, rstd, 1e-5, 'silu')
+    want = reference(x, g, wt, bs, 1e-5, 'silu', dy)
+    for name, got in (('y', y[ends]), ('dx', dx[ends]), ('dw', dw), ('db', db)):
+        assert_within(got, want[name], want['tol_' + name] + EPS32 * want[name].abs(), name)

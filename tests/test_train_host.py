@@ -133,6 +133,15 @@ def test_group_norm_groups_are_numbered_in_32_bits():
         assert lib.kad_group_norm_work_elems(ctypes.byref(most), backward) == -1
 
 
+def test_group_norm_small_maps_of_many_images_fit_a_grid():
+    """More (image, set of groups) pairs than layers of a grid hold go to the kernels that take a batch by rows."""
+    lib = _ext.load()
+    few = _gn_args(n=65535, c=512, groups=64, h=2, w=2, x_cs=512, dy_cs=512)
+    many = _gn_args(n=65535, c=1024, groups=128, h=2, w=2, x_cs=1024, dy_cs=1024)
+    assert lib.kad_group_norm_work_elems(ctypes.byref(few), 0) == 0
+    assert lib.kad_group_norm_work_elems(ctypes.byref(many), 0) > 0
+
+
 def _table(host):
     n = host.numel() // ctypes.sizeof(_ext.AdamwChunk)
     return list((_ext.AdamwChunk * n).from_buffer_copy(bytes(host.numpy().tobytes())))
