@@ -74,6 +74,11 @@ Tensor channels_last_pixels(const Tensor& x, int64_t& cs) {
   return out;
 }
 
+// The kernels take each size as an int.
+void check_sizes(const Tensor& x) {
+  for (const int64_t d : x.sizes()) TORCH_CHECK_VALUE(d <= INT32_MAX, "sizes up to 2^31 - 1 expected, got ", x.sizes());
+}
+
 struct Norm {
   int64_t groups;
   double eps;
@@ -201,6 +206,7 @@ struct GroupNormActBackward : torch::autograd::Node {
 int checked_act(const Tensor& x, int64_t groups, const Tensor& weight, const Tensor& bias, double eps,
                 const std::optional<std::string_view>& act) {
   TORCH_CHECK_VALUE(x.dim() == 4, "input [N, C, H, W] expected");
+  check_sizes(x);
   const int64_t c = x.size(1);
   TORCH_CHECK_VALUE(groups >= 1 && c >= 1 && c % groups == 0, groups, " groups do not divide ", c, " channels");
   TORCH_CHECK_VALUE(!act || *act == "relu" || *act == "silu", "act '", act.value_or(""), "' is none of None, 'relu', 'silu'");
@@ -250,6 +256,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight, 
 
 std::tuple<Tensor, Tensor, Tensor> group_norm_act_forward(const Tensor& x, int64_t groups, const OptTensor& weight,
                                                           const OptTensor& bias, double eps, int act) {
+  check_sizes(x);
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard guard(x.device());
   const Tensor mean = floats(x, {x.size(0), groups}), rstd = floats(x, {x.size(0), groups});
@@ -262,6 +269,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> group_norm_act_backward(const Tensor
                                                                     const OptTensor& weight, const OptTensor& bias,
                                                                     const Tensor& mean, const Tensor& rstd, double eps, int act,
                                                                     bool need_x, bool need_weight, bool need_bias) {
+  check_sizes(x);
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard guard(x.device());
   for (const Tensor& t : {mean, rstd})

@@ -6,6 +6,7 @@ import torch
 from torch.utils.checkpoint import checkpoint
 
 import kadconv
+from kadconv import ops
 from tests import _adamw_ref as R
 
 pytestmark = pytest.mark.gpu
@@ -269,3 +270,15 @@ def test_group_norm_refusals_on_the_gpu():
         if words != 'one device':
             with pytest.raises(error, match=words):
                 kadconv.group_norm_act(*(a.cpu() if isinstance(a, torch.Tensor) else a for a in args))
+
+
+def test_sizes_past_an_int_are_refused():
+    """Before anything of such a size is allocated: the map is one value, expanded."""
+    x = torch.zeros(1, 1, 1, 1, dtype=torch.float16, device=DEV)
+    stat = torch.zeros(1, 1, device=DEV)
+    for big in (x.expand((1 << 32) + 1, 1, 1, 1), x.expand(1, 1, (1 << 32) + 1, 1), x.expand(1, 1 << 32, 1, 1)):
+        for call in (lambda: kadconv.group_norm_act(big, 1),
+                     lambda: ops.group_norm_act_forward(big, 1, None, None, 1e-5, None),
+                     lambda: ops.group_norm_act_backward(big, big, 1, None, None, stat, stat, 1e-5, None)):
+            with pytest.raises(ValueError, match='sizes'):
+                call()
