@@ -79,6 +79,26 @@ void check_sizes(const Tensor& x) {
   for (const int64_t d : x.sizes()) TORCH_CHECK_VALUE(d <= INT32_MAX, "sizes up to 2^31 - 1 expected, got ", x.sizes());
 }
 
+// What the kernels take as given of a map and its parameters: the checks of kadconv.ops._group_norm_check, and that
+// the map is on a GPU.
+void check_norm(const Tensor& x, int64_t groups, const Tensor& weight, const Tensor& bias, double eps) {
+  TORCH_CHECK_VALUE(x.dim() == 4, "input [N, C, H, W] expected");
+  check_sizes(x);
+  const int64_t c = x.size(1);
+  TORCH_CHECK_VALUE(groups >= 1 && c >= 1 && c % groups == 0, groups, " groups do not divide ", c, " channels");
+  TORCH_CHECK_VALUE(eps >= 0, "eps must be >= 0");
+  for (const Tensor* p : {&weight, &bias}) {
+    if (!p->defined()) continue;
+    TORCH_CHECK_VALUE(p->dim() == 1 && p->size(0) == c, "weight and bias must have shape (", c, ",), got ", p->sizes());
+    TORCH_CHECK_VALUE(p->device() == x.device(), "input, weight and bias must be on one device");
+    TORCH_CHECK_TYPE(p->scalar_type() == at::kFloat || p->scalar_type() == x.scalar_type(), "weight and bias must be float32 or ",
+                     x.scalar_type(), ", got ", p->scalar_type());
+  }
+  TORCH_CHECK_TYPE(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(),
+                   "weight and bias must share a dtype");
+  TORCH_CHECK_VALUE(x.is_cuda(), "a GPU map expected, got one on ", x.device());
+}
+
 struct Norm {
   int64_t groups;
   double eps;
@@ -202,31 +222,17 @@ struct GroupNormActBackward : torch::autograd::Node {
   }
 };
 
-// The checks of kadconv.ops._group_norm_check, and the activation's number.
-int checked_act(const Tensor& x, int64_t groups, const Tensor& weight, const Tensor& bias, double eps,
-                const std::optional<std::string_view>& act) {
-  TORCH_CHECK_VALUE(x.dim() == 4, "input [N, C, H, W] expected");
-  check_sizes(x);
-  const int64_t c = x.size(1);
-  TORCH_CHECK_VALUE(groups >= 1 && c >= 1 && c % groups == 0, groups, " groups do not divide ", c, " channels");
+// The activation's number, after its check.
+int checked_act(const std::optional<std::string_view>& act) {
   TORCH_CHECK_VALUE(!act || *act == "relu" || *act == "silu", "act '", act.value_or(""), "' is none of None, 'relu', 'silu'");
-  TORCH_CHECK_VALUE(eps >= 0, "eps must be >= 0");
-  for (const Tensor* p : {&weight, &bias}) {
-    if (!p->defined()) continue;
-    TORCH_CHECK_VALUE(p->dim() == 1 && p->size(0) == c, "weight and bias must have shape (", c, ",), got ", p->sizes());
-    TORCH_CHECK_VALUE(p->device() == x.device(), "input, weight and bias must be on one device");
-    TORCH_CHECK_TYPE(p->scalar_type() == at::kFloat || p->scalar_type() == x.scalar_type(), "weight and bias must be float32 or ",
-                     x.scalar_type(), ", got ", p->scalar_type());
-  }
-  TORCH_CHECK_TYPE(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(),
-                   "weight and bias must share a dtype");
   return !act ? KAD_ACT_NONE : *act == "relu" ? KAD_ACT_RELU : KAD_ACT_SILU;
 }
 
 Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps,
                       const std::optional<std::string_view>& act) {
   const Tensor w = defined(weight), b = defined(bias);
-  const Norm norm{groups, eps, checked_act(x, groups, w, b, eps, act)};
+  check_norm(x, groups, w, b, eps);
+  const Norm norm{groups, eps, checked_act(act)};
   std::shared_ptr<GroupNormActBackward> node;
   TORCH_CHECK_NOT_IMPLEMENTED(!(torch::autograd::isFwGradDefined(x) || torch::autograd::isFwGradDefined(w) ||
                                 torch::autograd::isFwGradDefined(b)),
@@ -256,11 +262,12 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight, 
 
 std::tuple<Tensor, Tensor, Tensor> group_norm_act_forward(const Tensor& x, int64_t groups, const OptTensor& weight,
                                                           const OptTensor& bias, double eps, int act) {
-  check_sizes(x);
+  const Tensor w = defined(weight), b = defined(bias);
+  check_norm(x, groups, w, b, eps);
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard guard(x.device());
   const Tensor mean = floats(x, {x.size(0), groups}), rstd = floats(x, {x.size(0), groups});
-  return {norm_forward(x, defined(weight), defined(bias), {groups, eps, act}, mean.mutable_data_ptr<float>(),
+  return {norm_forward(x, w, b, {groups, eps, act}, mean.mutable_data_ptr<float>(),
                        rstd.mutable_data_ptr<float>()),
           mean, rstd};
 }
@@ -269,7 +276,8 @@ std::tuple<OptTensor, OptTensor, OptTensor> group_norm_act_backward(const Tensor
                                                                     const OptTensor& weight, const OptTensor& bias,
                                                                     const Tensor& mean, const Tensor& rstd, double eps, int act,
                                                                     bool need_x, bool need_weight, bool need_bias) {
-  check_sizes(x);
+  const Tensor w = defined(weight), b = defined(bias);
+  check_norm(x, groups, w, b, eps);
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard guard(x.device());
   for (const Tensor& t : {mean, rstd})
@@ -278,7 +286,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> group_norm_act_backward(const Tensor
                       "mean and rstd must be the forward's");
   TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.device() == x.device(), "dy must have the map's shape and device");
   TORCH_CHECK_TYPE(dy.scalar_type() == x.scalar_type(), "dy must have the map's dtype");
-  auto [dx, dw, db] = norm_backward(dy, x, defined(weight), defined(bias), mean.const_data_ptr<float>(),
+  auto [dx, dw, db] = norm_backward(dy, x, w, b, mean.const_data_ptr<float>(),
                                     rstd.const_data_ptr<float>(), {groups, eps, act}, {need_x, need_weight, need_bias});
   const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
   return {opt(dx), opt(dw), opt(db)};

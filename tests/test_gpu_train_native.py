@@ -282,3 +282,18 @@ def test_sizes_past_an_int_are_refused():
                      lambda: ops.group_norm_act_backward(big, big, 1, None, None, stat, stat, 1e-5, None)):
             with pytest.raises(ValueError, match='sizes'):
                 call()
+
+
+def test_entries_check_weight_and_bias():
+    """Refused on the host by the functions below the autograd one, with nothing launched."""
+    x, w, b = (t.detach() for t in _case())
+    y, mean, rstd = ops.group_norm_act_forward(x, 3, w, b, 1e-5, 'silu')
+    for kw, error in ((dict(w=w[:23].contiguous()), ValueError), (dict(b=b.cpu()), ValueError), (dict(w=w.cpu()), ValueError),
+                      (dict(b=b.half()), TypeError), (dict(w=w.half(), b=b.half()), TypeError)):
+        p = {**dict(w=w, b=b), **kw}
+        with pytest.raises(error):
+            ops.group_norm_act_forward(x, 3, p['w'], p['b'], 1e-5, 'silu')
+        with pytest.raises(error):
+            ops.group_norm_act_backward(y, x, 3, p['w'], p['b'], mean, rstd, 1e-5, 'silu')
+        with pytest.raises(error):
+            torch.ops.kadconv.group_norm_act_backward(y, x, 3, p['w'], p['b'], mean, rstd, 1e-5, 'silu')

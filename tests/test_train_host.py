@@ -90,6 +90,32 @@ def test_group_norm_act_fake():
         assert dx.shape == x.shape and dw.shape == w.shape and db.numel() == 0
 
 
+@pytest.mark.parametrize('backward', [False, True], ids=['forward', 'backward'])
+def test_group_norm_entries_check_weight_and_bias(backward):
+    """The functions below the autograd one, and the gradient's operator: what they are given is checked before
+    anything is allocated or launched (here: before the map is found to be on the CPU)."""
+    x, stat = torch.zeros(2, 12, 3, 3, dtype=torch.float16), torch.zeros(2, 3)
+    ok = torch.ones(12)
+
+    def call(w, b, x=x, groups=3, eps=1e-5):
+        if backward:
+            kadconv.ops.group_norm_act_backward(x, x, groups, w, b, stat, stat, eps, 'silu')
+        else:
+            kadconv.ops.group_norm_act_forward(x, groups, w, b, eps, 'silu')
+    for w, b, error, words in ((torch.ones(11), None, ValueError, 'shape'), (ok, torch.ones(1, 12), ValueError, 'shape'),
+                               (None, torch.ones(13), ValueError, 'shape'), (ok, ok.half(), TypeError, 'share'),
+                               (ok.half(), ok, TypeError, 'share'), (ok.bfloat16(), None, TypeError, 'float32'),
+                               (ok.to('meta'), None, ValueError, 'one device'), (ok, ok, ValueError, 'GPU')):
+        with pytest.raises(error, match=words):
+            call(w, b)
+        if backward and words not in ('GPU', 'one device'):  # (a meta tensor goes to the operator's shapes)
+            with pytest.raises(error, match=words):
+                torch.ops.kadconv.group_norm_act_backward(x, x, 3, w, b, stat, stat, 1e-5, 'silu')
+    for kw, words in ((dict(x=x[0]), 'N, C, H, W'), (dict(groups=5), 'divide'), (dict(groups=0), 'divide'), (dict(eps=-1.0), 'eps')):
+        with pytest.raises(ValueError, match=words):
+            call(ok, ok, **kw)
+
+
 def _gn_args(**kw):
     a = _ext.GroupNormArgs()
     a.x = a.dy = a.out = a.mean = a.rstd = a.work = 256   # never dereferenced: rejected first
