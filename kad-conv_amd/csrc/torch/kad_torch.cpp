@@ -417,6 +417,8 @@ class AdamWTable {
   std::vector<int64_t> offsets() const { return offsets_; }
   std::vector<int64_t> numels() const { return numels_; }
   int64_t elems() const { return elems_; }
+  // Whether a graph holds a step's addresses.
+  bool captured() const { return !captured_.empty(); }
 
  private:
   static int64_t address(const Tensor& g) { return g.defined() && g.numel() ? (int64_t)g.const_data_ptr() : 0; }
@@ -500,7 +502,8 @@ PYBIND11_MODULE(_native, m) {
       .def_property_readonly("params", &AdamWTable::params)
       .def_property_readonly("offsets", &AdamWTable::offsets)
       .def_property_readonly("numels", &AdamWTable::numels)
-      .def_property_readonly("elems", &AdamWTable::elems);
+      .def_property_readonly("elems", &AdamWTable::elems)
+      .def_property_readonly("captured", &AdamWTable::captured);
   m.def("group_norm_act", &group_norm_act);
   m.def("group_norm_act_forward", &group_norm_act_forward);
   m.def("group_norm_act_backward", &group_norm_act_backward);

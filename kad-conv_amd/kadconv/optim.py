@@ -70,8 +70,16 @@ class AdamWPlan:
         self.device, self.state_elems = p0.device, self._table.elems
         self.set_grads(grads)
         self.state = self._new_state() if state is None else self._given_state(state)
-        self._table.set_state(*(self.state[n] for n in _NAMES[state_bits]), *(None, None) * (state_bits == 32),
-                              self.state.get('master'), state_bits, self.seed)
+        self._hand_over()
+
+    def _hand_over(self):
+        self._table.set_state(*(self.state[n] for n in _NAMES[self.state_bits]), *(None, None) * (self.state_bits == 32),
+                              self.state.get('master'), self.state_bits, self.seed)
+
+    def _reseed(self, seed):
+        if self.seed != int(seed) & 0xFFFFFFFF:
+            self.seed = int(seed) & 0xFFFFFFFF
+            self._hand_over()
 
     @functools.cached_property
     def params(self):
@@ -105,10 +113,20 @@ class AdamWPlan:
         for name, (n, dtype) in self._layout().items():
             state[name] = torch.zeros(n, dtype=torch.uint8 if dtype == torch.float8_e4m3fn else dtype,
                                       device=self.device).view(dtype)
+        self._copy_masters(state)
+        return state
+
+    def _copy_masters(self, state):
         if self.master_weights:
             for i, p in enumerate(self.params):
                 self.part(state['master'], i).copy_(p)
-        return state
+
+    def _start_over(self):
+        """The state of a plan that has not stepped, in the same buffers."""
+        for name, t in self.state.items():
+            if name != 'master':
+                t.view(torch.uint8 if t.dtype == torch.float8_e4m3fn else t.dtype).zero_()
+        self._copy_masters(self.state)
 
     def _given_state(self, state):
         layout = self._layout()
@@ -171,8 +189,12 @@ class AdamW(torch.optim.Optimizer):
         if isinstance(lr, torch.Tensor) and not capturable:
             raise ValueError('lr may be a GPU scalar only with capturable=True')
         self._plans = {}      # group -> [(plan, its parameters)]
+        self._retired = []    # plans that a captured graph may still write by
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights, seed=seed, capturable=capturable, step=0))
+
+    def _seed(self, gi, dtype):
+        return self.param_groups[gi]['seed'] + 2 * gi + (dtype == torch.float32)
 
     def _group_plans(self, gi):
         """[(plan, its parameters)] of group gi, one a dtype, made of all its parameters."""
@@ -186,7 +208,7 @@ class AdamW(torch.optim.Optimizer):
         for dtype, params in by_dtype.items():
             master = group['master_weights'] and dtype != torch.float32
             plan = AdamWPlan(params, [None] * len(params), state_bits=group['state_bits'], master_weights=master,
-                             seed=group['seed'] + 2 * gi + (dtype == torch.float32))
+                             seed=self._seed(gi, dtype))
             for i, p in enumerate(params):
                 mine = {name: (plan.scales if name.endswith('_scale') else plan.part)(buf, i)
                         for name, buf in plan.state.items()}
@@ -227,19 +249,45 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._plans = {}
+        self.__dict__.setdefault('_retired', [])
+
+    def _keep_plans(self, gi, plans):
+        """Takes up plans that were made for group gi before its options were loaded, if they are what these ask for."""
+        group = self.param_groups[gi]
+        followed = [p for _, params in plans for p in params]
+        if len(followed) != len(group['params']) or set(map(id, followed)) != set(map(id, group['params'])) or any(
+                plan.state_bits != group['state_bits'] or
+                plan.master_weights != bool(group['master_weights'] and params[0].dtype != torch.float32)
+                for plan, params in plans):
+            self._retired += [plan for plan, _ in plans if plan._table.captured]
+            return False
+        for plan, params in plans:
+            plan._reseed(self._seed(gi, params[0].dtype))
+        self._plans[gi] = plans
+        return True
 
     def load_state_dict(self, state_dict):
+        """As torch's.  Values are loaded into the buffers and the count of steps that this optimizer has, so that a
+        step captured into a graph goes on from them (with the rates, betas, eps and decay that it was captured
+        with).  Where the loaded options ask for other states (``state_bits``, ``master_weights``) these are made
+        anew, and a step has to be captured again."""
+        counts, states, plans = [group['step'] for group in self.param_groups], self.state, self._plans
         super().load_state_dict({'state': {}, 'param_groups': state_dict['param_groups']})
-        self._plans = {}
         saved = state_dict['state']
-        if not saved:
-            return
-        for gi, (group, old) in enumerate(zip(self.param_groups, state_dict['param_groups'])):
+        loads = []
+        for gi, (group, old, count) in enumerate(zip(self.param_groups, state_dict['param_groups'], counts)):
+            if isinstance(count, torch.Tensor) and group['capturable']:
+                group['step'] = count.copy_(torch.as_tensor(group['step']))
+            elif isinstance(group['step'], torch.Tensor):  # of the saved optimizer, or on another device
+                group['step'] = group['step'].to(device=group['params'][0].device, dtype=torch.int64, copy=True)
+            kept = gi in plans and self._keep_plans(gi, plans[gi])
+            if kept:
+                self.state.update((p, states[p]) for p in group['params'])
             if not any(k in saved for k in old['params']):
+                for plan, _ in plans[gi] if kept else ():
+                    plan._start_over()
                 continue
             self._group_plans(gi)
-            if isinstance(group['step'], torch.Tensor):  # of the saved optimizer, or on another device
-                group['step'] = group['step'].to(device=group['params'][0].device, dtype=torch.int64, copy=True)
             for p, k in zip(group['params'], old['params']):
                 if k not in saved:
                     raise ValueError('the state dict holds some of a group\'s states only')
@@ -252,5 +300,6 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError(f'{name}: {tuple(o.shape)} {o.dtype} in the state dict, {tuple(t.shape)} {t.dtype} here')
                     if group['state_bits'] == 8 and not _same_layout(o, t):
                         raise ValueError('8-bit states load into parameters of the same strides alone')
-                for name, t in mine.items():
-                    t.copy_(theirs[name])
+                    loads.append((t, o))
+        for t, o in loads:
+            t.copy_(o)

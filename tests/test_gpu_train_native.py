@@ -297,3 +297,87 @@ def test_entries_check_weight_and_bias():
             ops.group_norm_act_backward(y, x, 3, p['w'], p['b'], mean, rstd, 1e-5, 'silu')
         with pytest.raises(error):
             torch.ops.kadconv.group_norm_act_backward(y, x, 3, p['w'], p['b'], mean, rstd, 1e-5, 'silu')
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_captured_step_goes_on_from_a_loaded_state(bits):
+    """A step captured, a state loaded into the optimizer, replays: those of an optimizer that is not captured."""
+    dtype, gen = torch.bfloat16, torch.Generator().manual_seed(3)
+    sizes = (5000, 3, 256)
+    first = [torch.randn(n, generator=gen).to(DEV, dtype) for n in sizes]
+    a, b = ([torch.nn.Parameter(t.clone()) for t in first] for _ in range(2))
+    for p, q in zip(a, b):
+        p.grad, q.grad = torch.zeros_like(p), torch.zeros_like(q)
+    kw = dict(lr=1e-2, state_bits=bits, master_weights=True, seed=4)
+    oa, ob = kadconv.AdamW(a, capturable=True, **kw), kadconv.AdamW(b, **kw)
+
+    def grads():
+        for p, q in zip(a, b):
+            p.grad.copy_(torch.randn(p.shape, generator=gen))
+            q.grad.copy_(p.grad)
+
+    def same():
+        torch.cuda.synchronize()
+        assert oa.param_groups[0]['step'].item() == ob.param_groups[0]['step']
+        for p, q in zip(a, b):
+            # the graph computes its rates on the GPU: a bf16 parameter may be rounded the other way
+            torch.testing.assert_close(p, q, rtol=2.0 ** -8, atol=1e-9)
+            for name, t in oa.state[p].items():
+                torch.testing.assert_close(t.float(), ob.state[q][name].float(), rtol=1e-6, atol=1e-9)
+
+    grads()
+    oa.step(), ob.step()
+    saved = copy.deepcopy((oa.state_dict(), [p.detach().clone() for p in a]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        oa.step()
+    for _ in range(2):
+        grads()
+        graph.replay()
+        ob.step()
+    same()
+    where = {k: t.data_ptr() for k, t in oa.state[a[0]].items()}
+    state_dict, values = saved
+    with torch.no_grad():
+        for p, q, v in zip(a, b, values):
+            p.copy_(v), q.copy_(v)
+    oa.load_state_dict(state_dict)
+    state_dict['param_groups'][0].update(capturable=False, step=1)
+    ob.load_state_dict(state_dict)
+    assert where == {k: t.data_ptr() for k, t in oa.state[a[0]].items()}
+    same()
+    for _ in range(2):
+        grads()
+        graph.replay()
+        ob.step()
+    same()
+    # a state dict without states: as an optimizer that has not stepped
+    empty = dict(state={}, param_groups=copy.deepcopy(state_dict['param_groups']))
+    empty['param_groups'][0].update(capturable=True, step=0)
+    oa.load_state_dict(empty)
+    empty['param_groups'][0].update(capturable=False)
+    ob.load_state_dict(empty)
+    assert not any(t.float().any() for p in a for name, t in oa.state[p].items() if name != 'master')
+    for _ in range(2):
+        grads()
+        graph.replay()
+        ob.step()
+    same()
+
+
+def test_captured_step_outlives_a_load_that_replaces_it():
+    """Options loaded that ask for other states: the plan that a graph writes by stays, and eager steps go on."""
+    p = torch.nn.Parameter(torch.zeros(5000, device=DEV))
+    p.grad = torch.randn(5000, device=DEV)
+    opt, other = kadconv.AdamW([p], capturable=True), kadconv.AdamW([torch.nn.Parameter(torch.zeros(5000, device=DEV))], state_bits=8)
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    plan = opt._plans[0][0][0]
+    opt.load_state_dict(other.state_dict())
+    assert opt._retired == [plan] and opt.param_groups[0]['state_bits'] == 8
+    opt.step()
+    assert set(opt.state[p]) == {'exp_avg', 'exp_avg_scale', 'exp_avg_sq_root', 'exp_avg_sq_root_scale'}
