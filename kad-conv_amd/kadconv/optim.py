@@ -267,19 +267,26 @@ class AdamW(torch.optim.Optimizer):
         return True
 
     def load_state_dict(self, state_dict):
-        """As torch's.  Values are loaded into the buffers and the count of steps that this optimizer has, so that a
-        step captured into a graph goes on from them (with the rates, betas, eps and decay that it was captured
-        with).  Where the loaded options ask for other states (``state_bits``, ``master_weights``) these are made
+        """As torch's.  Values are loaded into the buffers, the count of steps and the GPU scalar ``lr`` that this
+        optimizer has, so that a step captured into a graph goes on from them (with the betas, eps, decay and, where
+        it is a number, the rate that it was captured with).  Where the loaded options ask for other states (``state_bits``, ``master_weights``) these are made
         anew, and a step has to be captured again."""
-        counts, states, plans = [group['step'] for group in self.param_groups], self.state, self._plans
+        before, states, plans = [(group['step'], group['lr']) for group in self.param_groups], self.state, self._plans
         super().load_state_dict({'state': {}, 'param_groups': state_dict['param_groups']})
         saved = state_dict['state']
         loads = []
-        for gi, (group, old, count) in enumerate(zip(self.param_groups, state_dict['param_groups'], counts)):
+        rates = {}  # what groups that share a rate's tensor load into it
+        for group, (_, lr) in zip(self.param_groups, before):
+            rates.setdefault(id(lr), set()).add(float(group['lr']))
+        for gi, (group, old, (count, lr)) in enumerate(zip(self.param_groups, state_dict['param_groups'], before)):
             if isinstance(count, torch.Tensor) and group['capturable']:
                 group['step'] = count.copy_(torch.as_tensor(group['step']))
             elif isinstance(group['step'], torch.Tensor):  # of the saved optimizer, or on another device
                 group['step'] = group['step'].to(device=group['params'][0].device, dtype=torch.int64, copy=True)
+            if isinstance(lr, torch.Tensor) and group['capturable'] and len(rates[id(lr)]) == 1:
+                group['lr'] = lr.copy_(torch.as_tensor(group['lr']))
+            elif isinstance(group['lr'], torch.Tensor):
+                group['lr'] = group['lr'].to(group['params'][0].device)
             kept = gi in plans and self._keep_plans(gi, plans[gi])
             if kept:
                 self.state.update((p, states[p]) for p in group['params'])

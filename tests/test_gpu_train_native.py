@@ -381,3 +381,34 @@ def test_captured_step_outlives_a_load_that_replaces_it():
     assert opt._retired == [plan] and opt.param_groups[0]['state_bits'] == 8
     opt.step()
     assert set(opt.state[p]) == {'exp_avg', 'exp_avg_scale', 'exp_avg_sq_root', 'exp_avg_sq_root_scale'}
+
+
+def test_loaded_rates_are_on_the_gpu():
+    """A rate that is a GPU scalar, from a state dict brought to host memory: into the optimizer's own scalar, which
+    a graph may read, and where two groups of one scalar load two rates, each into its own."""
+    p, q = (torch.nn.Parameter(torch.zeros(8, device=DEV)) for _ in range(2))
+    p.grad, q.grad = torch.ones(8, device=DEV), torch.ones(8, device=DEV)
+    lr = torch.tensor(1e-2, device=DEV)
+    opt = kadconv.AdamW([dict(params=[p]), dict(params=[q])], lr=lr, weight_decay=0.0, capturable=True)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    for group in saved['param_groups']:
+        group['lr'] = torch.tensor(0.25)
+        group['step'] = group['step'].cpu()
+    opt.load_state_dict(saved)
+    assert all(group['lr'] is lr for group in opt.param_groups) and lr.item() == 0.25
+    with torch.no_grad():
+        p.zero_(), q.zero_()
+    opt.step()
+    # a steady gradient's step is lr, up to eps and a few roundings
+    torch.testing.assert_close(p.detach(), torch.full_like(p, -0.25), rtol=1e-5, atol=0)
+    assert torch.equal(p, q)
+    saved['param_groups'][1]['lr'] = torch.tensor(0.5)
+    opt.load_state_dict(saved)
+    assert [group['lr'].item() for group in opt.param_groups] == [0.25, 0.5]
+    assert all(group['lr'].is_cuda for group in opt.param_groups)
+    opt.step()
+    fresh = kadconv.AdamW([dict(params=[p]), dict(params=[q])])
+    fresh.load_state_dict(saved)
+    assert all(group['lr'].is_cuda and group['step'].is_cuda for group in fresh.param_groups)
+    fresh.step()
