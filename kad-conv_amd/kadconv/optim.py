@@ -251,34 +251,33 @@ class AdamW(torch.optim.Optimizer):
         self._plans = {}
         self.__dict__.setdefault('_retired', [])
 
-    def _keep_plans(self, gi, plans):
-        """Takes up plans that were made for group gi before its options were loaded, if they are what these ask for."""
-        group = self.param_groups[gi]
+    @staticmethod
+    def _fit(group, plans):
+        """Whether plans that were made for a group are what its options ask for now."""
         followed = [p for _, params in plans for p in params]
-        if len(followed) != len(group['params']) or set(map(id, followed)) != set(map(id, group['params'])) or any(
-                plan.state_bits != group['state_bits'] or
-                plan.master_weights != bool(group['master_weights'] and params[0].dtype != torch.float32)
-                for plan, params in plans):
-            self._retired += [plan for plan, _ in plans if plan._table.captured]
-            return False
-        for plan, params in plans:
-            plan._reseed(self._seed(gi, params[0].dtype))
-        self._plans[gi] = plans
-        return True
+        return len(followed) == len(group['params']) and set(map(id, followed)) == set(map(id, group['params'])) and all(
+            plan.state_bits == group['state_bits'] and
+            plan.master_weights == bool(group['master_weights'] and params[0].dtype != torch.float32)
+            for plan, params in plans)
 
     def load_state_dict(self, state_dict):
         """As torch's.  Values are loaded into the buffers, the count of steps and the GPU scalar ``lr`` that this
         optimizer has, so that a step captured into a graph goes on from them (with the betas, eps, decay and, where
-        it is a number, the rate that it was captured with).  Where the loaded options ask for other states (``state_bits``, ``master_weights``) these are made
-        anew, and a step has to be captured again."""
-        before, states, plans = [(group['step'], group['lr']) for group in self.param_groups], self.state, self._plans
+        it is a number, the rate that it was captured with).  Where the loaded options ask for other states
+        (``state_bits``, ``master_weights``) these are made anew, and a step has to be captured again.  A state dict
+        that does not fit is refused, and leaves the optimizer as it is."""
+        groups, states, plans = self.param_groups, self.state, self._plans
         super().load_state_dict({'state': {}, 'param_groups': state_dict['param_groups']})
-        saved = state_dict['state']
-        loads = []
+        try:
+            loads = self._matched_states(state_dict, states, plans)
+        except Exception:  # refused: nothing has been written
+            self.param_groups, self.state, self._plans = groups, states, plans
+            raise
         rates = {}  # what groups that share a rate's tensor load into it
-        for group, (_, lr) in zip(self.param_groups, before):
-            rates.setdefault(id(lr), set()).add(float(group['lr']))
-        for gi, (group, old, (count, lr)) in enumerate(zip(self.param_groups, state_dict['param_groups'], before)):
+        for group, was in zip(self.param_groups, groups):
+            rates.setdefault(id(was['lr']), set()).add(float(group['lr']))
+        for gi, (group, was) in enumerate(zip(self.param_groups, groups)):
+            count, lr = was['step'], was['lr']
             if isinstance(count, torch.Tensor) and group['capturable']:
                 group['step'] = count.copy_(torch.as_tensor(group['step']))
             elif isinstance(group['step'], torch.Tensor):  # of the saved optimizer, or on another device
@@ -287,12 +286,26 @@ class AdamW(torch.optim.Optimizer):
                 group['lr'] = lr.copy_(torch.as_tensor(group['lr']))
             elif isinstance(group['lr'], torch.Tensor):
                 group['lr'] = group['lr'].to(group['params'][0].device)
-            kept = gi in plans and self._keep_plans(gi, plans[gi])
+            if gi in plans and self._plans.get(gi) is not plans[gi]:
+                self._retired += [plan for plan, _ in plans[gi] if plan._table.captured]
+            for plan, params in self._plans.get(gi, ()):
+                plan._reseed(self._seed(gi, params[0].dtype))
+        for load in loads:
+            load()
+
+    def _matched_states(self, state_dict, states, plans):
+        """The calls that load what a state dict holds, with plans and states for them: those that there were, where
+        they are what the loaded options ask for."""
+        saved, loads = state_dict['state'], []
+        for gi, (group, old) in enumerate(zip(self.param_groups, state_dict['param_groups'])):
+            if not set(self.defaults) <= set(old):
+                raise ValueError(f'the state dict\'s options lack {sorted(set(self.defaults) - set(old))}: of another optimizer?')
+            kept = gi in plans and self._fit(group, plans[gi])
             if kept:
+                self._plans[gi] = plans[gi]
                 self.state.update((p, states[p]) for p in group['params'])
             if not any(k in saved for k in old['params']):
-                for plan, _ in plans[gi] if kept else ():
-                    plan._start_over()
+                loads += [plan._start_over for plan, _ in plans[gi]] if kept else []
                 continue
             self._group_plans(gi)
             for p, k in zip(group['params'], old['params']):
@@ -307,6 +320,5 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError(f'{name}: {tuple(o.shape)} {o.dtype} in the state dict, {tuple(t.shape)} {t.dtype} here')
                     if group['state_bits'] == 8 and not _same_layout(o, t):
                         raise ValueError('8-bit states load into parameters of the same strides alone')
-                    loads.append((t, o))
-        for t, o in loads:
-            t.copy_(o)
+                    loads.append(functools.partial(t.copy_, o))
+        return loads

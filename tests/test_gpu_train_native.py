@@ -412,3 +412,28 @@ def test_loaded_rates_are_on_the_gpu():
     fresh.load_state_dict(saved)
     assert all(group['lr'].is_cuda and group['step'].is_cuda for group in fresh.param_groups)
     fresh.step()
+
+
+def test_refused_load_leaves_the_optimizer():
+    """A state dict whose second group does not fit: the error, and an optimizer that goes on as it was."""
+    def make():
+        gen = torch.Generator().manual_seed(6)
+        params = [torch.nn.Parameter(torch.randn(300, generator=gen).to(DEV)) for _ in range(2)]
+        for p in params:
+            p.grad = torch.randn(300, generator=gen).to(DEV)
+        opt = kadconv.AdamW([dict(params=params[:1]), dict(params=params[1:])], lr=1e-2)
+        opt.step()
+        return params, opt
+    (a, oa), (b, ob) = make(), make()
+    saved = copy.deepcopy(oa.state_dict())
+    for group in saved['param_groups']:
+        group.update(lr=0.5, step=40)
+    saved['state'][0]['exp_avg'].fill_(7)
+    saved['state'][1]['exp_avg'] = torch.zeros(299, device=DEV)
+    with pytest.raises(ValueError, match='exp_avg'):
+        oa.load_state_dict(saved)
+    assert [group['step'] for group in oa.param_groups] == [1, 1] and oa.param_groups[0]['lr'] == 1e-2
+    oa.step(), ob.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    for p, q in zip(a, b):
+        assert torch.equal(oa.state[p]['exp_avg'], ob.state[q]['exp_avg'])

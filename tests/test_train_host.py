@@ -246,6 +246,17 @@ def test_adamw_refusals():
         kadconv.AdamW([q]).step()
 
 
+def test_adamw_refuses_another_optimizers_state():
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.ones(4)
+    other = torch.optim.AdamW([p], lr=0.5)
+    other.step()
+    opt = kadconv.AdamW([p], lr=1e-2)
+    with pytest.raises(ValueError, match='another optimizer'):
+        opt.load_state_dict(other.state_dict())
+    assert opt.param_groups[0]['lr'] == 1e-2 and opt.param_groups[0]['step'] == 0 and not opt.state
+
+
 STRUCTS = {'kad_group_norm_args': _ext.GroupNormArgs, 'kad_adamw_args': _ext.AdamwArgs, 'kad_adamw_chunk': _ext.AdamwChunk}
 
 
