@@ -31,6 +31,9 @@ from . import _ext
 _NAMES = {32: ('exp_avg', 'exp_avg_sq'),
           8: ('exp_avg', 'exp_avg_sq_root', 'exp_avg_scale', 'exp_avg_sq_root_scale')}
 
+# Of a parameter group; torch's base class adds its own.
+_OPTIONS = {'lr', 'betas', 'eps', 'weight_decay', 'state_bits', 'master_weights', 'seed', 'capturable', 'step'}
+
 
 def _same_layout(a, b):
     return a.shape == b.shape and (a.stride() == b.stride() or all(
@@ -298,8 +301,8 @@ class AdamW(torch.optim.Optimizer):
         they are what the loaded options ask for."""
         saved, loads = state_dict['state'], []
         for gi, (group, old) in enumerate(zip(self.param_groups, state_dict['param_groups'])):
-            if not set(self.defaults) <= set(old):
-                raise ValueError(f'the state dict\'s options lack {sorted(set(self.defaults) - set(old))}: of another optimizer?')
+            if not _OPTIONS <= set(old):
+                raise ValueError(f'the state dict\'s options lack {sorted(_OPTIONS - set(old))}: of another optimizer?')
             kept = gi in plans and self._fit(group, plans[gi])
             if kept:
                 self._plans[gi] = plans[gi]
