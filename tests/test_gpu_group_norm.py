@@ -294,3 +294,25 @@ def test_refusals():
         xs = x.clone().requires_grad_(True)
         g, = torch.autograd.grad(kadconv.group_norm_act(xs, 2, wt, bs).square().sum(), xs, create_graph=True)
         g.sum().backward()
+
+
+@pytest.mark.parametrize('dtype', [F32, F16, BF16], ids=['f32', 'f16', 'bf16'])
+@pytest.mark.parametrize('at', [40.0, 400.0, 1020.0, 2.0 ** 25])
+@pytest.mark.parametrize('shape', [(2, 16, 4, 6, 5), (2, 16, 4, 61, 60), (1, 9000, 30, 2, 3)], ids=['small', 'split', 'wide'])
+def test_silu_far_from_zero(shape, at, dtype):
+    """Where e^-z is under half a step of 1, SiLU's slope 1 + z e^-z (1 + ...) is 1 in 32 bits, however large z: the
+    gradients are those without an activation, bit for bit.  Gradients dy that are small integers sum to db without
+    a rounding."""
+    n, c, g, h, w = shape
+    x, (wt, _) = make(n, c, h, w, dtype, 23), params(c)
+    wt = wt.clamp(0.2, 2.0)              # z within 10 of `at`: |xhat| of these sizes is under 5
+    bias = torch.full((c,), at, device=DEV)
+    gen = torch.Generator().manual_seed(24)
+    dy = torch.randint(-3, 4, (n, h, w, c), generator=gen).to(dtype).to(DEV).permute(0, 3, 1, 2)
+    grads = []
+    for act in ('silu', None):
+        leaves = [t.clone(memory_format=torch.preserve_format).requires_grad_(True) for t in (x, wt, bias)]
+        grads.append(torch.autograd.grad(kadconv.group_norm_act(leaves[0], g, *leaves[1:], act=act), leaves, dy))
+    assert torch.equal(grads[0][2].double(), dy.double().sum(dim=(0, 2, 3)))
+    for got, want, name in zip(*grads, ('dx', 'dw', 'db')):
+        assert torch.equal(got, want), name
