@@ -11,6 +11,7 @@
 #include <ATen/ops/zeros_like.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -20,6 +21,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -228,9 +230,20 @@ int checked_act(const std::optional<std::string_view>& act) {
   return !act ? KAD_ACT_NONE : *act == "relu" ? KAD_ACT_RELU : KAD_ACT_SILU;
 }
 
-Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps,
-                      const std::optional<std::string_view>& act) {
+// Whether calls are watched (a trace, a dispatch mode) or a tensor stands for another (fake, wrapped): the caller then
+// takes the registered operator, which such a program sees.  What is allocated and launched here, it would not.
+bool observed(std::initializer_list<const Tensor*> tensors) {
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::any_modes_set()) return true;
+  for (const Tensor* t : tensors)
+    if (t->defined() && (!t->has_storage() || t->key_set().has(c10::DispatchKey::Python))) return true;
+  return false;
+}
+
+// None where the call is observed.
+OptTensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps,
+                         const std::optional<std::string_view>& act) {
   const Tensor w = defined(weight), b = defined(bias);
+  if (observed({&x, &w, &b})) return std::nullopt;
   check_norm(x, groups, w, b, eps);
   const Norm norm{groups, eps, checked_act(act)};
   std::shared_ptr<GroupNormActBackward> node;

@@ -271,7 +271,9 @@ def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, act=None
     They compute on channels-last maps, dense or a slice of a wider map's channels; another layout is
     copied to it first.  The result is dense channels-last.  CPU maps run the plain composition."""
     if input.is_cuda and not torch.compiler.is_compiling():
-        return _ext.native().group_norm_act(input, num_groups, weight, bias, eps, act)  # with the same checks
+        y = _ext.native().group_norm_act(input, num_groups, weight, bias, eps, act)  # with the same checks
+        if y is not None:  # not traced, and no tensor a fake one
+            return y
     _group_norm_check(input, num_groups, weight, bias, eps, act)
     if input.is_cuda:
         return torch.ops.kadconv.group_norm_act(input, num_groups, weight, bias, eps, act)[0]

@@ -3,6 +3,9 @@ import copy
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 from torch.utils.checkpoint import checkpoint
 
 import kadconv
@@ -437,3 +440,47 @@ def test_refused_load_leaves_the_optimizer():
     assert all(torch.equal(p, q) for p, q in zip(a, b))
     for p, q in zip(a, b):
         assert torch.equal(oa.state[p]['exp_avg'], ob.state[q]['exp_avg'])
+
+
+class _Ops(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.seen.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize('grad', [False, True])
+def test_traced_call_is_in_the_trace(grad):
+    """A traced network computes on what it is given, not on the example."""
+    net = torch.nn.Sequential(kadconv.GroupNormAct(3, 24), torch.nn.Sigmoid()).to(DEV)
+    a, b = _case(0)[0].detach(), _case(1)[0].detach()
+    with torch.set_grad_enabled(grad):
+        traced = torch.jit.trace(net, a)
+        assert 'group_norm_act' in str(traced.inlined_graph)
+        for x in (a, b):
+            assert torch.equal(traced(x), net(x))
+        if grad:
+            b.requires_grad_(True)
+            assert torch.equal(*(torch.autograd.grad(f(b).square().sum(), b)[0] for f in (traced, net)))
+
+
+def test_dispatch_modes_see_the_call():
+    x, w, b = _case()
+    want = torch.autograd.grad(f(x, w, b).sum(), (x, w, b))
+    with _Ops() as mode:
+        got = torch.autograd.grad(f(x, w, b).sum(), (x, w, b))
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    assert 'kadconv.group_norm_act.default' in mode.seen and 'kadconv.group_norm_act_backward.default' in mode.seen
+    graph = make_fx(lambda t: f(t, w.detach(), b.detach()).relu())(x.detach())
+    other = _case(1)[0].detach()
+    assert torch.equal(graph(other), f(other, w.detach(), b.detach()).relu())
+
+
+def test_fake_maps_have_gradients():
+    with FakeTensorMode() as mode:
+        x, w, b = (mode.from_tensor(t) for t in _case())
+        grads = torch.autograd.grad(f(x, w, b).sum(), (x, w, b))
+    assert [g.shape for g in grads] == [t.shape for t in (x, w, b)]

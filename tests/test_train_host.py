@@ -90,6 +90,18 @@ def test_group_norm_act_fake():
         assert dx.shape == x.shape and dw.shape == w.shape and db.numel() == 0
 
 
+def test_group_norm_act_of_fake_gpu_maps():
+    """The public function on tensors without values, in their mode and outside of it: shapes, and nothing run."""
+    with FakeTensorMode():
+        x = torch.empty(2, 12, 5, 7, dtype=torch.float16, device='cuda').requires_grad_(True)
+        w = torch.empty(12, device='cuda', requires_grad=True)
+        y = kadconv.group_norm_act(x, 4, w, act='silu')
+        assert y.shape == x.shape and y.dtype == x.dtype and y.is_contiguous(memory_format=torch.channels_last)
+        with pytest.raises(ValueError, match='divide'):
+            kadconv.group_norm_act(x, 5, w)
+    assert type(kadconv.group_norm_act(x.detach(), 4)) is type(x)
+
+
 @pytest.mark.parametrize('backward', [False, True], ids=['forward', 'backward'])
 def test_group_norm_entries_check_weight_and_bias(backward):
     """The functions below the autograd one, and the gradient's operator: what they are given is checked before
