@@ -19,8 +19,9 @@ shapes instead of breaking the graph at an opaque Python call:
       in x's memory format.
   kadconv::group_norm_act(x, num_groups, weight?, bias?, eps, act?)
         -> (Tensor y, Tensor mean, Tensor rstd)
-      kadconv.ops.group_norm_act with the statistics its gradient uses; the
-      gradient is the operator kadconv::group_norm_act_backward.
+      kadconv.ops.group_norm_act with the statistics its gradient uses, which are
+      constants to autograd; the gradient is the operator
+      kadconv::group_norm_act_backward.
 
 The eager implementations run the HIP kernels; nothing here falls back to
 another implementation.
@@ -122,6 +123,7 @@ def _(dy, x, num_groups, weight, bias, mean, rstd, eps, act):
 
 def _group_norm_act_context(ctx, inputs, output):
     x, num_groups, weight, bias, eps, act = inputs
+    ctx.mark_non_differentiable(output[1], output[2])  # for the gradient's own use
     ctx.save_for_backward(x, weight, bias, output[1], output[2])
     ctx.rest = num_groups, eps, act
 

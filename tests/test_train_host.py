@@ -90,6 +90,19 @@ def test_group_norm_act_fake():
         assert dx.shape == x.shape and dw.shape == w.shape and db.numel() == 0
 
 
+def test_group_norm_statistics_have_no_gradient():
+    """mean and rstd of the operator are constants to autograd: a loss of them alone is refused, not taken for one of y."""
+    with FakeTensorMode():
+        x, w = torch.empty(2, 12, 5, 7).requires_grad_(True), torch.empty(12, requires_grad=True)
+        y, mean, rstd = torch.ops.kadconv.group_norm_act(x, 4, w, None, 1e-5, 'silu')
+        assert y.requires_grad and not mean.requires_grad and not rstd.requires_grad
+        for t in (mean, rstd):
+            with pytest.raises(RuntimeError, match='does not require grad'):
+                t.sum().backward()
+        dx, dw = torch.autograd.grad(y, (x, w), torch.empty_like(y))
+        assert dx.shape == x.shape and dw.shape == w.shape
+
+
 def test_group_norm_act_of_fake_gpu_maps():
     """The public function on tensors without values, in their mode and outside of it: shapes, and nothing run."""
     with FakeTensorMode():
