@@ -326,6 +326,7 @@ class AdamWTable {
                        "parameters must share a dtype and a device");
       TORCH_CHECK_VALUE(p.layout() == at::kStrided && p.is_non_overlapping_and_dense(),
                         "parameters must be dense: no gaps or overlaps in their memory");
+      given_.push_back(p);
       params_.push_back(p.detach());
       // views of one tensor share its version: it stands for all of them
       versioned_.push_back(p.is_view() ? Tensor(p._base()) : p);
@@ -377,6 +378,7 @@ class AdamWTable {
     at.reserve(params.size());
     for (size_t i = 0; i < params.size(); ++i) {
       const Tensor& p = params[i];
+      TORCH_CHECK(p.is_same(given_[i]), "a group's parameters are not those of the first step: make a new optimizer");
       // a parameter that moved (module.to) would be written at its old address
       TORCH_CHECK((int64_t)p.const_data_ptr() == at_[i] && p.strides() == params_[i].strides() && p.sizes() == params_[i].sizes(),
                   "a parameter has moved since the first step: make a new optimizer");
@@ -493,7 +495,7 @@ class AdamWTable {
       if (!t.is_inference()) torch::autograd::impl::bump_version(t);
   }
 
-  std::vector<Tensor> params_, versioned_, held_, stepped_, state_;
+  std::vector<Tensor> given_, params_, versioned_, held_, stepped_, state_;
   std::vector<int64_t> at_, numels_, offsets_, grad_at_;
   int64_t elems_ = 0;
   Tensor chunks_, scalars_;

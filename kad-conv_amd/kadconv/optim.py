@@ -23,6 +23,7 @@ of (seed, step, place): the same call gives the same result.  A segment that
 meets an infinity or NaN holds NaN from then on, as a single value does in 32 bits.
 """
 import functools
+import operator
 
 import torch
 
@@ -191,7 +192,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f'state_bits must be 32 or 8, got {state_bits}')
         if isinstance(lr, torch.Tensor) and not capturable:
             raise ValueError('lr may be a GPU scalar only with capturable=True')
-        self._plans = {}      # group -> [(plan, its parameters)]
+        self._plans = {}      # group -> [(plan, its parameters, picks them from the group's)]
         self._retired = []    # plans that a captured graph may still write by
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights, seed=seed, capturable=capturable, step=0))
@@ -200,15 +201,18 @@ class AdamW(torch.optim.Optimizer):
         return self.param_groups[gi]['seed'] + 2 * gi + (dtype == torch.float32)
 
     def _group_plans(self, gi):
-        """[(plan, its parameters)] of group gi, one a dtype, made of all its parameters."""
+        """``_plans`` of group gi, one a dtype, made of all its parameters."""
         if gi in self._plans:
             return self._plans[gi]
         group = self.param_groups[gi]
         by_dtype = {}
-        for p in group['params']:
-            by_dtype.setdefault(p.dtype, []).append(p)
+        for i, p in enumerate(group['params']):
+            by_dtype.setdefault(p.dtype, []).append(i)
         out = []
-        for dtype, params in by_dtype.items():
+        for dtype, at in by_dtype.items():
+            together = at[-1] - at[0] + 1 == len(at)
+            pick = operator.itemgetter(slice(at[0], at[-1] + 1)) if together else operator.itemgetter(*at)
+            params = list(pick(group['params']))
             master = group['master_weights'] and dtype != torch.float32
             plan = AdamWPlan(params, [None] * len(params), state_bits=group['state_bits'], master_weights=master,
                              seed=self._seed(gi, dtype))
@@ -218,7 +222,7 @@ class AdamW(torch.optim.Optimizer):
                 for name, t in self.state[p].items():  # of a copied or unpickled optimizer
                     mine[name].copy_(t)
                 self.state[p] = mine
-            out.append((plan, params))
+            out.append((plan, params, pick))
         self._plans[gi] = out
         return out
 
@@ -234,17 +238,17 @@ class AdamW(torch.optim.Optimizer):
             if not any(p.grad is not None for p in group['params']):
                 continue
             plans = self._group_plans(gi)
-            if sum(len(params) for _, params in plans) != len(group['params']):
+            if sum(len(params) for _, params, _ in plans) != len(group['params']):
                 raise RuntimeError('a group has gained or lost parameters since the first step: make a new optimizer')
-            for plan, params in plans:
-                plan._table.follow(params)
+            for plan, _, pick in plans:
+                plan._table.follow(pick(group['params']))
             if group['capturable']:
                 if not isinstance(group['step'], torch.Tensor):
                     group['step'] = torch.tensor(group['step'], dtype=torch.int64, device=plans[0][0].device)
                 group['step'].add_(1)
             else:
                 group['step'] += 1
-            for plan, _ in plans:
+            for plan, *_ in plans:
                 plan.step(group['step'], lr=group['lr'], betas=group['betas'], eps=group['eps'],
                           weight_decay=group['weight_decay'], grad_scale=grad_scale)
         return loss
@@ -257,11 +261,12 @@ class AdamW(torch.optim.Optimizer):
     @staticmethod
     def _fit(group, plans):
         """Whether plans that were made for a group are what its options ask for now."""
-        followed = [p for _, params in plans for p in params]
-        return len(followed) == len(group['params']) and set(map(id, followed)) == set(map(id, group['params'])) and all(
+        followed = [p for _, params, _ in plans for p in params]
+        picked = [p for *_, pick in plans for p in pick(group['params'])] if len(followed) == len(group['params']) else []
+        return len(picked) == len(followed) and all(map(operator.is_, picked, followed)) and all(
             plan.state_bits == group['state_bits'] and
             plan.master_weights == bool(group['master_weights'] and params[0].dtype != torch.float32)
-            for plan, params in plans)
+            for plan, params, _ in plans)
 
     def load_state_dict(self, state_dict):
         """As torch's.  Values are loaded into the buffers, the count of steps and the GPU scalar ``lr`` that this
@@ -290,8 +295,8 @@ class AdamW(torch.optim.Optimizer):
             elif isinstance(group['lr'], torch.Tensor):
                 group['lr'] = group['lr'].to(group['params'][0].device)
             if gi in plans and self._plans.get(gi) is not plans[gi]:
-                self._retired += [plan for plan, _ in plans[gi] if plan._table.captured]
-            for plan, params in self._plans.get(gi, ()):
+                self._retired += [plan for plan, *_ in plans[gi] if plan._table.captured]
+            for plan, params, _ in self._plans.get(gi, ()):
                 plan._reseed(self._seed(gi, params[0].dtype))
         for load in loads:
             load()
@@ -308,7 +313,7 @@ class AdamW(torch.optim.Optimizer):
                 self._plans[gi] = plans[gi]
                 self.state.update((p, states[p]) for p in group['params'])
             if not any(k in saved for k in old['params']):
-                loads += [plan._start_over for plan, _ in plans[gi]] if kept else []
+                loads += [plan._start_over for plan, *_ in plans[gi]] if kept else []
                 continue
             self._group_plans(gi)
             for p, k in zip(group['params'], old['params']):

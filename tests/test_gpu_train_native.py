@@ -484,3 +484,46 @@ def test_fake_maps_have_gradients():
         x, w, b = (mode.from_tensor(t) for t in _case())
         grads = torch.autograd.grad(f(x, w, b).sum(), (x, w, b))
     assert [g.shape for g in grads] == [t.shape for t in (x, w, b)]
+
+
+def test_replaced_parameters_are_noticed():
+    """Another parameter in the same place, a group gone with another in its place, two that changed places: errors
+    that leave the parameters and the count of steps as they are."""
+    def param(dtype=torch.float32):
+        p = torch.nn.Parameter(torch.zeros(8, dtype=dtype, device=DEV))
+        p.grad = torch.ones_like(p)
+        return p
+
+    def refused(opt, params):
+        steps = [group['step'] for group in opt.param_groups]
+        before = [p.detach().clone() for p in params]
+        with pytest.raises(RuntimeError, match='new optimizer'):
+            opt.step()
+        assert steps == [group['step'] for group in opt.param_groups]
+        assert all(torch.equal(p, q) for p, q in zip(params, before))
+
+    p, new = param(), param()
+    opt = kadconv.AdamW([p])
+    opt.step()
+    opt.param_groups[0]['params'][0] = new
+    refused(opt, [p, new])
+    a, b, c = param(), param(), param()
+    opt = kadconv.AdamW([dict(params=[a]), dict(params=[b])])
+    opt.step()
+    opt.param_groups.pop(0)
+    refused(opt, [a, b])
+    opt = kadconv.AdamW([a, b])
+    opt.step()
+    opt.param_groups[0]['params'].reverse()
+    refused(opt, [a, b])
+    # several dtypes in a group: a plan each
+    h, i, new = param(torch.float16), param(torch.float16), param(torch.float16)
+    opt = kadconv.AdamW([a, h, b, i])
+    opt.step(), opt.step()
+    assert h.any() and torch.equal(h, i)
+    opt.param_groups[0]['params'][3] = new
+    refused(opt, [a, h, b, i, new])
+    opt = kadconv.AdamW([a, h, c])       # one of a dtype alone
+    opt.step(), opt.step()
+    opt.param_groups[0]['params'][1] = new
+    refused(opt, [a, h, c, new])
