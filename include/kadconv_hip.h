@@ -642,6 +642,8 @@ typedef struct kad_adamw_args {
   uint32_t seed;          /* of the 8-bit states' stochastic rounding */
   int dtype;              /* of param and grad */
   int state_bits;         /* 32 or 8 */
+  int follow;             /* with masters: a param that is not its master rounded (someone wrote it) replaces it first;
+                           * 0 saves reading param */
 } kad_adamw_args;
 
 int kad_adamw_step(const kad_adamw_args *a, void *stream);

@@ -114,10 +114,18 @@ struct Step {
   float beta1, beta2, keep1, keep2, eps;  // keep = 1 - beta, rounded from 64 bits
 };
 
+// What a step starts from in place of a master m whose parameter p someone else may have written: m while p is m
+// rounded, else p.
+template <typename T>
+__device__ __forceinline__ float followed(float m, float p) { return to_f32(from_f32<T>(m)) == p ? m : p; }
+
+// Where a step's 32-bit parameters come from.
+enum Source { PARAM, MASTER, FOLLOW };  // FOLLOW: the master, unless the parameter is another value
+
 constexpr int PIECE = 1024;  // values of a chunk that a wave takes at a time
 
 // 32-bit states: a lane takes 4 consecutive values of each of a piece's 4 segments, all on their way at once.
-template <typename T, bool MASTER, bool PAST>
+template <typename T, Source FROM, bool PAST>
 __global__ __launch_bounds__(256) void adamw32_kernel(Step a) {
   const kad_adamw_chunk ch = a.chunks[blockIdx.x];
   const kad_adamw_scalars s = a.scalars ? *a.scalars : a.values;
@@ -129,14 +137,15 @@ __global__ __launch_bounds__(256) void adamw32_kernel(Step a) {
   float* master = a.master + ch.offset;
   constexpr int ROWS = PIECE / SEG;
   for (int first = threadIdx.x / 64 * PIECE; first < ch.count; first += 4 * PIECE) {
-    float gv[ROWS][4], pv[ROWS][4], m[ROWS][4], v[ROWS][4];
+    float gv[ROWS][4], pv[ROWS][4], own[ROWS][4], m[ROWS][4], v[ROWS][4];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       const int i = first + r * SEG + (threadIdx.x & 63) * 4, left = ch.count - i;
       if (left <= 0) continue;
       load<4, PAST>(g + i, left, gv[r]);
-      if (MASTER) load<4, PAST>(master + i, 4, pv[r]);  // state buffers are whole segments
+      if (FROM != PARAM) load<4, PAST>(master + i, 4, pv[r]);  // state buffers are whole segments
       else load<4, PAST>(p + i, left, pv[r]);
+      if (FROM == FOLLOW) load<4, PAST>(p + i, left, own[r]);
       load<4, PAST>(exp_avg + i, 4, m[r]);
       load<4, PAST>(exp_avg_sq + i, 4, v[r]);
     }
@@ -150,6 +159,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(Step a) {
 #pragma clang fp contract(off)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
+          if (FROM == FOLLOW) pv[r][k] = followed<T>(pv[r][k], own[r][k]);
           const float gk = gv[r][k] * gs;
           m[r][k] = m[r][k] * a.beta1 + gk * a.keep1;
           v[r][k] = v[r][k] * a.beta2 + (gk * gk) * a.keep2;
@@ -158,7 +168,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(Step a) {
       }
       store<4, true>(exp_avg + i, 4, m[r]);
       store<4, true>(exp_avg_sq + i, 4, v[r]);
-      if (MASTER) store<4, true>(master + i, 4, pv[r]);
+      if (FROM != PARAM) store<4, true>(master + i, 4, pv[r]);
       store<4, true>(p + i, left, pv[r]);
     }
   }
@@ -211,7 +221,7 @@ __device__ __forceinline__ uint4 encode16(const float v[16], const uint32_t r[16
 }
 
 // 8-bit states: a lane takes 16 consecutive values, a row of 16 lanes a segment.
-template <typename T, bool MASTER>
+template <typename T, Source FROM>
 __global__ __launch_bounds__(256) void adamw8_kernel(Step a) {
   const kad_adamw_chunk ch = a.chunks[blockIdx.x];
   const kad_adamw_scalars s = a.scalars ? *a.scalars : a.values;
@@ -227,10 +237,11 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Step a) {
     T* p = (T*)ch.param + i;
     const uint4 mq = *mc, uq = *uc;
     float ms = a.exp_avg_scale[row], us = a.exp_avg_sq_scale[row];
-    float gv[16], pv[16], m[16], u[16];
+    float gv[16], pv[16], own[16], m[16], u[16];
     load<16>((const T*)ch.grad + i, left, gv);
-    if (MASTER) load<16>(a.master + pos, 16, pv);  // state buffers are whole segments
+    if (FROM != PARAM) load<16>(a.master + pos, 16, pv);  // state buffers are whole segments
     else load<16>(p, left, pv);
+    if (FROM == FOLLOW) load<16>(p, left, own);
     decode4(mq.x, ms, m);
     decode4(mq.y, ms, m + 4);
     decode4(mq.z, ms, m + 8);
@@ -247,6 +258,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Step a) {
 #pragma clang fp contract(off)
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
+        if (FROM == FOLLOW) pv[k] = followed<T>(pv[k], own[k]);
         const float gk = gv[k] * gs;
         m[k] = m[k] * a.beta1 + gk * a.keep1;
         u[k] = sqrtf((u[k] * u[k]) * a.beta2 + (gk * gk) * a.keep2);
@@ -254,7 +266,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Step a) {
       }
     }
     if (left > 0) {
-      if (MASTER) store<16>(a.master + pos, 16, pv);
+      if (FROM != PARAM) store<16>(a.master + pos, 16, pv);
       store<16>(p, left, pv);
     }
     if (left < 16) {
@@ -302,20 +314,20 @@ int check_rates(const kad_adamw_args* a, const char* what) {
   return KAD_OK;
 }
 
-template <typename T, bool MASTER>
+template <typename T, Source FROM>
 void launch(const kad_adamw_args& a, const Step& s, hipStream_t st) {
   const dim3 grid((unsigned)a.nchunks), block(256);
-  if (a.state_bits == 8) adamw8_kernel<T, MASTER><<<grid, block, 0, st>>>(s);
+  if (a.state_bits == 8) adamw8_kernel<T, FROM><<<grid, block, 0, st>>>(s);
   // What one step moves is met by the next, as far as the 256 MB cache before memory holds it; beyond, loads go past it
   // too (fp32: 8 M values 40 us against 43 so, 12 M 68 against 62, 32 M 172 against 159).
-  else if (a.values * 28 > (256 << 20)) adamw32_kernel<T, MASTER, true><<<grid, block, 0, st>>>(s);
-  else adamw32_kernel<T, MASTER, false><<<grid, block, 0, st>>>(s);
+  else if (a.values * 28 > (256 << 20)) adamw32_kernel<T, FROM, true><<<grid, block, 0, st>>>(s);
+  else adamw32_kernel<T, FROM, false><<<grid, block, 0, st>>>(s);
 }
 template <typename T>
 void launch(const kad_adamw_args& a, const Step& s, hipStream_t st) {
   if constexpr (sizeof(T) == 2)
-    if (a.master) return launch<T, true>(a, s, st);
-  launch<T, false>(a, s, st);
+    if (a.master) return a.follow ? launch<T, FOLLOW>(a, s, st) : launch<T, MASTER>(a, s, st);
+  launch<T, PARAM>(a, s, st);
 }
 
 }  // namespace

@@ -353,6 +353,14 @@ class AdamWTable {
     args_.master = (float*)mutable_pointer(state_[4]);
     args_.state_bits = state_bits;
     args_.seed = seed;
+    masters_match();
+  }
+
+  // The masters are what to go on from, whatever was done to the parameters before.
+  void masters_match() {
+    seen_.clear();
+    if (state_[4].defined())
+      for (const Tensor& t : versioned_) seen_.push_back(version(t));
   }
 
   // Steps by these gradients from now on, and keeps them.
@@ -438,6 +446,8 @@ class AdamWTable {
  private:
   static int64_t address(const Tensor& g) { return g.defined() && g.numel() ? (int64_t)g.const_data_ptr() : 0; }
 
+  static int64_t version(const Tensor& t) { return t.is_inference() ? 0 : (int64_t)t._version(); }
+
   static void check_grad(const Tensor& p, const Tensor& g) {
     TORCH_CHECK_VALUE(g.layout() == at::kStrided, "gradients must be dense tensors");
     TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type() && g.device() == p.device(), "a gradient is ", g.scalar_type(),
@@ -483,20 +493,29 @@ class AdamWTable {
     args_.weight_decay = weight_decay;
     const c10::DeviceGuard guard(params_[0].device());
     const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream(params_[0].device().index());
-    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+    const bool captured = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+    if (captured) {
       // a graph reads the table whenever it is replayed, also after another one has been laid out
       if (captured_.empty() || !captured_.back().is_same(chunks_)) captured_.push_back(chunks_);
     } else if (stream != chunks_stream_) {
       c10::hip::HIPCachingAllocator::recordStream(chunks_.storage().data_ptr(), stream);
     }
+    // A parameter written since its last step (its version tells) takes over from its master.  What will be written
+    // between replays of a graph is not known: its steps always look.
+    args_.follow = captured;
+    for (size_t i = 0; i < seen_.size() && !args_.follow; ++i) args_.follow = grad_at_[i] && version(versioned_[i]) != seen_[i];
     check(kad_adamw_step(&args_, (void*)stream.stream()), "kad_adamw_step");
     // the kernel wrote them: what is kept by a parameter's version (packed weights, saved tensors) is stale
     for (const Tensor& t : stepped_)
       if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+    if (!captured)
+      for (size_t i = 0; i < seen_.size(); ++i)
+        if (grad_at_[i]) seen_[i] = version(versioned_[i]);
   }
 
   std::vector<Tensor> given_, params_, versioned_, held_, stepped_, state_;
   std::vector<int64_t> at_, numels_, offsets_, grad_at_;
+  std::vector<int64_t> seen_;  // with masters: the parameters' versions after their last steps
   int64_t elems_ = 0;
   Tensor chunks_, scalars_;
   std::vector<Tensor> captured_;
@@ -510,6 +529,7 @@ PYBIND11_MODULE(_native, m) {
   py::class_<AdamWTable>(m, "AdamWTable")
       .def(py::init<const std::vector<Tensor>&>())
       .def("set_state", &AdamWTable::set_state)
+      .def("masters_match", &AdamWTable::masters_match)
       .def("set_grads", &AdamWTable::set_grads)
       .def("follow", &AdamWTable::follow)
       .def("step", &AdamWTable::step)

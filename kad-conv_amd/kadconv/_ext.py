@@ -123,7 +123,8 @@ class AdamwArgs(ctypes.Structure):
     _fields_ = [(f, c_vp) for f in ('chunks', 'exp_avg', 'exp_avg_sq', 'exp_avg_scale', 'exp_avg_sq_scale', 'master',
                                     'grad_scale', 'scalars')] + \
                [(f, ctypes.c_double) for f in ('lr', 'beta1', 'beta2', 'eps', 'weight_decay')] + \
-               [('step', c_i64), ('nchunks', c_i64), ('values', c_i64), ('seed', ctypes.c_uint32), ('dtype', c_int), ('state_bits', c_int)]
+               [('step', c_i64), ('nchunks', c_i64), ('values', c_i64), ('seed', ctypes.c_uint32), ('dtype', c_int), ('state_bits', c_int),
+                ('follow', c_int)]
 
 
 ADAMW_SEG = 256          # KAD_ADAMW_SEG

@@ -60,6 +60,10 @@ class AdamWPlan:
     them; ``state``: a dict of flat state buffers to use as they are, in place of new ones of zeros (and
     masters copied from the parameters); ``seed``: of the 8-bit states' stochastic rounding.
 
+    With masters, values of a parameter that were written since its last step (a state dict loaded, an average swapped
+    in, a clamp) take over from theirs.  A write that its version does not tell, through ``.data`` or to an inference
+    tensor, is taken up by captured steps alone.
+
     ``plan.state`` holds the buffers."""
 
     def __init__(self, params, grads, state_bits=32, master_weights=False, state=None, seed=0):
@@ -300,6 +304,9 @@ class AdamW(torch.optim.Optimizer):
                 plan._reseed(self._seed(gi, params[0].dtype))
         for load in loads:
             load()
+        for made in self._plans.values():
+            for plan, *_ in made:
+                plan._table.masters_match()
 
     def _matched_states(self, state_dict, states, plans):
         """The calls that load what a state dict holds, with plans and states for them: those that there were, where

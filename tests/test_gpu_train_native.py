@@ -527,3 +527,70 @@ def test_replaced_parameters_are_noticed():
     opt.step(), opt.step()
     opt.param_groups[0]['params'][1] = new
     refused(opt, [a, h, c, new])
+
+
+@pytest.mark.parametrize('views', [False, True])
+@pytest.mark.parametrize('captured', [False, True])
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('bits', [32, 8])
+def test_written_parameters_take_over_from_their_masters(bits, dtype, captured, views):
+    """Some values of a parameter written between steps: the step is that of a plan whose masters hold these values
+    there, and elsewhere (also where a value was written as it was) what they held."""
+    gen = torch.Generator().manual_seed(8)
+    sizes = (1000, 257, 5)
+    flat = torch.randn(1280 if views else 0, generator=gen).to(DEV, dtype)
+    at = (0, 1001, 1264)
+    params = [flat[a:a + n] if views else torch.randn(n, generator=gen).to(DEV, dtype) for a, n in zip(at, sizes)]
+    grads = [torch.randn(n, generator=gen).to(DEV, dtype) for n in sizes]
+    kw = dict(state_bits=bits, master_weights=True, seed=3)
+    plan = kadconv.AdamWPlan(params, grads, **kw)
+    t = torch.tensor(1, device=DEV)
+    plan.step(t, lr=1e-3)
+    if captured:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan.step(t, lr=1e-3)
+    for k in range(2, 5):
+        t.fill_(k)
+        params[0][100:300] = 0.5
+        params[0][500:600].clamp_(-0.2, 0.2)
+        params[1].mul_(1)
+        params[2][3] = float('inf') if k == 4 else -7.0
+        masters, values = plan.state['master'].clone(), [p.clone() for p in params]
+        for i, p in enumerate(params):
+            m = plan.part(masters, i)
+            m.copy_(torch.where(m.to(dtype) == p, m, p.float()))
+        assert (plan.state['master'] != masters).any() and (plan.state['master'] == masters).sum() > 1000
+        other = kadconv.AdamWPlan(values, grads, state=dict({n: s.clone() for n, s in plan.state.items()}, master=masters), **kw)
+        graph.replay() if captured else plan.step(t, lr=1e-3)
+        other.step(t, lr=1e-3)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(params, values)), k
+        for name, s in plan.state.items():
+            assert all(torch.equal(plan.part(s, i), other.part(other.state[name], i)) for i in range(3) if 'scale' not in name)
+
+
+def test_loaded_model_and_optimizer_in_either_order():
+    """Masters are more than the parameters tell: a model's and its optimizer's state dicts, loaded in either order
+    between steps, leave the masters' bits as they were saved."""
+    def make():
+        p = torch.nn.Parameter(torch.linspace(-1, 1, 300, device=DEV, dtype=torch.bfloat16))
+        p.grad = torch.linspace(1, 2, 300, device=DEV, dtype=torch.bfloat16)
+        opt = kadconv.AdamW([p], master_weights=True)
+        opt.step()
+        return p, opt
+    p, opt = make()
+    opt.step()
+    saved = copy.deepcopy((p.detach(), opt.state_dict()))
+    opt.step()
+    for first in ('model', 'optimizer'):
+        q, other = make()
+        for what in sorted(('model', 'optimizer'), key=lambda w: w != first):
+            if what == 'model':
+                with torch.no_grad():
+                    q.copy_(saved[0])
+            else:
+                other.load_state_dict(saved[1])
+        other.step()
+        assert torch.equal(q, p) and torch.equal(other.state[q]['master'], opt.state[p]['master']), first
