@@ -253,8 +253,8 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Step a) {
     {
       // Each product and sum is rounded by itself, as written: a held number depends on which side of a border its
       // value falls, so a program that computes this formula in 32 bits gets the same states, and a parameter is
-      // its master rounded.  The quotient goes into the parameter alone: the hardware's reciprocal (off by one
-      // step at most) costs a third of a division.
+      // its master rounded.  So is the quotient, where 32 bits of it are kept; a 16-bit parameter alone takes the
+      // hardware's reciprocal (off by one step of 32 bits at most, 2^-12 of its own), a third of a division.
 #pragma clang fp contract(off)
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
@@ -262,7 +262,8 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Step a) {
         const float gk = gv[k] * gs;
         m[k] = m[k] * a.beta1 + gk * a.keep1;
         u[k] = sqrtf((u[k] * u[k]) * a.beta2 + (gk * gk) * a.keep2);
-        pv[k] = pv[k] * s.decay - (s.rate * m[k]) * __builtin_amdgcn_rcpf(u[k] * s.inv_root + a.eps);
+        const float top = s.rate * m[k], below = u[k] * s.inv_root + a.eps;
+        pv[k] = pv[k] * s.decay - (FROM == PARAM && sizeof(T) == 2 ? top * __builtin_amdgcn_rcpf(below) : top / below);
       }
     }
     if (left > 0) {

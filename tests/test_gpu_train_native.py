@@ -1,6 +1,7 @@
 """What the autograd node and the optimizer's table in C++ have to keep of a torch program's rules."""
 import copy
 
+import numpy as np
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -594,3 +595,34 @@ def test_loaded_model_and_optimizer_in_either_order():
                 other.load_state_dict(saved[1])
         other.step()
         assert torch.equal(q, p) and torch.equal(other.state[q]['master'], opt.state[p]['master']), first
+
+
+@pytest.mark.parametrize('master', [False, True], ids=['f32', 'bf16_master'])
+@pytest.mark.parametrize('bits', [32, 8])
+def test_parameters_of_32_bits_are_those_of_the_formula_in_32_bits(bits, master):
+    """Parameters and masters in fp32 after a step, bit for bit as the CPU's operations round the formula, each
+    operation by itself: no fewer bits in the quotient, whatever holds the states."""
+    n, lr, (b1, b2), eps, wd = 256 * 512, 3e-3, (0.9, 0.999), 1e-8, 0.1
+    gen = torch.Generator().manual_seed(12)
+    dtype = torch.bfloat16 if master else torch.float32
+    start = torch.randn(n, generator=gen) * (torch.rand(n, generator=gen) < 0.5)   # half of them 0: the quotient alone
+    p = start.to(DEV, dtype)
+    g = torch.empty(n, dtype=dtype, device=DEV)
+    plan = kadconv.AdamWPlan([p], [g], state_bits=bits, master_weights=master)
+    for t in (1, 2, 3):
+        g.copy_(torch.randn(n, generator=gen) * torch.exp(3 * torch.randn(n, generator=gen)) * 1e-3)
+        st = {k: v.cpu() for k, v in plan.state.items()}
+        x, gc = (st['master'] if master else p.cpu()), g.float().cpu()
+        f32 = lambda v: torch.tensor(v, dtype=torch.float64).float()
+        if bits == 8:
+            m, u = (st[k].float() * st[k + '_scale'].repeat_interleave(256) for k in ('exp_avg', 'exp_avg_sq_root'))
+            v = u * u
+        else:
+            m, v = st['exp_avg'], st['exp_avg_sq']
+        m = m * f32(b1) + gc * f32(1 - b1)
+        v = v * f32(b2) + (gc * gc) * f32(1 - b2)
+        u = torch.from_numpy(np.sqrt(v.numpy()))   # rounded; torch's on the CPU is off by a step for one in six
+        want = x * f32(1 - lr * wd) - (f32(lr / (1 - b1 ** t)) * m) / (u * f32(1 / (1 - b2 ** t) ** 0.5) + f32(eps))
+        plan.step(t, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd)
+        got = plan.state['master'] if master else p
+        assert torch.equal(got.cpu(), want), (t, int((got.cpu() != want).sum()))
