@@ -101,6 +101,11 @@ void check_norm(const Tensor& x, int64_t groups, const Tensor& weight, const Ten
   TORCH_CHECK_VALUE(x.is_cuda(), "a GPU map expected, got one on ", x.device());
 }
 
+void check_gradient(const Tensor& dy, const Tensor& x) {
+  TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.device() == x.device(), "dy must have the map's shape and device");
+  TORCH_CHECK_TYPE(dy.scalar_type() == x.scalar_type(), "dy must have the map's dtype");
+}
+
 struct Norm {
   int64_t groups;
   double eps;
@@ -204,6 +209,9 @@ struct GroupNormActBackward : torch::autograd::Node {
     const Tensor& dy = grads[0];
     if (!dy.defined()) return out;
     const Tensor xs = x.unpack(), ws = weight.unpack(), bs = bias.unpack();
+    // a hook on saved tensors may have put others in their place
+    check_norm(xs, norm.groups, ws, bs, norm.eps);
+    check_gradient(dy, xs);
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::DeviceGuard guard(xs.device());
@@ -297,8 +305,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> group_norm_act_backward(const Tensor
     TORCH_CHECK_VALUE(t.is_contiguous() && t.scalar_type() == at::kFloat && t.device() == x.device() && t.dim() == 2 &&
                           t.size(0) == x.size(0) && t.size(1) == groups,
                       "mean and rstd must be the forward's");
-  TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.device() == x.device(), "dy must have the map's shape and device");
-  TORCH_CHECK_TYPE(dy.scalar_type() == x.scalar_type(), "dy must have the map's dtype");
+  check_gradient(dy, x);
   auto [dx, dw, db] = norm_backward(dy, x, w, b, mean.const_data_ptr<float>(),
                                     rstd.const_data_ptr<float>(), {groups, eps, act}, {need_x, need_weight, need_bias});
   const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };

@@ -626,3 +626,13 @@ def test_parameters_of_32_bits_are_those_of_the_formula_in_32_bits(bits, master)
         plan.step(t, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd)
         got = plan.state['master'] if master else p
         assert torch.equal(got.cpu(), want), (t, int((got.cpu() != want).sum()))
+
+
+@pytest.mark.parametrize('change', [lambda t: t.half(), lambda t: t.cpu(), lambda t: t[:1]], ids=['dtype', 'device', 'shape'])
+def test_saved_tensors_that_a_hook_replaced_are_checked(change):
+    """What unpacking gives is compared with the gradient before a kernel reads it as the map."""
+    x, w, b = _case()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        y = f(x, w, b)
+    with pytest.raises((TypeError, ValueError)):
+        torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
