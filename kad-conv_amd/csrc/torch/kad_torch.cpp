@@ -190,8 +190,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& dy, const Tensor&
 }
 
 struct GroupNormActBackward : torch::autograd::Node {
-  torch::autograd::SavedVariable x, weight, bias;
-  Tensor stats;
+  torch::autograd::SavedVariable x, weight, bias, stats;  // stats: means and reciprocal deviations [2, N, groups]
   Norm norm;
 
   std::string name() const override { return "GroupNormActBackward"; }
@@ -201,6 +200,7 @@ struct GroupNormActBackward : torch::autograd::Node {
     x.reset_data();
     weight.reset_data();
     bias.reset_data();
+    stats.reset_data();
   }
 
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
@@ -208,16 +208,19 @@ struct GroupNormActBackward : torch::autograd::Node {
     torch::autograd::variable_list out(3);
     const Tensor& dy = grads[0];
     if (!dy.defined()) return out;
-    const Tensor xs = x.unpack(), ws = weight.unpack(), bs = bias.unpack();
+    const Tensor xs = x.unpack(), ws = weight.unpack(), bs = bias.unpack(), st = stats.unpack();
     // a hook on saved tensors may have put others in their place
     check_norm(xs, norm.groups, ws, bs, norm.eps);
     check_gradient(dy, xs);
+    TORCH_CHECK_VALUE(st.is_contiguous() && st.scalar_type() == at::kFloat && st.device() == xs.device() &&
+                          st.sizes() == at::IntArrayRef({2, xs.size(0), norm.groups}),
+                      "the statistics must be the forward's");
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::DeviceGuard guard(xs.device());
-      const float* mean = stats.const_data_ptr<float>();
+      const float* mean = st.const_data_ptr<float>();
       std::tie(out[0], out[1], out[2]) =
-          norm_backward(dy, xs, ws, bs, mean, mean + stats.numel() / 2, norm,
+          norm_backward(dy, xs, ws, bs, mean, mean + st.numel() / 2, norm,
                         {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2)});
     }
     if (c10::GradMode::is_enabled() && torch::autograd::compute_requires_grad(dy, xs, ws, bs)) {
@@ -275,7 +278,7 @@ OptTensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weigh
     y = norm_forward(x, w, b, norm, mean, mean + x.size(0) * groups);
   }
   if (node) {
-    node->stats = stats;
+    node->stats = torch::autograd::SavedVariable(stats, false);
     torch::autograd::set_history(y, node);
   }
   return y;

@@ -636,3 +636,32 @@ def test_saved_tensors_that_a_hook_replaced_are_checked(change):
         y = f(x, w, b)
     with pytest.raises((TypeError, ValueError)):
         torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+
+
+def test_statistics_are_saved_as_the_map_is():
+    """Hooks see them, and they are freed with the rest of what a graph has saved."""
+    x, w, b = _case()
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.shape) or t, lambda t: t):
+        f(x, w, b)
+    assert sorted(map(tuple, seen)) == sorted([tuple(x.shape), (24,), (24,), (2, 2, 3)])
+
+    class Kept:
+        alive = 0
+
+        def __init__(self, t):
+            self.t = t
+            Kept.alive += 1
+
+        def __del__(self):
+            Kept.alive -= 1
+
+    with torch.autograd.graph.saved_tensors_hooks(Kept, lambda k: k.t):
+        y = f(x, w, b)
+    assert Kept.alive == 4
+    torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    assert Kept.alive == 0 and y.grad_fn is not None
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:1] if t.dim() == 3 else t):
+        y = f(x, w, b)
+    with pytest.raises(ValueError, match='statistics'):
+        torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
