@@ -356,6 +356,7 @@ class AdamWTable {
   void set_state(const Tensor& exp_avg, const Tensor& exp_avg_sq, const OptTensor& exp_avg_scale,
                  const OptTensor& exp_avg_sq_scale, const OptTensor& master, int state_bits, uint32_t seed) {
     state_ = {exp_avg, exp_avg_sq, defined(exp_avg_scale), defined(exp_avg_sq_scale), defined(master)};
+    if (!state_stream_) state_stream_ = stream();
     args_.exp_avg = exp_avg.mutable_data_ptr();
     args_.exp_avg_sq = exp_avg_sq.mutable_data_ptr();
     args_.exp_avg_scale = (float*)mutable_pointer(state_[2]);
@@ -431,8 +432,10 @@ class AdamWTable {
     const Tensor rate = defined(lr_at);
     if (rate.defined()) check_scalar("lr", rate, at::kFloat, "torch.float32");
     const c10::DeviceGuard guard(params_[0].device());
-    if (!scalars_.defined())
+    if (!scalars_.defined()) {
       scalars_ = at::empty({(int64_t)sizeof(kad_adamw_scalars)}, params_[0].options().dtype(at::kByte));
+      scalars_stream_ = stream();
+    }
     args_.step = 0;
     args_.lr = lr;
     args_.beta1 = beta1;
@@ -455,6 +458,8 @@ class AdamWTable {
 
  private:
   static int64_t address(const Tensor& g) { return g.defined() && g.numel() ? (int64_t)g.const_data_ptr() : 0; }
+
+  c10::hip::HIPStream stream() const { return c10::hip::getCurrentHIPStream(params_[0].device().index()); }
 
   static int64_t version(const Tensor& t) { return t.is_inference() ? 0 : (int64_t)t._version(); }
 
@@ -480,7 +485,7 @@ class AdamWTable {
     if (count)
       kad_adamw_chunks(at_.data(), grad_at.data(), numels_.data(), n, bytes, (kad_adamw_chunk*)host.mutable_data_ptr(), &elems);
     chunks_ = host.to(params_[0].device());
-    chunks_stream_ = c10::hip::getCurrentHIPStream(params_[0].device().index());
+    chunks_stream_ = stream();
     args_.chunks = (const kad_adamw_chunk*)chunks_.const_data_ptr();
     args_.nchunks = count;
     args_.values = 0;
@@ -502,19 +507,24 @@ class AdamWTable {
     args_.eps = eps;
     args_.weight_decay = weight_decay;
     const c10::DeviceGuard guard(params_[0].device());
-    const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream(params_[0].device().index());
+    const c10::hip::HIPStream st = stream();
     const bool captured = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
     if (captured) {
       // a graph reads the table whenever it is replayed, also after another one has been laid out
       if (captured_.empty() || !captured_.back().is_same(chunks_)) captured_.push_back(chunks_);
-    } else if (stream != chunks_stream_) {
-      c10::hip::HIPCachingAllocator::recordStream(chunks_.storage().data_ptr(), stream);
+    } else {  // what the table holds is not given to others, when it dies, before this stream is through with it
+      const auto used = [&](const Tensor& t, const std::optional<c10::hip::HIPStream>& own) {
+        if (t.defined() && own != st) c10::hip::HIPCachingAllocator::recordStream(t.storage().data_ptr(), st);
+      };
+      used(chunks_, chunks_stream_);
+      if (args_.scalars) used(scalars_, scalars_stream_);
+      for (const Tensor& t : state_) used(t, state_stream_);
     }
     // A parameter written since its last step (its version tells) takes over from its master.  What will be written
     // between replays of a graph is not known: its steps always look.
     args_.follow = captured;
     for (size_t i = 0; i < seen_.size() && !args_.follow; ++i) args_.follow = grad_at_[i] && version(versioned_[i]) != seen_[i];
-    check(kad_adamw_step(&args_, (void*)stream.stream()), "kad_adamw_step");
+    check(kad_adamw_step(&args_, (void*)st.stream()), "kad_adamw_step");
     // the kernel wrote them: what is kept by a parameter's version (packed weights, saved tensors) is stale
     for (const Tensor& t : stepped_)
       if (!t.is_inference()) torch::autograd::impl::bump_version(t);
@@ -529,7 +539,7 @@ class AdamWTable {
   int64_t elems_ = 0;
   Tensor chunks_, scalars_;
   std::vector<Tensor> captured_;
-  std::optional<c10::hip::HIPStream> chunks_stream_;
+  std::optional<c10::hip::HIPStream> chunks_stream_, scalars_stream_, state_stream_;  // that they were made on
   kad_adamw_args args_{};
 };
 

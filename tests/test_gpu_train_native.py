@@ -665,3 +665,27 @@ def test_statistics_are_saved_as_the_map_is():
         y = f(x, w, b)
     with pytest.raises(ValueError, match='statistics'):
         torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+
+
+def test_buffers_of_a_plan_outlive_their_kernels_on_another_stream():
+    """A plan stepped on a stream that is still busy, and dropped: its table, scalars and states (which were made on
+    the first stream) are not free yet, as the allocator counts them, and are once the stream is through."""
+    def held_back():  # blocks that are freed, but wait for a stream
+        stats = torch.cuda.memory_stats()
+        return stats['active.all.current'] - stats['allocation.all.current']
+
+    p, g = torch.zeros(5000, device=DEV), torch.ones(5000, device=DEV)
+    t = torch.tensor(1, device=DEV)
+    side = torch.cuda.Stream()
+    plan = kadconv.AdamWPlan([p], [g], state_bits=8)
+    plan.step(t)
+    torch.cuda.synchronize()
+    before = held_back()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        plan.step(t)
+    del plan
+    assert held_back() - before == 2 + 4
+    torch.cuda.synchronize()
+    torch.empty(1, device=DEV)  # the allocator looks at its events
+    assert held_back() == before
