@@ -47,18 +47,29 @@ def _compile(src, force):
 
 
 def _compile_native(force):
-    """The binding's object: host code only, against torch's headers."""
-    obj = os.path.join(OBJ, os.path.basename(NATIVE_SRC) + '.o')
-    newest = max(os.path.getmtime(f) for f in [NATIVE_SRC, *_deps()])
-    if not force and os.path.exists(obj) and os.path.getmtime(obj) >= newest:
-        return obj, None
+    """The binding's object: host code only, against torch's headers.  What it was built for is recorded beside it:
+    these headers' classes change from one version of torch to the next."""
+    import torch
     from torch.utils import cpp_extension
+    obj = os.path.join(OBJ, os.path.basename(NATIVE_SRC) + '.o')
     dirs = cpp_extension.include_paths() + ['/opt/rocm/include', sysconfig.get_paths()['include']]
     # the platform's name is what HIP's own headers ask for outside hipcc
     cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM', '-I', INCLUDE]
     cmd += [w for d in dirs for w in ('-isystem', d)] + ['-c', NATIVE_SRC, '-o', obj]
+    built_for = '\n'.join([f'torch {torch.__version__}', f'hip {torch.version.hip}', str(sysconfig.get_config_var('SOABI')),
+                           ' '.join(cmd)])
+    record = obj + '.for'
+    newest = max(os.path.getmtime(f) for f in [NATIVE_SRC, *_deps()])
+    if not force and os.path.exists(obj) and os.path.getmtime(obj) >= newest and os.path.exists(record):
+        with open(record) as f:
+            if f.read() == built_for:
+                return obj, None
     r = subprocess.run(cmd, capture_output=True, text=True)
-    return obj, f'{" ".join(cmd)}\n{r.stdout}\n{r.stderr}' if r.returncode else None
+    if r.returncode:
+        return obj, f'{" ".join(cmd)}\n{r.stdout}\n{r.stderr}'
+    with open(record, 'w') as f:
+        f.write(built_for)
+    return obj, None
 
 
 def _link_native(obj):

@@ -1,6 +1,7 @@
 """The training operators without a GPU: refusals, the CPU composition, the chunk table, the C ABI's checks
 and the layout of its structs."""
 import ctypes
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -318,3 +319,34 @@ def test_group_norm_c_refuses_far_pixels():
     lib = _ext.load()
     for kw in (dict(x_cs=(1 << 20) + 8), dict(dy_cs=(1 << 20) + 8)):
         assert lib.kad_group_norm_bwd(ctypes.byref(_gn_args(**kw)), None) == -1
+
+
+def test_binding_is_built_again_for_another_torch(tmp_path, monkeypatch):
+    """The object of the binding is used again for the same sources, torch, Python and command, and for no other."""
+    spec = importlib.util.spec_from_file_location('kad_build', os.path.join(ROOT, 'kad-conv_amd', 'build.py'))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    ran = []
+
+    def run(cmd, **_):
+        ran.append(cmd)
+        open(cmd[cmd.index('-o') + 1], 'w').close()
+        return subprocess.CompletedProcess(cmd, 0, '', '')
+
+    monkeypatch.setattr(build, 'OBJ', str(tmp_path))
+    monkeypatch.setattr(build.subprocess, 'run', run)
+
+    def compiles(n):
+        assert build._compile_native(False) == (str(tmp_path / 'kad_torch.cpp.o'), None)
+        assert len(ran) == n
+    compiles(1)
+    compiles(1)
+    monkeypatch.setattr(torch, '__version__', '9.0')
+    compiles(2)
+    compiles(2)
+    monkeypatch.setattr(torch.version, 'hip', '9.0')
+    compiles(3)
+    monkeypatch.setattr(build, 'INCLUDE', str(tmp_path / '..' / 'include'))
+    monkeypatch.setattr(build, '_deps', lambda: [])
+    compiles(4)
+    compiles(4)
