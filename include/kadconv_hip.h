@@ -610,7 +610,7 @@ typedef struct kad_adamw_chunk {
 
 /* Cuts n tensors (host arrays: addresses and numbers of values; tensors of 0 values are passed over) into
  * chunks, and lays their states out one after the other; a tensor whose gradient's address is 0 has its
- * place among the states but no chunk.  Returns the number of chunks and the length of
+ * place among the states but no chunk.  Other addresses are multiples of elem_bytes.  Returns the number of chunks and the length of
  * the state buffers in *state_elems; chunks (host memory) may be NULL: count only.  Host only. */
 int64_t kad_adamw_chunks(const int64_t *params, const int64_t *grads, const int64_t *numels, int n, int elem_bytes,
                          kad_adamw_chunk *chunks, int64_t *state_elems);

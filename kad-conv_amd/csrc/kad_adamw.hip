@@ -25,6 +25,7 @@ namespace kad {
 namespace {
 
 constexpr int SEG = KAD_ADAMW_SEG, CHUNK = KAD_ADAMW_CHUNK;
+constexpr int64_t MOST_VALUES = (int64_t)1 << 48;  // of a tensor and of a table: any number of bytes fits 64 bits
 constexpr float E4M3_MAX = 448.0f;
 // Largest magnitude of a segment below which it is held as zeros: its scale would no longer be a normal float.
 constexpr float SEG_TINY = 0x1p-110f;
@@ -342,7 +343,9 @@ extern "C" int64_t kad_adamw_chunks(const int64_t* params, const int64_t* grads,
   KAD_CHECK_ARG(n == 0 || (params && grads && numels), "kad_adamw_chunks: null pointer");
   int64_t count = 0, at = 0;
   for (int i = 0; i < n; ++i) {
-    KAD_CHECK_ARG(numels[i] >= 0 && numels[i] <= ((int64_t)1 << 48), "kad_adamw_chunks: bad number of values");
+    KAD_CHECK_ARG(numels[i] >= 0 && numels[i] <= MOST_VALUES, "kad_adamw_chunks: bad number of values");
+    KAD_CHECK_ARG(numels[i] == 0 || !grads[i] || (params[i] && (params[i] | grads[i]) % elem_bytes == 0),
+                  "kad_adamw_chunks: addresses must be multiples of the element's size, and params' not 0");
     for (int64_t k = 0; k < numels[i]; k += CHUNK, ++count) {
       if (!grads[i]) break;
       if (!chunks) continue;
@@ -354,6 +357,7 @@ extern "C" int64_t kad_adamw_chunks(const int64_t* params, const int64_t* grads,
       c.reserved = 0;
     }
     at += (numels[i] + SEG - 1) / SEG * SEG;
+    KAD_CHECK_ARG(at <= MOST_VALUES, "kad_adamw_chunks: too many values");
   }
   if (state_elems) *state_elems = at;
   return count;

@@ -235,6 +235,20 @@ def test_adamw_chunks_of_one_tensor_past_32_bits():
     assert lib.kad_adamw_chunks(*one, 1, 4, None, None) == -1
 
 
+def test_adamw_chunks_refuse_addresses_a_kernel_cannot_use():
+    """A table is read by the kernel as it is: no null or misaligned address gets into one, and no count that runs over."""
+    for params, grads, bytes_ in (([0], [4096], 4), ([4098], [8192], 4), ([4096], [8193], 2), ([4096, 2], [8192, 8196], 4)):
+        with pytest.raises(RuntimeError, match='addresses'):
+            _ext.adamw_chunks(params, grads, [5] * len(params), bytes_)
+    # without a gradient or without values there is no chunk
+    table, elems = _ext.adamw_chunks([0, 4096, 0], [0, 8192, 16], [5, 5, 0], 4)
+    assert len(_table(table)) == 1 and elems == 512
+    n = 3
+    most = [(ctypes.c_int64 * n)(*[v] * n) for v in (4096, 0, 1 << 47)]
+    assert _ext.load().kad_adamw_chunks(*most, 2, 4, None, None) == 0
+    assert _ext.load().kad_adamw_chunks(*most, n, 4, None, None) == -1 and b'too many' in _ext.load().kad_last_error()
+
+
 @pytest.mark.parametrize('kw', [dict(dtype=9), dict(state_bits=16), dict(chunks=None), dict(exp_avg=None), dict(step=0),
                                 dict(beta1=1.0), dict(beta2=-0.1), dict(eps=-1.0), dict(lr=float('nan')),
                                 dict(weight_decay=-1.0), dict(state_bits=8), dict(master=256, dtype=_ext.KAD_F32),
