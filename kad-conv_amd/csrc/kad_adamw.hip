@@ -123,11 +123,12 @@ __device__ __forceinline__ float followed(float m, float p) { return to_f32(from
 // Where a step's 32-bit parameters come from.
 enum Source { PARAM, MASTER, FOLLOW };  // FOLLOW: the master, unless the parameter is another value
 
+constexpr int THREADS = 256;
 constexpr int PIECE = 1024;  // values of a chunk that a wave takes at a time
 
 // 32-bit states: a lane takes 4 consecutive values of each of a piece's 4 segments, all on their way at once.
 template <typename T, Source FROM, bool PAST>
-__global__ __launch_bounds__(256) void adamw32_kernel(Step a) {
+__global__ __launch_bounds__(THREADS) void adamw32_kernel(Step a) {
   const kad_adamw_chunk ch = a.chunks[blockIdx.x];
   const kad_adamw_scalars s = a.scalars ? *a.scalars : a.values;
   const float gs = a.grad_scale ? *a.grad_scale : 1.0f;
@@ -223,7 +224,7 @@ __device__ __forceinline__ uint4 encode16(const float v[16], const uint32_t r[16
 
 // 8-bit states: a lane takes 16 consecutive values, a row of 16 lanes a segment.
 template <typename T, Source FROM>
-__global__ __launch_bounds__(256) void adamw8_kernel(Step a) {
+__global__ __launch_bounds__(THREADS) void adamw8_kernel(Step a) {
   const kad_adamw_chunk ch = a.chunks[blockIdx.x];
   const kad_adamw_scalars s = a.scalars ? *a.scalars : a.values;
   const float gs = a.grad_scale ? *a.grad_scale : 1.0f;
@@ -318,7 +319,7 @@ int check_rates(const kad_adamw_args* a, const char* what) {
 
 template <typename T, Source FROM>
 void launch(const kad_adamw_args& a, const Step& s, hipStream_t st) {
-  const dim3 grid((unsigned)a.nchunks), block(256);
+  const dim3 grid((unsigned)a.nchunks), block(THREADS);
   if (a.state_bits == 8) adamw8_kernel<T, FROM><<<grid, block, 0, st>>>(s);
   // What one step moves is met by the next, as far as the 256 MB cache before memory holds it; beyond, loads go past it
   // too (fp32: 8 M values 40 us against 43 so, 12 M 68 against 62, 32 M 172 against 159).
@@ -367,7 +368,8 @@ extern "C" int kad_adamw_step(const kad_adamw_args* a, void* stream) {
   KAD_CHECK_ARG(a, "kad_adamw_step: null pointer");
   KAD_CHECK_ARG(a->dtype == KAD_F32 || a->dtype == KAD_F16 || a->dtype == KAD_BF16, "kad_adamw_step: bad dtype");
   KAD_CHECK_ARG(a->state_bits == 32 || a->state_bits == 8, "kad_adamw_step: state_bits must be 32 or 8");
-  KAD_CHECK_ARG(a->nchunks >= 0 && a->nchunks < ((int64_t)1 << 31), "kad_adamw_step: too many chunks");
+  // a block a chunk, and a grid has fewer than 2^32 threads
+  KAD_CHECK_ARG(a->nchunks >= 0 && a->nchunks <= UINT32_MAX / THREADS, "kad_adamw_step: too many chunks");
   if (a->nchunks == 0) return KAD_OK;
   KAD_CHECK_ARG(a->chunks && a->exp_avg && a->exp_avg_sq, "kad_adamw_step: null pointer");
   KAD_CHECK_ARG(a->state_bits == 32 || (a->exp_avg_scale && a->exp_avg_sq_scale), "kad_adamw_step: 8-bit states need scales");

@@ -297,6 +297,15 @@ def test_adamw_refuses_another_optimizers_state():
     assert opt.param_groups[0]['lr'] == 1e-2 and opt.param_groups[0]['step'] == 0 and not opt.state
 
 
+@pytest.mark.parametrize('nchunks', [1 << 24, 1 << 40])
+def test_adamw_c_refuses_more_blocks_than_a_grid_holds(nchunks):
+    lib = _ext.load()
+    a = _ext.AdamwArgs()
+    a.chunks = a.exp_avg = a.exp_avg_sq = 256   # never dereferenced: rejected first
+    a.beta1, a.beta2, a.step, a.nchunks, a.dtype, a.state_bits = 0.9, 0.99, 1, nchunks, _ext.KAD_F16, 32
+    assert lib.kad_adamw_step(ctypes.byref(a), None) == -1 and b'too many chunks' in lib.kad_last_error()
+
+
 STRUCTS = {'kad_group_norm_args': _ext.GroupNormArgs, 'kad_adamw_args': _ext.AdamwArgs, 'kad_adamw_chunk': _ext.AdamwChunk}
 
 
