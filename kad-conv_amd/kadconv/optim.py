@@ -296,7 +296,7 @@ class AdamW(torch.optim.Optimizer):
                 group['step'] = group['step'].to(device=group['params'][0].device, dtype=torch.int64, copy=True)
             if isinstance(lr, torch.Tensor) and group['capturable'] and len(rates[id(lr)]) == 1:
                 group['lr'] = lr.copy_(torch.as_tensor(group['lr']))
-            elif isinstance(group['lr'], torch.Tensor):
+            elif isinstance(group['lr'], torch.Tensor) and group['params']:
                 group['lr'] = group['lr'].to(group['params'][0].device)
             if gi in plans and self._plans.get(gi) is not plans[gi]:
                 self._retired += [plan for plan, *_ in plans[gi] if plan._table.captured]

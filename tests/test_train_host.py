@@ -297,6 +297,15 @@ def test_adamw_refuses_another_optimizers_state():
     assert opt.param_groups[0]['lr'] == 1e-2 and opt.param_groups[0]['step'] == 0 and not opt.state
 
 
+def test_adamw_loads_a_group_without_parameters():
+    p = torch.nn.Parameter(torch.zeros(4))
+    for lr in (1e-2, torch.tensor(1e-2)):
+        a, b = (kadconv.AdamW([dict(params=[]), dict(params=[p])], lr=v, capturable=True) for v in (lr, 1e-3))
+        for opt in (a, b):
+            opt.load_state_dict(a.state_dict())
+            assert [float(group['lr']) for group in opt.param_groups] == [pytest.approx(1e-2)] * 2
+
+
 @pytest.mark.parametrize('nchunks', [1 << 24, 1 << 40])
 def test_adamw_c_refuses_more_blocks_than_a_grid_holds(nchunks):
     lib = _ext.load()
