@@ -139,12 +139,6 @@ struct Geo {
 // x / d for x in [0, 2^16), from 1 / d: an integer division is some forty instructions.
 __device__ __forceinline__ int over(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-  return v;
-}
-
 // Count, mean and squares about the mean of some values.
 struct Moments {
   float n, mean, m2;
