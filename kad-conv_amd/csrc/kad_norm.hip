@@ -15,7 +15,7 @@
 // 41 MB, [16, 256, 200, 200] bf16 205 and 331 us against 174 and 303).  Its stores pass the caches by, which leaves
 // x in them: a bare read and a bare copy of 41 MB take 23.3 us in two launches, 19.1 us with such stores (one copy
 // alone: 17.4, 12.5).
-// [8, 256, 100, 100] fp16 (41 MB): 25.0 us forward (statistics 9, result 16), backward 44 us (sums 21,
+// [8, 256, 100, 100] fp16 (41 MB): 25.2 us forward (statistics 9, result 16), backward 43 us (sums 21,
 // dx 22), where a bare read of x and dy takes 13.6 us, and their vector operations 11 and 12: what a block does
 // beside its rows (1 us of launch, 2 of places, weights and tiles joined, 1 of sums joined) is the rest.
 //
@@ -44,8 +44,10 @@ __device__ __forceinline__ void store_param(void* p, int i, int dtype, float v) 
   else ((bf16_t*)p)[i] = (bf16_t)v;
 }
 
-// 1 / (1 + e^-z): 0 where e^-z overflows.  For 16-bit maps with the hardware's reciprocal alone (off by one step of
-// 32 bits at most, 2^-12 of a step of theirs); for fp32 ones the quotient rounded.
+// 1 / (1 + e^-z): 0 where e^-z overflows.  For fp32 maps the quotient rounded.  For 16-bit ones the hardware's reciprocal
+// alone, off by one step of 32 bits at most: 2^-12 of a step of y and dx, and in a term of dw and db no more than its
+// other roundings.  Rounded, [16, 128, 200, 200] bf16 takes 90.2 and 144 us, with the reciprocal 88.0 and 137 (backward:
+// both launches); [8, 256, 100, 100] fp16 26.9 and 45.0, and 25.5 and 42.9.
 template <typename T>
 __device__ __forceinline__ float logistic(float z) {
   return sizeof(T) == 2 ? __builtin_amdgcn_rcpf(1.0f + __expf(-z)) : sigmoidf_(z);
@@ -1145,9 +1147,10 @@ bool resident(const kad_group_norm_args& a, Geo& o, int& threads) {
   if (a.groups % q) q = a.groups;
   if (!lay_out(a, q, o)) return false;
   // One launch, but a block's columns of D or few channels are pieces of lines that other blocks fetch too, and
-  // one CU reads them: up to 32 KB a block this beats the split kernels ([1, 64, 20, 20] fp16: 4.8 us against 8.1,
-  // [2, 48, 13, 17] fp32: 4.5 against 7.4, [16, 512, 25, 25] in 16 groups 13 against 15), at 64 KB most of it is
-  // lost (8 blocks: 11.1 against 8.9; 256 blocks: 13.8 against 17.0), at 256 KB they take half the time.
+  // one CU reads them.  One launch against the split kernels' two, in us: up to 32 KB a block 4.8 against 8.1
+  // ([1, 64, 20, 20] fp16), 4.5 against 7.4 ([2, 48, 13, 17] fp32), 13 against 15 ([16, 512, 25, 25] in 16 groups); at
+  // 64 KB 11.1 against 8.9 with 8 blocks, 13.8 against 17.0 with 256; at 256 KB twice theirs.  So the limit is where one
+  // launch wins whatever the number of blocks; what many blocks of 33 to 64 KB would gain by it is left.
   if ((int64_t)o.full * o.S * 16 > 32 * 1024) return false;
   int rows = ceil_div(o.full, MOST_RESIDENT);
   if (rows < ceil_div(64, o.S)) rows = ceil_div(64, o.S);

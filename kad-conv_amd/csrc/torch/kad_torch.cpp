@@ -2,8 +2,8 @@
 //
 // A group norm's forward and backward are a few microseconds on the GPU.  As a Python autograd function the
 // pair took 170 us of host time (its backward runs on the engine's thread, and each switch between the two
-// threads moves the interpreter's state from core to core); as an autograd node of C++ it takes 61, half of them
-// the engine's own.
+// threads moves the interpreter's state from core to core); as an autograd node of C++ it takes 61 to 64, half of
+// them the engine's own (and 36 in one of six runs).
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/ops/empty.h>
@@ -510,7 +510,8 @@ class AdamWTable {
     const c10::hip::HIPStream st = stream();
     const bool captured = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
     if (captured) {
-      // a graph reads the table whenever it is replayed, also after another one has been laid out
+      // a graph reads the table whenever it is replayed, also after another one has been laid out; when it dies is not
+      // known here, so a table (32 bytes a chunk) that was captured stays as long as this object
       if (captured_.empty() || !captured_.back().is_same(chunks_)) captured_.push_back(chunks_);
     } else {  // what the table holds is not given to others, when it dies, before this stream is through with it
       const auto used = [&](const Tensor& t, const std::optional<c10::hip::HIPStream>& own) {

@@ -233,7 +233,9 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, closure=None, grad_scale=None):
         """One step; ``grad_scale``: a float32 GPU scalar that gradients are multiplied by (a clipping or loss
-        scale's factor)."""
+        scale's factor).  A step by gradients that are not finite is not skipped: their parameters are lost, and
+        with 8-bit states the rest of their segments of 256 a step later.  A loop whose loss scale may be too large
+        looks at the gradients first, as torch.amp.GradScaler does."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
