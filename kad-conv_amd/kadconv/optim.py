@@ -197,7 +197,7 @@ class AdamW(torch.optim.Optimizer):
         if isinstance(lr, torch.Tensor) and not capturable:
             raise ValueError('lr may be a GPU scalar only with capturable=True')
         self._plans = {}      # group -> [(plan, its parameters, picks them from the group's)]
-        self._retired = []    # plans that a captured graph may still write by
+        self._retired, self._retired_scalars = [], []   # plans, and counts and rates, that a captured graph may still use
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights, seed=seed, capturable=capturable, step=0))
 
@@ -263,6 +263,7 @@ class AdamW(torch.optim.Optimizer):
         super().__setstate__(state)
         self._plans = {}
         self.__dict__.setdefault('_retired', [])
+        self.__dict__.setdefault('_retired_scalars', [])
 
     @staticmethod
     def _fit(group, plans):
@@ -278,7 +279,8 @@ class AdamW(torch.optim.Optimizer):
         """As torch's.  Values are loaded into the buffers, the count of steps and the GPU scalar ``lr`` that this
         optimizer has, so that a step captured into a graph goes on from them (with the betas, eps, decay and, where
         it is a number, the rate that it was captured with).  Where the loaded options ask for other states
-        (``state_bits``, ``master_weights``) these are made anew, and a step has to be captured again.  A state dict
+        (``state_bits``, ``master_weights``) or no GPU scalars (``capturable``) these are made anew, and a step has to
+        be captured again.  A state dict
         that does not fit is refused, and leaves the optimizer as it is."""
         groups, states, plans = self.param_groups, self.state, self._plans
         super().load_state_dict({'state': {}, 'param_groups': state_dict['param_groups']})
@@ -300,8 +302,12 @@ class AdamW(torch.optim.Optimizer):
                 group['lr'] = lr.copy_(torch.as_tensor(group['lr']))
             elif isinstance(group['lr'], torch.Tensor) and group['params']:
                 group['lr'] = group['lr'].to(group['params'][0].device)
-            if gi in plans and self._plans.get(gi) is not plans[gi]:
-                self._retired += [plan for plan, *_ in plans[gi] if plan._table.captured]
+            captured = [plan for plan, *_ in plans.get(gi, ()) if plan._table.captured]
+            if captured and self._plans.get(gi) is not plans[gi]:
+                self._retired += captured
+            if captured:
+                self._retired_scalars += [old for old, new in ((count, group['step']), (lr, group['lr']))
+                                          if isinstance(old, torch.Tensor) and old is not new]
             for plan, params, _ in self._plans.get(gi, ()):
                 plan._reseed(self._seed(gi, params[0].dtype))
         for load in loads:

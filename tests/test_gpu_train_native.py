@@ -689,3 +689,30 @@ def test_buffers_of_a_plan_outlive_their_kernels_on_another_stream():
     torch.cuda.synchronize()
     torch.empty(1, device=DEV)  # the allocator looks at its events
     assert held_back() == before
+
+
+def test_captured_scalars_outlive_a_load_that_replaces_them():
+    """Options loaded that count in Python, and rates that groups shared and share no more: what a graph reads and
+    writes stays allocated."""
+    p, q = (torch.nn.Parameter(torch.zeros(8, device=DEV)) for _ in range(2))
+    p.grad, q.grad = torch.ones(8, device=DEV), torch.ones(8, device=DEV)
+    lr = torch.tensor(1e-2, device=DEV)
+    opt = kadconv.AdamW([dict(params=[p]), dict(params=[q])], lr=lr, capturable=True)
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    counts = [group['step'] for group in opt.param_groups]
+    saved = copy.deepcopy(opt.state_dict())
+    for group, rate in zip(saved['param_groups'], (0.25, 0.5)):
+        group['lr'] = torch.tensor(rate)
+    opt.load_state_dict(saved)
+    assert [group['step'] for group in opt.param_groups] == counts
+    assert [t is lr for t in opt._retired_scalars] == [True, True]
+    for group in saved['param_groups']:
+        group.update(capturable=False, lr=1e-2, step=7)
+    opt.load_state_dict(saved)
+    assert all(any(t is c for t in opt._retired_scalars) for c in counts)
+    opt.step()
+    assert [group['step'] for group in opt.param_groups] == [8, 8]
