@@ -3,7 +3,7 @@
 // A group norm's forward and backward are a few microseconds on the GPU.  As a Python autograd function the
 // pair took 170 us of host time (its backward runs on the engine's thread, and each switch between the two
 // threads moves the interpreter's state from core to core); as an autograd node of C++ it takes 61 to 64, half of
-// them the engine's own (and 36 in one of six runs).
+// them the engine's own (and 36 in two of eight runs).
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/ops/empty.h>

@@ -716,3 +716,24 @@ def test_captured_scalars_outlive_a_load_that_replaces_them():
     assert all(any(t is c for t in opt._retired_scalars) for c in counts)
     opt.step()
     assert [group['step'] for group in opt.param_groups] == [8, 8]
+
+
+def test_masters_of_more_than_the_last_cache_holds():
+    """The same in one plan, whose loads go past the caches, and in two whose do not: masters, and written parameters."""
+    n, half = 12_000_007, 4096 * 1400
+    gen = torch.Generator(device=DEV).manual_seed(21)
+    p = torch.randn(n, generator=gen, device=DEV).bfloat16()
+    g = torch.randn(n, generator=gen, device=DEV).bfloat16()
+    q = [p[:half].clone(), p[half:].clone()]
+    whole = kadconv.AdamWPlan([p], [g], master_weights=True)
+    parts = [kadconv.AdamWPlan([v], [w.clone()], master_weights=True) for v, w in zip(q, (g[:half], g[half:]))]
+    for t in (1, 2, 3):
+        whole.step(t)
+        for plan in parts:
+            plan.step(t)
+        if t == 2:   # so that the third step compares
+            for v in (p, *q):
+                v.clamp_(-0.5, 0.5)
+    assert torch.equal(p, torch.cat(q)) and p.abs().max() < 0.51
+    for name in ('exp_avg', 'exp_avg_sq', 'master'):
+        assert torch.equal(whole.state[name][:n], torch.cat([parts[0].state[name][:half], parts[1].state[name][:n - half]])), name
