@@ -654,6 +654,32 @@ int kad_adamw_step(const kad_adamw_args *a, void *stream);
 int kad_adamw_hyper(const kad_adamw_args *a, const int64_t *step, const float *lr, kad_adamw_scalars *scalars,
                     void *stream);
 
+/* Layer norm of rows: y = weight (x - mean) rstd + bias, rstd = 1 / sqrt(var + eps), mean and (biased) var over the c
+ * values of a row. */
+typedef struct kad_layer_norm_args {
+  const void *x;          /* [rows][x_rs], dtype: values [0, c) of each row */
+  const void *dy;         /* backward: gradient of y, [rows][dy_rs], dtype */
+  void *out;              /* forward: y, backward: dx (or NULL: not wanted); dense [rows][c], dtype */
+  const void *weight;     /* [c], param_dtype, or NULL: ones */
+  const void *bias;       /* [c], param_dtype, or NULL: zeros; not read backward */
+  float *mean, *rstd;     /* [rows]: forward writes them (both NULL: not wanted), backward reads them */
+  void *dweight, *dbias;  /* backward: [c], param_dtype, or NULL: not wanted */
+  float *work;            /* backward: kad_layer_norm_work_elems floats; need not be initialised, free after the call */
+  int64_t rows;           /* 1 .. 2^40 */
+  int64_t x_rs, dy_rs;    /* elements from row to row (any, at least c; at most 2^31 - 1) */
+  int c;                  /* 1 .. KAD_LAYER_NORM_MOST */
+  float eps;
+  int dtype, param_dtype; /* param_dtype: KAD_F32, or dtype */
+} kad_layer_norm_args;
+
+#define KAD_LAYER_NORM_MOST 16384
+
+/* Floats of scratch that a backward call on these sizes needs, or KAD_EINVAL. */
+int64_t kad_layer_norm_work_elems(const kad_layer_norm_args *a);
+
+int kad_layer_norm_fwd(const kad_layer_norm_args *a, void *stream);
+int kad_layer_norm_bwd(const kad_layer_norm_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,22 +27,10 @@
 // Statistics.  A variance from sums of squares loses all digits where the mean is large, and a shift by the
 // first value does where that one is an outlier: a thread takes means and squares about them over a few
 // rows in registers and merges these (Chan's formula), so 32 bits suffice for any order of the values.
-#include "kad_common.h"
+#include "kad_vec.h"
 
 namespace kad {
 namespace {
-
-__device__ __forceinline__ float load_param(const void* p, int i, int dtype, float none) {
-  if (!p) return none;
-  if (dtype == KAD_F32) return ((const float*)p)[i];
-  if (dtype == KAD_F16) return (float)((const half_t*)p)[i];
-  return (float)((const bf16_t*)p)[i];
-}
-__device__ __forceinline__ void store_param(void* p, int i, int dtype, float v) {
-  if (dtype == KAD_F32) ((float*)p)[i] = v;
-  else if (dtype == KAD_F16) ((half_t*)p)[i] = (half_t)v;
-  else ((bf16_t*)p)[i] = (bf16_t)v;
-}
 
 // 1 / (1 + e^-z): 0 where e^-z overflows.  For fp32 maps the quotient rounded.  For 16-bit ones the hardware's reciprocal
 // alone, off by one step of 32 bits at most: 2^-12 of a step of y and dx, and in a term of dw and db no more than its
@@ -66,61 +54,6 @@ __device__ __forceinline__ float act_grad(float z, float dy) {
     return dy * (s + y * (1.0f - s));
   }
   return ACT == KAD_ACT_RELU ? (z > 0.f ? dy : 0.f) : dy;
-}
-
-template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
-// 16 bytes at a T's alignment.
-typedef int intx4_at2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef int intx4_at4 __attribute__((ext_vector_type(4), aligned(4)));
-template <typename T> struct Loose { typedef intx4_at2 type; };
-template <> struct Loose<float> { typedef intx4_at4 type; };
-template <typename T> using loose = typename Loose<T>::type;
-
-// 16 bytes at an address that need only be a T's (the memory unit takes wide accesses at any address).
-template <typename T>
-__device__ __forceinline__ intx4 load_vec(const T* p) {
-  intx4 r;
-  __builtin_memcpy(&r, p, 16);
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void unpack(intx4 r, float v[VEC<T>]) {
-  T t[VEC<T>];
-  __builtin_memcpy(t, &r, 16);
-#pragma unroll
-  for (int i = 0; i < VEC<T>; ++i) v[i] = to_f32(t[i]);
-}
-// Forgets what was computed from a held vector: otherwise its unpacked values stay in registers too.
-__device__ __forceinline__ void repack(intx4& r) { asm volatile("" : "+v"(r)); }
-template <typename T>
-__device__ __forceinline__ intx4 pack(const float v[VEC<T>]) {
-  T t[VEC<T>];
-#pragma unroll
-  for (int i = 0; i < VEC<T>; ++i) t[i] = from_f32<T>(v[i]);
-  intx4 r;
-  __builtin_memcpy(&r, t, 16);
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void store_vec(T* p, const float v[VEC<T>]) {
-  const intx4 r = pack<T>(v);
-  __builtin_memcpy(p, &r, 16);
-}
-// Past the caches.
-template <typename T>
-__device__ __forceinline__ void stream_vec(T* p, const float v[VEC<T>]) {
-  __builtin_nontemporal_store(pack<T>(v), (loose<T>*)p);
-}
-template <typename T>
-__device__ __forceinline__ void load_some(const T* p, int n, float v[VEC<T>]) {
-#pragma unroll
-  for (int i = 0; i < VEC<T>; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
-}
-template <typename T>
-__device__ __forceinline__ void store_some(T* p, int n, const float v[VEC<T>]) {
-#pragma unroll
-  for (int i = 0; i < VEC<T>; ++i)
-    if (i < n) p[i] = from_f32<T>(v[i]);
 }
 
 // How a block's columns (q groups of D channels, W in all) are cut into rows and vectors.

@@ -4,62 +4,9 @@
 // pair took 170 us of host time (its backward runs on the engine's thread, and each switch between the two
 // threads moves the interpreter's state from core to core); as an autograd node of C++ it takes 61 to 64, half of
 // them the engine's own (and 36 in two of eight runs).
-#include <ATen/core/Tensor.h>
-#include <ATen/hip/EmptyTensor.h>
-#include <ATen/ops/empty.h>
-#include <ATen/ops/empty_like.h>
-#include <ATen/ops/zeros_like.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/GradMode.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/hip/HIPCachingAllocator.h>
-#include <c10/hip/HIPGraphsC10Utils.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/FunctionsManual.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/autograd/variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/csrc/utils/pybind.h>
-
-#include <algorithm>
-#include <string_view>
-#include <tuple>
-#include <unordered_set>
-#include <vector>
-
-#include "kadconv_hip.h"
+#include "kad_torch.h"
 
 namespace {
-
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-
-void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", kad_last_error()); }
-
-void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-
-int dtype_of(const Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return KAD_F32;
-    case at::kHalf: return KAD_F16;
-    case at::kBFloat16: return KAD_BF16;
-    default: TORCH_CHECK_TYPE(false, "unsupported dtype ", t.scalar_type(), "; expected float32, float16 or bfloat16");
-  }
-}
-
-Tensor defined(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
-Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
-const void* pointer(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-void* mutable_pointer(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
-
-// A dense channels-last map of x's shape, dtype and device.
-Tensor map_like(const Tensor& x) {
-  const int64_t n = x.size(0), c = x.size(1), h = x.size(2), w = x.size(3);
-  return at::detail::empty_strided_cuda({n, c, h, w}, {h * w * c, 1, w * c, c}, x.scalar_type(), x.device());
-}
 
 // x [N, C, H, W] where it is channels-last, dense or a slice of the channels of a dense map; otherwise a dense
 // channels-last copy.  cs: elements from pixel to pixel.  A slice whose channels are not a multiple of 16 bytes
@@ -128,10 +75,6 @@ kad_group_norm_args norm_args(const Tensor& x, int64_t cs, const Tensor& weight,
   a.dtype = dtype_of(x);
   a.param_dtype = weight.defined() ? dtype_of(weight) : bias.defined() ? dtype_of(bias) : KAD_F32;
   return a;
-}
-
-Tensor floats(const Tensor& x, at::IntArrayRef sizes) {
-  return at::detail::empty_cuda(sizes, at::kFloat, x.device(), std::nullopt);
 }
 
 Tensor scratch(const kad_group_norm_args& a, int backward, const Tensor& x) {
@@ -239,15 +182,6 @@ struct GroupNormActBackward : torch::autograd::Node {
 int checked_act(const std::optional<std::string_view>& act) {
   TORCH_CHECK_VALUE(!act || *act == "relu" || *act == "silu", "act '", act.value_or(""), "' is none of None, 'relu', 'silu'");
   return !act ? KAD_ACT_NONE : *act == "relu" ? KAD_ACT_RELU : KAD_ACT_SILU;
-}
-
-// Whether calls are watched (a trace, a dispatch mode) or a tensor stands for another (fake, wrapped): the caller then
-// takes the registered operator, which such a program sees.  What is allocated and launched here, it would not.
-bool observed(std::initializer_list<const Tensor*> tensors) {
-  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::any_modes_set()) return true;
-  for (const Tensor* t : tensors)
-    if (t->defined() && (!t->has_storage() || t->key_set().has(c10::DispatchKey::Python))) return true;
-  return false;
 }
 
 // None where the call is observed.
@@ -563,4 +497,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("group_norm_act", &group_norm_act);
   m.def("group_norm_act_forward", &group_norm_act_forward);
   m.def("group_norm_act_backward", &group_norm_act_backward);
+  bind_rows(m);
 }

@@ -11,11 +11,12 @@ custom operators ``torch.ops.kadconv.deform_conv2d`` / ``layer_fwd`` /
 ``group_norm_act`` (kadconv.library).
 """
 from . import library  # registers the kadconv:: custom operators
-from .blocks import Conv1x1SiLU, GroupNormAct, KADDown, SqueezeExcitation
+from .blocks import Conv1x1SiLU, GroupNormAct, KADDown, LayerNorm, SqueezeExcitation
 from .fast import disable_fast_inference, enable_fast_inference
 from .kad_conv import DSC, LCSA, KADConv
-from .ops import deform_conv2d, group_norm_act
+from .ops import deform_conv2d, group_norm_act, layer_norm
 from .optim import AdamW, AdamWPlan
 
 __all__ = ['KADConv', 'DSC', 'LCSA', 'enable_fast_inference', 'disable_fast_inference', 'deform_conv2d',
-           'Conv1x1SiLU', 'SqueezeExcitation', 'KADDown', 'group_norm_act', 'GroupNormAct', 'AdamW', 'AdamWPlan']
+           'Conv1x1SiLU', 'SqueezeExcitation', 'KADDown', 'group_norm_act', 'GroupNormAct', 'AdamW', 'AdamWPlan',
+           'layer_norm', 'LayerNorm']

@@ -115,6 +115,12 @@ class GroupNormArgs(ctypes.Structure):
                [('eps', ctypes.c_float), ('act', c_int), ('dtype', c_int), ('param_dtype', c_int)]
 
 
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [(f, c_vp) for f in ('x', 'dy', 'out', 'weight', 'bias', 'mean', 'rstd', 'dweight', 'dbias', 'work')] + \
+               [(f, c_i64) for f in ('rows', 'x_rs', 'dy_rs')] + [('c', c_int), ('eps', ctypes.c_float), ('dtype', c_int),
+                                                                  ('param_dtype', c_int)]
+
+
 class AdamwChunk(ctypes.Structure):
     _fields_ = [('param', c_vp), ('grad', c_vp), ('offset', c_i64), ('count', c_int), ('reserved', c_int)]
 
@@ -128,6 +134,7 @@ class AdamwArgs(ctypes.Structure):
 
 
 ADAMW_SEG = 256          # KAD_ADAMW_SEG
+LAYER_NORM_MOST = 16384  # KAD_LAYER_NORM_MOST
 ADAMW_SCALARS = 4        # 4-byte words of kad_adamw_scalars
 
 
@@ -203,6 +210,9 @@ SIGNATURES = {
     'kad_group_norm_work_elems': (c_i64, [ctypes.POINTER(GroupNormArgs), c_int]),
     'kad_group_norm_fwd': (c_int, [ctypes.POINTER(GroupNormArgs), c_vp]),
     'kad_group_norm_bwd': (c_int, [ctypes.POINTER(GroupNormArgs), c_vp]),
+    'kad_layer_norm_work_elems': (c_i64, [ctypes.POINTER(LayerNormArgs)]),
+    'kad_layer_norm_fwd': (c_int, [ctypes.POINTER(LayerNormArgs), c_vp]),
+    'kad_layer_norm_bwd': (c_int, [ctypes.POINTER(LayerNormArgs), c_vp]),
     'kad_adamw_chunks': (c_i64, [c_vp, c_vp, c_vp, c_int, c_int, c_vp, ctypes.POINTER(c_i64)]),
     'kad_adamw_step': (c_int, [ctypes.POINTER(AdamwArgs), c_vp]),
     'kad_adamw_hyper': (c_int, [ctypes.POINTER(AdamwArgs), c_vp, c_vp, c_vp, c_vp]),

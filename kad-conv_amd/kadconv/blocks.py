@@ -14,10 +14,11 @@
   with up = bilinear (align_corners=False) to (H // 2, W // 2).
 * ``GroupNormAct`` -- group norm and an activation on channels-last maps, for
   layers trained at a batch too small for batch statistics.
+* ``LayerNorm`` -- layer norm of rows or of each pixel's channels.
 
 The first three: eval-mode GPU inputs run the HIP kernels (no fallback: a missing library
 raises); training mode or CPU inputs run the plain torch composition.
-``GroupNormAct`` runs them in training mode too: its kernels have a backward.
+``GroupNormAct`` and ``LayerNorm`` run them in training mode too: their kernels have a backward.
 """
 import torch
 import torch.nn as nn
@@ -167,3 +168,26 @@ class GroupNormAct(nn.Module):
 
     def extra_repr(self):
         return f'{self.num_groups}, {self.num_channels}, eps={self.eps}, affine={self.weight is not None}, act={self.act!r}'
+
+
+class LayerNorm(nn.Module):
+    """Layer norm of rows of ``num_channels`` values, along the last axis or, with ``dim=1``, of each pixel of a map
+    [N, C, H, W]; parameters as torch.nn.LayerNorm's, so its state dicts load."""
+
+    def __init__(self, num_channels, eps=1e-5, affine=True, dim=-1):
+        super().__init__()
+        if num_channels < 1:
+            raise ValueError(f'at least one channel expected, got {num_channels}')
+        if dim not in (-1, 1):
+            raise ValueError(f'dim must be -1 or 1, got {dim}')
+        self.num_channels, self.eps, self.dim = num_channels, eps, dim
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+
+    def forward(self, x):
+        if x.shape[self.dim] != self.num_channels:
+            raise ValueError(f'rows of {self.num_channels} values expected, got {tuple(x.shape)} along axis {self.dim}')
+        return ops.layer_norm(x, self.weight, self.bias, self.eps, self.dim)
+
+    def extra_repr(self):
+        return f'{self.num_channels}, eps={self.eps}, affine={self.weight is not None}, dim={self.dim}'

@@ -22,6 +22,8 @@ shapes instead of breaking the graph at an opaque Python call:
       kadconv.ops.group_norm_act with the statistics its gradient uses, which are
       constants to autograd; the gradient is the operator
       kadconv::group_norm_act_backward.
+  kadconv::layer_norm(x, weight?, bias?, eps, dim) -> (Tensor y, Tensor mean, Tensor rstd)
+      kadconv.ops.layer_norm, likewise, with kadconv::layer_norm_backward.
 
 The eager implementations run the HIP kernels; nothing here falls back to
 another implementation.
@@ -136,3 +138,61 @@ def _group_norm_act_grad(ctx, dy, _mean, _rstd):
 
 
 group_norm_act.register_autograd(_group_norm_act_grad, setup_context=_group_norm_act_context)
+
+
+def _rows_empty(x, dim, c=None, dtype=None):
+    """A dense result for x's rows (of c values each)."""
+    from . import ops
+    axis = ops._row_axis(x, dim)
+    shape = list(x.shape)
+    own = shape.pop(axis)
+    return x.new_empty((*shape, own if c is None else c), dtype=dtype or x.dtype).movedim(-1, axis)
+
+
+@torch.library.custom_op('kadconv::layer_norm', mutates_args=())
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
+               dim: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    from . import ops
+    if not x.is_cuda:
+        raise ValueError('kadconv::layer_norm needs a GPU tensor')
+    return ops.layer_norm_forward(x, weight, bias, eps, dim)
+
+
+@layer_norm.register_fake
+def _(x, weight, bias, eps, dim):
+    from . import ops
+    mean = x.new_empty((x.numel() // x.shape[ops._row_axis(x, dim)],), dtype=torch.float32)
+    return _rows_empty(x, dim), mean, torch.empty_like(mean)
+
+
+@torch.library.custom_op('kadconv::layer_norm_backward', mutates_args=())
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None,
+                        mean: torch.Tensor, rstd: torch.Tensor, eps: float,
+                        dim: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    from . import ops
+    dx, dw, db = ops.layer_norm_backward(dy, x, weight, bias, mean, rstd, eps, dim)
+    none = mean.new_empty(0)
+    return dx, none if dw is None else dw, none.clone() if db is None else db
+
+
+@layer_norm_backward.register_fake
+def _(dy, x, weight, bias, mean, rstd, eps, dim):
+    def like(p):
+        return mean.new_empty(0) if p is None else torch.empty_like(p, memory_format=torch.contiguous_format)
+    return _rows_empty(x, dim), like(weight), like(bias)
+
+
+def _layer_norm_context(ctx, inputs, output):
+    x, weight, bias, eps, dim = inputs
+    ctx.mark_non_differentiable(output[1], output[2])  # for the gradient's own use
+    ctx.save_for_backward(x, weight, bias, output[1], output[2])
+    ctx.rest = eps, dim
+
+
+def _layer_norm_grad(ctx, dy, _mean, _rstd):
+    x, weight, bias, mean, rstd = ctx.saved_tensors
+    dx, dw, db = torch.ops.kadconv.layer_norm_backward(dy, x, weight, bias, mean, rstd, *ctx.rest)
+    return dx, None if weight is None else dw, None if bias is None else db, None, None
+
+
+layer_norm.register_autograd(_layer_norm_grad, setup_context=_layer_norm_context)

@@ -8,7 +8,9 @@
   (north-star piece 3; KAD-CNet ``Conv`` after Conv-BN fusion).
 * ``squeeze_excitation`` -- SE block: GAP, FC-ReLU-FC-sigmoid, channel scale.
 * ``group_norm_act`` -- group norm and an activation on channels-last maps,
-  differentiable (the others are inference-only on the GPU).
+  differentiable (the ones above are inference-only on the GPU).
+* ``layer_norm`` -- layer norm of rows, or of each pixel of a channels-last map
+  over its channels, differentiable.
 
 GPU entry points never fall back to another implementation: if the HIP library
 is missing they raise ``kadconv._ext.KadExtensionError``.
@@ -278,3 +280,79 @@ def group_norm_act(input, num_groups, weight=None, bias=None, eps=1e-5, act=None
     if input.is_cuda:
         return torch.ops.kadconv.group_norm_act(input, num_groups, weight, bias, eps, act)[0]
     return _group_norm_act_cpu(input, num_groups, weight, bias, eps, act)
+
+
+def _row_axis(x, dim):
+    """The axis along which rows run: the last one, or 1 of [N, C, H, W]."""
+    nd = x.dim()
+    if nd < 1:
+        raise ValueError('an input with at least one axis expected')
+    if dim in (-1, nd - 1):
+        return nd - 1
+    if nd != 4 or dim not in (1, -3):
+        raise ValueError(f'dim must be the last axis, or 1 for [N, C, H, W]; got {dim} for {nd} axes')
+    return 1
+
+
+def _check_param(p, x, c, name):
+    if p is None:
+        return
+    if tuple(p.shape) != (c,):
+        raise ValueError(f'{name} must have shape ({c},), got {tuple(p.shape)}')
+    if p.device != x.device:
+        raise ValueError(f'input and {name} must be on one device')
+    if p.dtype not in (torch.float32, x.dtype):
+        raise TypeError(f'{name} must be float32 or {x.dtype}, got {p.dtype}')
+
+
+def _layer_norm_check(x, weight, bias, eps, dim):
+    c = x.shape[_row_axis(x, dim)]
+    if c < 1:
+        raise ValueError('rows of at least one value expected')
+    if not eps >= 0:
+        raise ValueError('eps must be >= 0')
+    _check_param(weight, x, c, 'weight')
+    _check_param(bias, x, c, 'bias')
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError('weight and bias must share a dtype')
+    if x.is_cuda:
+        _ext.kad_dtype(x.dtype)
+        if c > _ext.LAYER_NORM_MOST:
+            raise ValueError(f'rows of up to {_ext.LAYER_NORM_MOST} values expected on the GPU, got {c}')
+
+
+def _layer_norm_cpu(x, weight, bias, eps, dim):
+    axis = _row_axis(x, dim)
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    v = x.to(wide).movedim(axis, -1)
+    y = F.layer_norm(v, v.shape[-1:], None if weight is None else weight.to(wide), None if bias is None else bias.to(wide), eps)
+    return y.to(x.dtype).movedim(-1, axis)
+
+
+def layer_norm_forward(x, weight, bias, eps, dim):
+    """(y, mean, rstd) of a GPU tensor; mean and rstd [rows] in fp32 are what the gradient needs."""
+    return _ext.native().layer_norm_forward(x, weight, bias, eps, dim)
+
+
+def layer_norm_backward(dy, x, weight, bias, mean, rstd, eps, dim, need_x=True, need_weight=True, need_bias=True):
+    """(dx, dweight, dbias) of layer_norm; None for what is not needed or has no tensor."""
+    return _ext.native().layer_norm_backward(dy, x, weight, bias, mean, rstd, eps, dim, need_x, need_weight, need_bias)
+
+
+def layer_norm(input, weight=None, bias=None, eps=1e-5, dim=-1):
+    """Layer norm of rows: the last axis of ``input`` [..., C], or with ``dim=1`` the channels of each pixel of a map
+    [N, C, H, W]; ``weight`` and ``bias`` [C] (float32 or input's dtype) or None.  Statistics and normalisation are
+    computed in 32 bits and rounded once to input's dtype.
+
+    GPU tensors (fp32, fp16, bf16; rows of up to 16384 values) run the gfx950 HIP kernels, forward and backward (once
+    differentiable).  Rows that lie a fixed distance apart, as those of channels-last maps and of slices along their
+    axis do, are read where they are; others are copied first.  The result is dense (a map's: channels-last).  CPU
+    tensors run the plain composition."""
+    if input.is_cuda and not torch.compiler.is_compiling():
+        y = _ext.native().layer_norm(input, weight, bias, eps, dim)  # with the same checks
+        if y is not None:  # not traced, and no tensor a fake one
+            return y
+    _layer_norm_check(input, weight, bias, eps, dim)
+    if input.is_cuda:
+        return torch.ops.kadconv.layer_norm(input, weight, bias, eps, dim)[0]
+    return _layer_norm_cpu(input, weight, bias, eps, dim)
