@@ -680,6 +680,44 @@ int64_t kad_layer_norm_work_elems(const kad_layer_norm_args *a);
 int kad_layer_norm_fwd(const kad_layer_norm_args *a, void *stream);
 int kad_layer_norm_bwd(const kad_layer_norm_args *a, void *stream);
 
+/* Distillation from a teacher's top logits.  Row r has v logits z and k entries, of which entry e counts if its index i_e
+ * lies in [0, v) and its logit t_e is not -infinity.  With p = softmax(t / T) over the entries that count and
+ * q = softmax(z / T):
+ *   loss = T^2 sum_e p_e (log p_e - log q[i_e]),   dz_j = dloss T (q_j - sum of p_e with i_e = j),
+ * both 0 for a row without such entries, whatever its logits are.  Row r lies at (n, p) = (r / inner, r % inner). */
+typedef struct kad_distill_args {
+  const void *logits;     /* [rows][z_rs], dtype: values [0, v) of each row */
+  const void *teacher;    /* entry e of row (n, p) at n t_sn + p t_sp + e t_sk, teacher_dtype */
+  const void *index;      /* likewise with i_sn, i_sp, i_sk; int32_t or int64_t */
+  const float *dloss;     /* backward: of each row (KAD_REDUCE_NONE), or one */
+  void *dlogits;          /* backward: dense [rows][v], dtype */
+  float *stats;           /* [rows][2]: the largest logit and 1 / sum exp((z - largest) / T), 0 for a row without entries;
+                             forward writes them (NULL: not wanted), backward reads them */
+  float *loss;            /* forward: of each row (KAD_REDUCE_NONE), or one */
+  float *share;           /* KAD_REDUCE_MEAN: one float, 1 / the number of rows that have entries (0 if none); forward writes
+                             it, backward reads it */
+  float *work;            /* forward: kad_distill_work_elems floats; need not be initialised, free after the call */
+  int64_t rows;           /* 1 .. 2^31 - 1 */
+  int64_t z_rs;           /* elements from row to row (any, at least v; at most 2^31 - 1) */
+  int64_t inner;          /* >= 1 */
+  int64_t t_sn, t_sp, t_sk, i_sn, i_sp, i_sk;  /* >= 0 */
+  int v, k;               /* v: 1 .. 2^30, k: 1 .. KAD_DISTILL_MOST */
+  float temperature;      /* > 0 */
+  int reduction;
+  int dtype, teacher_dtype, index_bits; /* index_bits: 32 or 64 */
+} kad_distill_args;
+
+#define KAD_DISTILL_MOST 1024
+#define KAD_REDUCE_NONE 0
+#define KAD_REDUCE_SUM 1
+#define KAD_REDUCE_MEAN 2
+
+/* Floats of scratch that a forward call on these sizes needs, or KAD_EINVAL. */
+int64_t kad_distill_work_elems(const kad_distill_args *a);
+
+int kad_distill_fwd(const kad_distill_args *a, void *stream);
+int kad_distill_bwd(const kad_distill_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

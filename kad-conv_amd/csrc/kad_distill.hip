@@ -1,0 +1,581 @@
+// Distillation from a teacher's top logits: the loss of rows of logits, and its gradient.
+//
+//   p = softmax(t / T) over a row's entries (t_e at class i_e), q = softmax(z / T)
+//   loss = T^2 sum_e p_e (log p_e - log q[i_e]) = T^2 (sum_e e_e ((t_e - tm) - (z_i - zm)) / T / S + log(Z / S))
+//          with e_e = exp((t_e - tm) / T), S = sum e, Z = sum_j exp((z_j - zm) / T), tm and zm the largest of each
+//   dz_j = dloss T (q_j - sum of p_e with i_e = j)
+//
+// Memory bounds it: forward reads z once (the largest value and the sum in one pass), backward reads z and writes dz;
+// what the classes of the entries are is looked up in z, a few values a row.
+//
+// Two forms.  Up to MOST_SMALL classes a row stays in the registers of up to 64 lanes (kad_rows.h), many rows a wave;
+// beyond, a block walks a row, or a part of one where rows are few: forward these parts are joined in a second launch,
+// backward each writes its own classes.
+//
+// An index may come twice: its p add up, in no order that could change them: of small rows in LDS as whole numbers of
+// 2^-62 (a p of 2^-38 and more keeps its 24 bits; of what is smaller, no more than 2^-62 of the row's weight is lost),
+// of large ones by the entry that comes first, in the entries' order.
+#include "kad_rows.h"
+
+namespace kad {
+namespace {
+
+constexpr int MOST_SMALL = 1024;
+constexpr int MOST_BLOCKS = 1 << 20;  // a grid has at most 2^32 threads
+constexpr float INF = __builtin_inff();
+
+__device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// A row's entries.
+struct Entries {
+  const kad_distill_args& a;
+  int64_t t0, i0;
+  __device__ __forceinline__ Entries(const kad_distill_args& args, int64_t row) : a(args) {
+    int64_t n = 0, p = row;
+    if (a.inner < a.rows) {
+      n = (uint32_t)row / (uint32_t)a.inner;
+      p = row - n * a.inner;
+    }
+    t0 = n * a.t_sn + p * a.t_sp;
+    i0 = n * a.i_sn + p * a.i_sp;
+  }
+  // Whether entry e counts; its class and logit.
+  __device__ __forceinline__ bool get(int e, int& at, float& t) const {
+    const int64_t i = i0 + e * a.i_sk, ti = t0 + e * a.t_sk;
+    const int64_t c = a.index_bits == 32 ? (int64_t)((const int32_t*)a.index)[i] : ((const int64_t*)a.index)[i];
+    t = a.teacher_dtype == KAD_F32 ? ((const float*)a.teacher)[ti]
+        : a.teacher_dtype == KAD_F16 ? (float)((const half_t*)a.teacher)[ti] : (float)((const bf16_t*)a.teacher)[ti];
+    at = (int)c;
+    return c >= 0 && c < a.v && t != -INF;
+  }
+};
+
+struct Scales {
+  float inv_t, c2;  // 1 / T, log2(e) / T
+  __device__ __forceinline__ explicit Scales(float t) : inv_t(1.0f / t), c2(1.44269504f / t) {}
+};
+
+// One entry's part of S and of sum e ((t - tm) - (z - zm)).  An entry that weighs nothing does not meet log q = -inf.
+__device__ __forceinline__ void add_entry(float t, float tm, float z, float zm, float c2, float& s, float& d) {
+  const float e = exp2_((t - tm) * c2);
+  s += e;
+  d += e == 0.f ? 0.f : e * ((t - tm) - (z - zm));
+}
+__device__ __forceinline__ float row_loss(float T, float s, float d, float zsum, const Scales& c) {
+  return T * T * (d / s * c.inv_t + logf(zsum / s));
+}
+
+// A block's losses and rows that count, as a pair of work.
+__device__ __forceinline__ void leave_part(const kad_distill_args& a, float loss, unsigned count) {
+  __shared__ float red[32];
+  if (a.reduction == KAD_REDUCE_NONE) return;
+  float n = (float)count;
+  loss = lanes_sum(loss, 64);
+  n = lanes_sum(n, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    red[2 * (threadIdx.x >> 6)] = loss;
+    red[2 * (threadIdx.x >> 6) + 1] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < (int)blockDim.x >> 6; ++w) {
+    loss += red[2 * w];
+    n += red[2 * w + 1];
+  }
+  a.work[2 * blockIdx.x] = loss;
+  a.work[2 * blockIdx.x + 1] = n;  // a whole number under 2^24: a block has fewer rows
+}
+
+__device__ __forceinline__ void leave_row(const kad_distill_args& a, int64_t row, bool counts, float zm, float zsum, float loss) {
+  if (a.stats) {
+    a.stats[2 * row] = zm;
+    a.stats[2 * row + 1] = counts ? 1.0f / zsum : 0.f;
+  }
+  if (a.reduction == KAD_REDUCE_NONE) a.loss[row] = loss;
+}
+
+__global__ __launch_bounds__(1024) void distill_join_kernel(kad_distill_args a, int parts) {
+  __shared__ float red[16];
+  __shared__ unsigned nred[16];
+  float s = 0.f;
+  unsigned n = 0;
+  for (int i = threadIdx.x; i < parts; i += 1024) {
+    s += a.work[2 * i];
+    n += (unsigned)a.work[2 * i + 1];
+  }
+  s = lanes_sum(s, 64);
+  for (int m = 1; m < 64; m <<= 1) n += __shfl_xor(n, m);
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = s;
+    nred[threadIdx.x >> 6] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < 16; ++w) {
+    s += red[w];
+    n += nred[w];
+  }
+  const float share = n ? 1.0f / (float)n : 0.f;
+  if (a.reduction == KAD_REDUCE_MEAN) {
+    if (a.share) *a.share = share;
+    *a.loss = n ? s / (float)n : 0.f;
+  } else {
+    *a.loss = s;
+  }
+}
+
+// What dlogits are multiplied by, and 0 or NaN where a row's are.
+__device__ __forceinline__ float row_factor(const kad_distill_args& a, int64_t row) {
+  const float g = a.dloss[a.reduction == KAD_REDUCE_NONE ? row : 0];
+  return g * a.temperature * (a.reduction == KAD_REDUCE_MEAN ? *a.share : 1.f);
+}
+
+// ---------------------------------------------------------------------------- rows in registers
+template <typename T, int VV, int U, bool RAGGED>
+__global__ __launch_bounds__(256) void distill_small_fwd_kernel(kad_distill_args a, int G) {
+  const int sub = threadIdx.x / G, l = threadIdx.x & (G - 1), per = 256 / G;
+  const Place<VV, U, RAGGED> o(l, G, a.v);
+  const Scales c(a.temperature);
+  const int64_t step = (int64_t)gridDim.x * per, last = a.rows - 1;
+  float total = 0.f;
+  unsigned count = 0;
+  for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows; base += step) {
+    const bool live = base + sub <= last;
+    const int64_t row = live ? base + sub : last;
+    const T* z = (const T*)a.logits + row * a.z_rs;
+    Piece<T, VV> raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u].load(z + o.at[u]);
+    const Entries en(a, row);
+    float tm = -INF, any = 0.f, t;
+    int at;
+    for (int e = l; e < a.k; e += G)
+      if (en.get(e, at, t)) {
+        any = 1.f;
+        tm = fmaxf(tm, t);
+      }
+    any = lanes_max(any, G);
+    tm = lanes_max(tm, G);
+    float x[U][VV], zm = -INF, zsum = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      raw[u].get(x[u]);
+#pragma unroll
+      for (int e = 0; e < VV; ++e) zm = fmaxf(zm, x[u][e]);
+    }
+    zm = lanes_max(zm, G);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int e = 0; e < VV; ++e) x[u][e] = exp2_((x[u][e] - zm) * c.c2);
+      zsum += o.own(u, x[u]);
+    }
+    zsum = lanes_sum(zsum, G);
+    float s = 0.f, d = 0.f;
+    for (int e = l; e < a.k; e += G)
+      if (en.get(e, at, t)) add_entry(t, tm, to_f32(z[at]), zm, c.c2, s, d);
+    s = lanes_sum(s, G);
+    d = lanes_sum(d, G);
+    if (l == 0 && live) {
+      const float loss = any != 0.f ? row_loss(a.temperature, s, d, zsum, c) : 0.f;
+      leave_row(a, row, any != 0.f, zm, zsum, loss);
+      total += loss;
+      count += any != 0.f;
+    }
+  }
+  leave_part(a, total, count);
+}
+
+template <typename T, int VV, int U, bool RAGGED>
+__global__ __launch_bounds__(256) void distill_small_bwd_kernel(kad_distill_args a, int G) {
+  extern __shared__ unsigned long long sums[];  // [rows of the block][v]: sums of p in units of 2^-62
+  const int sub = threadIdx.x / G, l = threadIdx.x & (G - 1), per = 256 / G;
+  const Place<VV, U, RAGGED> o(l, G, a.v);
+  const Scales c(a.temperature);
+  const int64_t step = (int64_t)gridDim.x * per, last = a.rows - 1;
+  unsigned long long* mine = sums + sub * a.v;
+  for (int i = threadIdx.x; i < per * a.v; i += 256) sums[i] = 0;
+  for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows; base += step) {
+    const bool live = base + sub <= last;
+    const int64_t row = live ? base + sub : last;
+    const T* z = (const T*)a.logits + row * a.z_rs;
+    Piece<T, VV> raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u].load(z + o.at[u]);
+    const float zm = a.stats[2 * row], inv = a.stats[2 * row + 1], f = row_factor(a, row);
+    const Entries en(a, row);
+    float tm = -INF, s = 0.f, t;
+    int at;
+    for (int e = l; e < a.k; e += G)
+      if (en.get(e, at, t)) tm = fmaxf(tm, t);
+    tm = lanes_max(tm, G);
+    for (int e = l; e < a.k; e += G)
+      if (en.get(e, at, t)) s += exp2_((t - tm) * c.c2);
+    s = lanes_sum(s, G);
+    const float unit = 0x1p62f / s;
+    __syncthreads();  // sums are 0
+    for (int e = l; e < a.k; e += G)
+      if (en.get(e, at, t) && s == s) atomicAdd(mine + at, (unsigned long long)(exp2_((t - tm) * c.c2) * unit));
+    __syncthreads();
+    float x[U][VV];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      raw[u].get(x[u]);
+#pragma unroll
+      for (int e = 0; e < VV; ++e) {
+        const float q = exp2_((x[u][e] - zm) * c.c2) * inv, p = (float)mine[o.at[u] + e] * 0x1p-62f;
+        x[u][e] = inv == 0.f ? 0.f : f * (s == s ? q - p : s);
+      }
+    }
+    __syncthreads();  // what two vectors share is read twice before it is cleared
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!o.on[u]) continue;
+#pragma unroll
+      for (int e = 0; e < VV; ++e) mine[o.at[u] + e] = 0;
+      if (live) put<T, VV>((T*)a.dlogits + row * a.v + o.at[u], x[u]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------- rows of any length
+// A thread's largest value and sum of exp((z - largest) / T).
+struct Soft {
+  float m = -INF, s = 0.f;
+  // The base of differences: 0 while all values are -inf, whose exponentials are 0.
+  static __device__ __forceinline__ float base(float m) { return m == -INF ? 0.f : m; }
+  template <int N>
+  __device__ __forceinline__ void add(const float* v, int skip, float c2) {
+    float n = m;
+#pragma unroll
+    for (int e = 0; e < N; ++e) n = fmaxf(n, v[e]);
+    const float b = base(n);
+    s *= exp2_((m - b) * c2);
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += e >= skip ? exp2_((v[e] - b) * c2) : 0.f;
+    m = n;
+  }
+  __device__ __forceinline__ void join(float om, float os, float c2) {
+    const float n = fmaxf(m, om), b = base(n);
+    s = s * exp2_((m - b) * c2) + os * exp2_((om - b) * c2);
+    m = n;
+  }
+};
+
+// Joined over a block of 256 threads.
+__device__ __forceinline__ Soft join_block(Soft v, float c2, float* red) {
+  const float m = lanes_max(v.m, 64), b = Soft::base(m);
+  float s = lanes_sum(v.s * exp2_((v.m - b) * c2), 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    red[2 * (threadIdx.x >> 6)] = m;
+    red[2 * (threadIdx.x >> 6) + 1] = s;
+  }
+  __syncthreads();
+  Soft r;
+  r.m = red[0];
+  r.s = red[1];
+  for (int w = 1; w < 4; ++w) r.join(red[2 * w], red[2 * w + 1], c2);
+  return r;
+}
+
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = lanes_sum(v, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return red[0] + red[1] + red[2] + red[3];
+}
+__device__ __forceinline__ float block_max(float v, float* red) {
+  v = lanes_max(v, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// The row's loss, given its Soft: by a block of 256 threads.
+template <typename T>
+__device__ __forceinline__ float entries_loss(const kad_distill_args& a, const Entries& en, const T* z, const Soft& soft,
+                                              const Scales& c, float* red, bool& counts) {
+  float tm = -INF, any = 0.f, s = 0.f, d = 0.f, t;
+  int at;
+  for (int e = threadIdx.x; e < a.k; e += 256)
+    if (en.get(e, at, t)) {
+      any = 1.f;
+      tm = fmaxf(tm, t);
+    }
+  counts = block_max(any, red) != 0.f;
+  tm = block_max(tm, red);
+  for (int e = threadIdx.x; e < a.k; e += 256)
+    if (en.get(e, at, t)) add_entry(t, tm, to_f32(z[at]), soft.m, c.c2, s, d);
+  s = block_sum(s, red);
+  d = block_sum(d, red);
+  return counts ? row_loss(a.temperature, s, d, soft.s, c) : 0.f;
+}
+
+// The Soft of values [begin, end), which are VEC<T> at least.
+template <typename T>
+__device__ __forceinline__ Soft soft_of(const T* z, int begin, int end, float c2) {
+  constexpr int V = VEC<T>, AT_ONCE = 4;
+  Soft r;
+  const int n = (end - begin + V - 1) / V;
+  for (int j = threadIdx.x; j < n; j += AT_ONCE * 256) {
+    intx4 raw[AT_ONCE];
+    int skip[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = begin + (j + u * 256) * V, at = i < end - V ? i : end - V;
+      skip[u] = i < end ? i - at : V;
+      raw[u] = load_vec(z + at);
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      float v[V];
+      unpack<T>(raw[u], v);
+      r.add<V>(v, skip[u], c2);
+    }
+  }
+  return r;
+}
+
+// sum and largest of no values, or of -inf alone: the softmax is not defined
+__device__ __forceinline__ Soft settled(Soft v) {
+  if (!(v.s > 0.f)) v.s = __builtin_nanf("");
+  return v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void distill_large_fwd_kernel(kad_distill_args a) {
+  __shared__ float red[8];
+  const Scales c(a.temperature);
+  float total = 0.f;
+  unsigned count = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* z = (const T*)a.logits + row * a.z_rs;
+    const Soft soft = settled(join_block(soft_of(z, 0, a.v, c.c2), c.c2, red));
+    bool counts;
+    const float loss = entries_loss(a, Entries(a, row), z, soft, c, red, counts);
+    if (threadIdx.x == 0) {
+      leave_row(a, row, counts, soft.m, soft.s, loss);
+      total += loss;
+      count += counts;
+    }
+  }
+  leave_part(a, total, count);
+}
+
+// Where rows are few: a part of one a block, [rows][parts][2] behind the blocks' losses in work.
+template <typename T>
+__global__ __launch_bounds__(256) void distill_part_kernel(kad_distill_args a, int part, float* softs) {
+  __shared__ float red[8];
+  const Scales c(a.temperature);
+  const int64_t row = blockIdx.x;
+  const int begin = blockIdx.y * part, end = begin + part < a.v ? begin + part : a.v;
+  const Soft soft = join_block(soft_of((const T*)a.logits + row * a.z_rs, begin, end, c.c2), c.c2, red);
+  if (threadIdx.x) return;
+  softs[2 * (row * gridDim.y + blockIdx.y)] = soft.m;
+  softs[2 * (row * gridDim.y + blockIdx.y) + 1] = soft.s;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void distill_parts_fwd_kernel(kad_distill_args a, int parts, const float* softs) {
+  __shared__ float red[8];
+  const Scales c(a.temperature);
+  const int64_t row = blockIdx.x;
+  Soft mine;
+  if ((int)threadIdx.x < parts) {
+    mine.m = softs[2 * (row * parts + threadIdx.x)];
+    mine.s = softs[2 * (row * parts + threadIdx.x) + 1];
+  }
+  const Soft soft = settled(join_block(mine, c.c2, red));
+  bool counts;
+  const float loss = entries_loss(a, Entries(a, row), (const T*)a.logits + row * a.z_rs, soft, c, red, counts);
+  if (threadIdx.x == 0) leave_row(a, row, counts, soft.m, soft.s, loss);
+  leave_part(a, threadIdx.x ? 0.f : loss, threadIdx.x == 0 && counts);
+}
+
+// Rows from the last to the first: the forward pass left the last ones in the memory-side cache.
+template <typename T>
+__global__ __launch_bounds__(256) void distill_large_bwd_kernel(kad_distill_args a, int part) {
+  constexpr int V = VEC<T>, AT_ONCE = 4;
+  __shared__ float red[8];
+  __shared__ int at_of[KAD_DISTILL_MOST];
+  __shared__ float p_of[KAD_DISTILL_MOST];
+  const Scales c(a.temperature);
+  const int begin = blockIdx.y * part, end = begin + part < a.v ? begin + part : a.v, n = (end - begin + V - 1) / V;
+  for (int64_t turn = blockIdx.x; turn < a.rows; turn += gridDim.x) {
+    const int64_t row = a.rows - 1 - turn;
+    const T* z = (const T*)a.logits + row * a.z_rs;
+    T* dz = (T*)a.dlogits + row * a.v;
+    const float zm = a.stats[2 * row], inv = a.stats[2 * row + 1], f = row_factor(a, row);
+    const Entries en(a, row);
+    float tm = -INF, s = 0.f, t;
+    int at;
+    for (int e = threadIdx.x; e < a.k; e += 256)
+      if (en.get(e, at, t)) tm = fmaxf(tm, t);
+    tm = block_max(tm, red);
+    for (int e = threadIdx.x; e < a.k; e += 256) {
+      const bool counts = en.get(e, at, t);
+      const float w = counts ? exp2_((t - tm) * c.c2) : 0.f;
+      at_of[e] = counts ? at : -1;
+      p_of[e] = w;
+      s += w;
+    }
+    s = block_sum(s, red);  // NaN, or a row that counts: 1 at least
+    const float norm = 1.0f / s, scale = s == s ? f * inv : s;
+    for (int j = threadIdx.x; j < n; j += AT_ONCE * 256) {
+      intx4 raw[AT_ONCE];
+  #pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = begin + (j + u * 256) * V;
+        raw[u] = load_vec(z + (i < end - V ? i : end - V));
+      }
+  #pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = begin + (j + u * 256) * V;
+        float v[V];
+        unpack<T>(raw[u], v);
+  #pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = inv == 0.f ? 0.f : scale * exp2_((v[e] - zm) * c.c2);
+        if (i < end) store_vec(dz + (i < end - V ? i : end - V), v);
+      }
+    }
+    if (inv == 0.f) continue;
+    // The entries' classes again, once all of the block's stores are done.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.k; e += 256) {
+      const int mine = at_of[e];
+      if (mine < begin || mine >= end) continue;
+      float p = 0.f;
+      bool again = false;
+      for (int i = 0; i < a.k; ++i) {
+        const bool same = at_of[i] == mine;
+        p += same ? p_of[i] : 0.f;
+        again |= same && i < e;
+      }
+      if (!again) dz[mine] = from_f32<T>(f * (exp2_((to_f32(z[mine]) - zm) * c.c2) * inv - p * norm));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------- host
+struct Shape {
+  int vv, u, G;
+  int64_t blocks;  // whose losses are joined
+  int part, parts; // large rows: classes of a block, blocks of a row
+};
+
+Shape shape_of(const kad_distill_args& a, bool backward) {
+  Shape s{};
+  const int v = 16 / dtype_size(a.dtype);
+  if (a.v <= MOST_SMALL) {
+    s.vv = a.v >= v ? v : 1;
+    const int vecs = ceil_div(a.v, s.vv);
+    s.u = 1;
+    while (vecs > 64 * s.u) s.u *= 2;
+    s.G = 1;
+    while (s.G * s.u < vecs) s.G *= 2;
+    const int64_t turns = (a.rows + 256 / s.G - 1) / (256 / s.G);
+    s.blocks = turns < 2048 ? turns : 2048;
+    return s;
+  }
+  s.blocks = a.rows < 2048 || backward ? a.rows : 2048;
+  s.parts = 1;
+  s.part = a.v;
+  const int64_t wanted = backward ? 2048 : 1024;
+  if (a.rows * 2 <= wanted && a.v >= 8192) {
+    int64_t parts = wanted / a.rows, most = a.v / 4096;
+    parts = parts < most ? parts : most;
+    if (parts > 256) parts = 256;
+    s.part = round_up((int)((a.v + parts - 1) / parts), v);
+    // a last part shorter than a vector could not be read in one
+    while (s.parts = ceil_div(a.v, s.part), s.parts > 1 && a.v - (s.parts - 1) * s.part < v) s.part += v;
+  }
+  return s;
+}
+
+int check_args(const kad_distill_args* a, const char* what) {
+  const auto is_dtype = [](int t) { return t == KAD_F32 || t == KAD_F16 || t == KAD_BF16; };
+  KAD_CHECK_ARG(a, "%s: null pointer", what);
+  KAD_CHECK_ARG(is_dtype(a->dtype) && is_dtype(a->teacher_dtype), "%s: bad dtype", what);
+  KAD_CHECK_ARG(a->index_bits == 32 || a->index_bits == 64, "%s: index_bits must be 32 or 64", what);
+  KAD_CHECK_ARG(a->rows > 0 && a->rows <= INT32_MAX, "%s: 1 to 2^31 - 1 rows expected", what);
+  KAD_CHECK_ARG(a->v > 0 && a->v <= 1 << 30, "%s: 1 to 2^30 classes expected", what);
+  KAD_CHECK_ARG(a->k > 0 && a->k <= KAD_DISTILL_MOST, "%s: 1 to %d entries expected", what, KAD_DISTILL_MOST);
+  KAD_CHECK_ARG(a->temperature > 0.f && a->temperature < INF, "%s: temperature must be positive", what);
+  KAD_CHECK_ARG(a->reduction >= KAD_REDUCE_NONE && a->reduction <= KAD_REDUCE_MEAN, "%s: unknown reduction", what);
+  return KAD_OK;
+}
+
+int check_call(const kad_distill_args* a, bool backward, const char* what) {
+  if (int rc = check_args(a, what)) return rc;
+  KAD_CHECK_ARG(a->logits && a->teacher && a->index, "%s: null pointer", what);
+  KAD_CHECK_ARG(backward ? a->dloss && a->dlogits && a->stats : a->loss != nullptr, "%s: null pointer", what);
+  KAD_CHECK_ARG(!backward || a->reduction != KAD_REDUCE_MEAN || a->share, "%s: share is missing", what);
+  KAD_CHECK_ARG(backward || a->work || kad_distill_work_elems(a) == 0, "%s: work is missing", what);
+  KAD_CHECK_ARG(a->z_rs >= a->v && a->z_rs <= INT32_MAX, "%s: z_rs does not fit v", what);
+  KAD_CHECK_ARG(a->inner >= 1, "%s: inner must be at least 1", what);
+  KAD_CHECK_ARG(a->t_sn >= 0 && a->t_sp >= 0 && a->t_sk >= 0 && a->i_sn >= 0 && a->i_sp >= 0 && a->i_sk >= 0,
+                "%s: strides must not be negative", what);
+  return KAD_OK;
+}
+
+template <typename T, int VV, int U, bool RAGGED>
+void launch_small(const kad_distill_args& a, const Shape& s, bool backward, hipStream_t st) {
+  if (backward)
+    distill_small_bwd_kernel<T, VV, U, RAGGED><<<s.blocks, 256, (256 / s.G) * a.v * sizeof(unsigned long long), st>>>(a, s.G);
+  else
+    distill_small_fwd_kernel<T, VV, U, RAGGED><<<s.blocks, 256, 0, st>>>(a, s.G);
+}
+
+template <typename T, int U>
+void launch_small(const kad_distill_args& a, const Shape& s, bool backward, hipStream_t st) {
+  if (a.v % VEC<T>) launch_small<T, VEC<T>, U, true>(a, s, backward, st);
+  else launch_small<T, VEC<T>, U, false>(a, s, backward, st);
+}
+
+template <typename T>
+void launch(const kad_distill_args& a, bool backward, hipStream_t st) {
+  const Shape s = shape_of(a, backward);
+  if (s.G) {
+    if (s.vv == 1) launch_small<T, 1, 1, false>(a, s, backward, st);
+    else if (s.u == 1) launch_small<T, 1>(a, s, backward, st);
+    else if (s.u == 2) launch_small<T, 2>(a, s, backward, st);
+    else if constexpr (sizeof(T) == 4) launch_small<T, 4>(a, s, backward, st);
+  } else if (backward) {
+    distill_large_bwd_kernel<T><<<dim3(a.rows < MOST_BLOCKS ? a.rows : MOST_BLOCKS, s.parts), 256, 0, st>>>(a, s.part);
+  } else if (s.parts > 1) {
+    float* softs = a.work + 2 * s.blocks;
+    distill_part_kernel<T><<<dim3(a.rows, s.parts), 256, 0, st>>>(a, s.part, softs);
+    distill_parts_fwd_kernel<T><<<a.rows, 256, 0, st>>>(a, s.parts, softs);
+  } else {
+    distill_large_fwd_kernel<T><<<s.blocks, 256, 0, st>>>(a);
+  }
+  if (!backward && a.reduction != KAD_REDUCE_NONE) distill_join_kernel<<<1, 1024, 0, st>>>(a, (int)s.blocks);
+}
+
+int run(const kad_distill_args* a, bool backward, void* stream, const char* what) {
+  if (int rc = check_call(a, backward, what)) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  if (a->dtype == KAD_F32) launch<float>(*a, backward, st);
+  else if (a->dtype == KAD_F16) launch<half_t>(*a, backward, st);
+  else launch<bf16_t>(*a, backward, st);
+  return check_launch(what);
+}
+
+}  // namespace
+}  // namespace kad
+
+using namespace kad;
+
+extern "C" int64_t kad_distill_work_elems(const kad_distill_args* a) {
+  if (int rc = check_args(a, "kad_distill_work_elems")) return rc;
+  const Shape s = shape_of(*a, false);
+  return (a->reduction == KAD_REDUCE_NONE && s.parts <= 1 ? 0 : 2 * s.blocks) + (s.parts > 1 ? 2 * a->rows * s.parts : 0);
+}
+
+extern "C" int kad_distill_fwd(const kad_distill_args* a, void* stream) { return run(a, false, stream, "kad_distill_fwd"); }
+
+extern "C" int kad_distill_bwd(const kad_distill_args* a, void* stream) { return run(a, true, stream, "kad_distill_bwd"); }

@@ -7,118 +7,16 @@
 // Memory bounds it: a row stays in registers (at most 16 values a thread), so x is read once and y written once, x and dy
 // read once and dx written.
 //
-// Layout.  A row belongs to G threads (a power of two, 1 .. 1024), each with U 16-byte vectors of V values.  Where V does
-// not divide c, the last vector is moved back to end with the row: what it shares with the one before is computed and
-// written twice, with the same bits, and counted once in sums.  So any c >= V is read in whole vectors, at any alignment;
-// shorter rows go a value a thread.  A block walks rows with its parameters (and, backward, its share of dw and db) in
-// registers, the next row's values on their way while it computes.
+// Layout.  A row belongs to G threads (1 .. 1024), each with U vectors (kad_rows.h).  A block walks rows with its
+// parameters (and, backward, its share of dw and db) in registers, the next row's values on their way while it computes.
 //
 // Sums.  The variance is that of the differences to the mean, in 32 bits, whose own mean corrects both: a row of one value
-// repeated is 0 everywhere.  All sums are joined in an order that the sizes
-// alone decide: dw and db first over a block's rows, then over blocks in a second launch.
-#include "kad_vec.h"
+// repeated is 0 everywhere.  All sums are joined in an order that the sizes alone decide: dw and db first over a block's
+// rows, then over blocks in a second launch.
+#include "kad_rows.h"
 
 namespace kad {
 namespace {
-
-// Sum over the G (a power of two, at most 64) threads that share a row, by lane permutations of the vector unit.
-__device__ __forceinline__ float lanes_sum(float v, int G) {
-#define KAD_DPP(x, ctrl) __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), ctrl, 0xf, 0xf, true))
-  if (G >= 2) v += KAD_DPP(v, 0xB1);    // lane ^ 1
-  if (G >= 4) v += KAD_DPP(v, 0x4E);    // lane ^ 2
-  if (G >= 8) v += KAD_DPP(v, 0x141);   // 7 - lane of eight: the other four, whose values are equal by now
-  if (G >= 16) v += KAD_DPP(v, 0x140);  // 15 - lane of sixteen
-#undef KAD_DPP
-  if (G >= 32) v = sum_xor16(v);
-  if (G >= 64) v = sum_xor32(v);
-  return v;
-}
-
-// Over all threads of a row; beyond a wave through red (one float a wave and call), with one barrier.
-__device__ __forceinline__ float row_sum(float v, int G, float* red) {
-  v = lanes_sum(v, G);
-  if (G > 64) {
-    const int wave = threadIdx.x >> 6, waves = G >> 6, first = wave & ~(waves - 1);
-    if ((threadIdx.x & 63) == 0) red[wave] = v;
-    __syncthreads();
-    v = red[first];
-    for (int i = 1; i < waves; ++i) v += red[first + i];
-  }
-  return v;
-}
-
-// Two at once (two floats a wave).
-__device__ __forceinline__ void row_sums(float& v, float& w, int G, float* red) {
-  v = lanes_sum(v, G);
-  w = lanes_sum(w, G);
-  if (G > 64) {
-    const int wave = threadIdx.x >> 6, waves = G >> 6, first = wave & ~(waves - 1);
-    if ((threadIdx.x & 63) == 0) {
-      red[2 * wave] = v;
-      red[2 * wave + 1] = w;
-    }
-    __syncthreads();
-    v = red[2 * first];
-    w = red[2 * first + 1];
-    for (int i = 1; i < waves; ++i) {
-      v += red[2 * (first + i)];
-      w += red[2 * (first + i) + 1];
-    }
-  }
-}
-
-// VV values of a thread's vector: V, or 1 for rows shorter than a vector.
-template <typename T, int VV>
-struct Piece {
-  intx4 raw;
-  __device__ __forceinline__ void load(const T* p, bool on) {
-    if (VV > 1) {
-      raw = load_vec(p);
-    } else {
-      T v = p[0];
-      raw = intx4{0, 0, 0, 0};
-      __builtin_memcpy(&raw, &v, sizeof(T));
-    }
-  }
-  __device__ __forceinline__ void get(float v[VV]) const {
-    if constexpr (VV > 1) {
-      unpack<T>(raw, v);
-    } else {
-      T t;
-      __builtin_memcpy(&t, &raw, sizeof(T));
-      v[0] = to_f32(t);
-    }
-  }
-};
-template <typename T, int VV>
-__device__ __forceinline__ void put(T* p, const float v[VV]) {
-  if constexpr (VV > 1) stream_vec<T>(p, v);
-  else p[0] = from_f32<T>(v[0]);
-}
-
-// Where a thread's vectors lie in a row.  RAGGED: VV does not divide c.
-template <int VV, int U, bool RAGGED>
-struct Place {
-  int at[U];     // first value
-  int skip[U];   // how many of the vector's first values belong to the vector before
-  bool on[U];    // there is a vector
-  __device__ __forceinline__ Place(int l, int G, int c) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = (l + u * G) * VV;
-      on[u] = j < c;
-      at[u] = j < c - VV ? j : c - VV;
-      skip[u] = RAGGED ? j - at[u] : 0;
-    }
-  }
-  // Sum of the values that are its own.
-  __device__ __forceinline__ float own(int u, const float v[VV]) const {
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < VV; ++e) s += !RAGGED || e >= skip[u] ? v[e] : 0.f;
-    return on[u] ? s : 0.f;
-  }
-};
 
 template <typename Q, int VV, int U, bool RAGGED>
 __device__ __forceinline__ void params(const void* p, float none, const Place<VV, U, RAGGED>& o, float f[U][VV]) {
@@ -151,7 +49,7 @@ __global__ __launch_bounds__(MOST) void layer_norm_fwd_kernel(kad_layer_norm_arg
   const auto fetch = [&](int64_t row) {
     const T* x = (const T*)a.x + (row < last ? row : last) * a.x_rs;
 #pragma unroll
-    for (int u = 0; u < U; ++u) next[u].load(x + o.at[u], true);
+    for (int u = 0; u < U; ++u) next[u].load(x + o.at[u]);
   };
   fetch(base + sub);
   for (; base < a.rows; base += step) {
@@ -219,8 +117,8 @@ __global__ __launch_bounds__(MOST) void layer_norm_bwd_kernel(kad_layer_norm_arg
     const T *x = (const T*)a.x + row * a.x_rs, *d = (const T*)a.dy + row * a.dy_rs;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      nx[u].load(x + o.at[u], true);
-      nd[u].load(d + o.at[u], true);
+      nx[u].load(x + o.at[u]);
+      nd[u].load(d + o.at[u]);
     }
     nmean = a.mean[row];
     nrstd = a.rstd[row];

@@ -1,6 +1,8 @@
 // kadconv._native: operators on rows, which are the last axis of a tensor or the channels of a map's pixels.
 #include "kad_torch.h"
 
+#include <cmath>
+
 namespace {
 
 // The number of the axis along which rows run, as dim says: the last one, or the channels of [N, C, H, W].
@@ -281,10 +283,244 @@ std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_backward(const Tensor& dy
   return {opt(dx), opt(dw), opt(db)};
 }
 
+// ---------------------------------------------------------------------------- distillation
+struct Distill {
+  double temperature;
+  int reduction;
+  int64_t dim;
+};
+
+int checked_reduction(std::string_view r) {
+  TORCH_CHECK_VALUE(r == "none" || r == "sum" || r == "mean", "reduction '", r, "' is none of 'none', 'sum', 'mean'");
+  return r == "none" ? KAD_REDUCE_NONE : r == "sum" ? KAD_REDUCE_SUM : KAD_REDUCE_MEAN;
+}
+
+// What the kernels take as given: the checks of kadconv.ops._distill_check, and that the tensors are on a GPU.
+bool check_distill(const Tensor& x, const Tensor& t, const Tensor& index, double temperature, int64_t dim) {
+  const bool map = is_map(x, dim);
+  const int64_t nd = x.dim(), axis = map ? 1 : nd - 1;
+  TORCH_CHECK_VALUE(x.size(axis) >= 1, "at least one class expected");
+  TORCH_CHECK_VALUE(t.dim() == nd && t.sizes() == index.sizes(), "teacher_logits and teacher_index must have one shape and the axes of logits");
+  for (int64_t d = 0; d < nd; ++d)
+    TORCH_CHECK_VALUE(d == axis || t.size(d) == x.size(d), "teacher_logits must have the shape of logits but for the classes, got ",
+                      t.sizes(), " for ", x.sizes());
+  TORCH_CHECK_VALUE(t.size(axis) >= 1 && t.size(axis) <= KAD_DISTILL_MOST, "1 to ", KAD_DISTILL_MOST, " entries expected, got ",
+                    t.size(axis));
+  TORCH_CHECK_VALUE(x.device() == t.device() && x.device() == index.device(), "logits and the teacher's tensors must be on one device");
+  TORCH_CHECK_TYPE(index.scalar_type() == at::kInt || index.scalar_type() == at::kLong,
+                   "teacher_index must be torch.int32 or torch.int64, got ", index.scalar_type());
+  TORCH_CHECK_VALUE(temperature > 0 && std::isfinite((float)temperature) && (float)temperature > 0, "temperature must be positive");
+  TORCH_CHECK_VALUE(x.is_cuda(), "a GPU tensor expected, got one on ", x.device());
+  dtype_of(x);
+  dtype_of(t);
+  return map;
+}
+
+// Where the entries lie: of row (n, p), n sn + p sp + e sk.
+struct Strided {
+  Tensor held;
+  int64_t sn, sp, sk;
+};
+
+Strided entries_of(const Tensor& t, bool map) {
+  if (map) {
+    const int64_t h = t.size(2), w = t.size(3);
+    Strided r{t, t.stride(0), w > 1 ? t.stride(3) : t.stride(2), t.stride(1)};
+    if (h > 1 && w > 1 && t.stride(2) != w * t.stride(3)) {
+      r.held = t.contiguous();
+      r.sn = t.size(1) * h * w, r.sp = 1, r.sk = h * w;
+    }
+    return r;
+  }
+  Strided r{t, 0, t.size(-1), t.stride(-1)};
+  bool first = true;
+  int64_t expected = 0;
+  for (int64_t i = t.dim() - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (first) r.sp = expected = t.stride(i), first = false;
+    if (t.stride(i) != expected) {
+      r.held = t.contiguous();
+      r.sp = t.size(-1), r.sk = 1;
+      return r;
+    }
+    expected *= t.size(i);
+  }
+  return r;
+}
+
+kad_distill_args distill_args(const Rows& x, const Strided& t, const Strided& i, bool map, const Distill& o) {
+  kad_distill_args a{};
+  a.logits = x.held.const_data_ptr();
+  a.teacher = t.held.const_data_ptr();
+  a.index = i.held.const_data_ptr();
+  a.rows = x.count;
+  a.z_rs = x.rs;
+  a.inner = map ? x.held.size(2) * x.held.size(3) : x.count;
+  a.t_sn = t.sn, a.t_sp = t.sp, a.t_sk = t.sk;
+  a.i_sn = i.sn, a.i_sp = i.sp, a.i_sk = i.sk;
+  a.v = (int)x.c;
+  a.k = (int)t.held.size(map ? 1 : -1);
+  a.temperature = (float)o.temperature;
+  a.reduction = o.reduction;
+  a.dtype = dtype_of(x.held);
+  a.teacher_dtype = dtype_of(t.held);
+  a.index_bits = i.held.scalar_type() == at::kInt ? 32 : 64;
+  return a;
+}
+
+c10::DimVector row_sizes(const Tensor& x, bool map) {
+  c10::DimVector s(x.sizes());
+  s.erase(s.begin() + (map ? 1 : x.dim() - 1));
+  return s;
+}
+
+void check_classes(const Tensor& x, bool map) {
+  TORCH_CHECK_VALUE(row_length(x, map) <= 1 << 30 && row_count(x, map) <= INT32_MAX, "up to 2^30 classes and 2^31 - 1 rows expected, got ",
+                    x.sizes());
+}
+
+// The loss, with stats [rows, 2] (where wanted) and share [1] written.
+Tensor distill_run(const Tensor& x, bool map, const Tensor& t, const Tensor& index, const Distill& o, const Tensor& stats,
+                   const Tensor& share) {
+  check_classes(x, map);
+  Tensor loss = o.reduction == KAD_REDUCE_NONE ? floats(x, row_sizes(x, map)) : floats(x, {});
+  if (!x.numel()) {
+    loss.zero_();
+    if (share.defined()) share.zero_();
+    return loss;
+  }
+  const Rows r = rows_of(x, map);
+  const Strided te = entries_of(t, map), ie = entries_of(index, map);
+  kad_distill_args a = distill_args(r, te, ie, map, o);
+  a.loss = loss.mutable_data_ptr<float>();
+  a.stats = (float*)mutable_pointer(stats);
+  a.share = (float*)mutable_pointer(share);
+  const int64_t n = kad_distill_work_elems(&a);
+  if (n < 0) check((int)n, "kad_distill_work_elems");
+  const Tensor work = n ? floats(x, {n}) : Tensor();
+  a.work = (float*)mutable_pointer(work);
+  check(kad_distill_fwd(&a, stream_of(x)), "kad_distill_fwd");
+  return loss;
+}
+
+void check_saved(const Tensor& x, bool map, const Tensor& stats, const Tensor& share) {
+  const auto floats_like = [&](const Tensor& t, at::IntArrayRef sizes) {
+    return t.is_contiguous() && t.scalar_type() == at::kFloat && t.device() == x.device() && t.sizes() == sizes;
+  };
+  TORCH_CHECK_VALUE(floats_like(stats, {row_count(x, map), 2}) && floats_like(share, {1}), "stats and share must be the forward's");
+}
+
+Tensor distill_gradient(const Tensor& dloss, const Tensor& x, bool map, const Tensor& t, const Tensor& index, const Tensor& stats,
+                        const Tensor& share, const Distill& o) {
+  check_classes(x, map);
+  TORCH_CHECK_VALUE(dloss.device() == x.device() && dloss.scalar_type() == at::kFloat &&
+                        (o.reduction == KAD_REDUCE_NONE ? dloss.sizes() == at::IntArrayRef(row_sizes(x, map)) : dloss.numel() == 1),
+                    "dloss must be float32 with the shape and device of the loss");
+  Tensor dx = dense_like(x, map);
+  if (!x.numel()) return dx;
+  const Rows r = rows_of(x, map);
+  const Strided te = entries_of(t, map), ie = entries_of(index, map);
+  const Tensor g = dloss.contiguous();
+  kad_distill_args a = distill_args(r, te, ie, map, o);
+  a.dloss = g.const_data_ptr<float>();
+  a.dlogits = dx.mutable_data_ptr();
+  a.stats = const_cast<float*>(stats.const_data_ptr<float>());
+  a.share = const_cast<float*>(share.const_data_ptr<float>());
+  check(kad_distill_bwd(&a, stream_of(x)), "kad_distill_bwd");
+  return dx;
+}
+
+struct DistillBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable x, t, index, stats, share;
+  Distill o;
+
+  std::string name() const override { return "DistillBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto* v : {&x, &t, &index, &stats, &share}) v->reset_data();
+  }
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    torch::autograd::variable_list out(1);
+    const Tensor& dloss = grads[0];
+    if (!dloss.defined() || !task_should_compute_output(0)) return out;
+    const Tensor xs = x.unpack(), ts = t.unpack(), is = index.unpack(), st = stats.unpack(), sh = share.unpack();
+    // a hook on saved tensors may have put others in their place
+    const bool map = check_distill(xs, ts, is, o.temperature, o.dim);
+    check_saved(xs, map, st, sh);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const c10::DeviceGuard guard(xs.device());
+      out[0] = distill_gradient(dloss, xs, map, ts, is, st, sh, o);
+    }
+    if (c10::GradMode::is_enabled() && torch::autograd::compute_requires_grad(dloss, xs))
+      out = once_differentiable(std::move(out), "kadconv.distill_loss");
+    return out;
+  }
+};
+
+// None where the call is observed.
+OptTensor distill_loss(const Tensor& x, const Tensor& t, const Tensor& index, double temperature, std::string_view reduction,
+                       int64_t dim) {
+  if (observed({&x, &t, &index})) return std::nullopt;
+  const bool map = check_distill(x, t, index, temperature, dim);
+  const Distill o{temperature, checked_reduction(reduction), dim};
+  check_no_forward_grad({&x, &t}, "kadconv.distill_loss");
+  std::shared_ptr<DistillBackward> node;
+  if (torch::autograd::compute_requires_grad(x)) {
+    node = new_node<DistillBackward>(torch::autograd::collect_next_edges(x));
+    node->x = torch::autograd::SavedVariable(x, false);
+    node->t = torch::autograd::SavedVariable(t.detach(), false);
+    node->index = torch::autograd::SavedVariable(index, false);
+    node->o = o;
+  }
+  Tensor loss, stats, share;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::DeviceGuard guard(x.device());
+    if (node) {
+      stats = floats(x, {row_count(x, map), 2});
+      share = floats(x, {1});
+    }
+    loss = distill_run(x, map, t, index, o, stats, share);
+  }
+  if (node) {
+    node->stats = torch::autograd::SavedVariable(stats, false);
+    node->share = torch::autograd::SavedVariable(share, false);
+    torch::autograd::set_history(loss, node);
+  }
+  return loss;
+}
+
+std::tuple<Tensor, Tensor, Tensor> distill_loss_forward(const Tensor& x, const Tensor& t, const Tensor& index, double temperature,
+                                                        std::string_view reduction, int64_t dim) {
+  const bool map = check_distill(x, t, index, temperature, dim);
+  const Distill o{temperature, checked_reduction(reduction), dim};
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x.device());
+  const Tensor stats = floats(x, {row_count(x, map), 2}), share = floats(x, {1});
+  return {distill_run(x, map, t, index, o, stats, share), stats, share};
+}
+
+Tensor distill_loss_backward(const Tensor& dloss, const Tensor& x, const Tensor& t, const Tensor& index, const Tensor& stats,
+                             const Tensor& share, double temperature, std::string_view reduction, int64_t dim) {
+  const bool map = check_distill(x, t, index, temperature, dim);
+  const Distill o{temperature, checked_reduction(reduction), dim};
+  check_saved(x, map, stats, share);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x.device());
+  return distill_gradient(dloss, x, map, t, index, stats, share, o);
+}
+
 }  // namespace
 
 void kad_torch::bind_rows(py::module_& m) {
   m.def("layer_norm", &layer_norm);
   m.def("layer_norm_forward", &layer_norm_forward);
   m.def("layer_norm_backward", &layer_norm_backward);
+  m.def("distill_loss", &distill_loss);
+  m.def("distill_loss_forward", &distill_loss_forward);
+  m.def("distill_loss_backward", &distill_loss_backward);
 }

@@ -14,9 +14,9 @@ from . import library  # registers the kadconv:: custom operators
 from .blocks import Conv1x1SiLU, GroupNormAct, KADDown, LayerNorm, SqueezeExcitation
 from .fast import disable_fast_inference, enable_fast_inference
 from .kad_conv import DSC, LCSA, KADConv
-from .ops import deform_conv2d, group_norm_act, layer_norm
+from .ops import deform_conv2d, distill_loss, group_norm_act, layer_norm
 from .optim import AdamW, AdamWPlan
 
 __all__ = ['KADConv', 'DSC', 'LCSA', 'enable_fast_inference', 'disable_fast_inference', 'deform_conv2d',
            'Conv1x1SiLU', 'SqueezeExcitation', 'KADDown', 'group_norm_act', 'GroupNormAct', 'AdamW', 'AdamWPlan',
-           'layer_norm', 'LayerNorm']
+           'layer_norm', 'LayerNorm', 'distill_loss']

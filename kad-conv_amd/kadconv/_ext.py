@@ -121,6 +121,13 @@ class LayerNormArgs(ctypes.Structure):
                                                                   ('param_dtype', c_int)]
 
 
+class DistillArgs(ctypes.Structure):
+    _fields_ = [(f, c_vp) for f in ('logits', 'teacher', 'index', 'dloss', 'dlogits', 'stats', 'loss', 'share', 'work')] + \
+               [(f, c_i64) for f in ('rows', 'z_rs', 'inner', 't_sn', 't_sp', 't_sk', 'i_sn', 'i_sp', 'i_sk')] + \
+               [('v', c_int), ('k', c_int), ('temperature', ctypes.c_float)] + \
+               [(f, c_int) for f in ('reduction', 'dtype', 'teacher_dtype', 'index_bits')]
+
+
 class AdamwChunk(ctypes.Structure):
     _fields_ = [('param', c_vp), ('grad', c_vp), ('offset', c_i64), ('count', c_int), ('reserved', c_int)]
 
@@ -135,6 +142,7 @@ class AdamwArgs(ctypes.Structure):
 
 ADAMW_SEG = 256          # KAD_ADAMW_SEG
 LAYER_NORM_MOST = 16384  # KAD_LAYER_NORM_MOST
+DISTILL_MOST = 1024      # KAD_DISTILL_MOST
 ADAMW_SCALARS = 4        # 4-byte words of kad_adamw_scalars
 
 
@@ -213,6 +221,9 @@ SIGNATURES = {
     'kad_layer_norm_work_elems': (c_i64, [ctypes.POINTER(LayerNormArgs)]),
     'kad_layer_norm_fwd': (c_int, [ctypes.POINTER(LayerNormArgs), c_vp]),
     'kad_layer_norm_bwd': (c_int, [ctypes.POINTER(LayerNormArgs), c_vp]),
+    'kad_distill_work_elems': (c_i64, [ctypes.POINTER(DistillArgs)]),
+    'kad_distill_fwd': (c_int, [ctypes.POINTER(DistillArgs), c_vp]),
+    'kad_distill_bwd': (c_int, [ctypes.POINTER(DistillArgs), c_vp]),
     'kad_adamw_chunks': (c_i64, [c_vp, c_vp, c_vp, c_int, c_int, c_vp, ctypes.POINTER(c_i64)]),
     'kad_adamw_step': (c_int, [ctypes.POINTER(AdamwArgs), c_vp]),
     'kad_adamw_hyper': (c_int, [ctypes.POINTER(AdamwArgs), c_vp, c_vp, c_vp, c_vp]),

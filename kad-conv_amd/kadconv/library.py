@@ -24,6 +24,9 @@ shapes instead of breaking the graph at an opaque Python call:
       kadconv::group_norm_act_backward.
   kadconv::layer_norm(x, weight?, bias?, eps, dim) -> (Tensor y, Tensor mean, Tensor rstd)
       kadconv.ops.layer_norm, likewise, with kadconv::layer_norm_backward.
+  kadconv::distill_loss(logits, teacher_logits, teacher_index, temperature, reduction, dim)
+        -> (Tensor loss, Tensor stats, Tensor share)
+      kadconv.ops.distill_loss, likewise, with kadconv::distill_loss_backward.
 
 The eager implementations run the HIP kernels; nothing here falls back to
 another implementation.
@@ -196,3 +199,49 @@ def _layer_norm_grad(ctx, dy, _mean, _rstd):
 
 
 layer_norm.register_autograd(_layer_norm_grad, setup_context=_layer_norm_context)
+
+
+@torch.library.custom_op('kadconv::distill_loss', mutates_args=())
+def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, temperature: float,
+                 reduction: str, dim: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    from . import ops
+    if not logits.is_cuda:
+        raise ValueError('kadconv::distill_loss needs a GPU tensor')
+    return ops.distill_loss_forward(logits, teacher_logits, teacher_index, temperature, reduction, dim)
+
+
+@distill_loss.register_fake
+def _(logits, teacher_logits, teacher_index, temperature, reduction, dim):
+    from . import ops
+    axis = ops._row_axis(logits, dim)
+    shape = [n for d, n in enumerate(logits.shape) if d != axis]
+    rows = logits.numel() // logits.shape[axis]
+    loss = logits.new_empty(shape if reduction == 'none' else (), dtype=torch.float32)
+    return loss, logits.new_empty((rows, 2), dtype=torch.float32), logits.new_empty((1,), dtype=torch.float32)
+
+
+@torch.library.custom_op('kadconv::distill_loss_backward', mutates_args=())
+def distill_loss_backward(dloss: torch.Tensor, logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
+                          stats: torch.Tensor, share: torch.Tensor, temperature: float, reduction: str, dim: int) -> torch.Tensor:
+    from . import ops
+    return ops.distill_loss_backward(dloss, logits, teacher_logits, teacher_index, stats, share, temperature, reduction, dim)
+
+
+@distill_loss_backward.register_fake
+def _(dloss, logits, teacher_logits, teacher_index, stats, share, temperature, reduction, dim):
+    return _rows_empty(logits, dim)
+
+
+def _distill_loss_context(ctx, inputs, output):
+    logits, teacher_logits, teacher_index, temperature, reduction, dim = inputs
+    ctx.mark_non_differentiable(output[1], output[2])  # for the gradient's own use
+    ctx.save_for_backward(logits, teacher_logits, teacher_index, output[1], output[2])
+    ctx.rest = temperature, reduction, dim
+
+
+def _distill_loss_grad(ctx, dloss, _stats, _share):
+    dz = torch.ops.kadconv.distill_loss_backward(dloss, *ctx.saved_tensors, *ctx.rest)
+    return dz, None, None, None, None, None
+
+
+distill_loss.register_autograd(_distill_loss_grad, setup_context=_distill_loss_context)

@@ -11,6 +11,7 @@
   differentiable (the ones above are inference-only on the GPU).
 * ``layer_norm`` -- layer norm of rows, or of each pixel of a channels-last map
   over its channels, differentiable.
+* ``distill_loss`` -- distillation from a teacher's top logits, differentiable.
 
 GPU entry points never fall back to another implementation: if the HIP library
 is missing they raise ``kadconv._ext.KadExtensionError``.
@@ -356,3 +357,93 @@ def layer_norm(input, weight=None, bias=None, eps=1e-5, dim=-1):
     if input.is_cuda:
         return torch.ops.kadconv.layer_norm(input, weight, bias, eps, dim)[0]
     return _layer_norm_cpu(input, weight, bias, eps, dim)
+
+
+_REDUCTIONS = ('none', 'sum', 'mean')
+
+
+def _distill_check(x, t, index, temperature, reduction, dim):
+    axis = _row_axis(x, dim)
+    if x.shape[axis] < 1:
+        raise ValueError('at least one class expected')
+    if t.dim() != x.dim() or t.shape != index.shape:
+        raise ValueError('teacher_logits and teacher_index must have one shape and the axes of logits')
+    if any(d != axis and t.shape[d] != x.shape[d] for d in range(x.dim())):
+        raise ValueError('teacher_logits must have the shape of logits but for the classes, got '
+                         f'{tuple(t.shape)} for {tuple(x.shape)}')
+    if not 1 <= t.shape[axis] <= _ext.DISTILL_MOST:
+        raise ValueError(f'1 to {_ext.DISTILL_MOST} entries expected, got {t.shape[axis]}')
+    if not x.device == t.device == index.device:
+        raise ValueError("logits and the teacher's tensors must be on one device")
+    if index.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f'teacher_index must be torch.int32 or torch.int64, got {index.dtype}')
+    if not 0 < temperature < float('inf'):
+        raise ValueError('temperature must be positive')
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction {reduction!r} is none of 'none', 'sum', 'mean'")
+    for v in (x, t):
+        if x.is_cuda:
+            _ext.kad_dtype(v.dtype)
+        elif not v.is_floating_point():
+            raise TypeError(f'logits must be floating-point numbers, got {v.dtype}')
+
+
+def _distill_cpu(x, t, index, temperature, reduction, dim):
+    axis = _row_axis(x, dim)
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    z = x.to(wide).movedim(axis, -1) / temperature
+    t = t.detach().to(wide).movedim(axis, -1) / temperature
+    index = index.movedim(axis, -1).long()
+    counts = (index >= 0) & (index < z.shape[-1]) & (t != -float('inf'))
+    live = counts.any(-1)
+    t = torch.where(counts, t, torch.full_like(t, -float('inf'))).masked_fill(~live[..., None], 0.0)
+    log_p = F.log_softmax(t, -1)
+    p = log_p.exp()
+    z = torch.where(live[..., None], z, torch.zeros_like(z))  # a row without entries: 0, whatever its logits are
+    log_q = F.log_softmax(z, -1).gather(-1, index.clamp(0, z.shape[-1] - 1))
+    weighs = live[..., None] & (p != 0)
+    terms = p * (log_p - torch.where(weighs, log_q, torch.zeros_like(log_q)))
+    loss = temperature ** 2 * torch.where(weighs, terms, torch.zeros_like(p)).sum(-1)
+    if reduction == 'none':
+        return loss.to(torch.promote_types(torch.float32, x.dtype))
+    loss = loss.sum()
+    return loss / live.sum().clamp(min=1) if reduction == 'mean' else loss
+
+
+def distill_loss_forward(logits, teacher_logits, teacher_index, temperature, reduction, dim):
+    """(loss, stats, share) on the GPU; stats [rows, 2] and share [1] in fp32 are what the gradient needs."""
+    return _ext.native().distill_loss_forward(logits, teacher_logits, teacher_index, temperature, reduction, dim)
+
+
+def distill_loss_backward(dloss, logits, teacher_logits, teacher_index, stats, share, temperature, reduction, dim):
+    """The gradient of the logits."""
+    return _ext.native().distill_loss_backward(dloss, logits, teacher_logits, teacher_index, stats, share, temperature,
+                                               reduction, dim)
+
+
+def distill_loss(logits, teacher_logits, teacher_index, temperature=1.0, reduction='mean', dim=-1):
+    """The divergence of a student's softmax from a teacher's, of whose classes only the best are known:
+
+        p = softmax(t / T) over a row's entries, q = softmax(z / T) over all classes,
+        loss = T^2 sum_e p_e (log p_e - log q[i_e])
+
+    ``logits`` z [..., V] (or with ``dim=1`` maps [N, V, H, W]); ``teacher_logits`` t and ``teacher_index`` i (int32 or
+    int64), of the same shape but for K entries in place of the V classes, as torch.topk returns them.  An entry whose
+    index lies outside of [0, V) or whose logit is -infinity does not count; an index that comes twice has both weights.
+    A row without entries that count is 0 and has no gradient, whatever its logits are; a row that has some, but logits
+    of -infinity alone, is NaN.
+
+    ``reduction``: 'none' (a row's loss each, float32), 'sum', or 'mean' over the rows that have entries (0 if none has).
+    Sums are taken in 32 bits and in an order that the sizes decide.  The teacher's tensors are constants.
+
+    GPU tensors (fp32, fp16, bf16; up to 1024 entries) run the gfx950 HIP kernels, forward and backward (once
+    differentiable); logits are read where they are if their rows lie a fixed distance apart.  The gradient is dense (a
+    map's: channels-last).  CPU tensors run the plain composition."""
+    if logits.is_cuda and not torch.compiler.is_compiling():
+        loss = _ext.native().distill_loss(logits, teacher_logits, teacher_index, temperature, reduction, dim)  # with the same checks
+        if loss is not None:  # not traced, and no tensor a fake one
+            return loss
+    _distill_check(logits, teacher_logits, teacher_index, temperature, reduction, dim)
+    if logits.is_cuda:
+        return torch.ops.kadconv.distill_loss(logits, teacher_logits, teacher_index, temperature, reduction, dim)[0]
+    return _distill_cpu(logits, teacher_logits, teacher_index, temperature, reduction, dim)

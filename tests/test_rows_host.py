@@ -85,3 +85,100 @@ def test_layer_norm_work():
     a = _ln_args(rows=1 << 40, c=16384, x_rs=16384, dy_rs=16384)
     assert 0 < lib.kad_layer_norm_work_elems(ctypes.byref(a)) <= 1024 * 2 * 16384
     assert lib.kad_layer_norm_work_elems(ctypes.byref(_ln_args(c=0))) == -1
+
+
+# ---------------------------------------------------------------------------- distillation
+def _logits(dim=-1):
+    g = torch.Generator().manual_seed(1)
+    shape = (3, 6, 5) if dim == -1 else (3, 5, 2, 3)
+    z = torch.randn(shape, generator=g, dtype=torch.float64)
+    top = torch.topk(torch.randn(shape, generator=g, dtype=torch.float64), 3, dim=dim)
+    return z, top.values, top.indices
+
+
+@pytest.mark.parametrize('dim', [-1, 1])
+def test_distill_plain(dim):
+    from tests._distill_ref import reference
+    z, t, i = _logits(dim)
+    i.movedim(dim, -1)[0] = -1
+    z.movedim(dim, -1)[0] = float('nan')
+    zs = z.clone().requires_grad_(True)
+    rows = [a.movedim(dim, -1).reshape(-1, a.shape[dim]) for a in (z, t, i)]
+    loss = kadconv.distill_loss(zs, t, i, 2.0, 'none', dim)
+    g = torch.rand(loss.shape, dtype=torch.float64)
+    ref = reference(*rows, 2.0, g.reshape(-1))
+    assert torch.allclose(loss.reshape(-1), ref['loss'], atol=1e-12)
+    dz, = torch.autograd.grad(loss, zs, g)
+    assert torch.allclose(dz.movedim(dim, -1).reshape(-1, z.shape[dim]), ref['dz'], atol=1e-12)
+    mean = kadconv.distill_loss(z, t, i, 2.0, 'mean', dim)
+    assert torch.allclose(mean, ref['loss'].sum() / ref['live'].sum(), atol=1e-12)
+    full = torch.topk(torch.randn(4, 6, dtype=torch.float64), 6, dim=1)  # all classes: the divergence itself
+    z = torch.randn(4, 6, dtype=torch.float64)
+    p = torch.zeros(4, 6, dtype=torch.float64).scatter(1, full.indices, torch.softmax(full.values, 1))
+    want = torch.nn.functional.kl_div(torch.log_softmax(z, 1), p, reduction='batchmean')
+    assert torch.allclose(kadconv.distill_loss(z, full.values, full.indices), want, atol=1e-12)
+
+
+def test_distill_refusals():
+    z, t, i = _logits()
+    for args, match in (((z[..., :0], t, i), 'class'), ((z, t[0], i[0]), 'one shape'), ((z, t, i[..., :2]), 'one shape'),
+                        ((z[:2], t, i), 'shape of logits'), ((z, t[..., :0], i[..., :0]), 'entries')):
+        with pytest.raises(ValueError, match=match):
+            kadconv.distill_loss(*args)
+    for temperature in (0.0, -1.0, float('inf'), float('nan')):
+        with pytest.raises(ValueError, match='temperature'):
+            kadconv.distill_loss(z, t, i, temperature)
+    with pytest.raises(ValueError, match='reduction'):
+        kadconv.distill_loss(z, t, i, reduction='max')
+    with pytest.raises(ValueError, match='dim must'):
+        kadconv.distill_loss(z, t, i, dim=1)
+    with pytest.raises(TypeError, match='int32'):
+        kadconv.distill_loss(z, t, i.short())
+    with pytest.raises(TypeError, match='floating'):
+        kadconv.distill_loss(z.long(), t, i)
+    with pytest.raises(ValueError, match='GPU'):
+        _ext.native().distill_loss(z.float(), t.float(), i, 1.0, 'mean', -1)
+    with pytest.raises(ValueError, match='needs a GPU'):
+        torch.ops.kadconv.distill_loss(z, t, i, 1.0, 'mean', -1)
+
+
+def _distill_args(**kw):
+    a = _ext.DistillArgs()
+    for f in ('logits', 'teacher', 'index', 'dloss', 'dlogits', 'stats', 'loss', 'share', 'work'):
+        setattr(a, f, 4096)
+    a.rows, a.v, a.z_rs, a.inner, a.k, a.temperature, a.reduction = 3, 8, 8, 3, 2, 1.0, 2
+    a.t_sp = a.i_sp = 2
+    a.t_sk = a.i_sk = 1
+    a.dtype = a.teacher_dtype = _ext.KAD_F16
+    a.index_bits = 64
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize('kw', [dict(logits=None), dict(teacher=None), dict(index=None), dict(loss=None), dict(work=None), dict(rows=0),
+                                dict(rows=1 << 31), dict(v=0), dict(v=(1 << 30) + 1), dict(k=0), dict(k=1025), dict(z_rs=7),
+                                dict(z_rs=1 << 31), dict(inner=0), dict(t_sk=-1), dict(i_sn=-1), dict(temperature=0.0), dict(reduction=3),
+                                dict(dtype=9), dict(teacher_dtype=-1), dict(index_bits=16)], ids=str)
+def test_distill_c_refuses(kw):
+    lib = _ext.load()
+    assert lib.kad_distill_fwd(ctypes.byref(_distill_args(**kw)), None) == -1
+    assert b'kad_distill' in lib.kad_last_error()
+
+
+@pytest.mark.parametrize('kw', [dict(dloss=None), dict(dlogits=None), dict(stats=None), dict(share=None)], ids=str)
+def test_distill_backward_c_refuses(kw):
+    assert _ext.load().kad_distill_bwd(ctypes.byref(_distill_args(**kw)), None) == -1
+
+
+def test_distill_work():
+    """Two floats for each block that has losses, and for each part of a row."""
+    lib = _ext.load()
+    def work(**kw):
+        return lib.kad_distill_work_elems(ctypes.byref(_distill_args(**kw)))
+    assert work(reduction=0) == 0 and work() == 2
+    for v in list(range(8192, 8400)) + list(range(100000, 100100)) + [1 << 30]:
+        for rows in (1, 2, 7, 511, 512):
+            for dtype in (0, 1):
+                n = work(rows=rows, v=v, z_rs=v, dtype=dtype)
+                assert 2 * rows <= n <= 2 * rows + 2 * rows * 256
