@@ -718,6 +718,49 @@ int64_t kad_distill_work_elems(const kad_distill_args *a);
 int kad_distill_fwd(const kad_distill_args *a, void *stream);
 int kad_distill_bwd(const kad_distill_args *a, void *stream);
 
+/* Matrices in 8 bits, a scale for each block of 128: a row of c numbers is held as round_up(c, 128) e4m3 codes (zeros
+ * behind the last) and a scale byte for each 128 of them, x = code * 2^(scale - 127), in rows of
+ * round_up(ceil(c / 128), 4) bytes (127 behind the last).  The scale is the smallest power of two with
+ * max |x| <= 448 * scale over the block's finite values (1 for zeros alone, 2^-127 at least); codes are rounded to
+ * nearest, ties to even; what is not finite is NaN. */
+typedef struct kad_quant8_args {
+  const void *x;              /* [rows][x_rs], dtype: values [0, c) of each row */
+  void *codes, *scales;       /* along the rows: [rows][..] as above; both NULL: not wanted */
+  void *t_codes, *t_scales;   /* along the columns, of the transposed matrix: [c][..]; both NULL: not wanted */
+  void *sums;                 /* [c], sums_dtype: of each column, or NULL */
+  float *work;                /* kad_quant8_work_elems floats (sums only); need not be initialised, free after the call */
+  int64_t rows;               /* 1 .. 2^31 - 128; fewer than 2^24 tiles of 128 x 128 values */
+  int64_t x_rs;               /* elements from row to row (any, at least c; at most 2^31 - 1) */
+  int c;                      /* 1 .. KAD_QUANT8_MOST */
+  int dtype, sums_dtype;
+} kad_quant8_args;
+
+#define KAD_QUANT8_MOST (1 << 20)
+
+int64_t kad_quant8_work_elems(const kad_quant8_args *a);
+int kad_quant8(const kad_quant8_args *a, void *stream);
+
+/* out = act(a b^T + bias): a [m][k] and b [n][k] in 8 bits along k (as kad_quant8 writes them), or a as values
+ * (a_scales NULL), which are brought to 8 bits on the way; then m is at most KAD_GEMM8_FEW.
+ * Sums are 32-bit.  Those of 32-bit results are taken from exact products; for 16-bit results the 8-bit matrix instruction
+ * cuts the products of eight consecutive k to 2^-13 of the largest of them. */
+typedef struct kad_gemm8_args {
+  const void *a, *a_scales;
+  const void *b, *b_scales;
+  const void *bias;           /* [n], bias_dtype, or NULL */
+  void *out;                  /* dense [m][n], dtype */
+  float *work;                /* kad_gemm8_work_elems floats; need not be initialised, free after the call */
+  int64_t a_rs;               /* a as values: elements from row to row (>= k) */
+  int m, n, k;                /* >= 1; k at most KAD_QUANT8_MOST; fewer than 2^24 tiles of 64 x 64 results */
+  int act;                    /* KAD_ACT_NONE, KAD_ACT_RELU or KAD_ACT_SILU */
+  int dtype, a_dtype, bias_dtype; /* a_dtype: of a as values */
+} kad_gemm8_args;
+
+#define KAD_GEMM8_FEW 64
+
+int64_t kad_gemm8_work_elems(const kad_gemm8_args *a);
+int kad_gemm8(const kad_gemm8_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

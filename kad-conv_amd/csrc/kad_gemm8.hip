@@ -1,0 +1,431 @@
+// Products of matrices in 8 bits with a scale for each block of 128 (kad_block8.h):
+//
+//   out[m][n] = act(sum over blocks of 2^(sa + sb - 254) sum over the block of a b + bias[n])
+//
+// The scales are powers of two, so the scaled matrix instruction takes them as they are: one of 16 x 16 x 128 meets one
+// block of each of its rows, and the sums need no arithmetic beside it.  Every 8-bit matrix instruction cuts the products
+// of eight consecutive k to 2^-13 of the largest of them (found by giving it single products: 2^3 next to 2^16 is kept,
+// 2^2 is not) before it adds them up in 32 bits.  Of normally distributed numbers that is 1.3e-5 of a result, of codes with
+// all bits random 5e-5: under the rounding of a 16-bit result.  For 32-bit results (EXACT) codes become fp16 numbers, which
+// hold them exactly, the fp16 instruction sums a block in 32 bits (1e-7), and the scales are applied to its sum.
+//
+// Two forms.  Many rows: tiles of BM x BN results, both operands' codes of 128 columns at a time copied to LDS past the
+// registers, one stage ahead.  Few rows (KAD_GEMM8_FEW): b's codes are read once, straight into the instruction's
+// operands; a block takes 16 rows of b, its waves take every eighth 128 columns and join in LDS.  a as values is brought
+// to 8 bits in those registers, by each block for itself: a launch less, and a is small.
+//
+// The instruction computes b a^T: a lane then holds four results of one row of out that follow each other.
+#include "kad_block8.h"
+
+namespace kad {
+namespace {
+
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+
+constexpr int LINE = BLOCK8;        // bytes of a row in a stage: one block of codes
+constexpr int KB_GROUP = 4;         // scales are read by fours
+
+__device__ __forceinline__ float activate(float z, int act) {
+  if (act == KAD_ACT_SILU) return z * sigmoidf_(z);
+  return act == KAD_ACT_RELU ? (z > 0.f ? z : z != z ? z : 0.f) : z;
+}
+
+template <bool EXACT> struct Operand;
+template <> struct Operand<false> {
+  intx8 v;
+  __device__ __forceinline__ void set(intx4 lo, intx4 hi) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+  }
+};
+template <> struct Operand<true> {
+  half8_t v[4];
+  __device__ __forceinline__ void set(intx4 lo, intx4 hi) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int w = q < 2 ? lo[2 * q + i] : hi[2 * (q - 2) + i];
+        const auto a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+        v[q][4 * i] = a[0];
+        v[q][4 * i + 1] = a[1];
+        v[q][4 * i + 2] = b[0];
+        v[q][4 * i + 3] = b[1];
+      }
+    }
+  }
+};
+
+// acc += a block of b's 16 rows times one of a's 16, of whose scales byte Q of sb and sa is this block's.  EXACT: eb are
+// the scales of the four rows of b whose results the lane holds.
+template <int Q>
+__device__ __forceinline__ void multiply(floatx4& acc, const Operand<false>& b, const Operand<false>& a, int sb, int sa, const int*) {
+  acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, acc, 0, 0, Q, sb, Q, sa);
+}
+template <int Q>
+__device__ __forceinline__ void multiply(floatx4& acc, const Operand<true>& b, const Operand<true>& a, int, int sa, const int* eb) {
+  floatx4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(b.v[q], a.v[q], t, 0, 0, 0);
+  const int ea = ((sa >> (8 * Q)) & 255) - 254;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] += __builtin_amdgcn_ldexpf(t[i], ea + eb[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_four(T* p, const float* v, int n) {
+  T t[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = from_f32<T>(v[i]);
+  if (n >= 4) {
+    __builtin_memcpy(p, t, sizeof(t));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = t[i];
+  }
+}
+
+// Four results of row m from column n on; parts: 32-bit sums that are joined later, in place of out.
+template <typename T>
+__device__ __forceinline__ void finish(const kad_gemm8_args& a, float* part, int m, int n, const floatx4& acc) {
+  if (m >= a.m || n >= a.n) return;
+  float v[4];
+  if (part) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = acc[i];
+    store_four<float>(part + (int64_t)m * a.n + n, v, a.n - n);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float b = a.bias && n + i < a.n ? load_param(a.bias, n + i, a.bias_dtype, 0.f) : 0.f;
+    v[i] = activate(acc[i] + b, a.act);
+  }
+  store_four<T>((T*)a.out + (int64_t)m * a.n + n, v, a.n - n);
+}
+
+// ---------------------------------------------------------------------------- many rows
+struct Tiles {
+  int tm, tn;      // tiles of rows and columns
+  int splits, per; // parts of k, and the 128s of k in each (a multiple of KB_GROUP)
+};
+
+// Blocks go to the eight XCDs in turn: each gets a run of tiles, which walks the rows of a few columns' worth of tiles, so
+// that what shares an L2 shares operands.
+__device__ __forceinline__ bool tile_of(const Tiles& o, int& m, int& n, int& split) {
+  constexpr int XCDS = 8, GROUP = 8;
+  const int total = o.tm * o.tn * o.splits, run = (total + XCDS - 1) / XCDS;
+  int id = (int)(blockIdx.x % XCDS) * run + (int)(blockIdx.x / XCDS);
+  if (id >= total || (int)(blockIdx.x / XCDS) >= run) return false;
+  split = id / (o.tm * o.tn);
+  id -= split * (o.tm * o.tn);
+  const int first = id / (GROUP * o.tm) * GROUP, wide = o.tn - first < GROUP ? o.tn - first : GROUP;
+  id -= first * o.tm;
+  m = id / wide;
+  n = first + id - m * wide;
+  return true;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool EXACT>
+__global__ __launch_bounds__(64 * WM * WN) void gemm8_tile_kernel(kad_gemm8_args a, Tiles o) {
+  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int CA = BM / 8 / WAVES, CB = BN / 8 / WAVES;  // copies of a wave and stage: 8 rows each
+  __shared__ __attribute__((aligned(128))) char s0[(BM + BN) * LINE];
+  __shared__ __attribute__((aligned(128))) char s1[(BM + BN) * LINE];
+  int m0, n0, split;
+  if (!tile_of(o, m0, n0, split)) return;
+  m0 *= BM;
+  n0 *= BN;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int blocks = (a.k + BLOCK8 - 1) / BLOCK8, kp = blocks * BLOCK8, ks = (blocks + 3) / 4 * 4;
+  const int begin = split * o.per, end = begin + o.per < blocks ? begin + o.per : blocks;
+  // rows past the last read as zeros
+  const int rows_a = a.m - m0 < BM ? a.m - m0 : BM, rows_b = a.n - n0 < BN ? a.n - n0 : BN;
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc((const char*)a.a + (int64_t)m0 * kp, rows_a * kp);
+  const __amdgpu_buffer_rsrc_t rb = make_rsrc((const char*)a.b + (int64_t)n0 * kp, rows_b * kp);
+  // 16-byte piece p of row r lies at piece p ^ (r & 7) of its line: lanes that read one piece of eight rows meet all banks
+  const uint32_t off = (uint32_t)(lane >> 3) * kp + (((lane & 7) ^ (lane >> 3)) << 4);
+  const auto stage = [&](char* s, int kb) {
+#pragma unroll
+    for (int i = 0; i < CA; ++i) {
+      const int r = (i * WAVES + wave) * 8;
+      dma16(ra, s + r * LINE, off + (uint32_t)r * kp, kb * BLOCK8);
+    }
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+      const int r = (i * WAVES + wave) * 8;
+      dma16(rb, s + (BM + r) * LINE, off + (uint32_t)r * kp, kb * BLOCK8);
+    }
+  };
+  const int wm = wave / WN, wn = wave % WN, r16 = lane & 15, g = lane >> 4;
+  const int line_a = (wm * TM * 16 + r16) * LINE, line_b = (BM + wn * TN * 16 + r16) * LINE;
+  const int piece0 = ((2 * g) ^ (r16 & 7)) << 4, piece1 = ((2 * g + 1) ^ (r16 & 7)) << 4;
+  const auto fetch = [&](const char* s, int line, int frag, Operand<EXACT>& v) {
+    const char* p = s + line + frag * 16 * LINE;
+    v.set(*(const intx4*)(p + piece0), *(const intx4*)(p + piece1));
+  };
+  // scales of the lane's rows, four blocks of k in each
+  const unsigned char *sa = (const unsigned char*)a.a_scales, *sb = (const unsigned char*)a.b_scales;
+  int32_t scale_a[TM], scale_b[TN];
+  const auto scales = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int r = m0 + wm * TM * 16 + i * 16 + r16;
+      scale_a[i] = *(const int32_t*)(sa + (int64_t)(r < a.m ? r : a.m - 1) * ks + kb);
+    }
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+      const int r = n0 + wn * TN * 16 + i * 16 + r16;
+      scale_b[i] = *(const int32_t*)(sb + (int64_t)(r < a.n ? r : a.n - 1) * ks + kb);
+    }
+  };
+  floatx4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  stage(s0, begin);
+#define KAD_STEP(Q, NOW, NEXT)                                                           \
+  if (kb + Q < end) {                                                                    \
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");             \
+    if (kb + Q + 1 < end) stage(NEXT, kb + Q + 1);                                       \
+    Operand<EXACT> fb[TN], fa;                                                           \
+    int eb[TN][4];                                                                       \
+    _Pragma("unroll") for (int j = 0; j < TN; ++j) {                                     \
+      fetch(NOW, line_b, j, fb[j]);                                                      \
+      if (EXACT) {                                                                       \
+        const int e = (scale_b[j] >> (8 * Q)) & 255;                                     \
+        _Pragma("unroll") for (int i = 0; i < 4; ++i) eb[j][i] = __shfl(e, 4 * g + i);   \
+      }                                                                                  \
+    }                                                                                    \
+    _Pragma("unroll") for (int i = 0; i < TM; ++i) {                                     \
+      fetch(NOW, line_a, i, fa);                                                         \
+      _Pragma("unroll") for (int j = 0; j < TN; ++j)                                     \
+        multiply<Q>(acc[i][j], fb[j], fa, scale_b[j], scale_a[i], eb[j]);                \
+    }                                                                                    \
+  }
+  for (int kb = begin; kb < end; kb += KB_GROUP) {
+    scales(kb);
+    KAD_STEP(0, s0, s1)
+    KAD_STEP(1, s1, s0)
+    KAD_STEP(2, s0, s1)
+    KAD_STEP(3, s1, s0)
+  }
+#undef KAD_STEP
+  float* part = o.splits > 1 ? a.work + (int64_t)split * a.m * a.n : nullptr;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      finish<T>(a, part, m0 + (wm * TM + i) * 16 + r16, n0 + (wn * TN + j) * 16 + 4 * g, acc[i][j]);
+}
+
+// The parts of k, in order.
+template <typename T>
+__global__ __launch_bounds__(256) void gemm8_join_kernel(kad_gemm8_args a, int splits) {
+  const int64_t all = (int64_t)a.m * a.n, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
+    float s = a.work[i];
+#pragma unroll 4
+    for (int p = 1; p < splits; ++p) s += a.work[p * all + i];
+    if (a.bias) s += load_param(a.bias, (int)(i % a.n), a.bias_dtype, 0.f);
+    ((T*)a.out)[i] = from_f32<T>(activate(s, a.act));
+  }
+}
+
+// ---------------------------------------------------------------------------- few rows
+constexpr int FEW_WAVES = 8;
+
+// 32 values of a row from column k on as codes, and their block's scale: the four lanes of a row hold a block.
+template <typename X>
+__device__ __forceinline__ int to_codes(const X* p, int left, intx4& lo, intx4& hi) {
+  constexpr int V = VEC<X>;
+  float x[32];
+  if (left >= 32) {
+#pragma unroll
+    for (int i = 0; i < 32; i += V) {
+      intx4 raw = load_vec(p + i);
+      unpack<X>(raw, x + i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = i < left ? to_f32(p[i]) : 0.f;
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const uint32_t b = magnitude(x[i]);
+    m = m > b ? m : b;
+  }
+  uint32_t other = __shfl_xor(m, 16);
+  m = m > other ? m : other;
+  other = __shfl_xor(m, 32);
+  m = m > other ? m : other;
+  const int s = scale_of(m);
+  const float inv = inverse(s);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    lo[i] = codes_of(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], inv);
+    hi[i] = codes_of(x[16 + 4 * i], x[17 + 4 * i], x[18 + 4 * i], x[19 + 4 * i], inv);
+  }
+  return s;
+}
+
+// X: a's type as values, or unsigned char: a in 8 bits.
+template <typename T, typename X, int MT, bool EXACT>
+__global__ __launch_bounds__(64 * FEW_WAVES) void gemm8_few_kernel(kad_gemm8_args a) {
+  __shared__ floatx4 red[FEW_WAVES][MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16, row_b = n0 + r16 < a.n ? n0 + r16 : a.n - 1;
+  const int blocks = (a.k + BLOCK8 - 1) / BLOCK8, kp = blocks * BLOCK8, ks = (blocks + 3) / 4 * 4;
+  const char* codes_b = (const char*)a.b + (int64_t)row_b * kp + 32 * g;
+  const unsigned char* scales_b = (const unsigned char*)a.b_scales + (int64_t)row_b * ks;
+  floatx4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int kb = wave; kb < blocks; kb += FEW_WAVES) {
+    Operand<EXACT> fb;
+    fb.set(*(const intx4*)(codes_b + kb * BLOCK8), *(const intx4*)(codes_b + kb * BLOCK8 + 16));
+    const int sb = scales_b[kb];
+    int eb[4];
+    if (EXACT)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) eb[i] = __shfl(sb, 4 * g + i);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = i * 16 + r16;
+      intx4 lo, hi;
+      int s;
+      if constexpr (sizeof(X) == 1) {
+        const int row = m < a.m ? m : a.m - 1;  // what comes of rows past the last is not stored
+        const intx4* p = (const intx4*)((const char*)a.a + (int64_t)row * kp + kb * BLOCK8 + 32 * g);
+        lo = p[0];
+        hi = p[1];
+        s = ((const unsigned char*)a.a_scales)[(int64_t)row * ks + kb];
+      } else {
+        const int k = kb * BLOCK8 + 32 * g, left = m < a.m ? a.k - k : 0;
+        s = to_codes((const X*)a.a + (left > 0 ? m * a.a_rs + k : 0), left, lo, hi);
+      }
+      Operand<EXACT> fa;
+      fa.set(lo, hi);
+      multiply<0>(acc[i], fb, fa, sb, s, eb);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) red[wave][i][lane] = acc[i];
+  __syncthreads();
+  for (int i = wave; i < MT; i += FEW_WAVES) {
+    floatx4 s = red[0][i][lane];
+    const int waves = blocks < FEW_WAVES ? blocks : FEW_WAVES;
+    for (int w = 1; w < waves; ++w) s += red[w][i][lane];
+    finish<T>(a, nullptr, i * 16 + r16, n0 + 4 * g, s);
+  }
+}
+
+// ---------------------------------------------------------------------------- host
+constexpr int CUS = 256;
+
+struct Plan {
+  int bm, bn;
+  Tiles o;
+};
+
+Plan plan_of(const kad_gemm8_args& a) {
+  Plan p;
+  const int blocks = ceil_div(a.k, BLOCK8);
+  const bool exact = a.dtype == KAD_F32;
+  const auto count = [&](int bm, int bn) { return (int64_t)ceil_div(a.m, bm) * ceil_div(a.n, bn); };
+  p.bm = p.bn = !exact && count(256, 256) >= CUS ? 256 : count(128, 128) >= CUS ? 128 : 64;
+  p.o.tm = ceil_div(a.m, p.bm);
+  p.o.tn = ceil_div(a.n, p.bn);
+  const int64_t tiles = (int64_t)p.o.tm * p.o.tn;
+  int64_t splits = tiles >= CUS ? 1 : CUS * 2 / tiles;
+  const int most = ceil_div(blocks, 2 * KB_GROUP);
+  if (splits > most) splits = most;
+  p.o.per = round_up(ceil_div(blocks, (int)splits), KB_GROUP);
+  p.o.splits = ceil_div(blocks, p.o.per);
+  return p;
+}
+
+bool few(const kad_gemm8_args& a) { return a.m <= KAD_GEMM8_FEW; }
+
+template <typename T, typename X, int MT>
+void launch_few(const kad_gemm8_args& a, hipStream_t st) {
+  gemm8_few_kernel<T, X, MT, sizeof(T) == 4><<<ceil_div(a.n, 16), 64 * FEW_WAVES, 0, st>>>(a);
+}
+
+template <typename T, typename X>
+void launch_few(const kad_gemm8_args& a, hipStream_t st) {
+  if (a.m <= 16) launch_few<T, X, 1>(a, st);
+  else if (a.m <= 32) launch_few<T, X, 2>(a, st);
+  else launch_few<T, X, 4>(a, st);
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+void launch_tiles(const kad_gemm8_args& a, const Tiles& o, hipStream_t st) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  const int total = o.tm * o.tn * o.splits, blocks = ceil_div(total, 8) * 8;
+  gemm8_tile_kernel<T, BM, BN, WM, WN, EXACT><<<blocks, 64 * WM * WN, 0, st>>>(a, o);
+}
+
+template <typename T>
+void launch(const kad_gemm8_args& a, hipStream_t st) {
+  if (few(a)) {
+    if (a.a_scales) launch_few<T, unsigned char>(a, st);
+    else if (a.a_dtype == KAD_F32) launch_few<T, float>(a, st);
+    else if (a.a_dtype == KAD_F16) launch_few<T, half_t>(a, st);
+    else launch_few<T, bf16_t>(a, st);
+    return;
+  }
+  const Plan p = plan_of(a);
+  if constexpr (sizeof(T) == 2)
+    if (p.bm == 256) launch_tiles<T, 256, 256, 2, 4>(a, p.o, st);
+  if (p.bm == 128) launch_tiles<T, 128, 128, 2, 2>(a, p.o, st);
+  if (p.bm == 64) launch_tiles<T, 64, 64, 2, 2>(a, p.o, st);
+  if (p.o.splits > 1) {
+    const int64_t n = ((int64_t)a.m * a.n + 255) / 256;
+    gemm8_join_kernel<T><<<n < 4096 ? n : 4096, 256, 0, st>>>(a, p.o.splits);
+  }
+}
+
+int check_args(const kad_gemm8_args* a, const char* what) {
+  const auto is_dtype = [](int t) { return t == KAD_F32 || t == KAD_F16 || t == KAD_BF16; };
+  KAD_CHECK_ARG(a, "%s: null pointer", what);
+  KAD_CHECK_ARG(is_dtype(a->dtype), "%s: bad dtype", what);
+  KAD_CHECK_ARG(a->m > 0 && a->n > 0 && a->k > 0 && a->k <= KAD_QUANT8_MOST && a->m <= INT32_MAX - 255 && a->n <= INT32_MAX - 255,
+                "%s: bad sizes", what);
+  KAD_CHECK_ARG((int64_t)ceil_div(a->m, 64) * ceil_div(a->n, 64) < 1 << 24, "%s: fewer than 2^24 tiles of 64 x 64 results expected", what);
+  KAD_CHECK_ARG(a->act == KAD_ACT_NONE || a->act == KAD_ACT_RELU || a->act == KAD_ACT_SILU, "%s: unknown activation", what);
+  KAD_CHECK_ARG(a->a_scales || (is_dtype(a->a_dtype) && few(*a)), "%s: a as values: of a known dtype, and at most %d rows", what,
+                KAD_GEMM8_FEW);
+  KAD_CHECK_ARG(!a->bias || is_dtype(a->bias_dtype), "%s: bad bias_dtype", what);
+  return KAD_OK;
+}
+
+}  // namespace
+}  // namespace kad
+
+using namespace kad;
+
+extern "C" int64_t kad_gemm8_work_elems(const kad_gemm8_args* a) {
+  if (int rc = check_args(a, "kad_gemm8_work_elems")) return rc;
+  if (few(*a)) return 0;
+  const Plan p = plan_of(*a);
+  return p.o.splits > 1 ? (int64_t)p.o.splits * a->m * a->n : 0;
+}
+
+extern "C" int kad_gemm8(const kad_gemm8_args* a, void* stream) {
+  const char* what = "kad_gemm8";
+  if (int rc = check_args(a, what)) return rc;
+  KAD_CHECK_ARG(a->a && a->b && a->b_scales && a->out, "%s: null pointer", what);
+  KAD_CHECK_ARG(((uintptr_t)a->b | (a->a_scales ? (uintptr_t)a->a : 0)) % 16 == 0, "%s: codes must be aligned to 16 bytes", what);
+  KAD_CHECK_ARG(((uintptr_t)a->b_scales | (uintptr_t)a->a_scales) % 4 == 0, "%s: scales must be aligned to 4 bytes", what);
+  KAD_CHECK_ARG(a->a_scales || (a->a_rs >= a->k && a->a_rs <= INT32_MAX), "%s: a_rs does not fit k", what);
+  KAD_CHECK_ARG(a->work || kad_gemm8_work_elems(a) == 0, "%s: work is missing", what);
+  const hipStream_t st = (hipStream_t)stream;
+  if (a->dtype == KAD_F32) launch<float>(*a, st);
+  else if (a->dtype == KAD_F16) launch<half_t>(*a, st);
+  else launch<bf16_t>(*a, st);
+  return check_launch(what);
+}

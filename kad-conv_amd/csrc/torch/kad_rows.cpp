@@ -514,12 +514,384 @@ Tensor distill_loss_backward(const Tensor& dloss, const Tensor& x, const Tensor&
   return distill_gradient(dloss, x, map, t, index, stats, share, o);
 }
 
+// ---------------------------------------------------------------------------- products in 8 bits
+int64_t blocks8(int64_t k) { return (k + 127) / 128; }
+int64_t codes8(int64_t k) { return blocks8(k) * 128; }
+int64_t scales8(int64_t k) { return (blocks8(k) + 3) / 4 * 4; }
+
+// Rows of k numbers in 8 bits (kadconv_hip.h).
+struct Held8 {
+  Tensor codes, scales;
+  bool defined() const { return codes.defined(); }
+};
+
+Held8 new_held(const Tensor& x, c10::DimVector sizes, int64_t k) {
+  Held8 h;
+  sizes.push_back(codes8(k));
+  h.codes = at::detail::empty_cuda(sizes, at::kFloat8_e4m3fn, x.device(), std::nullopt);
+  sizes.back() = scales8(k);
+  h.scales = at::detail::empty_cuda(sizes, at::kFloat8_e8m0fnu, x.device(), std::nullopt);
+  return h;
+}
+
+void check_held(const Tensor& codes, const Tensor& scales, int64_t rows, int64_t k, const Tensor& x, const char* name) {
+  TORCH_CHECK_TYPE(codes.scalar_type() == at::kFloat8_e4m3fn && scales.scalar_type() == at::kFloat8_e8m0fnu, name,
+                   ": codes must be torch.float8_e4m3fn and scales torch.float8_e8m0fnu");
+  TORCH_CHECK_VALUE(codes.is_contiguous() && scales.is_contiguous() && codes.device() == x.device() && scales.device() == x.device() &&
+                        codes.dim() >= 1 && scales.dim() == codes.dim() && codes.size(-1) == codes8(k) &&
+                        scales.size(-1) == scales8(k) && codes.numel() == rows * codes8(k) && scales.numel() == rows * scales8(k),
+                    name, ": ", rows, " dense rows of ", codes8(k), " codes and ", scales8(k), " scales on ", x.device(), " expected, got ",
+                    codes.sizes(), " and ", scales.sizes());
+}
+
+// What is wanted of a matrix: along its rows, along its columns, and their sums.
+void quantize(const Rows& r, const Held8& along, const Held8& across, const Tensor& sums, const Tensor& x) {
+  kad_quant8_args a{};
+  a.x = r.held.const_data_ptr();
+  a.x_rs = r.rs;
+  a.rows = r.count;
+  a.c = (int)r.c;
+  a.codes = mutable_pointer(along.codes);
+  a.scales = mutable_pointer(along.scales);
+  a.t_codes = mutable_pointer(across.codes);
+  a.t_scales = mutable_pointer(across.scales);
+  a.sums = mutable_pointer(sums);
+  a.dtype = dtype_of(r.held);
+  a.sums_dtype = sums.defined() ? dtype_of(sums) : KAD_F32;
+  const int64_t n = kad_quant8_work_elems(&a);
+  if (n < 0) check((int)n, "kad_quant8_work_elems");
+  const Tensor work = n ? floats(x, {n}) : Tensor();
+  a.work = (float*)mutable_pointer(work);
+  check(kad_quant8(&a, stream_of(x)), "kad_quant8");
+}
+
+// out = act(a b^T + bias), a in 8 bits or, where it has no scales, as values in rows a_rs apart.
+void product(const Tensor& a, const Tensor& a_scales, int64_t a_rs, const Held8& b, int64_t m, int64_t n, int64_t k, const Tensor& bias,
+             int act, const Tensor& out) {
+  TORCH_CHECK_VALUE(m <= INT32_MAX - 255 && n <= INT32_MAX - 255, "too many rows: ", m, " and ", n);
+  kad_gemm8_args g{};
+  g.a = a.const_data_ptr();
+  g.a_scales = pointer(a_scales);
+  g.a_rs = a_rs;
+  g.b = b.codes.const_data_ptr();
+  g.b_scales = b.scales.const_data_ptr();
+  g.bias = pointer(bias);
+  g.out = out.mutable_data_ptr();
+  g.m = (int)m;
+  g.n = (int)n;
+  g.k = (int)k;
+  g.act = act;
+  g.dtype = dtype_of(out);
+  g.a_dtype = a_scales.defined() ? KAD_F32 : dtype_of(a);
+  g.bias_dtype = bias.defined() ? dtype_of(bias) : KAD_F32;
+  const int64_t elems = kad_gemm8_work_elems(&g);
+  if (elems < 0) check((int)elems, "kad_gemm8_work_elems");
+  const Tensor work = elems ? floats(out, {elems}) : Tensor();
+  g.work = (float*)mutable_pointer(work);
+  check(kad_gemm8(&g, stream_of(out)), "kad_gemm8");
+}
+
+// The same for values: by way of 8 bits along k, in memory where they are many.
+void product_of_values(const Rows& r, const Held8& b, int64_t n, const Tensor& bias, int act, const Tensor& out) {
+  if (r.count <= KAD_GEMM8_FEW) return product(r.held, Tensor(), r.rs, b, r.count, n, r.c, bias, act, out);
+  const Held8 h = new_held(r.held, {r.count}, r.c);
+  quantize(r, h, {}, Tensor(), r.held);
+  product(h.codes, h.scales, 0, b, r.count, n, r.c, bias, act, out);
+}
+
+void check_quantized(const Tensor& x, int64_t k) {
+  TORCH_CHECK_VALUE(k >= 1 && k <= KAD_QUANT8_MOST, "rows of 1 to ", KAD_QUANT8_MOST, " values expected, got ", k);
+  TORCH_CHECK_VALUE(x.is_cuda(), "a GPU tensor expected, got one on ", x.device());
+  dtype_of(x);
+}
+
+// x [..., K] (or a map's pixels) as codes and scales [..., ...].
+std::tuple<Tensor, Tensor> quantize8(const Tensor& x, int64_t dim) {
+  const bool map = is_map(x, dim);
+  check_quantized(x, row_length(x, map));
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x.device());
+  const int64_t k = row_length(x, map);
+  Held8 h = new_held(x, row_sizes(x, map), k);
+  if (x.numel()) quantize(rows_of(x, map), h, {}, Tensor(), x);
+  return {h.codes, h.scales};
+}
+
+at::ScalarType checked_result(at::ScalarType t) {
+  TORCH_CHECK_TYPE(t == at::kFloat || t == at::kHalf || t == at::kBFloat16, "unsupported dtype ", t, "; expected float32, float16 or bfloat16");
+  return t;
+}
+
+// a [..., K] b [N, K]^T, both in 8 bits.
+Tensor matmul8(const Tensor& a, const Tensor& a_scales, const Tensor& b, const Tensor& b_scales, int64_t k, const OptTensor& bias,
+               const std::optional<std::string_view>& act, at::ScalarType dtype) {
+  TORCH_CHECK_VALUE(a.is_cuda(), "a GPU tensor expected, got one on ", a.device());
+  TORCH_CHECK_VALUE(k >= 1 && k <= KAD_QUANT8_MOST, "rows of 1 to ", KAD_QUANT8_MOST, " values expected, got ", k);
+  TORCH_CHECK_VALUE(a.dim() >= 1 && b.dim() == 2, "a of at least one axis and b of two expected");
+  const int64_t m = a.numel() / std::max<int64_t>(a.size(-1), 1), n = b.size(0);
+  check_held(a, a_scales, m, k, a, "a");
+  check_held(b, b_scales, n, k, a, "b");
+  const Tensor bi = dense(defined(bias));
+  if (bi.defined()) {
+    TORCH_CHECK_VALUE(bi.dim() == 1 && bi.size(0) == n && bi.device() == a.device(), "bias must have shape (", n, ",) on ", a.device());
+    dtype_of(bi);
+  }
+  const int ac = checked_act(act);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(a.device());
+  c10::DimVector sizes(a.sizes());
+  sizes.back() = n;
+  Tensor out = at::detail::empty_cuda(sizes, checked_result(dtype), a.device(), std::nullopt);
+  if (out.numel()) product(a, a_scales, 0, {b, b_scales}, m, n, k, bi, ac, out);
+  return out;
+}
+
+// What the kernels take as given: the checks of kadconv.block8._linear8_check, and that the input is on a GPU.
+bool check_linear8(const Tensor& x, int64_t n, int64_t k, const Tensor& bias, int64_t dim) {
+  const bool map = is_map(x, dim);
+  check_quantized(x, row_length(x, map));
+  TORCH_CHECK_VALUE(row_length(x, map) == k, "rows of ", k, " values expected, got ", row_length(x, map));
+  TORCH_CHECK_VALUE(n >= 1, "a weight of at least one row expected");
+  check_param(bias, x, n, "bias");
+  return map;
+}
+
+bool check_weight8(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t dim) {
+  TORCH_CHECK_VALUE(weight.dim() == 2, "weight [N, K] expected");
+  TORCH_CHECK_VALUE(weight.device() == x.device(), "input and weight must be on one device");
+  TORCH_CHECK_TYPE(weight.scalar_type() == at::kFloat || weight.scalar_type() == x.scalar_type(), "weight must be float32 or ",
+                   x.scalar_type(), ", got ", weight.scalar_type());
+  return check_linear8(x, weight.size(0), weight.size(1), bias, dim);
+}
+
+Tensor result_like(const Tensor& x, bool map, int64_t n) {
+  if (map) {
+    const int64_t b = x.size(0), h = x.size(2), w = x.size(3);
+    return at::detail::empty_strided_cuda({b, n, h, w}, {h * w * n, 1, w * n, n}, x.scalar_type(), x.device());
+  }
+  c10::DimVector sizes(x.sizes());
+  sizes.back() = n;
+  return at::detail::empty_cuda(sizes, x.scalar_type(), x.device(), std::nullopt);
+}
+
+// What the gradients need of a forward pass: x and w along their columns.
+struct Across {
+  Held8 x, w;
+};
+
+// y of values and a weight, which are brought to 8 bits; `across`: where wanted, along the columns in the same reads.
+Tensor linear8_run(const Tensor& x, bool map, const Tensor& weight, const Tensor& bias, int act, bool across_x, bool across_w,
+                   Across& across) {
+  const int64_t n = weight.size(0), k = weight.size(1);
+  Tensor y = result_like(x, map, n);
+  const Rows w = rows_of(weight, false);
+  const Held8 wh = new_held(x, {n}, k);
+  if (across_w) across.w = new_held(x, {k}, n);
+  quantize(w, wh, across.w, Tensor(), x);
+  const int64_t m = row_count(x, map);
+  if (across_x) across.x = new_held(x, {k}, std::max<int64_t>(m, 1));
+  if (!m) return y;
+  const Rows r = rows_of(x, map);
+  const Tensor b = dense(bias);
+  if (!across_x) {
+    product_of_values(r, wh, n, b, act, y);
+  } else if (m <= KAD_GEMM8_FEW) {
+    quantize(r, {}, across.x, Tensor(), x);
+    product(r.held, Tensor(), r.rs, wh, m, n, k, b, act, y);
+  } else {
+    const Held8 h = new_held(x, {m}, k);
+    quantize(r, h, across.x, Tensor(), x);
+    product(h.codes, h.scales, 0, wh, m, n, k, b, act, y);
+  }
+  return y;
+}
+
+struct Linear8Sizes {
+  int64_t m, n, k, dim;
+  at::ScalarType x, weight, bias;
+};
+
+// x: for its sizes and device.  dx, dw and db of dy, those that are needed.
+std::tuple<Tensor, Tensor, Tensor> linear8_gradients(const Tensor& dy, bool map, const Linear8Sizes& o, const Across& across,
+                                                     bool need_x, bool need_weight, bool need_bias) {
+  Tensor dx = need_x ? result_like(dy, map, o.k) : Tensor();
+  Tensor dw = need_weight ? at::detail::empty_cuda({o.n, o.k}, o.weight, dy.device(), std::nullopt) : Tensor();
+  Tensor db = need_bias ? at::detail::empty_cuda({o.n}, o.bias, dy.device(), std::nullopt) : Tensor();
+  if (!o.m) {  // sums over nothing
+    if (need_weight) dw.zero_();
+    if (need_bias) db.zero_();
+    return {dx, dw, db};
+  }
+  if (!(need_x || need_weight || need_bias)) return {};
+  const Rows r = rows_of(dy, map);
+  const bool in_memory = need_x && o.m > KAD_GEMM8_FEW;
+  Held8 along, down;
+  if (in_memory) along = new_held(dy, {o.m}, o.n);
+  if (need_weight) down = new_held(dy, {o.n}, o.m);
+  if (in_memory || need_weight || need_bias) quantize(r, along, down, db, dy);
+  if (in_memory) product(along.codes, along.scales, 0, across.w, o.m, o.k, o.n, Tensor(), KAD_ACT_NONE, dx);
+  else if (need_x) product(r.held, Tensor(), r.rs, across.w, o.m, o.k, o.n, Tensor(), KAD_ACT_NONE, dx);
+  if (need_weight) product(down.codes, down.scales, 0, across.x, o.n, o.k, o.m, Tensor(), KAD_ACT_NONE, dw);
+  return {dx, dw, db};
+}
+
+struct Linear8Backward : torch::autograd::Node {
+  torch::autograd::SavedVariable x_codes, x_scales, w_codes, w_scales;  // along their columns
+  Linear8Sizes o;
+  bool map, has_x, has_w;
+  c10::DimVector sizes;  // of y
+
+  std::string name() const override { return "Linear8Backward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto* v : {&x_codes, &x_scales, &w_codes, &w_scales}) v->reset_data();
+  }
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    torch::autograd::variable_list out(3);
+    const Tensor& dy = grads[0];
+    if (!dy.defined()) return out;
+    TORCH_CHECK_VALUE(dy.is_cuda() && dy.sizes() == at::IntArrayRef(sizes), "dy must have the result's shape and device");
+    TORCH_CHECK_TYPE(dy.scalar_type() == o.x, "dy must have the result's dtype");
+    const bool need_x = has_w && task_should_compute_output(0), need_w = has_x && task_should_compute_output(1),
+               need_b = task_should_compute_output(2);
+    Across across;
+    if (need_w) {
+      across.x = {x_codes.unpack(), x_scales.unpack()};
+      check_held(across.x.codes, across.x.scales, o.k, std::max<int64_t>(o.m, 1), dy, "the saved input");
+    }
+    if (need_x) {
+      across.w = {w_codes.unpack(), w_scales.unpack()};
+      check_held(across.w.codes, across.w.scales, o.k, o.n, dy, "the saved weight");
+    }
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const c10::DeviceGuard guard(dy.device());
+      std::tie(out[0], out[1], out[2]) = linear8_gradients(dy, map, o, across, need_x, need_w, need_b);
+    }
+    // rounding to 8 bits has no second derivative
+    if (c10::GradMode::is_enabled()) out = once_differentiable(std::move(out), "kadconv.linear8");
+    return out;
+  }
+};
+
+// None where the call is observed.
+OptTensor linear8(const Tensor& x, const Tensor& weight, const OptTensor& bias, const std::optional<std::string_view>& act, int64_t dim) {
+  const Tensor b = defined(bias);
+  if (observed({&x, &weight, &b})) return std::nullopt;
+  const bool map = check_weight8(x, weight, b, dim);
+  const int ac = checked_act(act);
+  check_no_forward_grad({&x, &weight, &b}, "kadconv.linear8");
+  const bool grad = torch::autograd::compute_requires_grad(x, weight, b);
+  TORCH_CHECK_NOT_IMPLEMENTED(!grad || ac == KAD_ACT_NONE, "kadconv.linear8 with an activation has no gradient");
+  std::shared_ptr<Linear8Backward> node;
+  Tensor y;
+  Across across;
+  if (grad) node = new_node<Linear8Backward>(torch::autograd::collect_next_edges(x, weight, b));
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::DeviceGuard guard(x.device());
+    y = linear8_run(x, map, weight, b, ac, node && weight.requires_grad(), node && x.requires_grad(), across);
+  }
+  if (node) {
+    node->o = {row_count(x, map), weight.size(0), weight.size(1), dim, x.scalar_type(), weight.scalar_type(),
+               b.defined() ? b.scalar_type() : at::kFloat};
+    node->map = map;
+    node->sizes = c10::DimVector(y.sizes());
+    node->has_x = across.x.defined();
+    node->has_w = across.w.defined();
+    if (node->has_x) {
+      node->x_codes = torch::autograd::SavedVariable(across.x.codes, false);
+      node->x_scales = torch::autograd::SavedVariable(across.x.scales, false);
+    }
+    if (node->has_w) {
+      node->w_codes = torch::autograd::SavedVariable(across.w.codes, false);
+      node->w_scales = torch::autograd::SavedVariable(across.w.scales, false);
+    }
+    torch::autograd::set_history(y, node);
+  }
+  return y;
+}
+
+Tensor linear8_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, const std::optional<std::string_view>& act, int64_t dim) {
+  const Tensor b = defined(bias);
+  const bool map = check_weight8(x, weight, b, dim);
+  const int ac = checked_act(act);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x.device());
+  Across across;
+  return linear8_run(x, map, weight, b, ac, false, false, across);
+}
+
+std::tuple<OptTensor, OptTensor, OptTensor> linear8_backward(const Tensor& dy, const Tensor& x, const Tensor& weight, const OptTensor& bias,
+                                                             int64_t dim, bool need_x, bool need_weight, bool need_bias) {
+  const Tensor b = defined(bias);
+  const bool map = check_weight8(x, weight, b, dim);
+  const Linear8Sizes o{row_count(x, map), weight.size(0), weight.size(1), dim, x.scalar_type(), weight.scalar_type(),
+                       b.defined() ? b.scalar_type() : at::kFloat};
+  c10::DimVector sizes(x.sizes());
+  sizes[map ? 1 : x.dim() - 1] = o.n;
+  TORCH_CHECK_VALUE(dy.device() == x.device() && dy.sizes() == at::IntArrayRef(sizes), "dy must have the result's shape and device");
+  TORCH_CHECK_TYPE(dy.scalar_type() == o.x, "dy must have the result's dtype");
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x.device());
+  Across across;
+  if (need_weight && o.m) {
+    across.x = new_held(x, {o.k}, o.m);
+    quantize(rows_of(x, map), {}, across.x, Tensor(), x);
+  }
+  if (need_x && o.m) {
+    across.w = new_held(x, {o.k}, o.n);
+    quantize(rows_of(weight, false), {}, across.w, Tensor(), x);
+  }
+  auto [dx, dw, db] = linear8_gradients(dy, map, o, across, need_x, need_weight, need_bias && b.defined());
+  return {opt(dx), opt(dw), opt(db)};
+}
+
+// With a weight that is kept in 8 bits.  None where the call is observed.
+Tensor linear8_kept_run(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t k, const Tensor& b,
+                        const std::optional<std::string_view>& act, int64_t dim) {
+  TORCH_CHECK_VALUE(codes.dim() == 2, "a weight [N, K] expected");
+  const int64_t n = codes.size(0);
+  const bool map = check_linear8(x, n, k, b, dim);
+  check_held(codes, scales, n, k, x, "weight");
+  const int ac = checked_act(act);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x.device());
+  Tensor y = result_like(x, map, n);
+  if (y.numel()) product_of_values(rows_of(x, map), {codes, scales}, n, dense(b), ac, y);
+  return y;
+}
+
+OptTensor linear8_kept(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t k, const OptTensor& bias,
+                       const std::optional<std::string_view>& act, int64_t dim) {
+  const Tensor b = defined(bias);
+  if (observed({&x, &codes, &scales, &b})) return std::nullopt;
+  check_no_forward_grad({&x, &b}, "kadconv.linear8");
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::compute_requires_grad(x, b), "kadconv.linear8 with a weight in 8 bits has no gradient");
+  return linear8_kept_run(x, codes, scales, k, b, act, dim);
+}
+
+Tensor linear8_kept_forward(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t k, const OptTensor& bias,
+                            const std::optional<std::string_view>& act, int64_t dim) {
+  return linear8_kept_run(x, codes, scales, k, defined(bias), act, dim);
+}
+
 }  // namespace
 
 void kad_torch::bind_rows(py::module_& m) {
   m.def("layer_norm", &layer_norm);
   m.def("layer_norm_forward", &layer_norm_forward);
   m.def("layer_norm_backward", &layer_norm_backward);
+  m.def("quantize8", &quantize8);
+  m.def("matmul8", &matmul8);
+  m.def("linear8", &linear8);
+  m.def("linear8_forward", &linear8_forward);
+  m.def("linear8_backward", &linear8_backward);
+  m.def("linear8_kept", &linear8_kept);
+  m.def("linear8_kept_forward", &linear8_kept_forward);
   m.def("distill_loss", &distill_loss);
   m.def("distill_loss_forward", &distill_loss_forward);
   m.def("distill_loss_backward", &distill_loss_backward);

@@ -178,12 +178,6 @@ struct GroupNormActBackward : torch::autograd::Node {
   }
 };
 
-// The activation's number, after its check.
-int checked_act(const std::optional<std::string_view>& act) {
-  TORCH_CHECK_VALUE(!act || *act == "relu" || *act == "silu", "act '", act.value_or(""), "' is none of None, 'relu', 'silu'");
-  return !act ? KAD_ACT_NONE : *act == "relu" ? KAD_ACT_RELU : KAD_ACT_SILU;
-}
-
 // None where the call is observed.
 OptTensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps,
                          const std::optional<std::string_view>& act) {

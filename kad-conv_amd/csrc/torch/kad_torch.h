@@ -71,6 +71,12 @@ inline bool observed(std::initializer_list<const Tensor*> tensors) {
   return false;
 }
 
+// The activation's number, after its check.
+inline int checked_act(const std::optional<std::string_view>& act) {
+  TORCH_CHECK_VALUE(!act || *act == "relu" || *act == "silu", "act '", act.value_or(""), "' is none of None, 'relu', 'silu'");
+  return !act ? KAD_ACT_NONE : *act == "relu" ? KAD_ACT_RELU : KAD_ACT_SILU;
+}
+
 // The entry points of kad_rows.cpp.
 void bind_rows(py::module_& m);
 

@@ -11,7 +11,8 @@ custom operators ``torch.ops.kadconv.deform_conv2d`` / ``layer_fwd`` /
 ``group_norm_act`` (kadconv.library).
 """
 from . import library  # registers the kadconv:: custom operators
-from .blocks import Conv1x1SiLU, GroupNormAct, KADDown, LayerNorm, SqueezeExcitation
+from .block8 import Block8, linear8, matmul8, quantize8
+from .blocks import Conv1x1SiLU, GroupNormAct, KADDown, LayerNorm, Linear8, SqueezeExcitation
 from .fast import disable_fast_inference, enable_fast_inference
 from .kad_conv import DSC, LCSA, KADConv
 from .ops import deform_conv2d, distill_loss, group_norm_act, layer_norm
@@ -19,4 +20,5 @@ from .optim import AdamW, AdamWPlan
 
 __all__ = ['KADConv', 'DSC', 'LCSA', 'enable_fast_inference', 'disable_fast_inference', 'deform_conv2d',
            'Conv1x1SiLU', 'SqueezeExcitation', 'KADDown', 'group_norm_act', 'GroupNormAct', 'AdamW', 'AdamWPlan',
-           'layer_norm', 'LayerNorm', 'distill_loss']
+           'layer_norm', 'LayerNorm', 'distill_loss',
+           'Block8', 'quantize8', 'matmul8', 'linear8', 'Linear8']

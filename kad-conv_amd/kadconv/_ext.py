@@ -128,6 +128,16 @@ class DistillArgs(ctypes.Structure):
                [(f, c_int) for f in ('reduction', 'dtype', 'teacher_dtype', 'index_bits')]
 
 
+class Quant8Args(ctypes.Structure):
+    _fields_ = [(f, c_vp) for f in ('x', 'codes', 'scales', 't_codes', 't_scales', 'sums', 'work')] + \
+               [('rows', c_i64), ('x_rs', c_i64), ('c', c_int), ('dtype', c_int), ('sums_dtype', c_int)]
+
+
+class Gemm8Args(ctypes.Structure):
+    _fields_ = [(f, c_vp) for f in ('a', 'a_scales', 'b', 'b_scales', 'bias', 'out', 'work')] + [('a_rs', c_i64)] + \
+               [(f, c_int) for f in ('m', 'n', 'k', 'act', 'dtype', 'a_dtype', 'bias_dtype')]
+
+
 class AdamwChunk(ctypes.Structure):
     _fields_ = [('param', c_vp), ('grad', c_vp), ('offset', c_i64), ('count', c_int), ('reserved', c_int)]
 
@@ -143,6 +153,7 @@ class AdamwArgs(ctypes.Structure):
 ADAMW_SEG = 256          # KAD_ADAMW_SEG
 LAYER_NORM_MOST = 16384  # KAD_LAYER_NORM_MOST
 DISTILL_MOST = 1024      # KAD_DISTILL_MOST
+QUANT8_MOST = 1 << 20    # KAD_QUANT8_MOST
 ADAMW_SCALARS = 4        # 4-byte words of kad_adamw_scalars
 
 
@@ -224,6 +235,10 @@ SIGNATURES = {
     'kad_distill_work_elems': (c_i64, [ctypes.POINTER(DistillArgs)]),
     'kad_distill_fwd': (c_int, [ctypes.POINTER(DistillArgs), c_vp]),
     'kad_distill_bwd': (c_int, [ctypes.POINTER(DistillArgs), c_vp]),
+    'kad_quant8_work_elems': (c_i64, [ctypes.POINTER(Quant8Args)]),
+    'kad_quant8': (c_int, [ctypes.POINTER(Quant8Args), c_vp]),
+    'kad_gemm8_work_elems': (c_i64, [ctypes.POINTER(Gemm8Args)]),
+    'kad_gemm8': (c_int, [ctypes.POINTER(Gemm8Args), c_vp]),
     'kad_adamw_chunks': (c_i64, [c_vp, c_vp, c_vp, c_int, c_int, c_vp, ctypes.POINTER(c_i64)]),
     'kad_adamw_step': (c_int, [ctypes.POINTER(AdamwArgs), c_vp]),
     'kad_adamw_hyper': (c_int, [ctypes.POINTER(AdamwArgs), c_vp, c_vp, c_vp, c_vp]),

@@ -15,16 +15,17 @@
 * ``GroupNormAct`` -- group norm and an activation on channels-last maps, for
   layers trained at a batch too small for batch statistics.
 * ``LayerNorm`` -- layer norm of rows or of each pixel's channels.
+* ``Linear8`` -- a linear layer or 1 x 1 convolution whose products are in 8 bits.
 
 The first three: eval-mode GPU inputs run the HIP kernels (no fallback: a missing library
 raises); training mode or CPU inputs run the plain torch composition.
-``GroupNormAct`` and ``LayerNorm`` run them in training mode too: their kernels have a backward.
+``GroupNormAct``, ``LayerNorm`` and ``Linear8`` run them in training mode too: their kernels have a backward.
 """
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import _ext, ops
+from . import _ext, block8, ops
 
 
 def _use_hip(module, x):
@@ -191,3 +192,46 @@ class LayerNorm(nn.Module):
 
     def extra_repr(self):
         return f'{self.num_channels}, eps={self.eps}, affine={self.weight is not None}, dim={self.dim}'
+
+
+class Linear8(nn.Module):
+    """x W^T + b along the last axis or, with ``dim=1``, of each pixel of a map [N, C, H, W] (a 1 x 1 convolution), the
+    products in 8 bits (``kadconv.linear8``); parameters as torch.nn.Linear's, so its state dicts load.
+
+    In eval mode, where nothing is differentiated, W is kept in 8 bits and laid out anew when it has changed (seen by its
+    version: a write through ``.data`` is not), and ``act`` is applied in the same launch.  Other calls go by W itself."""
+
+    def __init__(self, in_features, out_features, bias=True, act=None, dim=-1):
+        super().__init__()
+        if in_features < 1 or out_features < 1:
+            raise ValueError(f'positive sizes expected, got {in_features} and {out_features}')
+        if act not in (None, 'relu', 'silu'):
+            raise ValueError(f"act {act!r} is none of None, 'relu', 'silu'")
+        if dim not in (-1, 1):
+            raise ValueError(f'dim must be -1 or 1, got {dim}')
+        self.in_features, self.out_features, self.act, self.dim = in_features, out_features, act, dim
+        like = nn.Linear(in_features, out_features, bias)
+        self.weight, self.bias = like.weight, like.bias
+        self._kept = None  # (weight, its version, the weight in 8 bits)
+
+    def __getstate__(self):
+        return {**self.__dict__, '_kept': None}  # a copy of the module lays out its own
+
+    def _weight8(self):
+        w, kept = self.weight.detach(), self._kept
+        if w.is_inference():
+            return block8.quantize8(w)
+        # the weight that was laid out is held, so that its address is no other's
+        if kept is None or kept[0].data_ptr() != w.data_ptr() or (kept[0].dtype, kept[1]) != (w.dtype, self.weight._version):
+            kept = self._kept = w, self.weight._version, block8.quantize8(w)
+        return kept[2]
+
+    def forward(self, x):
+        grad = torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters()))
+        if grad and self.act is not None:
+            return {'relu': F.relu, 'silu': F.silu}[self.act](block8.linear8(x, self.weight, self.bias, None, self.dim))
+        keep = not (grad or self.training or torch.compiler.is_compiling()) and x.is_cuda
+        return block8.linear8(x, self._weight8() if keep else self.weight, self.bias, self.act, self.dim)
+
+    def extra_repr(self):
+        return f'{self.in_features}, {self.out_features}, bias={self.bias is not None}, act={self.act!r}, dim={self.dim}'

@@ -24,6 +24,11 @@ shapes instead of breaking the graph at an opaque Python call:
       kadconv::group_norm_act_backward.
   kadconv::layer_norm(x, weight?, bias?, eps, dim) -> (Tensor y, Tensor mean, Tensor rstd)
       kadconv.ops.layer_norm, likewise, with kadconv::layer_norm_backward.
+  kadconv::linear8(x, weight, bias?, act?, dim) -> Tensor
+  kadconv::linear8_kept(x, codes, scales, size, bias?, act?, dim) -> Tensor
+  kadconv::quantize8(x, dim) -> (Tensor codes, Tensor scales)
+  kadconv::matmul8(a_codes, a_scales, b_codes, b_scales, size, bias?, act?, dtype) -> Tensor
+      those of kadconv.block8; the first's gradient is kadconv::linear8_backward.
   kadconv::distill_loss(logits, teacher_logits, teacher_index, temperature, reduction, dim)
         -> (Tensor loss, Tensor stats, Tensor share)
       kadconv.ops.distill_loss, likewise, with kadconv::distill_loss_backward.
@@ -245,3 +250,83 @@ def _distill_loss_grad(ctx, dloss, _stats, _share):
 
 
 distill_loss.register_autograd(_distill_loss_grad, setup_context=_distill_loss_context)
+
+
+@torch.library.custom_op('kadconv::quantize8', mutates_args=())
+def quantize8(x: torch.Tensor, dim: int) -> tuple[torch.Tensor, torch.Tensor]:
+    from . import _ext
+    return _ext.native().quantize8(x, dim)
+
+
+@quantize8.register_fake
+def _(x, dim):
+    from . import ops
+    axis = ops._row_axis(x, dim)
+    shape = [n for d, n in enumerate(x.shape) if d != axis]
+    blocks = -(-x.shape[axis] // 128)
+    return (x.new_empty((*shape, blocks * 128), dtype=torch.float8_e4m3fn),
+            x.new_empty((*shape, -(-blocks // 4) * 4), dtype=torch.float8_e8m0fnu))
+
+
+@torch.library.custom_op('kadconv::matmul8', mutates_args=())
+def matmul8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, size: int,
+            bias: torch.Tensor | None, act: str | None, dtype: torch.dtype) -> torch.Tensor:
+    from . import _ext
+    return _ext.native().matmul8(a, a_scales, b, b_scales, size, bias, act, dtype)
+
+
+@matmul8.register_fake
+def _(a, a_scales, b, b_scales, size, bias, act, dtype):
+    return a.new_empty((*a.shape[:-1], b.shape[0]), dtype=dtype)
+
+
+@torch.library.custom_op('kadconv::linear8', mutates_args=())
+def linear8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, act: str | None, dim: int) -> torch.Tensor:
+    from . import block8
+    return block8.linear8_forward(x, weight, bias, act, dim)
+
+
+@linear8.register_fake
+def _(x, weight, bias, act, dim):
+    return _rows_empty(x, dim, weight.shape[0])
+
+
+@torch.library.custom_op('kadconv::linear8_backward', mutates_args=())
+def linear8_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
+                     dim: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    from . import block8
+    dx, dw, db = block8.linear8_backward(dy, x, weight, bias, dim)
+    return dx, dw, dw.new_empty(0) if db is None else db
+
+
+@linear8_backward.register_fake
+def _(dy, x, weight, bias, dim):
+    dw = torch.empty_like(weight, memory_format=torch.contiguous_format)
+    return _rows_empty(x, dim), dw, dw.new_empty(0) if bias is None else torch.empty_like(bias, memory_format=torch.contiguous_format)
+
+
+def _linear8_context(ctx, inputs, output):
+    x, weight, bias, _, dim = inputs
+    ctx.save_for_backward(x, weight, bias)
+    ctx.dim = dim
+
+
+def _linear8_grad(ctx, dy):
+    x, weight, bias = ctx.saved_tensors
+    dx, dw, db = torch.ops.kadconv.linear8_backward(dy, x, weight, bias, ctx.dim)
+    return dx, dw, None if bias is None else db, None, None
+
+
+linear8.register_autograd(_linear8_grad, setup_context=_linear8_context)
+
+
+@torch.library.custom_op('kadconv::linear8_kept', mutates_args=())
+def linear8_kept(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, size: int, bias: torch.Tensor | None,
+                 act: str | None, dim: int) -> torch.Tensor:
+    from . import _ext
+    return _ext.native().linear8_kept_forward(x, codes, scales, size, bias, act, dim)
+
+
+@linear8_kept.register_fake
+def _(x, codes, scales, size, bias, act, dim):
+    return _rows_empty(x, dim, codes.shape[0])

@@ -182,3 +182,147 @@ def test_distill_work():
             for dtype in (0, 1):
                 n = work(rows=rows, v=v, z_rs=v, dtype=dtype)
                 assert 2 * rows <= n <= 2 * rows + 2 * rows * 256
+
+
+# ---------------------------------------------------------------------------- products in 8 bits
+def test_quantize8_plain():
+    from tests._block8_ref import held, numbers
+    g = torch.Generator().manual_seed(2)
+    for k in (1, 100, 128, 129, 700):
+        x = torch.randn(5, k, generator=g) * torch.exp(3 * torch.randn(5, k, generator=g))
+        x[0, 0] = float('nan')
+        x[1] = 0
+        q = kadconv.quantize8(x)
+        codes, powers = held(x)
+        assert q.shape == (5, k) and q.codes.shape[1] == -(-k // 128) * 128 and q.scales.shape[1] % 4 == 0
+        got = q.codes[:, :k].float().double()
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(codes)) and torch.equal(torch.isnan(got), torch.isnan(codes))
+        assert torch.equal(q.scales.view(torch.uint8)[:, :powers.shape[1]].int() - 127, powers.int())
+        assert torch.equal(torch.nan_to_num(q.dequantize(torch.float64)), torch.nan_to_num(numbers(x)))
+
+
+def test_linear8_plain():
+    from tests._block8_ref import numbers
+    g = torch.Generator().manual_seed(3)
+    x, w, b, dy = (torch.randn(*s, generator=g) for s in ((2, 6, 3, 4), (5, 6), (5,), (2, 5, 3, 4)))
+    rows, drows = x.permute(0, 2, 3, 1).reshape(-1, 6), dy.permute(0, 2, 3, 1).reshape(-1, 5)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = kadconv.linear8(*leaves, dim=1)
+    want = numbers(rows) @ numbers(w).t() + b.double()
+    assert torch.allclose(y.permute(0, 2, 3, 1).reshape(-1, 5).double(), want, atol=1e-5)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    assert torch.allclose(dx.permute(0, 2, 3, 1).reshape(-1, 6).double(), numbers(drows) @ numbers(w.t()).t(), atol=1e-5)
+    assert torch.allclose(dw.double(), numbers(drows.t()) @ numbers(rows.t()).t(), atol=1e-5)
+    assert torch.allclose(db, drows.sum(0), atol=1e-5)
+    kept = kadconv.quantize8(w)
+    served = kadconv.linear8(x, kept, b, 'silu', dim=1)
+    assert torch.allclose(served, torch.nn.functional.silu(y.detach()), atol=1e-5)
+    assert torch.equal(kadconv.linear8(x, w, b, 'silu', dim=1), served)
+    z = kadconv.matmul8(kadconv.quantize8(x, dim=1), kept, b, 'relu', torch.float32)
+    assert torch.allclose(z.permute(0, 3, 1, 2), y.detach().clamp(min=0), atol=1e-5)
+    m = kadconv.Linear8(6, 5, act='silu', dim=1)
+    m.load_state_dict(torch.nn.Linear(6, 5).state_dict())
+    m(x).sum().backward()
+    assert m.weight.grad.shape == (5, 6)
+    m.eval()
+    with torch.no_grad():
+        assert m(x).shape == (2, 5, 3, 4)
+    x0 = torch.empty(0, 6, requires_grad=True)
+    assert not torch.autograd.grad(kadconv.linear8(x0, leaves[1]).sum(), leaves[1])[0].any()
+
+
+def test_block8_refusals():
+    x, w = torch.randn(3, 40), torch.randn(5, 40)
+    q = kadconv.quantize8(w)
+    for args in ((q.codes, q.scales, 129), (q.codes, q.scales, 0), (q.codes[:4], q.scales, 40), (q.codes, q.scales[:, :1], 40)):
+        with pytest.raises(ValueError):
+            kadconv.Block8(*args)
+    with pytest.raises(TypeError):
+        kadconv.Block8(q.codes.view(torch.uint8), q.scales, 40)
+    for bad in (x.double(), x.long()):
+        with pytest.raises(TypeError):
+            kadconv.quantize8(bad)
+        with pytest.raises(TypeError):
+            kadconv.linear8(bad, q)
+    with pytest.raises(ValueError):
+        kadconv.quantize8(x[:, :0])
+    with pytest.raises(ValueError, match='dim must'):
+        kadconv.quantize8(x, dim=0)
+    for args, match in (((x[:, :39], w), 'rows of 40'), ((x, w[0]), 'weight'), ((x, w, torch.zeros(4)), 'bias'),
+                        ((x, w, None, 'gelu'), 'act')):
+        with pytest.raises(ValueError, match=match):
+            kadconv.linear8(*args)
+    with pytest.raises(TypeError, match='weight'):
+        kadconv.linear8(x, w.half())
+    with pytest.raises(NotImplementedError, match='8 bits'):
+        kadconv.linear8(x.requires_grad_(True), q)
+    with pytest.raises(NotImplementedError, match='activation'):
+        kadconv.linear8(x, w, act='relu')
+    x = x.detach()
+    with pytest.raises(TypeError, match='Block8'):
+        kadconv.matmul8(x, q)
+    with pytest.raises(ValueError, match='expected'):
+        kadconv.matmul8(kadconv.quantize8(x[:, :39]), q)
+    with pytest.raises(TypeError, match='dtype'):
+        kadconv.matmul8(kadconv.quantize8(x), q, dtype=torch.float64)
+    with pytest.raises(ValueError, match='bias'):
+        kadconv.matmul8(kadconv.quantize8(x), q, torch.zeros(4))
+    for args in ((0, 4), (4, 0), (4, 4, True, 'tanh'), (4, 4, True, None, 2)):
+        with pytest.raises(ValueError):
+            kadconv.Linear8(*args)
+    with pytest.raises(ValueError, match='GPU'):
+        _ext.native().linear8(x, w, None, None, -1)
+    with pytest.raises(ValueError, match='GPU'):
+        _ext.native().quantize8(x, -1)
+
+
+def _quant_args(**kw):
+    a = _ext.Quant8Args()
+    for f in ('x', 'codes', 'scales', 't_codes', 't_scales', 'sums', 'work'):
+        setattr(a, f, 4096)
+    a.rows, a.x_rs, a.c, a.dtype, a.sums_dtype = 3, 8, 8, 1, 0
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize('kw', [dict(x=None), dict(codes=None), dict(scales=None), dict(t_codes=None), dict(codes=4104), dict(work=None),
+                                dict(rows=0), dict(rows=1 << 31), dict(c=0), dict(c=(1 << 20) + 1), dict(x_rs=7), dict(x_rs=1 << 31),
+                                dict(dtype=3), dict(sums_dtype=3), dict(rows=1 << 30, c=1 << 20, x_rs=1 << 20),
+                                dict(codes=None, scales=None, t_codes=None, t_scales=None, sums=None)], ids=str)
+def test_quant8_c_refuses(kw):
+    lib = _ext.load()
+    assert lib.kad_quant8(ctypes.byref(_quant_args(**kw)), None) == -1
+    assert b'kad_quant8' in lib.kad_last_error()
+
+
+def _gemm_args(**kw):
+    a = _ext.Gemm8Args()
+    for f in ('a', 'a_scales', 'b', 'b_scales', 'bias', 'out', 'work'):
+        setattr(a, f, 4096)
+    a.a_rs, a.m, a.n, a.k, a.dtype = 8, 3, 4, 8, 1
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize('kw', [dict(a=None), dict(b=None), dict(b_scales=None), dict(out=None), dict(m=0), dict(n=0), dict(k=0),
+                                dict(k=(1 << 20) + 1), dict(m=(1 << 31) - 100), dict(act=7), dict(dtype=5), dict(bias_dtype=-1),
+                                dict(a_scales=None, m=65), dict(a_scales=None, a_rs=7), dict(a_scales=None, a_dtype=4), dict(b=4104),
+                                dict(a=4104), dict(b_scales=4098), dict(a_scales=4098), dict(m=1 << 20, n=1 << 20),
+                                dict(m=100, k=100000, work=None)], ids=str)
+def test_gemm8_c_refuses(kw):
+    lib = _ext.load()
+    assert lib.kad_gemm8(ctypes.byref(_gemm_args(**kw)), None) == -1
+    assert b'kad_gemm8' in lib.kad_last_error()
+
+
+def test_gemm8_parts_cover_k():
+    """Floats of scratch: none, or one matrix for each part of k."""
+    lib = _ext.load()
+    for m in (1, 64, 65, 1000, 70000):
+        for n in (1, 300, 5000):
+            for k in (1, 128, 1000, 20000, 1 << 20):
+                for dtype in (0, 1):
+                    w = lib.kad_gemm8_work_elems(ctypes.byref(_gemm_args(m=m, n=n, k=k, dtype=dtype)))
+                    assert w >= 0 and w % (m * n) == 0 and w // (m * n) != 1 and w // (m * n) <= 512
