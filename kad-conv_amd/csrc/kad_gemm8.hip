@@ -25,8 +25,10 @@ typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
 constexpr int LINE = BLOCK8;        // bytes of a row in a stage: one block of codes
 constexpr int KB_GROUP = 4;         // scales are read by fours
 
+// For 16-bit results the hardware's reciprocal alone, off by one step of 32 bits at most.
+template <typename T>
 __device__ __forceinline__ float activate(float z, int act) {
-  if (act == KAD_ACT_SILU) return z * sigmoidf_(z);
+  if (act == KAD_ACT_SILU) return sizeof(T) == 2 ? z * __builtin_amdgcn_rcpf(1.0f + __expf(-z)) : z * sigmoidf_(z);
   return act == KAD_ACT_RELU ? (z > 0.f ? z : z != z ? z : 0.f) : z;
 }
 
@@ -86,22 +88,18 @@ __device__ __forceinline__ void store_four(T* p, const float* v, int n) {
   }
 }
 
-// Four results of row m from column n on; parts: 32-bit sums that are joined later, in place of out.
 template <typename T>
-__device__ __forceinline__ void finish(const kad_gemm8_args& a, float* part, int m, int n, const floatx4& acc) {
+__device__ __forceinline__ float bias_at(const kad_gemm8_args& a, int n) {
+  return a.bias && n < a.n ? load_param(a.bias, n, a.bias_dtype, 0.f) : 0.f;
+}
+
+// Four results of row m from column n on.
+template <typename T>
+__device__ __forceinline__ void finish(const kad_gemm8_args& a, int m, int n, const floatx4& acc) {
   if (m >= a.m || n >= a.n) return;
   float v[4];
-  if (part) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = acc[i];
-    store_four<float>(part + (int64_t)m * a.n + n, v, a.n - n);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float b = a.bias && n + i < a.n ? load_param(a.bias, n + i, a.bias_dtype, 0.f) : 0.f;
-    v[i] = activate(acc[i] + b, a.act);
-  }
+  for (int i = 0; i < 4; ++i) v[i] = activate<T>(acc[i] + bias_at<T>(a, n + i), a.act);
   store_four<T>((T*)a.out + (int64_t)m * a.n + n, v, a.n - n);
 }
 
@@ -127,10 +125,53 @@ __device__ __forceinline__ bool tile_of(const Tiles& o, int& m, int& n, int& spl
   return true;
 }
 
+// A wave's 16-bit results: two rows of fragments at a time by way of its part of LDS, so that whole lines are written.
+constexpr int store_bytes(int tn) { return 32 * (tn * 32 + 16); }
+template <typename T, int TM, int TN, int ACT>
+__device__ __forceinline__ void store_tile(const kad_gemm8_args& a, const floatx4 (&acc)[TM][TN], const float (&bias)[TN][4], char* lds,
+                                           int lane, int m1, int n1) {
+  constexpr int PITCH = TN * 32 + 16, PIECES = TN * 2, ROWS = 64 / PIECES;
+  const int r16 = lane & 15, g = lane >> 4, piece = lane % PIECES, row = lane / PIECES;
+  const int n = n1 + piece * 8, left = a.n - n;
+#pragma unroll
+  for (int i = 0; i < TM; i += 2) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        T t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = from_f32<T>(activate<T>(acc[i + h][j][e] + bias[j][e], ACT));
+        __builtin_memcpy(lds + (h * 16 + r16) * PITCH + (j * 16 + 4 * g) * 2, t, 8);
+      }
+    __builtin_amdgcn_wave_barrier();
+    intx4 v[32 / ROWS];
+#pragma unroll
+    for (int r = 0; r < 32 / ROWS; ++r) v[r] = *(const intx4*)(lds + (r * ROWS + row) * PITCH + piece * 16);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 32 / ROWS; ++r) {
+      const int m = m1 + i * 16 + r * ROWS + row;
+      if (m >= a.m || left <= 0) continue;
+      T* to = (T*)a.out + (int64_t)m * a.n + n;
+      if (left >= 8) {
+        __builtin_memcpy(to, &v[r], 16);
+      } else {
+        T t[8];
+        __builtin_memcpy(t, &v[r], 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < left) to[e] = t[e];
+      }
+    }
+  }
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN) void gemm8_tile_kernel(kad_gemm8_args a, Tiles o) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int CA = BM / 8 / WAVES, CB = BN / 8 / WAVES;  // copies of a wave and stage: 8 rows each
+  static_assert(WAVES % 2 == 0, "a wave's copies begin at rows 8 (wave & 1) of 16");
   __shared__ __attribute__((aligned(128))) char s0[(BM + BN) * LINE];
   __shared__ __attribute__((aligned(128))) char s1[(BM + BN) * LINE];
   int m0, n0, split;
@@ -144,8 +185,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm8_tile_kernel(kad_gemm8_args
   const int rows_a = a.m - m0 < BM ? a.m - m0 : BM, rows_b = a.n - n0 < BN ? a.n - n0 : BN;
   const __amdgpu_buffer_rsrc_t ra = make_rsrc((const char*)a.a + (int64_t)m0 * kp, rows_a * kp);
   const __amdgpu_buffer_rsrc_t rb = make_rsrc((const char*)a.b + (int64_t)n0 * kp, rows_b * kp);
-  // 16-byte piece p of row r lies at piece p ^ (r & 7) of its line: lanes that read one piece of eight rows meet all banks
-  const uint32_t off = (uint32_t)(lane >> 3) * kp + (((lane & 7) ^ (lane >> 3)) << 4);
+  // 16-byte piece p of row r lies at piece p ^ (r / 2 & 7) of its line: lanes that read one piece of 16 rows meet all 64 banks
+  const uint32_t off = (uint32_t)(lane >> 3) * kp + (((lane & 7) ^ ((wave & 1) << 2 | lane >> 4)) << 4);
   const auto stage = [&](char* s, int kb) {
 #pragma unroll
     for (int i = 0; i < CA; ++i) {
@@ -160,38 +201,42 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm8_tile_kernel(kad_gemm8_args
   };
   const int wm = wave / WN, wn = wave % WN, r16 = lane & 15, g = lane >> 4;
   const int line_a = (wm * TM * 16 + r16) * LINE, line_b = (BM + wn * TN * 16 + r16) * LINE;
-  const int piece0 = ((2 * g) ^ (r16 & 7)) << 4, piece1 = ((2 * g + 1) ^ (r16 & 7)) << 4;
+  const int piece0 = ((2 * g) ^ (r16 >> 1)) << 4, piece1 = ((2 * g + 1) ^ (r16 >> 1)) << 4;
   const auto fetch = [&](const char* s, int line, int frag, Operand<EXACT>& v) {
     const char* p = s + line + frag * 16 * LINE;
     v.set(*(const intx4*)(p + piece0), *(const intx4*)(p + piece1));
   };
-  // scales of the lane's rows, four blocks of k in each
-  const unsigned char *sa = (const unsigned char*)a.a_scales, *sb = (const unsigned char*)a.b_scales;
-  int32_t scale_a[TM], scale_b[TN];
+  // scales of the lane's rows, four blocks of k in each, a group ahead; past the last row 0, for codes of 0
+  const __amdgpu_buffer_rsrc_t rsa = make_rsrc((const char*)a.a_scales + (int64_t)m0 * ks, rows_a * ks);
+  const __amdgpu_buffer_rsrc_t rsb = make_rsrc((const char*)a.b_scales + (int64_t)n0 * ks, rows_b * ks);
+  const uint32_t off_sa = (uint32_t)(wm * TM * 16 + r16) * ks, off_sb = (uint32_t)(wn * TN * 16 + r16) * ks;
+  int scale_a[TM], scale_b[TN], next_a[TM], next_b[TN];
   const auto scales = [&](int kb) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int r = m0 + wm * TM * 16 + i * 16 + r16;
-      scale_a[i] = *(const int32_t*)(sa + (int64_t)(r < a.m ? r : a.m - 1) * ks + kb);
-    }
+    for (int i = 0; i < TM; ++i) next_a[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, off_sa + (uint32_t)(i * 16 * ks), kb, 0);
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-      const int r = n0 + wn * TN * 16 + i * 16 + r16;
-      scale_b[i] = *(const int32_t*)(sb + (int64_t)(r < a.n ? r : a.n - 1) * ks + kb);
-    }
+    for (int i = 0; i < TN; ++i) next_b[i] = __builtin_amdgcn_raw_buffer_load_b32(rsb, off_sb + (uint32_t)(i * 16 * ks), kb, 0);
   };
   floatx4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  scales(begin);
   stage(s0, begin);
+  // a's operands one ahead of the instructions that they feed
 #define KAD_STEP(Q, NOW, NEXT)                                                           \
   if (kb + Q < end) {                                                                    \
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");             \
+    if (Q == 0) {                                                                        \
+      _Pragma("unroll") for (int i = 0; i < TM; ++i) scale_a[i] = next_a[i];             \
+      _Pragma("unroll") for (int i = 0; i < TN; ++i) scale_b[i] = next_b[i];             \
+    }                                                                                    \
     if (kb + Q + 1 < end) stage(NEXT, kb + Q + 1);                                       \
-    Operand<EXACT> fb[TN], fa;                                                           \
+    if (Q == 0 && kb + KB_GROUP < end) scales(kb + KB_GROUP);                            \
+    Operand<EXACT> fb[TN], fa[2];                                                        \
     int eb[TN][4];                                                                       \
+    fetch(NOW, line_a, 0, fa[0]);                                                        \
     _Pragma("unroll") for (int j = 0; j < TN; ++j) {                                     \
       fetch(NOW, line_b, j, fb[j]);                                                      \
       if (EXACT) {                                                                       \
@@ -200,25 +245,54 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm8_tile_kernel(kad_gemm8_args
       }                                                                                  \
     }                                                                                    \
     _Pragma("unroll") for (int i = 0; i < TM; ++i) {                                     \
-      fetch(NOW, line_a, i, fa);                                                         \
+      if (i + 1 < TM) fetch(NOW, line_a, i + 1, fa[(i + 1) & 1]);                        \
       _Pragma("unroll") for (int j = 0; j < TN; ++j)                                     \
-        multiply<Q>(acc[i][j], fb[j], fa, scale_b[j], scale_a[i], eb[j]);                \
+        multiply<Q>(acc[i][j], fb[j], fa[i & 1], scale_b[j], scale_a[i], eb[j]);         \
+    }                                                                                    \
+    if (!EXACT) {                                                                        \
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 + 2 * TN, 0);                        \
+      _Pragma("unroll") for (int i = 0; i < TM; ++i) {                                   \
+        if (i + 1 < TM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);               \
+        __builtin_amdgcn_sched_group_barrier(0x008, TN, 0);                              \
+      }                                                                                  \
     }                                                                                    \
   }
   for (int kb = begin; kb < end; kb += KB_GROUP) {
-    scales(kb);
     KAD_STEP(0, s0, s1)
     KAD_STEP(1, s1, s0)
     KAD_STEP(2, s0, s1)
     KAD_STEP(3, s1, s0)
   }
 #undef KAD_STEP
-  float* part = o.splits > 1 ? a.work + (int64_t)split * a.m * a.n : nullptr;
+  const int m1 = m0 + wm * TM * 16, n1 = n0 + wn * TN * 16;
+  if (o.splits > 1) {  // 32-bit sums that are joined later
+    float* part = a.work + (int64_t)split * a.m * a.n;
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int m = m1 + i * 16 + r16, n = n1 + j * 16 + 4 * g;
+        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if (m < a.m && n < a.n) store_four<float>(part + (int64_t)m * a.n + n, v, a.n - n);
+      }
+    return;
+  }
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) finish<T>(a, m1 + i * 16 + r16, n1 + j * 16 + 4 * g, acc[i][j]);
+  } else {
+    float bias[TN][4];
 #pragma unroll
     for (int j = 0; j < TN; ++j)
-      finish<T>(a, part, m0 + (wm * TM + i) * 16 + r16, n0 + (wn * TN + j) * 16 + 4 * g, acc[i][j]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bias[j][i] = bias_at<T>(a, n1 + j * 16 + 4 * g + i);
+    __syncthreads();
+    if (a.act == KAD_ACT_SILU) store_tile<T, TM, TN, KAD_ACT_SILU>(a, acc, bias, s0 + wave * store_bytes(TN), lane, m1, n1);
+    else if (a.act == KAD_ACT_RELU) store_tile<T, TM, TN, KAD_ACT_RELU>(a, acc, bias, s0 + wave * store_bytes(TN), lane, m1, n1);
+    else store_tile<T, TM, TN, KAD_ACT_NONE>(a, acc, bias, s0 + wave * store_bytes(TN), lane, m1, n1);
+  }
 }
 
 // The parts of k, in order.
@@ -230,7 +304,7 @@ __global__ __launch_bounds__(256) void gemm8_join_kernel(kad_gemm8_args a, int s
 #pragma unroll 4
     for (int p = 1; p < splits; ++p) s += a.work[p * all + i];
     if (a.bias) s += load_param(a.bias, (int)(i % a.n), a.bias_dtype, 0.f);
-    ((T*)a.out)[i] = from_f32<T>(activate(s, a.act));
+    ((T*)a.out)[i] = from_f32<T>(activate<T>(s, a.act));
   }
 }
 
@@ -319,7 +393,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void gemm8_few_kernel(kad_gemm8_arg
     floatx4 s = red[0][i][lane];
     const int waves = blocks < FEW_WAVES ? blocks : FEW_WAVES;
     for (int w = 1; w < waves; ++w) s += red[w][i][lane];
-    finish<T>(a, nullptr, i * 16 + r16, n0 + 4 * g, s);
+    finish<T>(a, i * 16 + r16, n0 + 4 * g, s);
   }
 }
 
