@@ -295,6 +295,208 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm8_tile_kernel(kad_gemm8_args
   }
 }
 
+// Tiles of 256 x 256 results for 16-bit results: 8 waves of 128 x 64, the 32 x 32 x 64 instruction, and a ring of four stages
+// of 64 columns, so that three are on their way while one is used: with two stages of 128 the copies' latency was the step's
+// time (4900 cycles, of which the instructions take 2048).
+//
+// The copies are written as assembly: of ones that it knows the compiler waits for more than a step needs before it reads
+// LDS (it does not tell all stages apart), which ends the run ahead.  They write no register but m0, which nothing else
+// here uses, and every wait for them is one of KAD_STEP's.  Scales go the same way, two groups of four blocks in turn.
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+__device__ __forceinline__ intx4 resource(const void* base, uint32_t bytes) {
+  const uint64_t at = (uint64_t)base;
+  return intx4{__builtin_amdgcn_readfirstlane((int)(uint32_t)at), __builtin_amdgcn_readfirstlane((int)(at >> 32 & 0xFFFF)),
+               __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+// 16 or 4 bytes a lane from byte off + at of the resource to LDS, the lanes' one after the other; nothing is known to be
+// there before a wait for vmcnt.
+__device__ __forceinline__ void copy16(intx4 r, uint32_t lds, uint32_t off, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(r), "s"(at)
+               : "memory");
+}
+__device__ __forceinline__ void copy4(intx4 r, uint32_t lds, uint32_t off, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(r), "s"(at)
+               : "memory");
+}
+
+constexpr int WIDE = 256, HALF = 64;  // rows of a tile, bytes of a row in a stage
+
+template <typename T, int ACT>
+__device__ __forceinline__ void store_wide(const kad_gemm8_args& a, const floatx16 (&acc)[4][2], const float (&bias)[2][16], char* lds,
+                                           int lane, int m1, int n1) {
+  constexpr int PITCH = 64 * 2 + 16;
+  const int r32 = lane & 31, h = lane >> 5, piece = lane & 7, row = lane >> 3;
+  const int n = n1 + piece * 8, left = a.n - n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        T t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = from_f32<T>(activate<T>(acc[i][j][4 * q + e] + bias[j][4 * q + e], ACT));
+        __builtin_memcpy(lds + r32 * PITCH + (j * 32 + 8 * q + 4 * h) * 2, t, 8);
+      }
+    __builtin_amdgcn_wave_barrier();
+    intx4 v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = *(const intx4*)(lds + (r * 8 + row) * PITCH + piece * 16);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = m1 + i * 32 + r * 8 + row;
+      if (m >= a.m || left <= 0) continue;
+      T* to = (T*)a.out + (int64_t)m * a.n + n;
+      if (left >= 8) {
+        __builtin_memcpy(to, &v[r], 16);
+      } else {
+        T t[8];
+        __builtin_memcpy(t, &v[r], 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < left) to[e] = t[e];
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(512) void gemm8_wide_kernel(kad_gemm8_args a, Tiles o) {
+  __shared__ __attribute__((aligned(128))) char s0[2 * WIDE * HALF];
+  __shared__ __attribute__((aligned(128))) char s1[2 * WIDE * HALF];
+  __shared__ __attribute__((aligned(128))) char s2[2 * WIDE * HALF];
+  __shared__ __attribute__((aligned(128))) char s3[2 * WIDE * HALF];
+  __shared__ __attribute__((aligned(128))) char c0[2 * WIDE * 4], c1[2 * WIDE * 4];
+  int m0, n0, split;
+  if (!tile_of(o, m0, n0, split)) return;
+  m0 *= WIDE;
+  n0 *= WIDE;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int blocks = (a.k + BLOCK8 - 1) / BLOCK8, kp = blocks * BLOCK8, ks = (blocks + 3) / 4 * 4;
+  const int begin = split * o.per, end = begin + o.per < blocks ? begin + o.per : blocks, steps = 2 * (end - begin);
+  // rows past the last read as zeros
+  const int rows_a = a.m - m0 < WIDE ? a.m - m0 : WIDE, rows_b = a.n - n0 < WIDE ? a.n - n0 : WIDE;
+  const intx4 ra = resource((const char*)a.a + (int64_t)m0 * kp, rows_a * kp), rb = resource((const char*)a.b + (int64_t)n0 * kp, rows_b * kp);
+  // 16-byte piece p of row r lies at piece p ^ (r / 2 & 3) of its 64 bytes: lanes that read one piece of 8 rows meet 32 banks
+  const uint32_t off = (uint32_t)(lane >> 2) * kp + (((lane & 3) ^ (lane >> 3 & 3)) << 4);
+  const auto stage = [&](const char* s, int step) {
+    const uint32_t at = begin * BLOCK8 + step * HALF, to = lds_address(s);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = (i * 8 + wave) * 16;
+      copy16(ra, to + r * HALF, off + (uint32_t)r * kp, at);
+      copy16(rb, to + (WIDE + r) * HALF, off + (uint32_t)r * kp, at);
+    }
+  };
+  const int wm = wave >> 2, wn = wave & 3, r32 = lane & 31, h = lane >> 5;
+  const int line_a = (wm * 128 + r32) * HALF, line_b = (WIDE + wn * 64 + r32) * HALF;
+  const int piece0 = ((2 * h) ^ (r32 >> 1 & 3)) << 4, piece1 = ((2 * h + 1) ^ (r32 >> 1 & 3)) << 4;
+  const auto fetch = [&](const char* s, int line, int frag, intx8& v) {
+    const char* p = s + line + frag * 32 * HALF;
+    const intx4 lo = *(const intx4*)(p + piece0), hi = *(const intx4*)(p + piece1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+  };
+  // scales of 64 rows of a (the first four waves) or b, four blocks of k in each; past the last row 0, for codes of 0
+  const intx4 rs = wave < 4 ? resource((const char*)a.a_scales + (int64_t)m0 * ks, rows_a * ks)
+                            : resource((const char*)a.b_scales + (int64_t)n0 * ks, rows_b * ks);
+  const auto scales = [&](const char* s, int kb) {
+    copy4(rs, lds_address(s) + wave * 256, (uint32_t)((wave & 3) * 64 + lane) * ks, kb < ks - 4 ? kb : ks - 4);
+  };
+  int scale_a[4], scale_b[2];
+  floatx16 acc[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  scales(c0, begin);
+  stage(s0, 0);
+  stage(s1, 1);
+  if (2 < steps) stage(s2, 2);
+  // Step s uses what was copied three steps ago: of the wave's own copies, those of the two stages after it (4 each) may be
+  // under way, and in two steps the one of scales between them.
+#define KAD_STEP(H, NOW, LATER)                                                                              \
+  if (base + H < steps) {                                                                                    \
+    if (base + H + 2 < steps) {                                                                              \
+      if (H % 8 == 5 || H % 8 == 6) asm volatile("s_waitcnt vmcnt(9) lgkmcnt(0)\n\ts_barrier" ::: "memory"); \
+      else asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");                          \
+    } else {                                                                                                 \
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");                               \
+    }                                                                                                        \
+    if (H % 8 == 4) scales(H < 8 ? c1 : c0, begin + (base + H + 4) / 2);                                     \
+    if (base + H + 3 < steps) stage(LATER, base + H + 3);                                                    \
+    if (H % 8 == 0) {                                                                                        \
+      const int* c = (const int*)(H < 8 ? c0 : c1);                                                          \
+      _Pragma("unroll") for (int i = 0; i < 4; ++i) scale_a[i] = c[wm * 128 + i * 32 + r32];                 \
+      _Pragma("unroll") for (int i = 0; i < 2; ++i) scale_b[i] = c[WIDE + wn * 64 + i * 32 + r32];           \
+    }                                                                                                        \
+    intx8 fa[4], fb[2];                                                                                      \
+    _Pragma("unroll") for (int j = 0; j < 2; ++j) fetch(NOW, line_b, j, fb[j]);                              \
+    _Pragma("unroll") for (int i = 0; i < 4; ++i) fetch(NOW, line_a, i, fa[i]);                              \
+    _Pragma("unroll") for (int i = 0; i < 4; ++i)                                                            \
+      _Pragma("unroll") for (int j = 0; j < 2; ++j)                                                          \
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j], fa[i], acc[i][j], 0, 0, H % 8 / 2, scale_b[j], H % 8 / 2, scale_a[i]); \
+    __builtin_amdgcn_sched_group_barrier(0x100, H % 8 == 0 ? 14 : 8, 0);                                     \
+    _Pragma("unroll") for (int i = 0; i < 4; ++i) {                                                          \
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);                                                     \
+      if (i < 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                                          \
+    }                                                                                                        \
+  }
+  for (int base = 0; base < steps; base += 16) {
+    KAD_STEP(0, s0, s3)
+    KAD_STEP(1, s1, s0)
+    KAD_STEP(2, s2, s1)
+    KAD_STEP(3, s3, s2)
+    KAD_STEP(4, s0, s3)
+    KAD_STEP(5, s1, s0)
+    KAD_STEP(6, s2, s1)
+    KAD_STEP(7, s3, s2)
+    KAD_STEP(8, s0, s3)
+    KAD_STEP(9, s1, s0)
+    KAD_STEP(10, s2, s1)
+    KAD_STEP(11, s3, s2)
+    KAD_STEP(12, s0, s3)
+    KAD_STEP(13, s1, s0)
+    KAD_STEP(14, s2, s1)
+    KAD_STEP(15, s3, s2)
+  }
+#undef KAD_STEP
+  const int m1 = m0 + wm * 128, n1 = n0 + wn * 64;
+  if (o.splits > 1) {  // 32-bit sums that are joined later
+    float* part = a.work + (int64_t)split * a.m * a.n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int m = m1 + i * 32 + r32, n = n1 + j * 32 + 8 * q + 4 * h;
+          const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          if (m < a.m && n < a.n) store_four<float>(part + (int64_t)m * a.n + n, v, a.n - n);
+        }
+    return;
+  }
+  float bias[2][16];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[j][4 * q + e] = bias_at<T>(a, n1 + j * 32 + 8 * q + 4 * h + e);
+  __syncthreads();
+  char* lds = (wave < 4 ? s0 : s1) + (wave & 3) * (32 * 144);
+  if (a.act == KAD_ACT_SILU) store_wide<T, KAD_ACT_SILU>(a, acc, bias, lds, lane, m1, n1);
+  else if (a.act == KAD_ACT_RELU) store_wide<T, KAD_ACT_RELU>(a, acc, bias, lds, lane, m1, n1);
+  else store_wide<T, KAD_ACT_NONE>(a, acc, bias, lds, lane, m1, n1);
+}
+
 // The parts of k, in order.
 template <typename T>
 __global__ __launch_bounds__(256) void gemm8_join_kernel(kad_gemm8_args a, int splits) {
@@ -410,7 +612,11 @@ Plan plan_of(const kad_gemm8_args& a) {
   const int blocks = ceil_div(a.k, BLOCK8);
   const bool exact = a.dtype == KAD_F32;
   const auto count = [&](int bm, int bn) { return (int64_t)ceil_div(a.m, bm) * ceil_div(a.n, bn); };
-  p.bm = p.bn = !exact && count(256, 256) >= CUS ? 256 : count(128, 128) >= CUS ? 128 : 64;
+  // A round of 256 x 256 tiles (one a CU) takes 3.1 / 4 of the time that their 128 x 128 ones take, two a CU at a time:
+  // [8192, 4096] x [4096, 4096] 126 us against 167; where it leaves CUs idle, [40000, 512] x [512, 512] 26.3 against 22.7.
+  const auto rounds = [](int64_t tiles, int at_once) { return (tiles + at_once - 1) / at_once; };
+  p.bm = p.bn = !exact && rounds(count(WIDE, WIDE), CUS) * 3.1 < rounds(count(128, 128), 2 * CUS) * 2 ? WIDE
+                : count(128, 128) >= CUS ? 128 : 64;
   p.o.tm = ceil_div(a.m, p.bm);
   p.o.tn = ceil_div(a.n, p.bn);
   const int64_t tiles = (int64_t)p.o.tm * p.o.tn;
@@ -454,7 +660,7 @@ void launch(const kad_gemm8_args& a, hipStream_t st) {
   }
   const Plan p = plan_of(a);
   if constexpr (sizeof(T) == 2)
-    if (p.bm == 256) launch_tiles<T, 256, 256, 2, 4>(a, p.o, st);
+    if (p.bm == WIDE) gemm8_wide_kernel<T><<<ceil_div(p.o.tm * p.o.tn * p.o.splits, 8) * 8, 512, 0, st>>>(a, p.o);
   if (p.bm == 128) launch_tiles<T, 128, 128, 2, 2>(a, p.o, st);
   if (p.bm == 64) launch_tiles<T, 64, 64, 2, 2>(a, p.o, st);
   if (p.o.splits > 1) {
