@@ -6,6 +6,12 @@ launch, with states in 8 bits if asked to.
     python -m kadcnet.finetune --steps 50 --batch 8 --size 640 --dtype bf16 --state-bits 8
 
 runs it on synthetic images: a cell's class is the largest of fixed random projections of its neck map.
+
+    python -m kadcnet.finetune --distill 4
+
+goes on with a smaller head that learns from the first one's 4 best logits of each cell alone (``kadconv.distill_loss``):
+1 x 1 convolutions whose products are in 8 bits (``kadconv.Linear8``), with ``kadconv.LayerNorm`` over each cell's channels.
+In eval mode it serves with its weights kept in 8 bits.
 """
 import argparse
 import time
@@ -31,6 +37,21 @@ class GroupNormHead(nn.Module):
             nn.Conv2d(c, width, 3, padding=1, bias=False), kadconv.GroupNormAct(groups, width),
             nn.Conv2d(width, width, 3, padding=1, bias=False), kadconv.GroupNormAct(groups, width),
             nn.Conv2d(width, classes, 1)) for c in channels)
+
+    def forward(self, maps):
+        return [scale(m) for scale, m in zip(self.scales, maps)]
+
+
+class StudentHead(nn.Module):
+    """Class logits of each cell from each neck map, cell by cell: two 1 x 1 convolutions in 8 bits with layer norm over the
+    channels and SiLU, and a third."""
+
+    def __init__(self, channels, classes, width=64):
+        super().__init__()
+        self.scales = nn.ModuleList(nn.Sequential(
+            kadconv.Linear8(c, width, dim=1), kadconv.LayerNorm(width, dim=1), nn.SiLU(),
+            kadconv.Linear8(width, width, dim=1), kadconv.LayerNorm(width, dim=1), nn.SiLU(),
+            kadconv.Linear8(width, classes, dim=1)) for c in channels)
 
     def forward(self, maps):
         return [scale(m) for scale, m in zip(self.scales, maps)]
@@ -78,6 +99,35 @@ def train_head(head, batches, lr=2e-3, weight_decay=1e-2, state_bits=8, seed=0):
     return torch.stack(losses)
 
 
+def top_logits(head, maps, entries):
+    """(logits, classes) of each cell's best ``entries`` classes, a pair of maps [N, entries, H, W] for each neck map: what a
+    student needs of its teacher."""
+    with torch.no_grad():
+        return [tuple(torch.topk(z, min(entries, z.shape[1]), dim=1)) for z in head(maps)]
+
+
+def distill_head(student, batches, temperature=2.0, lr=2e-3, weight_decay=1e-2, state_bits=8, seed=0):
+    """One step a batch of (neck maps, a teacher's top logits on them); the losses as a GPU tensor."""
+    masters = next(student.parameters()).dtype != torch.float32
+    optimizer = kadconv.AdamW(student.parameters(), lr=lr, weight_decay=weight_decay, state_bits=state_bits,
+                              master_weights=masters, seed=seed)
+    losses = []
+    for maps, top in batches:
+        loss = sum(kadconv.distill_loss(z, t, i, temperature, dim=1) for z, (t, i) in zip(student(maps), top)) / len(top)
+        optimizer.zero_grad()
+        loss.backward()
+        optimizer.step()
+        losses.append(loss.detach())
+    return torch.stack(losses)
+
+
+def agreement(student, teacher, maps):
+    """The share of cells whose best class both heads agree on."""
+    with torch.no_grad():
+        same = [(a.argmax(1) == b.argmax(1)).float().flatten() for a, b in zip(student(maps), teacher(maps))]
+    return torch.cat(same).mean().item()
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split('\n\n')[0])
     ap.add_argument('--steps', type=int, default=50)
@@ -88,9 +138,14 @@ def main(argv=None):
     ap.add_argument('--state-bits', type=int, choices=(8, 32), default=8)
     ap.add_argument('--lr', type=float, default=2e-3)
     ap.add_argument('--seed', type=int, default=0)
+    ap.add_argument('--distill', type=int, default=0, metavar='ENTRIES',
+                    help="then train a head of 8-bit 1 x 1 convolutions by the first one's best ENTRIES logits of each cell")
+    ap.add_argument('--temperature', type=float, default=2.0)
     a = ap.parse_args(argv)
     if a.steps < 1 or a.batch < 1 or a.size < 128 or a.size % 32:
         ap.error('steps and batch must be positive, size a multiple of 32 from 128 on')
+    if a.distill < 0 or not a.temperature > 0:
+        ap.error('distill must not be negative, and temperature positive')
     from .synthetic import build_kadcnet_s
     device, dtype = torch.device('cuda'), DTYPES[a.dtype]
     model = build_kadcnet_s(seed=a.seed).fuse().to(device, dtype)
@@ -117,6 +172,29 @@ def main(argv=None):
     tenth = max(1, a.steps // 10)
     print(f'{a.steps} steps of {a.batch} x 3 x {a.size} x {a.size} {a.dtype}, {a.state_bits}-bit states: {ms:.1f} ms a step, '
           f'loss {sum(losses[:tenth]) / tenth:.4f} -> {sum(losses[-tenth:]) / tenth:.4f}')
+    if a.distill:
+        losses = losses, distill(a, head, channels, maps)
+    return losses
+
+
+def distill(a, teacher, channels, maps):
+    """The student's part of the program: its losses."""
+    teacher.eval()
+
+    def batches():
+        for _ in range(a.steps):
+            m = maps()
+            yield m, top_logits(teacher, m, a.distill)
+
+    device, dtype = torch.device('cuda'), DTYPES[a.dtype]
+    student = StudentHead(channels, a.classes).to(device, dtype)
+    torch.cuda.synchronize()
+    start = time.perf_counter()
+    losses = distill_head(student, batches(), a.temperature, lr=a.lr, state_bits=a.state_bits, seed=a.seed).tolist()
+    ms = (time.perf_counter() - start) * 1e3 / a.steps
+    tenth = max(1, a.steps // 10)
+    print(f'student: {a.steps} steps by {a.distill} entries a cell: {ms:.1f} ms a step, loss {sum(losses[:tenth]) / tenth:.4f} -> '
+          f'{sum(losses[-tenth:]) / tenth:.4f}, served in 8 bits it agrees on {agreement(student.eval(), teacher, maps()):.3f} of the cells')
     return losses
 
 
