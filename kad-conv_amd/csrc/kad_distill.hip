@@ -132,12 +132,69 @@ __device__ __forceinline__ float row_factor(const kad_distill_args& a, int64_t r
 }
 
 // ---------------------------------------------------------------------------- rows in registers
-template <typename T, int VV, int U, bool RAGGED>
+constexpr int HELD = 8;  // entries of a lane that stay in registers too
+
+// A lane's entries: `chunk` that follow each other, at most HELD; those that do not count have class -1.
+struct Own {
+  int at[HELD];
+  float t[HELD];
+  int chunk;
+  __device__ __forceinline__ explicit Own(int c) : chunk(c) {}
+  template <typename Q>
+  __device__ __forceinline__ void logits(const Q* p) {
+    constexpr int V = VEC<Q>;
+#pragma unroll
+    for (int i = 0; i < HELD; i += V) unpack<Q>(load_vec(p + i), t + i);
+  }
+  __device__ __forceinline__ void load(const Entries& en, int l) {
+    const kad_distill_args& a = en.a;
+    const int e = l * chunk;
+    if (chunk == HELD && e + HELD <= a.k && a.t_sk == 1 && a.i_sk == 1) {
+      if (a.index_bits == 32) {
+        const int32_t* p = (const int32_t*)a.index + en.i0 + e;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) at[i] = p[i];
+      } else {
+        const int64_t* p = (const int64_t*)a.index + en.i0 + e;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) at[i] = p[i] >= 0 && p[i] < a.v ? (int)p[i] : -1;
+      }
+      if (a.teacher_dtype == KAD_F32) logits((const float*)a.teacher + en.t0 + e);
+      else if (a.teacher_dtype == KAD_F16) logits((const half_t*)a.teacher + en.t0 + e);
+      else logits((const bf16_t*)a.teacher + en.t0 + e);
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) at[i] = (uint32_t)at[i] < (uint32_t)a.v && t[i] != -INF ? at[i] : -1;
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      t[i] = 0.f;
+      at[i] = -1;
+      if (i < chunk && e + i < a.k && !en.get(e + i, at[i], t[i])) at[i] = -1;
+    }
+  }
+  __device__ __forceinline__ float largest() const {
+    float m = -INF;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) m = at[i] >= 0 ? fmaxf(m, t[i]) : m;
+    return m;
+  }
+  __device__ __forceinline__ bool any() const {
+    int m = -1;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) m = m > at[i] ? m : at[i];
+    return m >= 0;
+  }
+};
+
+// IN_REGS: a row's entries are at most HELD G; otherwise they are read again for each use.
+template <typename T, int VV, int U, bool RAGGED, bool IN_REGS>
 __global__ __launch_bounds__(256) void distill_small_fwd_kernel(kad_distill_args a, int G) {
   const int sub = threadIdx.x / G, l = threadIdx.x & (G - 1), per = 256 / G;
   const Place<VV, U, RAGGED> o(l, G, a.v);
   const Scales c(a.temperature);
   const int64_t step = (int64_t)gridDim.x * per, last = a.rows - 1;
+  Own own((a.k + G - 1) / G);
   float total = 0.f;
   unsigned count = 0;
   for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows; base += step) {
@@ -150,11 +207,20 @@ __global__ __launch_bounds__(256) void distill_small_fwd_kernel(kad_distill_args
     const Entries en(a, row);
     float tm = -INF, any = 0.f, t;
     int at;
-    for (int e = l; e < a.k; e += G)
-      if (en.get(e, at, t)) {
-        any = 1.f;
-        tm = fmaxf(tm, t);
-      }
+    float zi[HELD];
+    if (IN_REGS) {
+      own.load(en, l);
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) zi[i] = i < own.chunk && own.at[i] >= 0 ? to_f32(z[own.at[i]]) : 0.f;
+      tm = own.largest();
+      any = own.any() ? 1.f : 0.f;
+    } else {
+      for (int e = l; e < a.k; e += G)
+        if (en.get(e, at, t)) {
+          any = 1.f;
+          tm = fmaxf(tm, t);
+        }
+    }
     any = lanes_max(any, G);
     tm = lanes_max(tm, G);
     float x[U][VV], zm = -INF, zsum = 0.f;
@@ -173,8 +239,14 @@ __global__ __launch_bounds__(256) void distill_small_fwd_kernel(kad_distill_args
     }
     zsum = lanes_sum(zsum, G);
     float s = 0.f, d = 0.f;
-    for (int e = l; e < a.k; e += G)
-      if (en.get(e, at, t)) add_entry(t, tm, to_f32(z[at]), zm, c.c2, s, d);
+    if (IN_REGS) {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+        if (i < own.chunk && own.at[i] >= 0) add_entry(own.t[i], tm, zi[i], zm, c.c2, s, d);
+    } else {
+      for (int e = l; e < a.k; e += G)
+        if (en.get(e, at, t)) add_entry(t, tm, to_f32(z[at]), zm, c.c2, s, d);
+    }
     s = lanes_sum(s, G);
     d = lanes_sum(d, G);
     if (l == 0 && live) {
@@ -187,15 +259,31 @@ __global__ __launch_bounds__(256) void distill_small_fwd_kernel(kad_distill_args
   leave_part(a, total, count);
 }
 
-template <typename T, int VV, int U, bool RAGGED>
+// Sums of weights as whole numbers of 2^-62; `unit` is 2^62 of the weights' own unit.
+__device__ __forceinline__ void add_weight(unsigned long long* sum, float weight, float unit) {
+  const float u = weight * unit, hi = floorf(u * 0x1p-32f), lo = __builtin_fmaf(hi, -0x1p32f, u);  // both exact
+  atomicAdd(sum, (unsigned long long)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+__device__ __forceinline__ float weight_of(unsigned long long sum) {
+  return __builtin_fmaf((float)(uint32_t)(sum >> 32), 0x1p-30f, (float)(uint32_t)sum * 0x1p-62f);
+}
+// Orders a wave's accesses to LDS: the unit takes them in turn, so it is the compiler alone that has to.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <typename T, int VV, int U, bool RAGGED, bool IN_REGS>
 __global__ __launch_bounds__(256) void distill_small_bwd_kernel(kad_distill_args a, int G) {
-  extern __shared__ unsigned long long sums[];  // [rows of the block][v]: sums of p in units of 2^-62
+  extern __shared__ unsigned long long sums[];  // [rows of the block][v]; a row's are its own wave's
   const int sub = threadIdx.x / G, l = threadIdx.x & (G - 1), per = 256 / G;
   const Place<VV, U, RAGGED> o(l, G, a.v);
   const Scales c(a.temperature);
   const int64_t step = (int64_t)gridDim.x * per, last = a.rows - 1;
+  Own own((a.k + G - 1) / G);
   unsigned long long* mine = sums + sub * a.v;
   for (int i = threadIdx.x; i < per * a.v; i += 256) sums[i] = 0;
+  __syncthreads();
   for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows; base += step) {
     const bool live = base + sub <= last;
     const int64_t row = live ? base + sub : last;
@@ -207,28 +295,46 @@ __global__ __launch_bounds__(256) void distill_small_bwd_kernel(kad_distill_args
     const Entries en(a, row);
     float tm = -INF, s = 0.f, t;
     int at;
-    for (int e = l; e < a.k; e += G)
-      if (en.get(e, at, t)) tm = fmaxf(tm, t);
-    tm = lanes_max(tm, G);
-    for (int e = l; e < a.k; e += G)
-      if (en.get(e, at, t)) s += exp2_((t - tm) * c.c2);
+    if (IN_REGS) {
+      own.load(en, l);
+      tm = lanes_max(own.largest(), G);
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+        if (i < own.chunk) {
+          own.t[i] = exp2_((own.t[i] - tm) * c.c2);
+          s += own.at[i] >= 0 ? own.t[i] : 0.f;
+        }
+    } else {
+      for (int e = l; e < a.k; e += G)
+        if (en.get(e, at, t)) tm = fmaxf(tm, t);
+      tm = lanes_max(tm, G);
+      for (int e = l; e < a.k; e += G)
+        if (en.get(e, at, t)) s += exp2_((t - tm) * c.c2);
+    }
     s = lanes_sum(s, G);
     const float unit = 0x1p62f / s;
-    __syncthreads();  // sums are 0
-    for (int e = l; e < a.k; e += G)
-      if (en.get(e, at, t) && s == s) atomicAdd(mine + at, (unsigned long long)(exp2_((t - tm) * c.c2) * unit));
-    __syncthreads();
+    if (s == s) {
+      if (IN_REGS) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+          if (i < own.chunk && own.at[i] >= 0) add_weight(mine + own.at[i], own.t[i], unit);
+      } else {
+        for (int e = l; e < a.k; e += G)
+          if (en.get(e, at, t)) add_weight(mine + at, exp2_((t - tm) * c.c2), unit);
+      }
+    }
+    wave_order();
     float x[U][VV];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       raw[u].get(x[u]);
 #pragma unroll
       for (int e = 0; e < VV; ++e) {
-        const float q = exp2_((x[u][e] - zm) * c.c2) * inv, p = (float)mine[o.at[u] + e] * 0x1p-62f;
+        const float q = exp2_((x[u][e] - zm) * c.c2) * inv, p = weight_of(mine[o.at[u] + e]);
         x[u][e] = inv == 0.f ? 0.f : f * (s == s ? q - p : s);
       }
     }
-    __syncthreads();  // what two vectors share is read twice before it is cleared
+    wave_order();  // what two vectors share is read twice before it is cleared
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (!o.on[u]) continue;
@@ -236,6 +342,7 @@ __global__ __launch_bounds__(256) void distill_small_bwd_kernel(kad_distill_args
       for (int e = 0; e < VV; ++e) mine[o.at[u] + e] = 0;
       if (live) put<T, VV>((T*)a.dlogits + row * a.v + o.at[u], x[u]);
     }
+    wave_order();
   }
 }
 
@@ -476,7 +583,7 @@ Shape shape_of(const kad_distill_args& a, bool backward) {
     s.u = 1;
     while (vecs > 64 * s.u) s.u *= 2;
     s.G = 1;
-    while (s.G * s.u < vecs) s.G *= 2;
+    while (s.G * s.u < vecs || (s.G < 64 && s.G * HELD < a.k)) s.G *= 2;
     const int64_t turns = (a.rows + 256 / s.G - 1) / (256 / s.G);
     s.blocks = turns < 2048 ? turns : 2048;
     return s;
@@ -522,12 +629,18 @@ int check_call(const kad_distill_args* a, bool backward, const char* what) {
   return KAD_OK;
 }
 
-template <typename T, int VV, int U, bool RAGGED>
+template <typename T, int VV, int U, bool RAGGED, bool IN_REGS>
 void launch_small(const kad_distill_args& a, const Shape& s, bool backward, hipStream_t st) {
   if (backward)
-    distill_small_bwd_kernel<T, VV, U, RAGGED><<<s.blocks, 256, (256 / s.G) * a.v * sizeof(unsigned long long), st>>>(a, s.G);
+    distill_small_bwd_kernel<T, VV, U, RAGGED, IN_REGS><<<s.blocks, 256, (256 / s.G) * a.v * sizeof(unsigned long long), st>>>(a, s.G);
   else
-    distill_small_fwd_kernel<T, VV, U, RAGGED><<<s.blocks, 256, 0, st>>>(a, s.G);
+    distill_small_fwd_kernel<T, VV, U, RAGGED, IN_REGS><<<s.blocks, 256, 0, st>>>(a, s.G);
+}
+
+template <typename T, int VV, int U, bool RAGGED>
+void launch_small(const kad_distill_args& a, const Shape& s, bool backward, hipStream_t st) {
+  if (a.k <= HELD * s.G) launch_small<T, VV, U, RAGGED, true>(a, s, backward, st);
+  else launch_small<T, VV, U, RAGGED, false>(a, s, backward, st);
 }
 
 template <typename T, int U>
