@@ -756,7 +756,7 @@ typedef struct kad_gemm8_args {
   int dtype, a_dtype, bias_dtype; /* a_dtype: of a as values */
 } kad_gemm8_args;
 
-#define KAD_GEMM8_FEW 64
+#define KAD_GEMM8_FEW 32
 
 int64_t kad_gemm8_work_elems(const kad_gemm8_args *a);
 int kad_gemm8(const kad_gemm8_args *a, void *stream);

@@ -9,10 +9,10 @@
 // all bits random 5e-5: under the rounding of a 16-bit result.  For 32-bit results (EXACT) codes become fp16 numbers, which
 // hold them exactly, the fp16 instruction sums a block in 32 bits (1e-7), and the scales are applied to its sum.
 //
-// Two forms.  Many rows: tiles of BM x BN results, both operands' codes of 128 columns at a time copied to LDS past the
-// registers, one stage ahead.  Few rows (KAD_GEMM8_FEW): b's codes are read once, straight into the instruction's
-// operands; a block takes 16 rows of b, its waves take every eighth 128 columns and join in LDS.  a as values is brought
-// to 8 bits in those registers, by each block for itself: a launch less, and a is small.
+// Two forms.  Many rows: tiles of BM x BN results, both operands' codes copied to LDS past the registers, ahead of their use.
+// Few rows (KAD_GEMM8_FEW): b's codes are read once, straight into the instruction's operands; a block takes 16 rows of b,
+// its waves take every eighth 128 columns and join in LDS.  a as values is brought to 8 bits in those registers, by each
+// block for itself: a launch less, and a is small (at 48 rows and [8192, 4096] it is not: 48 us against 33).
 //
 // The instruction computes b a^T: a lane then holds four results of one row of out that follow each other.
 #include "kad_block8.h"
@@ -513,80 +513,127 @@ __global__ __launch_bounds__(256) void gemm8_join_kernel(kad_gemm8_args a, int s
 // ---------------------------------------------------------------------------- few rows
 constexpr int FEW_WAVES = 8;
 
-// 32 values of a row from column k on as codes, and their block's scale: the four lanes of a row hold a block.
-template <typename X>
-__device__ __forceinline__ int to_codes(const X* p, int left, intx4& lo, intx4& hi) {
-  constexpr int V = VEC<X>;
-  float x[32];
-  if (left >= 32) {
+// A lane's 32 numbers of a block: 8-bit ones, or values in registers until they are brought to 8 bits.  Rows past the last
+// read the last one's: what comes of them is not stored.
+template <typename X> struct Numbers {
+  static constexpr int V = VEC<X>;
+  intx4 raw[32 / V];
+  static __device__ __forceinline__ int whole(const kad_gemm8_args& a) { return a.k / BLOCK8; }  // blocks without an end of k
+  __device__ __forceinline__ void load(const kad_gemm8_args& a, int64_t, int64_t, int row, int kb, int g) {
+    const X* p = (const X*)a.a + row * a.a_rs + kb * BLOCK8 + 32 * g;
 #pragma unroll
-    for (int i = 0; i < 32; i += V) {
-      intx4 raw = load_vec(p + i);
-      unpack<X>(raw, x + i);
+    for (int i = 0; i < 32 / V; ++i) raw[i] = load_vec(p + i * V);
+  }
+  // Of the block where k ends: zeros behind.
+  __device__ __forceinline__ void load_end(const kad_gemm8_args& a, int row, int kb, int g) {
+    const X* p = (const X*)a.a + row * a.a_rs;
+    X v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int at = kb * BLOCK8 + 32 * g + i;
+      v[i] = p[at < a.k ? at : a.k - 1];
+      if (at >= a.k) v[i] = (X)0.f;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) x[i] = i < left ? to_f32(p[i]) : 0.f;
+    __builtin_memcpy(raw, v, sizeof(v));
   }
-  uint32_t m = 0;
+  // Their codes, and their block's scale: the four lanes of a row hold a block.
+  __device__ __forceinline__ int codes(intx4& lo, intx4& hi) const {
+    constexpr int WORDS = 32 * sizeof(X) / 4;
+    uint32_t w[WORDS];
+    __builtin_memcpy(w, raw, sizeof(w));
+    uint32_t m = largest_finite<X, WORDS>(w), other = __shfl_xor(m, 16);
+    m = m > other ? m : other;
+    other = __shfl_xor(m, 32);
+    m = m > other ? m : other;
+    const int s = scale_of<X>(m);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const uint32_t b = magnitude(x[i]);
-    m = m > b ? m : b;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(X) == 2) {
+        lo[i] = codes_of<X>(w[2 * i], w[2 * i + 1], s);
+        hi[i] = codes_of<X>(w[8 + 2 * i], w[9 + 2 * i], s);
+      } else {
+        lo[i] = codes_of(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3], s);
+        hi[i] = codes_of(w[16 + 4 * i], w[17 + 4 * i], w[18 + 4 * i], w[19 + 4 * i], s);
+      }
+    }
+    return s;
   }
-  uint32_t other = __shfl_xor(m, 16);
-  m = m > other ? m : other;
-  other = __shfl_xor(m, 32);
-  m = m > other ? m : other;
-  const int s = scale_of(m);
-  const float inv = inverse(s);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    lo[i] = codes_of(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], inv);
-    hi[i] = codes_of(x[16 + 4 * i], x[17 + 4 * i], x[18 + 4 * i], x[19 + 4 * i], inv);
+};
+template <> struct Numbers<unsigned char> {
+  intx4 lo, hi;
+  int scale;
+  static __device__ __forceinline__ int whole(const kad_gemm8_args& a) { return (a.k + BLOCK8 - 1) / BLOCK8; }
+  __device__ __forceinline__ void load(const kad_gemm8_args& a, int64_t kp, int64_t ks, int row, int kb, int g) {
+    const intx4* p = (const intx4*)((const char*)a.a + row * kp + kb * BLOCK8 + 32 * g);
+    lo = p[0];
+    hi = p[1];
+    scale = ((const unsigned char*)a.a_scales)[row * ks + kb];
   }
-  return s;
-}
+  __device__ __forceinline__ void load_end(const kad_gemm8_args&, int, int, int) {}
+  __device__ __forceinline__ int codes(intx4& l, intx4& h) const {
+    l = lo;
+    h = hi;
+    return scale;
+  }
+};
 
-// X: a's type as values, or unsigned char: a in 8 bits.
+// X: a's type as values, or unsigned char: a in 8 bits.  A wave has the loads of AT_ONCE blocks under way: they are made for
+// the last block again where there are fewer, since the compiler waits for all loads where branches around some meet
+// ([1, 4096] x [8192, 4096] bf16, weights from memory: 17.6 us with such branches, 12.7 without).
 template <typename T, typename X, int MT, bool EXACT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void gemm8_few_kernel(kad_gemm8_args a) {
+  constexpr int AT_ONCE = 4 / MT;
   __shared__ floatx4 red[FEW_WAVES][MT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16, row_b = n0 + r16 < a.n ? n0 + r16 : a.n - 1;
-  const int blocks = (a.k + BLOCK8 - 1) / BLOCK8, kp = blocks * BLOCK8, ks = (blocks + 3) / 4 * 4;
-  const char* codes_b = (const char*)a.b + (int64_t)row_b * kp + 32 * g;
-  const unsigned char* scales_b = (const unsigned char*)a.b_scales + (int64_t)row_b * ks;
+  const int blocks = (a.k + BLOCK8 - 1) / BLOCK8, whole = Numbers<X>::whole(a);
+  const int64_t kp = (int64_t)blocks * BLOCK8, ks = (blocks + 3) / 4 * 4;
+  const char* codes_b = (const char*)a.b + row_b * kp + 32 * g;
+  const unsigned char* scales_b = (const unsigned char*)a.b_scales + row_b * ks;
+  int row[MT];
   floatx4 acc[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-  for (int kb = wave; kb < blocks; kb += FEW_WAVES) {
-    Operand<EXACT> fb;
-    fb.set(*(const intx4*)(codes_b + kb * BLOCK8), *(const intx4*)(codes_b + kb * BLOCK8 + 16));
-    const int sb = scales_b[kb];
+  for (int i = 0; i < MT; ++i) {
+    row[i] = i * 16 + r16 < a.m ? i * 16 + r16 : a.m - 1;
+    acc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  const auto add = [&](intx4 lo, intx4 hi, int sb, const Numbers<X> (&x)[MT]) {
+    Operand<EXACT> fb, fa;
+    fb.set(lo, hi);
     int eb[4];
     if (EXACT)
 #pragma unroll
       for (int i = 0; i < 4; ++i) eb[i] = __shfl(sb, 4 * g + i);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const int m = i * 16 + r16;
-      intx4 lo, hi;
-      int s;
-      if constexpr (sizeof(X) == 1) {
-        const int row = m < a.m ? m : a.m - 1;  // what comes of rows past the last is not stored
-        const intx4* p = (const intx4*)((const char*)a.a + (int64_t)row * kp + kb * BLOCK8 + 32 * g);
-        lo = p[0];
-        hi = p[1];
-        s = ((const unsigned char*)a.a_scales)[(int64_t)row * ks + kb];
-      } else {
-        const int k = kb * BLOCK8 + 32 * g, left = m < a.m ? a.k - k : 0;
-        s = to_codes((const X*)a.a + (left > 0 ? m * a.a_rs + k : 0), left, lo, hi);
-      }
-      Operand<EXACT> fa;
-      fa.set(lo, hi);
+      intx4 l, h;
+      const int s = x[i].codes(l, h);
+      fa.set(l, h);
       multiply<0>(acc[i], fb, fa, sb, s, eb);
     }
+  };
+  for (int first = wave; first < whole; first += AT_ONCE * FEW_WAVES) {
+    intx4 lo[AT_ONCE], hi[AT_ONCE];
+    int sb[AT_ONCE];
+    Numbers<X> x[AT_ONCE][MT];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int kb = first + u * FEW_WAVES < whole ? first + u * FEW_WAVES : whole - 1;
+      lo[u] = *(const intx4*)(codes_b + kb * BLOCK8);
+      hi[u] = *(const intx4*)(codes_b + kb * BLOCK8 + 16);
+      sb[u] = scales_b[kb];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) x[u][i].load(a, kp, ks, row[i], kb, g);
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+      if (first + u * FEW_WAVES < whole) add(lo[u], hi[u], sb[u], x[u]);
+  }
+  if (whole < blocks && wave == whole % FEW_WAVES) {
+    Numbers<X> x[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i].load_end(a, row[i], whole, g);
+    add(*(const intx4*)(codes_b + whole * BLOCK8), *(const intx4*)(codes_b + whole * BLOCK8 + 16), scales_b[whole], x);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) red[wave][i][lane] = acc[i];
@@ -638,8 +685,7 @@ void launch_few(const kad_gemm8_args& a, hipStream_t st) {
 template <typename T, typename X>
 void launch_few(const kad_gemm8_args& a, hipStream_t st) {
   if (a.m <= 16) launch_few<T, X, 1>(a, st);
-  else if (a.m <= 32) launch_few<T, X, 2>(a, st);
-  else launch_few<T, X, 4>(a, st);
+  else launch_few<T, X, 2>(a, st);
 }
 
 template <typename T, int BM, int BN, int WM, int WN>

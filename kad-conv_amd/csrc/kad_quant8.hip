@@ -28,97 +28,115 @@ __device__ __forceinline__ uint32_t lanes_largest(uint32_t v) {
 template <typename T>
 __global__ __launch_bounds__(256) void quant8_kernel(kad_quant8_args a) {
   constexpr int V = VEC<T>, L = LANES<T>, D = DEEP<T>, SUBS = 256 / L;  // SUBS threads share a column
-  __shared__ uint32_t most[SUBS][BLOCK8];
+  __shared__ float column_sums[SUBS][BLOCK8];
+  __shared__ uint32_t most[SUBS][L * 4];                                // of a thread's columns, as its words hold them
   __shared__ __attribute__((aligned(16))) unsigned char flat[BLOCK8 * PITCH];
   const int t = threadIdx.x, l = t % L, sub = t / L;
   const int tiles = (a.c + BLOCK8 - 1) / BLOCK8;
   const int64_t band = blockIdx.x / tiles;
   const int tile = (int)(blockIdx.x - band * tiles), col = tile * BLOCK8 + l * V, left = a.c - col;
   const int64_t row0 = band * BLOCK8 + sub * D;
-  float x[D][V];
-  // whole vectors of whole rows first, all on their way at once
+  uint32_t x[D][4];
+  // whole vectors of whole rows, all on their way at once
   if (left >= V && row0 + D <= a.rows) {
-    intx4 raw[D];
     const T* p = (const T*)a.x + row0 * a.x_rs + col;
 #pragma unroll
-    for (int r = 0; r < D; ++r) raw[r] = load_vec(p + r * a.x_rs);
+    for (int r = 0; r < D; ++r) {
+      const intx4 v = load_vec(p + r * a.x_rs);
 #pragma unroll
-    for (int r = 0; r < D; ++r) unpack<T>(raw[r], x[r]);
+      for (int i = 0; i < 4; ++i) x[r][i] = v[i];
+    }
   } else {
 #pragma unroll
     for (int r = 0; r < D; ++r) {
       const int n = row0 + r < a.rows && left > 0 ? left : 0;
-      load_some((const T*)a.x + (n ? (row0 + r) * a.x_rs + col : 0), n, x[r]);
+      float v[V];
+      load_some((const T*)a.x + (n ? (row0 + r) * a.x_rs + col : 0), n, v);
+      const intx4 w = pack<T>(v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[r][i] = w[i];
     }
   }
   if (a.codes) {
     const int64_t kp = (int64_t)tiles * BLOCK8, kb = (tiles + 3) / 4 * 4;
 #pragma unroll
     for (int r = 0; r < D; ++r) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const uint32_t b = magnitude(x[r][e]);
-        m = m > b ? m : b;
-      }
-      const int s = scale_of(lanes_largest<L>(m));
+      const int s = scale_of<T>(lanes_largest<L>(largest_finite<T, 4>(x[r])));
       if (row0 + r >= a.rows) continue;
-      const float inv = inverse(s);
       int* to = (int*)((unsigned char*)a.codes + (row0 + r) * kp + col);
-#pragma unroll
-      for (int e = 0; e < V; e += 4) to[e / 4] = codes_of(x[r][e], x[r][e + 1], x[r][e + 2], x[r][e + 3], inv);
+      if constexpr (sizeof(T) == 2) {
+        to[0] = codes_of<T>(x[r][0], x[r][1], s);
+        to[1] = codes_of<T>(x[r][2], x[r][3], s);
+      } else {
+        to[0] = codes_of(x[r][0], x[r][1], x[r][2], x[r][3], s);
+      }
       unsigned char* sc = (unsigned char*)a.scales + (row0 + r) * kb;
       if (l == 0) sc[tile] = (unsigned char)s;
       if (tile == tiles - 1 && l < kb - tiles) sc[tiles + l] = 127;  // so that a row's scales can be read by fours
     }
   }
-  if (!a.t_codes && !a.sums) return;
-  float total[V];
-  uint32_t m[V];
+  if (a.sums) {
+    float total[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    total[e] = 0.f;
-    m[e] = 0;
+    for (int e = 0; e < V; ++e) total[e] = 0.f;
 #pragma unroll
     for (int r = 0; r < D; ++r) {
-      total[e] += x[r][e];
-      const uint32_t b = magnitude(x[r][e]);
-      m[e] = m[e] > b ? m[e] : b;
-    }
-  }
-  if (a.sums) {
+      float v[V];
+      unpack<T>(intx4{(int)x[r][0], (int)x[r][1], (int)x[r][2], (int)x[r][3]}, v);
 #pragma unroll
-    for (int e = 0; e < V; ++e) most[sub][l * V + e] = __float_as_uint(total[e]);
+      for (int e = 0; e < V; ++e) total[e] += v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) column_sums[sub][l * V + e] = total[e];
     __syncthreads();
     if (t < BLOCK8 && tile * BLOCK8 + t < a.c) {
-      float s = __uint_as_float(most[0][t]);
+      float s = column_sums[0][t];
 #pragma unroll
-      for (int i = 1; i < SUBS; ++i) s += __uint_as_float(most[i][t]);
+      for (int i = 1; i < SUBS; ++i) s += column_sums[i][t];
       a.work[band * a.c + tile * BLOCK8 + t] = s;
     }
-    __syncthreads();
   }
   if (!a.t_codes) return;
 #pragma unroll
-  for (int e = 0; e < V; ++e) most[sub][l * V + e] = m[e];
+  for (int i = 0; i < 4; ++i) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int r = 0; r < D; ++r) m = larger<T>(m, magnitudes<T>(x[r][i]));
+    if (!all_finite<T>(m)) {
+      m = 0;
+#pragma unroll
+      for (int r = 0; r < D; ++r) m = larger<T>(m, finite_of<T>(magnitudes<T>(x[r][i])));
+    }
+    most[sub][l * 4 + i] = m;
+  }
   __syncthreads();
   const int bands = (int)((a.rows + BLOCK8 - 1) / BLOCK8);
   const int64_t mp = (int64_t)bands * BLOCK8, mb = (bands + 3) / 4 * 4;
+  constexpr int PER = V / 4;  // columns of a word
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    uint32_t b = 0;
+  for (int i = 0; i < 4; ++i) {
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < SUBS; ++i) b = b > most[i][l * V + e] ? b : most[i][l * V + e];
-    const int s = scale_of(b);
-    const float inv = inverse(s);
-    int* to = (int*)(flat + (l * V + e) * PITCH + sub * D);
+    for (int k = 0; k < SUBS; ++k) m = larger<T>(m, most[k][l * 4 + i]);
 #pragma unroll
-    for (int r = 0; r < D; r += 4) to[r / 4] = codes_of(x[r][e], x[r + 1][e], x[r + 2][e], x[r + 3][e], inv);
-    if (sub == 0 && col + e < a.c) {
-      unsigned char* sc = (unsigned char*)a.t_scales + (col + e) * mb;
-      sc[band] = (unsigned char)s;
-      if (band == bands - 1)
-        for (int i = bands; i < mb; ++i) sc[i] = 127;
+    for (int h = 0; h < PER; ++h) {
+      const int s = scale_of<T>(PER == 1 ? m : h ? m >> 16 : m & 0xFFFFu), c = l * V + i * PER + h;
+      int* to = (int*)(flat + c * PITCH + sub * D);
+#pragma unroll
+      for (int r = 0; r < D; r += 4) {
+        if constexpr (PER == 1) {
+          to[r / 4] = codes_of(x[r][i], x[r + 1][i], x[r + 2][i], x[r + 3][i], s);
+        } else {  // the column's halves of two rows at a time
+          const uint32_t pick = h ? 0x07060302u : 0x05040100u;
+          to[r / 4] = codes_of<T>(__builtin_amdgcn_perm(x[r + 1][i], x[r][i], pick), __builtin_amdgcn_perm(x[r + 3][i], x[r + 2][i], pick), s);
+        }
+      }
+      if (sub == 0 && tile * BLOCK8 + c < a.c) {
+        unsigned char* sc = (unsigned char*)a.t_scales + (tile * BLOCK8 + c) * mb;
+        sc[band] = (unsigned char)s;
+        if (band == bands - 1)
+          for (int k = bands; k < mb; ++k) sc[k] = 127;
+      }
     }
   }
   __syncthreads();
