@@ -519,19 +519,32 @@ int64_t blocks8(int64_t k) { return (k + 127) / 128; }
 int64_t codes8(int64_t k) { return blocks8(k) * 128; }
 int64_t scales8(int64_t k) { return (blocks8(k) + 3) / 4 * 4; }
 
-// Rows of k numbers in 8 bits (kadconv_hip.h).
+// Rows of k numbers in 8 bits (kadconv_hip.h), of a caller or, codes and then scales, in a buffer of their own.
 struct Held8 {
-  Tensor codes, scales;
-  bool defined() const { return codes.defined(); }
+  Tensor buffer;
+  void *codes = nullptr, *scales = nullptr;
+  bool defined() const { return codes != nullptr; }
 };
 
-Held8 new_held(const Tensor& x, c10::DimVector sizes, int64_t k) {
-  Held8 h;
-  sizes.push_back(codes8(k));
-  h.codes = at::detail::empty_cuda(sizes, at::kFloat8_e4m3fn, x.device(), std::nullopt);
-  sizes.back() = scales8(k);
-  h.scales = at::detail::empty_cuda(sizes, at::kFloat8_e8m0fnu, x.device(), std::nullopt);
-  return h;
+int64_t held_bytes(int64_t rows, int64_t k) { return rows * (codes8(k) + scales8(k)); }
+
+Held8 held_in(const Tensor& buffer, int64_t rows, int64_t k) {
+  char* p = (char*)buffer.mutable_data_ptr();
+  return {buffer, p, p + rows * codes8(k)};
+}
+
+Held8 new_held(const Tensor& x, int64_t rows, int64_t k) {
+  return held_in(at::detail::empty_cuda({held_bytes(rows, k)}, at::kByte, x.device(), std::nullopt), rows, k);
+}
+
+Held8 held_of(const Tensor& codes, const Tensor& scales) {
+  return {Tensor(), const_cast<void*>(codes.const_data_ptr()), const_cast<void*>(scales.const_data_ptr())};
+}
+
+Held8 saved_held(const Tensor& buffer, int64_t rows, int64_t k, const Tensor& like, const char* name) {
+  TORCH_CHECK_VALUE(buffer.is_contiguous() && buffer.scalar_type() == at::kByte && buffer.device() == like.device() &&
+                        buffer.numel() == held_bytes(rows, k), name, " must be the forward's");
+  return held_in(buffer, rows, k);
 }
 
 void check_held(const Tensor& codes, const Tensor& scales, int64_t rows, int64_t k, const Tensor& x, const char* name) {
@@ -551,10 +564,10 @@ void quantize(const Rows& r, const Held8& along, const Held8& across, const Tens
   a.x_rs = r.rs;
   a.rows = r.count;
   a.c = (int)r.c;
-  a.codes = mutable_pointer(along.codes);
-  a.scales = mutable_pointer(along.scales);
-  a.t_codes = mutable_pointer(across.codes);
-  a.t_scales = mutable_pointer(across.scales);
+  a.codes = along.codes;
+  a.scales = along.scales;
+  a.t_codes = across.codes;
+  a.t_scales = across.scales;
   a.sums = mutable_pointer(sums);
   a.dtype = dtype_of(r.held);
   a.sums_dtype = sums.defined() ? dtype_of(sums) : KAD_F32;
@@ -565,16 +578,16 @@ void quantize(const Rows& r, const Held8& along, const Held8& across, const Tens
   check(kad_quant8(&a, stream_of(x)), "kad_quant8");
 }
 
-// out = act(a b^T + bias), a in 8 bits or, where it has no scales, as values in rows a_rs apart.
-void product(const Tensor& a, const Tensor& a_scales, int64_t a_rs, const Held8& b, int64_t m, int64_t n, int64_t k, const Tensor& bias,
-             int act, const Tensor& out) {
+// out = act(a b^T + bias), a in 8 bits or, where it has no scales, as values of a_dtype in rows a_rs apart.
+void product(const void* a, const void* a_scales, int64_t a_rs, int a_dtype, const Held8& b, int64_t m, int64_t n, int64_t k,
+             const Tensor& bias, int act, const Tensor& out) {
   TORCH_CHECK_VALUE(m <= INT32_MAX - 255 && n <= INT32_MAX - 255, "too many rows: ", m, " and ", n);
   kad_gemm8_args g{};
-  g.a = a.const_data_ptr();
-  g.a_scales = pointer(a_scales);
+  g.a = a;
+  g.a_scales = a_scales;
   g.a_rs = a_rs;
-  g.b = b.codes.const_data_ptr();
-  g.b_scales = b.scales.const_data_ptr();
+  g.b = b.codes;
+  g.b_scales = b.scales;
   g.bias = pointer(bias);
   g.out = out.mutable_data_ptr();
   g.m = (int)m;
@@ -582,7 +595,7 @@ void product(const Tensor& a, const Tensor& a_scales, int64_t a_rs, const Held8&
   g.k = (int)k;
   g.act = act;
   g.dtype = dtype_of(out);
-  g.a_dtype = a_scales.defined() ? KAD_F32 : dtype_of(a);
+  g.a_dtype = a_dtype;
   g.bias_dtype = bias.defined() ? dtype_of(bias) : KAD_F32;
   const int64_t elems = kad_gemm8_work_elems(&g);
   if (elems < 0) check((int)elems, "kad_gemm8_work_elems");
@@ -591,12 +604,19 @@ void product(const Tensor& a, const Tensor& a_scales, int64_t a_rs, const Held8&
   check(kad_gemm8(&g, stream_of(out)), "kad_gemm8");
 }
 
-// The same for values: by way of 8 bits along k, in memory where they are many.
+void product(const Held8& a, const Held8& b, int64_t m, int64_t n, int64_t k, const Tensor& bias, int act, const Tensor& out) {
+  product(a.codes, a.scales, 0, KAD_F32, b, m, n, k, bias, act, out);
+}
+void product(const Rows& a, const Held8& b, int64_t n, const Tensor& bias, int act, const Tensor& out) {
+  product(a.held.const_data_ptr(), nullptr, a.rs, dtype_of(a.held), b, a.count, n, a.c, bias, act, out);
+}
+
+// Of values: by way of 8 bits along k, in memory where they are many.
 void product_of_values(const Rows& r, const Held8& b, int64_t n, const Tensor& bias, int act, const Tensor& out) {
-  if (r.count <= KAD_GEMM8_FEW) return product(r.held, Tensor(), r.rs, b, r.count, n, r.c, bias, act, out);
-  const Held8 h = new_held(r.held, {r.count}, r.c);
+  if (r.count <= KAD_GEMM8_FEW) return product(r, b, n, bias, act, out);
+  const Held8 h = new_held(r.held, r.count, r.c);
   quantize(r, h, {}, Tensor(), r.held);
-  product(h.codes, h.scales, 0, b, r.count, n, r.c, bias, act, out);
+  product(h, b, r.count, n, r.c, bias, act, out);
 }
 
 void check_quantized(const Tensor& x, int64_t k) {
@@ -612,9 +632,13 @@ std::tuple<Tensor, Tensor> quantize8(const Tensor& x, int64_t dim) {
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard guard(x.device());
   const int64_t k = row_length(x, map);
-  Held8 h = new_held(x, row_sizes(x, map), k);
-  if (x.numel()) quantize(rows_of(x, map), h, {}, Tensor(), x);
-  return {h.codes, h.scales};
+  c10::DimVector sizes = row_sizes(x, map);
+  sizes.push_back(codes8(k));
+  const Tensor codes = at::detail::empty_cuda(sizes, at::kFloat8_e4m3fn, x.device(), std::nullopt);
+  sizes.back() = scales8(k);
+  const Tensor scales = at::detail::empty_cuda(sizes, at::kFloat8_e8m0fnu, x.device(), std::nullopt);
+  if (x.numel()) quantize(rows_of(x, map), held_of(codes, scales), {}, Tensor(), x);
+  return {codes, scales};
 }
 
 at::ScalarType checked_result(at::ScalarType t) {
@@ -642,7 +666,7 @@ Tensor matmul8(const Tensor& a, const Tensor& a_scales, const Tensor& b, const T
   c10::DimVector sizes(a.sizes());
   sizes.back() = n;
   Tensor out = at::detail::empty_cuda(sizes, checked_result(dtype), a.device(), std::nullopt);
-  if (out.numel()) product(a, a_scales, 0, {b, b_scales}, m, n, k, bi, ac, out);
+  if (out.numel()) product(held_of(a, a_scales), held_of(b, b_scales), m, n, k, bi, ac, out);
   return out;
 }
 
@@ -685,11 +709,11 @@ Tensor linear8_run(const Tensor& x, bool map, const Tensor& weight, const Tensor
   const int64_t n = weight.size(0), k = weight.size(1);
   Tensor y = result_like(x, map, n);
   const Rows w = rows_of(weight, false);
-  const Held8 wh = new_held(x, {n}, k);
-  if (across_w) across.w = new_held(x, {k}, n);
+  const Held8 wh = new_held(x, n, k);
+  if (across_w) across.w = new_held(x, k, n);
   quantize(w, wh, across.w, Tensor(), x);
   const int64_t m = row_count(x, map);
-  if (across_x) across.x = new_held(x, {k}, std::max<int64_t>(m, 1));
+  if (across_x) across.x = new_held(x, k, std::max<int64_t>(m, 1));
   if (!m) return y;
   const Rows r = rows_of(x, map);
   const Tensor b = dense(bias);
@@ -697,11 +721,11 @@ Tensor linear8_run(const Tensor& x, bool map, const Tensor& weight, const Tensor
     product_of_values(r, wh, n, b, act, y);
   } else if (m <= KAD_GEMM8_FEW) {
     quantize(r, {}, across.x, Tensor(), x);
-    product(r.held, Tensor(), r.rs, wh, m, n, k, b, act, y);
+    product(r, wh, n, b, act, y);
   } else {
-    const Held8 h = new_held(x, {m}, k);
+    const Held8 h = new_held(x, m, k);
     quantize(r, h, across.x, Tensor(), x);
-    product(h.codes, h.scales, 0, wh, m, n, k, b, act, y);
+    product(h, wh, m, n, k, b, act, y);
   }
   return y;
 }
@@ -726,17 +750,17 @@ std::tuple<Tensor, Tensor, Tensor> linear8_gradients(const Tensor& dy, bool map,
   const Rows r = rows_of(dy, map);
   const bool in_memory = need_x && o.m > KAD_GEMM8_FEW;
   Held8 along, down;
-  if (in_memory) along = new_held(dy, {o.m}, o.n);
-  if (need_weight) down = new_held(dy, {o.n}, o.m);
+  if (in_memory) along = new_held(dy, o.m, o.n);
+  if (need_weight) down = new_held(dy, o.n, o.m);
   if (in_memory || need_weight || need_bias) quantize(r, along, down, db, dy);
-  if (in_memory) product(along.codes, along.scales, 0, across.w, o.m, o.k, o.n, Tensor(), KAD_ACT_NONE, dx);
-  else if (need_x) product(r.held, Tensor(), r.rs, across.w, o.m, o.k, o.n, Tensor(), KAD_ACT_NONE, dx);
-  if (need_weight) product(down.codes, down.scales, 0, across.x, o.n, o.k, o.m, Tensor(), KAD_ACT_NONE, dw);
+  if (in_memory) product(along, across.w, o.m, o.k, o.n, Tensor(), KAD_ACT_NONE, dx);
+  else if (need_x) product(r, across.w, o.k, Tensor(), KAD_ACT_NONE, dx);
+  if (need_weight) product(down, across.x, o.n, o.k, o.m, Tensor(), KAD_ACT_NONE, dw);
   return {dx, dw, db};
 }
 
 struct Linear8Backward : torch::autograd::Node {
-  torch::autograd::SavedVariable x_codes, x_scales, w_codes, w_scales;  // along their columns
+  torch::autograd::SavedVariable x, w;  // in 8 bits along their columns
   Linear8Sizes o;
   bool map, has_x, has_w;
   c10::DimVector sizes;  // of y
@@ -745,7 +769,8 @@ struct Linear8Backward : torch::autograd::Node {
 
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    for (auto* v : {&x_codes, &x_scales, &w_codes, &w_scales}) v->reset_data();
+    x.reset_data();
+    w.reset_data();
   }
 
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
@@ -758,14 +783,9 @@ struct Linear8Backward : torch::autograd::Node {
     const bool need_x = has_w && task_should_compute_output(0), need_w = has_x && task_should_compute_output(1),
                need_b = task_should_compute_output(2);
     Across across;
-    if (need_w) {
-      across.x = {x_codes.unpack(), x_scales.unpack()};
-      check_held(across.x.codes, across.x.scales, o.k, std::max<int64_t>(o.m, 1), dy, "the saved input");
-    }
-    if (need_x) {
-      across.w = {w_codes.unpack(), w_scales.unpack()};
-      check_held(across.w.codes, across.w.scales, o.k, o.n, dy, "the saved weight");
-    }
+    // a hook on saved tensors may have put others in their place
+    if (need_w) across.x = saved_held(x.unpack(), o.k, std::max<int64_t>(o.m, 1), dy, "the saved input");
+    if (need_x) across.w = saved_held(w.unpack(), o.k, o.n, dy, "the saved weight");
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const c10::DeviceGuard guard(dy.device());
@@ -802,14 +822,8 @@ OptTensor linear8(const Tensor& x, const Tensor& weight, const OptTensor& bias, 
     node->sizes = c10::DimVector(y.sizes());
     node->has_x = across.x.defined();
     node->has_w = across.w.defined();
-    if (node->has_x) {
-      node->x_codes = torch::autograd::SavedVariable(across.x.codes, false);
-      node->x_scales = torch::autograd::SavedVariable(across.x.scales, false);
-    }
-    if (node->has_w) {
-      node->w_codes = torch::autograd::SavedVariable(across.w.codes, false);
-      node->w_scales = torch::autograd::SavedVariable(across.w.scales, false);
-    }
+    if (node->has_x) node->x = torch::autograd::SavedVariable(across.x.buffer, false);
+    if (node->has_w) node->w = torch::autograd::SavedVariable(across.w.buffer, false);
     torch::autograd::set_history(y, node);
   }
   return y;
@@ -839,11 +853,11 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear8_backward(const Tensor& dy, c
   const c10::DeviceGuard guard(x.device());
   Across across;
   if (need_weight && o.m) {
-    across.x = new_held(x, {o.k}, o.m);
+    across.x = new_held(x, o.k, o.m);
     quantize(rows_of(x, map), {}, across.x, Tensor(), x);
   }
   if (need_x && o.m) {
-    across.w = new_held(x, {o.k}, o.n);
+    across.w = new_held(x, o.k, o.n);
     quantize(rows_of(weight, false), {}, across.w, Tensor(), x);
   }
   auto [dx, dw, db] = linear8_gradients(dy, map, o, across, need_x, need_weight, need_bias && b.defined());
@@ -861,7 +875,7 @@ Tensor linear8_kept_run(const Tensor& x, const Tensor& codes, const Tensor& scal
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard guard(x.device());
   Tensor y = result_like(x, map, n);
-  if (y.numel()) product_of_values(rows_of(x, map), {codes, scales}, n, dense(b), ac, y);
+  if (y.numel()) product_of_values(rows_of(x, map), held_of(codes, scales), n, dense(b), ac, y);
   return y;
 }
 
