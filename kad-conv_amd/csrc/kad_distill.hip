@@ -353,14 +353,16 @@ struct Soft {
   // The base of differences: 0 while all values are -inf, whose exponentials are 0.
   static __device__ __forceinline__ float base(float m) { return m == -INF ? 0.f : m; }
   template <int N>
-  __device__ __forceinline__ void add(const float* v, int skip, float c2) {
+  __device__ __forceinline__ void add(const float* v, float c2) {  // what does not count is -inf
     float n = m;
 #pragma unroll
     for (int e = 0; e < N; ++e) n = fmaxf(n, v[e]);
     const float b = base(n);
     s *= exp2_((m - b) * c2);
+    float more = 0.f;
 #pragma unroll
-    for (int e = 0; e < N; ++e) s += e >= skip ? exp2_((v[e] - b) * c2) : 0.f;
+    for (int e = 0; e < N; ++e) more += exp2_((v[e] - b) * c2);
+    s += more;
     m = n;
   }
   __device__ __forceinline__ void join(float om, float os, float c2) {
@@ -402,46 +404,100 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// The row's loss, given its Soft: by a block of 256 threads.
+// What the entries come to, before the row's largest logit zm is known: with zr the largest logit of the entries' classes,
+// d = sum e ((t - tm) - (z_i - zr)), to which S (zm - zr) is added.
+struct Teacher {
+  float s, d, zr;
+  bool counts;
+};
 template <typename T>
-__device__ __forceinline__ float entries_loss(const kad_distill_args& a, const Entries& en, const T* z, const Soft& soft,
-                                              const Scales& c, float* red, bool& counts) {
-  float tm = -INF, any = 0.f, s = 0.f, d = 0.f, t;
-  int at;
-  for (int e = threadIdx.x; e < a.k; e += 256)
-    if (en.get(e, at, t)) {
+__device__ __forceinline__ Teacher teacher_of(const kad_distill_args& a, const Entries& en, const T* z, const Scales& c) {
+  constexpr int MOST = KAD_DISTILL_MOST / 256;
+  __shared__ float red[3][4];
+  float t[MOST], zi[MOST], tm = -INF, zr = -INF, any = 0.f;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    const int e = threadIdx.x + 256 * i;
+    t[i] = -INF;
+    zi[i] = 0.f;
+    int at;
+    float v;
+    if (e < a.k && en.get(e, at, v)) {
+      t[i] = v;
+      zi[i] = to_f32(z[at]);
+      tm = fmaxf(tm, v);
+      zr = fmaxf(zr, zi[i]);
       any = 1.f;
-      tm = fmaxf(tm, t);
     }
-  counts = block_max(any, red) != 0.f;
-  tm = block_max(tm, red);
-  for (int e = threadIdx.x; e < a.k; e += 256)
-    if (en.get(e, at, t)) add_entry(t, tm, to_f32(z[at]), soft.m, c.c2, s, d);
-  s = block_sum(s, red);
-  d = block_sum(d, red);
-  return counts ? row_loss(a.temperature, s, d, soft.s, c) : 0.f;
+  }
+  const int wave = threadIdx.x >> 6;
+  tm = lanes_max(tm, 64);
+  zr = lanes_max(zr, 64);
+  any = lanes_max(any, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    red[0][wave] = tm;
+    red[1][wave] = zr;
+    red[2][wave] = any;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    tm = fmaxf(tm, red[0][w]);
+    zr = fmaxf(zr, red[1][w]);
+    any = fmaxf(any, red[2][w]);
+  }
+  if (zr == -INF) zr = 0.f;  // no entry's class has weight: d is infinite
+  Teacher r{0.f, 0.f, zr, any != 0.f};
+#pragma unroll
+  for (int i = 0; i < MOST; ++i)
+    if (t[i] != -INF) add_entry(t[i], tm, zi[i], zr, c.c2, r.s, r.d);
+  r.s = lanes_sum(r.s, 64);
+  r.d = lanes_sum(r.d, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    red[0][wave] = r.s;
+    red[1][wave] = r.d;
+  }
+  __syncthreads();
+  r.s = red[0][0] + red[0][1] + red[0][2] + red[0][3];
+  r.d = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  return r;
+}
+__device__ __forceinline__ float large_loss(const kad_distill_args& a, const Teacher& t, const Soft& soft, const Scales& c) {
+  return t.counts ? row_loss(a.temperature, t.s, t.d + t.s * (soft.m - t.zr), soft.s, c) : 0.f;
 }
 
-// The Soft of values [begin, end), which are VEC<T> at least.
+// The Soft of values [begin, end), which are VEC<T> at least: the next vectors are on their way while some are added.
 template <typename T>
 __device__ __forceinline__ Soft soft_of(const T* z, int begin, int end, float c2) {
   constexpr int V = VEC<T>, AT_ONCE = 4;
   Soft r;
   const int n = (end - begin + V - 1) / V;
-  for (int j = threadIdx.x; j < n; j += AT_ONCE * 256) {
-    intx4 raw[AT_ONCE];
-    int skip[AT_ONCE];
+  intx4 next[AT_ONCE];
+  const auto fetch = [&](int j) {
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
-      const int i = begin + (j + u * 256) * V, at = i < end - V ? i : end - V;
-      skip[u] = i < end ? i - at : V;
-      raw[u] = load_vec(z + at);
+      const int i = begin + (j + u * 256) * V;
+      next[u] = load_vec(z + (i < end - V ? i : end - V));
     }
+  };
+  fetch(threadIdx.x);
+  for (int j = threadIdx.x; j - (int)threadIdx.x < n; j += AT_ONCE * 256) {
+    intx4 raw[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) raw[u] = next[u];
+    fetch(j + AT_ONCE * 256);
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = begin + (j + u * 256) * V;
       float v[V];
       unpack<T>(raw[u], v);
-      r.add<V>(v, skip[u], c2);
+      if (i > end - V) {  // moved back to end with the row: its first values are another thread's, or all are
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = e >= i - (end - V) ? v[e] : -INF;
+      }
+      r.add<V>(v, c2);
     }
   }
   return r;
@@ -461,13 +517,13 @@ __global__ __launch_bounds__(256) void distill_large_fwd_kernel(kad_distill_args
   unsigned count = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* z = (const T*)a.logits + row * a.z_rs;
+    const Teacher teacher = teacher_of(a, Entries(a, row), z, c);
     const Soft soft = settled(join_block(soft_of(z, 0, a.v, c.c2), c.c2, red));
-    bool counts;
-    const float loss = entries_loss(a, Entries(a, row), z, soft, c, red, counts);
     if (threadIdx.x == 0) {
-      leave_row(a, row, counts, soft.m, soft.s, loss);
+      const float loss = large_loss(a, teacher, soft, c);
+      leave_row(a, row, teacher.counts, soft.m, soft.s, loss);
       total += loss;
-      count += counts;
+      count += teacher.counts;
     }
   }
   leave_part(a, total, count);
@@ -496,10 +552,10 @@ __global__ __launch_bounds__(256) void distill_parts_fwd_kernel(kad_distill_args
     mine.s = softs[2 * (row * parts + threadIdx.x) + 1];
   }
   const Soft soft = settled(join_block(mine, c.c2, red));
-  bool counts;
-  const float loss = entries_loss(a, Entries(a, row), (const T*)a.logits + row * a.z_rs, soft, c, red, counts);
-  if (threadIdx.x == 0) leave_row(a, row, counts, soft.m, soft.s, loss);
-  leave_part(a, threadIdx.x ? 0.f : loss, threadIdx.x == 0 && counts);
+  const Teacher teacher = teacher_of(a, Entries(a, row), (const T*)a.logits + row * a.z_rs, c);
+  const float loss = large_loss(a, teacher, soft, c);
+  if (threadIdx.x == 0) leave_row(a, row, teacher.counts, soft.m, soft.s, loss);
+  leave_part(a, threadIdx.x ? 0.f : loss, threadIdx.x == 0 && teacher.counts);
 }
 
 // Rows from the last to the first: the forward pass left the last ones in the memory-side cache.
