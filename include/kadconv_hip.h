@@ -702,7 +702,7 @@ typedef struct kad_distill_args {
   int64_t inner;          /* >= 1 */
   int64_t t_sn, t_sp, t_sk, i_sn, i_sp, i_sk;  /* >= 0 */
   int v, k;               /* v: 1 .. 2^30, k: 1 .. KAD_DISTILL_MOST */
-  float temperature;      /* > 0 */
+  float temperature;      /* 1e-6 .. 1e6 */
   int reduction;
   int dtype, teacher_dtype, index_bits; /* index_bits: 32 or 64 */
 } kad_distill_args;
@@ -751,12 +751,13 @@ typedef struct kad_gemm8_args {
   void *out;                  /* dense [m][n], dtype */
   float *work;                /* kad_gemm8_work_elems floats; need not be initialised, free after the call */
   int64_t a_rs;               /* a as values: elements from row to row (>= k) */
-  int m, n, k;                /* >= 1; k at most KAD_QUANT8_MOST; fewer than 2^24 tiles of 64 x 64 results */
+  int m, n, k;                /* >= 1; k at most KAD_GEMM8_MOST; fewer than 2^24 tiles of 64 x 64 results */
   int act;                    /* KAD_ACT_NONE, KAD_ACT_RELU or KAD_ACT_SILU */
   int dtype, a_dtype, bias_dtype; /* a_dtype: of a as values */
 } kad_gemm8_args;
 
 #define KAD_GEMM8_FEW 32
+#define KAD_GEMM8_MOST (1 << 22)  /* 256 rows of codes lie within 2^31 bytes */
 
 int64_t kad_gemm8_work_elems(const kad_gemm8_args *a);
 int kad_gemm8(const kad_gemm8_args *a, void *stream);

@@ -667,7 +667,7 @@ int check_args(const kad_distill_args* a, const char* what) {
   KAD_CHECK_ARG(a->rows > 0 && a->rows <= INT32_MAX, "%s: 1 to 2^31 - 1 rows expected", what);
   KAD_CHECK_ARG(a->v > 0 && a->v <= 1 << 30, "%s: 1 to 2^30 classes expected", what);
   KAD_CHECK_ARG(a->k > 0 && a->k <= KAD_DISTILL_MOST, "%s: 1 to %d entries expected", what, KAD_DISTILL_MOST);
-  KAD_CHECK_ARG(a->temperature > 0.f && a->temperature < INF, "%s: temperature must be positive", what);
+  KAD_CHECK_ARG(a->temperature >= 1e-6f && a->temperature <= 1e6f, "%s: temperature must lie in 1e-6 to 1e6", what);
   KAD_CHECK_ARG(a->reduction >= KAD_REDUCE_NONE && a->reduction <= KAD_REDUCE_MEAN, "%s: unknown reduction", what);
   return KAD_OK;
 }

@@ -719,7 +719,7 @@ int check_args(const kad_gemm8_args* a, const char* what) {
   const auto is_dtype = [](int t) { return t == KAD_F32 || t == KAD_F16 || t == KAD_BF16; };
   KAD_CHECK_ARG(a, "%s: null pointer", what);
   KAD_CHECK_ARG(is_dtype(a->dtype), "%s: bad dtype", what);
-  KAD_CHECK_ARG(a->m > 0 && a->n > 0 && a->k > 0 && a->k <= KAD_QUANT8_MOST && a->m <= INT32_MAX - 255 && a->n <= INT32_MAX - 255,
+  KAD_CHECK_ARG(a->m > 0 && a->n > 0 && a->k > 0 && a->k <= KAD_GEMM8_MOST && a->m <= INT32_MAX - 255 && a->n <= INT32_MAX - 255,
                 "%s: bad sizes", what);
   KAD_CHECK_ARG((int64_t)ceil_div(a->m, 64) * ceil_div(a->n, 64) < 1 << 24, "%s: fewer than 2^24 tiles of 64 x 64 results expected", what);
   KAD_CHECK_ARG(a->act == KAD_ACT_NONE || a->act == KAD_ACT_RELU || a->act == KAD_ACT_SILU, "%s: unknown activation", what);

@@ -1,8 +1,6 @@
 // kadconv._native: operators on rows, which are the last axis of a tensor or the channels of a map's pixels.
 #include "kad_torch.h"
 
-#include <cmath>
-
 namespace {
 
 // The number of the axis along which rows run, as dim says: the last one, or the channels of [N, C, H, W].
@@ -309,7 +307,7 @@ bool check_distill(const Tensor& x, const Tensor& t, const Tensor& index, double
   TORCH_CHECK_VALUE(x.device() == t.device() && x.device() == index.device(), "logits and the teacher's tensors must be on one device");
   TORCH_CHECK_TYPE(index.scalar_type() == at::kInt || index.scalar_type() == at::kLong,
                    "teacher_index must be torch.int32 or torch.int64, got ", index.scalar_type());
-  TORCH_CHECK_VALUE(temperature > 0 && std::isfinite((float)temperature) && (float)temperature > 0, "temperature must be positive");
+  TORCH_CHECK_VALUE(temperature >= 1e-6 && temperature <= 1e6, "temperature must lie in 1e-6 to 1e6, got ", temperature);
   TORCH_CHECK_VALUE(x.is_cuda(), "a GPU tensor expected, got one on ", x.device());
   dtype_of(x);
   dtype_of(t);
@@ -500,7 +498,8 @@ std::tuple<Tensor, Tensor, Tensor> distill_loss_forward(const Tensor& x, const T
   const Distill o{temperature, checked_reduction(reduction), dim};
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard guard(x.device());
-  const Tensor stats = floats(x, {row_count(x, map), 2}), share = floats(x, {1});
+  const Tensor stats = floats(x, {row_count(x, map), 2});
+  const Tensor share = o.reduction == KAD_REDUCE_MEAN ? floats(x, {1}) : floats(x, {1}).zero_();
   return {distill_run(x, map, t, index, o, stats, share), stats, share};
 }
 
@@ -703,16 +702,22 @@ struct Across {
   Held8 x, w;
 };
 
+// The gradient of a weight is a product over the rows.
+void check_many(int64_t rows) {
+  TORCH_CHECK_VALUE(rows <= KAD_GEMM8_MOST, "a weight has a gradient of up to ", KAD_GEMM8_MOST, " rows, got ", rows);
+}
+
 // y of values and a weight, which are brought to 8 bits; `across`: where wanted, along the columns in the same reads.
 Tensor linear8_run(const Tensor& x, bool map, const Tensor& weight, const Tensor& bias, int act, bool across_x, bool across_w,
                    Across& across) {
   const int64_t n = weight.size(0), k = weight.size(1);
   Tensor y = result_like(x, map, n);
+  const int64_t m = row_count(x, map);
+  if (across_x) check_many(m);
   const Rows w = rows_of(weight, false);
   const Held8 wh = new_held(x, n, k);
   if (across_w) across.w = new_held(x, k, n);
   quantize(w, wh, across.w, Tensor(), x);
-  const int64_t m = row_count(x, map);
   if (across_x) across.x = new_held(x, k, std::max<int64_t>(m, 1));
   if (!m) return y;
   const Rows r = rows_of(x, map);
@@ -852,6 +857,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear8_backward(const Tensor& dy, c
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard guard(x.device());
   Across across;
+  if (need_weight) check_many(o.m);
   if (need_weight && o.m) {
     across.x = new_held(x, o.k, o.m);
     quantize(rows_of(x, map), {}, across.x, Tensor(), x);

@@ -214,7 +214,7 @@ def linear8(input, weight, bias=None, act=None, dim=-1):
     With numbers as weight and no ``act`` it is differentiable once.  Gradients pass the rounding as if it were not there,
     and are products in 8 bits themselves: that of x is dy W, both along N, that of W is dy^T x, both along the rows; that
     of the bias is the sum of dy.  For them x and W are kept in 8 bits, not as they are: later changes of either are not
-    seen.
+    seen.  The gradient of W takes up to 2^22 rows.
 
     GPU tensors (fp32, fp16, bf16) run the gfx950 HIP kernels; rows that lie a fixed distance apart are read where they
     are.  Up to 32 rows take one launch, their numbers brought to 8 bits by the product's own threads.  The result is

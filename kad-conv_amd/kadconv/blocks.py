@@ -186,7 +186,7 @@ class LayerNorm(nn.Module):
         self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
 
     def forward(self, x):
-        if x.shape[self.dim] != self.num_channels:
+        if x.shape[ops._row_axis(x, self.dim)] != self.num_channels:
             raise ValueError(f'rows of {self.num_channels} values expected, got {tuple(x.shape)} along axis {self.dim}')
         return ops.layer_norm(x, self.weight, self.bias, self.eps, self.dim)
 
@@ -199,7 +199,9 @@ class Linear8(nn.Module):
     products in 8 bits (``kadconv.linear8``); parameters as torch.nn.Linear's, so its state dicts load.
 
     In eval mode, where nothing is differentiated, W is kept in 8 bits and laid out anew when it has changed (seen by its
-    version: a write through ``.data`` is not), and ``act`` is applied in the same launch.  Other calls go by W itself."""
+    version: a write through ``.data`` is not), and ``act`` is applied in the same launch.  Other calls go by W itself, and
+    so does one that is captured into a graph: its replays follow W.  (For a graph that reads W in 8 bits only, capture
+    ``kadconv.linear8`` with ``kadconv.quantize8(W)``.)"""
 
     def __init__(self, in_features, out_features, bias=True, act=None, dim=-1):
         super().__init__()
@@ -212,7 +214,7 @@ class Linear8(nn.Module):
         self.in_features, self.out_features, self.act, self.dim = in_features, out_features, act, dim
         like = nn.Linear(in_features, out_features, bias)
         self.weight, self.bias = like.weight, like.bias
-        self._kept = None  # (weight, its version, the weight in 8 bits)
+        self._kept = None  # (weight, its version, the weight in 8 bits, the stream that it was laid out on, and when)
 
     def __getstate__(self):
         return {**self.__dict__, '_kept': None}  # a copy of the module lays out its own
@@ -222,15 +224,22 @@ class Linear8(nn.Module):
         if w.is_inference():
             return block8.quantize8(w)
         # the weight that was laid out is held, so that its address is no other's
+        stream = torch.cuda.current_stream(w.device)
         if kept is None or kept[0].data_ptr() != w.data_ptr() or (kept[0].dtype, kept[1]) != (w.dtype, self.weight._version):
-            kept = self._kept = w, self.weight._version, block8.quantize8(w)
+            kept = self._kept = w, self.weight._version, block8.quantize8(w), stream, stream.record_event()
+        if stream != kept[3]:  # laid out on another one
+            stream.wait_event(kept[4])
+            kept[2].codes.record_stream(stream)
+            kept[2].scales.record_stream(stream)
         return kept[2]
 
     def forward(self, x):
         grad = torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters()))
         if grad and self.act is not None:
             return {'relu': F.relu, 'silu': F.silu}[self.act](block8.linear8(x, self.weight, self.bias, None, self.dim))
-        keep = not (grad or self.training or torch.compiler.is_compiling()) and x.is_cuda
+        # the other calls: with gradients, traced, on fake tensors, captured
+        keep = not (grad or self.training or torch.compiler.is_compiling()) and x.is_cuda and \
+            type(self.weight) is nn.Parameter and not torch.cuda.is_current_stream_capturing()
         return block8.linear8(x, self._weight8() if keep else self.weight, self.bias, self.act, self.dim)
 
     def extra_repr(self):

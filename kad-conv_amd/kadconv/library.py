@@ -306,7 +306,9 @@ def _(dy, x, weight, bias, dim):
 
 
 def _linear8_context(ctx, inputs, output):
-    x, weight, bias, _, dim = inputs
+    x, weight, bias, act, dim = inputs
+    if act is not None:
+        raise NotImplementedError('kadconv.linear8 with an activation has no gradient')
     ctx.save_for_backward(x, weight, bias)
     ctx.dim = dim
 

@@ -377,8 +377,8 @@ def _distill_check(x, t, index, temperature, reduction, dim):
         raise ValueError("logits and the teacher's tensors must be on one device")
     if index.dtype not in (torch.int32, torch.int64):
         raise TypeError(f'teacher_index must be torch.int32 or torch.int64, got {index.dtype}')
-    if not 0 < temperature < float('inf'):
-        raise ValueError('temperature must be positive')
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f'temperature must lie in 1e-6 to 1e6, got {temperature}')
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction {reduction!r} is none of 'none', 'sum', 'mean'")
     for v in (x, t):
@@ -427,11 +427,11 @@ def distill_loss(logits, teacher_logits, teacher_index, temperature=1.0, reducti
         p = softmax(t / T) over a row's entries, q = softmax(z / T) over all classes,
         loss = T^2 sum_e p_e (log p_e - log q[i_e])
 
-    ``logits`` z [..., V] (or with ``dim=1`` maps [N, V, H, W]); ``teacher_logits`` t and ``teacher_index`` i (int32 or
-    int64), of the same shape but for K entries in place of the V classes, as torch.topk returns them.  An entry whose
-    index lies outside of [0, V) or whose logit is -infinity does not count; an index that comes twice has both weights.
-    A row without entries that count is 0 and has no gradient, whatever its logits are; a row that has some, but logits
-    of -infinity alone, is NaN.
+    at ``temperature`` T (1e-6 to 1e6).  ``logits`` z [..., V] (or with ``dim=1`` maps [N, V, H, W]); ``teacher_logits`` t
+    and ``teacher_index`` i (int32 or int64), of the same shape but for K entries in place of the V classes, as torch.topk
+    returns them.  An entry whose index lies outside of [0, V) or whose logit is -infinity does not count; an index that
+    comes twice has both weights.  A row without entries that count is 0 and has no gradient, whatever its logits are; a
+    row that has some, but logits of -infinity alone, is NaN.
 
     ``reduction``: 'none' (a row's loss each, float32), 'sum', or 'mean' over the rows that have entries (0 if none has).
     Sums are taken in 32 bits and in an order that the sizes decide.  The teacher's tensors are constants.

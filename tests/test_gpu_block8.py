@@ -419,8 +419,60 @@ def test_module():
         assert torch.equal(fresh(x), kadconv.linear8(x, fresh.weight, fresh.bias))
 
 
+def test_module_on_another_stream():
+    """The weight is laid out on one stream, behind much other work, and used on another at once."""
+    x, m = make(200, 300, F16, 1), kadconv.Linear8(300, 64).to(DEV, F16).eval()
+    busy = torch.randn(4096, 4096, device=DEV)
+    side = torch.cuda.Stream()
+    with torch.no_grad():
+        want = kadconv.linear8(x, kadconv.quantize8(m.weight), m.bias)
+        torch.cuda.synchronize()
+        for _ in range(20):
+            busy = busy @ busy
+            busy = busy / busy.norm()
+        m(x)
+        with torch.cuda.stream(side):
+            got = m(x)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_module_in_a_graph_follows_its_weight():
+    x, m = make(100, 300, F16, 1), kadconv.Linear8(300, 20, act='relu').to(DEV, F16).eval()
+    with torch.no_grad():
+        m(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = m(x)
+        for k in range(3):
+            m.weight.normal_()
+            graph.replay()
+            want = kadconv.linear8(x, m.weight, m.bias, 'relu')
+            torch.cuda.synchronize()
+            assert torch.equal(y, want) and torch.equal(m(x), want), k
+
+
+@pytest.mark.parametrize('rows', [(1 << 20) + 200, 1 << 22])
+def test_gradient_over_many_rows(rows):
+    """Sums over more than 2^20 rows, of numbers that 8 bits hold and whose sums 32 bits hold exactly."""
+    x = torch.randint(-1, 2, (rows, 3), device=DEV).to(F16)
+    dy = torch.randint(-1, 2, (rows, 2), device=DEV).to(F16)
+    w = torch.ones(2, 3, device=DEV)
+    _, dw, db = block8.linear8_backward(dy, x, w, torch.zeros(2, device=DEV), -1, need_x=False)
+    assert torch.equal(dw.double(), dy.double().t() @ x.double()) and torch.equal(db.double(), dy.double().sum(0))
+
+
 def test_refusals():
     x, w = make(3, 40, F32), make(5, 40, F32)
+    many = torch.zeros((1 << 22) + 1, 1, device=DEV, dtype=F16)
+    with pytest.raises(ValueError, match='rows'):
+        kadconv.linear8(many, torch.ones(1, 1, device=DEV, requires_grad=True))
+    with pytest.raises(ValueError, match='rows'):
+        block8.linear8_backward(many, many, torch.ones(1, 1, device=DEV), None, -1)
+    assert not kadconv.linear8(many, torch.ones(1, 1, device=DEV)).any()
+    with pytest.raises(NotImplementedError, match='activation'):
+        torch.ops.kadconv.linear8(x, w.clone().requires_grad_(True), None, 'silu', -1)
     q = kadconv.quantize8(w)
     with pytest.raises(TypeError):
         kadconv.linear8(x.double(), w)

@@ -46,6 +46,8 @@ def test_layer_norm_refusals():
         kadconv.LayerNorm(4, dim=2)
     with pytest.raises(ValueError, match='rows of 4'):
         kadconv.LayerNorm(4)(x)
+    with pytest.raises(ValueError, match='dim must'):
+        kadconv.LayerNorm(4, dim=1)(x[0])
     with pytest.raises(ValueError, match='needs a GPU'):
         torch.ops.kadconv.layer_norm(x, None, None, 1e-5, -1)
     native = _ext.native()
@@ -125,7 +127,7 @@ def test_distill_refusals():
                         ((z[:2], t, i), 'shape of logits'), ((z, t[..., :0], i[..., :0]), 'entries')):
         with pytest.raises(ValueError, match=match):
             kadconv.distill_loss(*args)
-    for temperature in (0.0, -1.0, float('inf'), float('nan')):
+    for temperature in (0.0, -1.0, 9e-7, 1.1e6, float('inf'), float('nan')):
         with pytest.raises(ValueError, match='temperature'):
             kadconv.distill_loss(z, t, i, temperature)
     with pytest.raises(ValueError, match='reduction'):
@@ -158,7 +160,7 @@ def _distill_args(**kw):
 
 @pytest.mark.parametrize('kw', [dict(logits=None), dict(teacher=None), dict(index=None), dict(loss=None), dict(work=None), dict(rows=0),
                                 dict(rows=1 << 31), dict(v=0), dict(v=(1 << 30) + 1), dict(k=0), dict(k=1025), dict(z_rs=7),
-                                dict(z_rs=1 << 31), dict(inner=0), dict(t_sk=-1), dict(i_sn=-1), dict(temperature=0.0), dict(reduction=3),
+                                dict(z_rs=1 << 31), dict(inner=0), dict(t_sk=-1), dict(i_sn=-1), dict(temperature=0.0), dict(temperature=1e7), dict(reduction=3),
                                 dict(dtype=9), dict(teacher_dtype=-1), dict(index_bits=16)], ids=str)
 def test_distill_c_refuses(kw):
     lib = _ext.load()
@@ -307,7 +309,7 @@ def _gemm_args(**kw):
 
 
 @pytest.mark.parametrize('kw', [dict(a=None), dict(b=None), dict(b_scales=None), dict(out=None), dict(m=0), dict(n=0), dict(k=0),
-                                dict(k=(1 << 20) + 1), dict(m=(1 << 31) - 100), dict(act=7), dict(dtype=5), dict(bias_dtype=-1),
+                                dict(k=(1 << 22) + 1), dict(m=(1 << 31) - 100), dict(act=7), dict(dtype=5), dict(bias_dtype=-1),
                                 dict(a_scales=None, m=65), dict(a_scales=None, a_rs=7), dict(a_scales=None, a_dtype=4), dict(b=4104),
                                 dict(a=4104), dict(b_scales=4098), dict(a_scales=4098), dict(m=1 << 20, n=1 << 20),
                                 dict(m=100, k=100000, work=None)], ids=str)
@@ -322,7 +324,7 @@ def test_gemm8_parts_cover_k():
     lib = _ext.load()
     for m in (1, 64, 65, 1000, 70000):
         for n in (1, 300, 5000):
-            for k in (1, 128, 1000, 20000, 1 << 20):
+            for k in (1, 128, 1000, 20000, 1 << 22):
                 for dtype in (0, 1):
                     w = lib.kad_gemm8_work_elems(ctypes.byref(_gemm_args(m=m, n=n, k=k, dtype=dtype)))
                     assert w >= 0 and w % (m * n) == 0 and w // (m * n) != 1 and w // (m * n) <= 512
