@@ -751,7 +751,8 @@ typedef struct kad_gemm8_args {
   void *out;                  /* dense [m][n], dtype */
   float *work;                /* kad_gemm8_work_elems floats; need not be initialised, free after the call */
   int64_t a_rs;               /* a as values: elements from row to row (>= k) */
-  int m, n, k;                /* >= 1; k at most KAD_GEMM8_MOST; fewer than 2^24 tiles of 64 x 64 results */
+  int m, n, k;                /* >= 1; k at most KAD_GEMM8_MOST; fewer than 2^24 tiles of 64 x 64 results;
+                                 n < 2^26 where m <= KAD_GEMM8_FEW */
   int act;                    /* KAD_ACT_NONE, KAD_ACT_RELU or KAD_ACT_SILU */
   int dtype, a_dtype, bias_dtype; /* a_dtype: of a as values */
 } kad_gemm8_args;

@@ -722,6 +722,7 @@ int check_args(const kad_gemm8_args* a, const char* what) {
   KAD_CHECK_ARG(a->m > 0 && a->n > 0 && a->k > 0 && a->k <= KAD_GEMM8_MOST && a->m <= INT32_MAX - 255 && a->n <= INT32_MAX - 255,
                 "%s: bad sizes", what);
   KAD_CHECK_ARG((int64_t)ceil_div(a->m, 64) * ceil_div(a->n, 64) < 1 << 24, "%s: fewer than 2^24 tiles of 64 x 64 results expected", what);
+  KAD_CHECK_ARG(!few(*a) || a->n < 1 << 26, "%s: up to %d rows: fewer than 2^26 columns expected", what, KAD_GEMM8_FEW);
   KAD_CHECK_ARG(a->act == KAD_ACT_NONE || a->act == KAD_ACT_RELU || a->act == KAD_ACT_SILU, "%s: unknown activation", what);
   KAD_CHECK_ARG(a->a_scales || (is_dtype(a->a_dtype) && few(*a)), "%s: a as values: of a known dtype, and at most %d rows", what,
                 KAD_GEMM8_FEW);

@@ -47,7 +47,7 @@ Rows rows_of(const Tensor& x, bool map) {
     fits = fits && s == expected;
     expected *= n;
   }
-  if (fits && r.rs >= c && r.rs <= INT32_MAX) return r;
+  if (fits && r.rs >= c && r.rs <= INT32_MAX && !x.is_neg()) return r;
   r.held = dense_like(x, map);
   r.held.copy_(x);
   r.rs = c;
@@ -418,7 +418,7 @@ Tensor distill_gradient(const Tensor& dloss, const Tensor& x, bool map, const Te
   if (!x.numel()) return dx;
   const Rows r = rows_of(x, map);
   const Strided te = entries_of(t, map), ie = entries_of(index, map);
-  const Tensor g = dloss.contiguous();
+  const Tensor g = dloss.contiguous().resolve_neg();
   kad_distill_args a = distill_args(r, te, ie, map, o);
   a.dloss = g.const_data_ptr<float>();
   a.dlogits = dx.mutable_data_ptr();
@@ -625,7 +625,7 @@ void check_quantized(const Tensor& x, int64_t k) {
 }
 
 // x [..., K] (or a map's pixels) as codes and scales [..., ...].
-std::tuple<Tensor, Tensor> quantize8(const Tensor& x, int64_t dim) {
+std::tuple<Tensor, Tensor> quantize8_forward(const Tensor& x, int64_t dim) {
   const bool map = is_map(x, dim);
   check_quantized(x, row_length(x, map));
   at::AutoDispatchBelowADInplaceOrView below;
@@ -640,14 +640,20 @@ std::tuple<Tensor, Tensor> quantize8(const Tensor& x, int64_t dim) {
   return {codes, scales};
 }
 
+// None where the call is observed.
+std::optional<std::tuple<Tensor, Tensor>> quantize8(const Tensor& x, int64_t dim) {
+  if (observed({&x})) return std::nullopt;
+  return quantize8_forward(x, dim);
+}
+
 at::ScalarType checked_result(at::ScalarType t) {
   TORCH_CHECK_TYPE(t == at::kFloat || t == at::kHalf || t == at::kBFloat16, "unsupported dtype ", t, "; expected float32, float16 or bfloat16");
   return t;
 }
 
 // a [..., K] b [N, K]^T, both in 8 bits.
-Tensor matmul8(const Tensor& a, const Tensor& a_scales, const Tensor& b, const Tensor& b_scales, int64_t k, const OptTensor& bias,
-               const std::optional<std::string_view>& act, at::ScalarType dtype) {
+Tensor matmul8_forward(const Tensor& a, const Tensor& a_scales, const Tensor& b, const Tensor& b_scales, int64_t k, const OptTensor& bias,
+                       const std::optional<std::string_view>& act, at::ScalarType dtype) {
   TORCH_CHECK_VALUE(a.is_cuda(), "a GPU tensor expected, got one on ", a.device());
   TORCH_CHECK_VALUE(k >= 1 && k <= KAD_QUANT8_MOST, "rows of 1 to ", KAD_QUANT8_MOST, " values expected, got ", k);
   TORCH_CHECK_VALUE(a.dim() >= 1 && b.dim() == 2, "a of at least one axis and b of two expected");
@@ -667,6 +673,14 @@ Tensor matmul8(const Tensor& a, const Tensor& a_scales, const Tensor& b, const T
   Tensor out = at::detail::empty_cuda(sizes, checked_result(dtype), a.device(), std::nullopt);
   if (out.numel()) product(held_of(a, a_scales), held_of(b, b_scales), m, n, k, bi, ac, out);
   return out;
+}
+
+// None where the call is observed.
+OptTensor matmul8(const Tensor& a, const Tensor& a_scales, const Tensor& b, const Tensor& b_scales, int64_t k, const OptTensor& bias,
+                  const std::optional<std::string_view>& act, at::ScalarType dtype) {
+  const Tensor bi = defined(bias);
+  if (observed({&a, &a_scales, &b, &b_scales, &bi})) return std::nullopt;
+  return matmul8_forward(a, a_scales, b, b_scales, k, bias, act, dtype);
 }
 
 // What the kernels take as given: the checks of kadconv.block8._linear8_check, and that the input is on a GPU.
@@ -906,7 +920,9 @@ void kad_torch::bind_rows(py::module_& m) {
   m.def("layer_norm_forward", &layer_norm_forward);
   m.def("layer_norm_backward", &layer_norm_backward);
   m.def("quantize8", &quantize8);
+  m.def("quantize8_forward", &quantize8_forward);
   m.def("matmul8", &matmul8);
+  m.def("matmul8_forward", &matmul8_forward);
   m.def("linear8", &linear8);
   m.def("linear8_forward", &linear8_forward);
   m.def("linear8_backward", &linear8_backward);

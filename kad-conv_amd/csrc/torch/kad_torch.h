@@ -62,12 +62,14 @@ inline Tensor floats(const Tensor& x, at::IntArrayRef sizes) {
   return at::detail::empty_cuda(sizes, at::kFloat, x.device(), std::nullopt);
 }
 
-// Whether calls are watched (a trace, a dispatch mode) or a tensor stands for another (fake, wrapped): the caller then
-// takes the registered operator, which such a program sees.  What is allocated and launched here, it would not.
+// Whether calls are watched (a trace, a dispatch mode) or a tensor stands for another (fake, wrapped, or a view that
+// negates what is stored): the caller then takes the registered operator, which such a program sees and which is given
+// the values themselves.  What is allocated and launched here, it would not see.
 inline bool observed(std::initializer_list<const Tensor*> tensors) {
   if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::any_modes_set()) return true;
   for (const Tensor* t : tensors)
-    if (t->defined() && (!t->has_storage() || t->key_set().has(c10::DispatchKey::Python))) return true;
+    if (t->defined() && (!t->has_storage() || t->key_set().has(c10::DispatchKey::Python) || t->is_neg() || t->_is_zerotensor()))
+      return true;
   return false;
 }
 

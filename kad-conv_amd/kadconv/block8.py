@@ -90,7 +90,8 @@ def quantize8(input, dim=-1):
     are [N, H, W, ...]) as a ``Block8``.  Not differentiable: the result is constants."""
     axis = _quantize_check(input, dim)
     if input.is_cuda:
-        codes, scales = torch.ops.kadconv.quantize8(input, dim) if torch.compiler.is_compiling() else _ext.native().quantize8(input, dim)
+        held = None if torch.compiler.is_compiling() else _ext.native().quantize8(input, dim)
+        codes, scales = held or torch.ops.kadconv.quantize8(input.detach(), dim)
     else:
         codes, scales = _quantize_cpu(input.detach().movedim(axis, -1))
     return Block8(codes, scales, input.shape[axis])
@@ -125,8 +126,9 @@ def matmul8(a, b, bias=None, act=None, dtype=torch.bfloat16):
     if dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f'unsupported dtype {dtype}; expected float32, float16 or bfloat16')
     if a.codes.is_cuda:
-        return torch.ops.kadconv.matmul8(a.codes, a.scales, b.codes, b.scales, a.size, bias, act, dtype) \
-            if torch.compiler.is_compiling() else _ext.native().matmul8(a.codes, a.scales, b.codes, b.scales, a.size, bias, act, dtype)
+        args = a.codes, a.scales, b.codes, b.scales, a.size, bias, act, dtype
+        y = None if torch.compiler.is_compiling() else _ext.native().matmul8(*args)
+        return torch.ops.kadconv.matmul8(*args) if y is None else y
     z = F.linear(a.dequantize(torch.float64), b.dequantize(torch.float64), None if bias is None else bias.double())
     return _act_cpu(z, act).to(dtype)
 

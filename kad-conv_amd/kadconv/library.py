@@ -255,7 +255,7 @@ distill_loss.register_autograd(_distill_loss_grad, setup_context=_distill_loss_c
 @torch.library.custom_op('kadconv::quantize8', mutates_args=())
 def quantize8(x: torch.Tensor, dim: int) -> tuple[torch.Tensor, torch.Tensor]:
     from . import _ext
-    return _ext.native().quantize8(x, dim)
+    return _ext.native().quantize8_forward(x, dim)
 
 
 @quantize8.register_fake
@@ -272,7 +272,7 @@ def _(x, dim):
 def matmul8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, size: int,
             bias: torch.Tensor | None, act: str | None, dtype: torch.dtype) -> torch.Tensor:
     from . import _ext
-    return _ext.native().matmul8(a, a_scales, b, b_scales, size, bias, act, dtype)
+    return _ext.native().matmul8_forward(a, a_scales, b, b_scales, size, bias, act, dtype)
 
 
 @matmul8.register_fake

@@ -309,7 +309,7 @@ def _gemm_args(**kw):
 
 
 @pytest.mark.parametrize('kw', [dict(a=None), dict(b=None), dict(b_scales=None), dict(out=None), dict(m=0), dict(n=0), dict(k=0),
-                                dict(k=(1 << 22) + 1), dict(m=(1 << 31) - 100), dict(act=7), dict(dtype=5), dict(bias_dtype=-1),
+                                dict(k=(1 << 22) + 1), dict(m=(1 << 31) - 100), dict(m=1, n=1 << 26), dict(act=7), dict(dtype=5), dict(bias_dtype=-1),
                                 dict(a_scales=None, m=65), dict(a_scales=None, a_rs=7), dict(a_scales=None, a_dtype=4), dict(b=4104),
                                 dict(a=4104), dict(b_scales=4098), dict(a_scales=4098), dict(m=1 << 20, n=1 << 20),
                                 dict(m=100, k=100000, work=None)], ids=str)
@@ -328,3 +328,21 @@ def test_gemm8_parts_cover_k():
                 for dtype in (0, 1):
                     w = lib.kad_gemm8_work_elems(ctypes.byref(_gemm_args(m=m, n=n, k=k, dtype=dtype)))
                     assert w >= 0 and w % (m * n) == 0 and w // (m * n) != 1 and w // (m * n) <= 512
+
+
+def test_fake_tensors():
+    """Calls on fake GPU tensors give fake results of the right shapes and types, and launch nothing."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(), torch.device('cuda'):
+        x, w = torch.empty(5, 70), torch.empty(9, 70)
+        held, kept = kadconv.quantize8(x), kadconv.quantize8(w)
+        assert held.codes.shape == (5, 128) and held.scales.shape == (5, 4) and held.shape == (5, 70)
+        y = kadconv.matmul8(held, kept, dtype=torch.float16)
+        assert y.shape == (5, 9) and y.dtype == torch.float16
+        assert kadconv.linear8(x, kept, act='relu').shape == kadconv.linear8(x, w).shape == (5, 9)
+        m = kadconv.Linear8(70, 9).eval()
+        with torch.no_grad():
+            assert m(x).shape == m(x).shape == (5, 9) and m._kept is None
+        assert kadconv.LayerNorm(70)(x).shape == (5, 70)
+        t, i = torch.empty(5, 3), torch.empty(5, 3, dtype=torch.int64)
+        assert kadconv.distill_loss(x, t, i).shape == () and kadconv.distill_loss(x, t, i, reduction='none').shape == (5,)
