@@ -741,7 +741,8 @@ int64_t kad_quant8_work_elems(const kad_quant8_args *a);
 int kad_quant8(const kad_quant8_args *a, void *stream);
 
 /* out = act(a b^T + bias): a [m][k] and b [n][k] in 8 bits along k (as kad_quant8 writes them), or a as values
- * (a_scales NULL), which are brought to 8 bits on the way; then m is at most KAD_GEMM8_FEW.
+ * (a_scales NULL), which are brought to 8 bits on the way where kad_gemm8_takes_values says 1: with m up to
+ * KAD_GEMM8_FEW, and with short rows of dtype and few columns.
  * Sums are 32-bit.  Those of 32-bit results are taken from exact products; for 16-bit results the 8-bit matrix instruction
  * cuts the products of eight consecutive k to 2^-13 of the largest of them. */
 typedef struct kad_gemm8_args {
@@ -761,6 +762,7 @@ typedef struct kad_gemm8_args {
 #define KAD_GEMM8_MOST (1 << 22)  /* 256 rows of codes lie within 2^31 bytes */
 
 int64_t kad_gemm8_work_elems(const kad_gemm8_args *a);
+int kad_gemm8_takes_values(const kad_gemm8_args *a);  /* 1 or 0; looks at sizes and types alone */
 int kad_gemm8(const kad_gemm8_args *a, void *stream);
 
 #ifdef __cplusplus

@@ -100,4 +100,21 @@ __device__ __forceinline__ uint32_t largest_finite(const uint32_t* w) {
   return largest_of<T>(m);
 }
 
+template <typename T> constexpr int LANES = BLOCK8 / VEC<T>;  // that share a row's block
+
+// Largest over the N (16 or 32) lanes of a row, by lane permutations of the vector unit.
+template <int N>
+__device__ __forceinline__ uint32_t lanes_largest(uint32_t v) {
+  const auto with = [&](uint32_t o) { v = v > o ? v : o; };
+  with(__builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true));   // lane ^ 1
+  with(__builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true));   // lane ^ 2
+  with(__builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true));  // 7 - lane of eight
+  with(__builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true));  // 15 - lane of sixteen
+  if (N == 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = r[0] > r[1] ? r[0] : r[1];
+  }
+  return v;
+}
+
 }  // namespace kad

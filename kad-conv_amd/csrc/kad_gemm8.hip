@@ -9,10 +9,12 @@
 // all bits random 5e-5: under the rounding of a 16-bit result.  For 32-bit results (EXACT) codes become fp16 numbers, which
 // hold them exactly, the fp16 instruction sums a block in 32 bits (1e-7), and the scales are applied to its sum.
 //
-// Two forms.  Many rows: tiles of BM x BN results, both operands' codes copied to LDS past the registers, ahead of their use.
+// Three forms.  Many rows: tiles of BM x BN results, both operands' codes copied to LDS past the registers, ahead of their use.
 // Few rows (KAD_GEMM8_FEW): b's codes are read once, straight into the instruction's operands; a block takes 16 rows of b,
 // its waves take every eighth 128 columns and join in LDS.  a as values is brought to 8 bits in those registers, by each
 // block for itself: a launch less, and a is small (at 48 rows and [8192, 4096] it is not: 48 us against 33).
+//
+// Many rows, short ones, and few columns: a block brings its rows of values to 8 bits once and keeps them in LDS.
 //
 // The instruction computes b a^T: a lane then holds four results of one row of out that follow each other.
 #include "kad_block8.h"
@@ -646,6 +648,146 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void gemm8_few_kernel(kad_gemm8_arg
   }
 }
 
+// ---------------------------------------------------------------------------- many short rows
+// a as values of the result's type: a block brings 64 rows to 8 bits, keeps their codes in LDS, and meets them with all of
+// b's rows, or a part, whose codes go straight into the instruction's operands.  So a is read once, and its codes take no
+// way through memory.
+constexpr int SHORT_ROWS = 64, SHORT_MOST = 512;  // rows of a block, their values
+
+template <typename T, int WM, int TN>
+__global__ __launch_bounds__(256) void gemm8_short_kernel(kad_gemm8_args a, int columns) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  constexpr int WN = 4 / WM, TM = 4 / WM, V = VEC<T>, L = LANES<T>, PER = 64 / L, GROUPS = 16 / PER;
+  extern __shared__ __attribute__((aligned(128))) char lds[];  // codes [blocks][64][128], scales [64][ks], the waves' results
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), m0 = blockIdx.x * SHORT_ROWS;
+  const int whole = a.k / BLOCK8, blocks = (a.k + BLOCK8 - 1) / BLOCK8, ks = (blocks + 3) / 4 * 4;
+  const int64_t kp = (int64_t)blocks * BLOCK8;
+  unsigned char* scales = (unsigned char*)lds + blocks * SHORT_ROWS * LINE;
+  char* results = (char*)scales + SHORT_ROWS * ks;
+  {
+    const int l = lane % L, sub = lane / L;
+    const T* p[GROUPS];
+#pragma unroll
+    for (int q = 0; q < GROUPS; ++q) {
+      const int m = m0 + wave * 16 + q * PER + sub;  // rows past the last read the last one: what comes of them is not stored
+      p[q] = (const T*)a.a + (m < a.m ? m : a.m - 1) * a.a_rs;
+    }
+    const auto put_codes = [&](int q, int kb, const uint32_t* w) {
+      const int r = wave * 16 + q * PER + sub, s = scale_of<T>(lanes_largest<L>(largest_finite<T, 4>(w)));
+      char* to = lds + (kb * SHORT_ROWS + r) * LINE;
+      if constexpr (sizeof(T) == 2) {
+        int* two = (int*)(to + (((l >> 1) ^ (r >> 1 & 7)) << 4) + (l & 1) * 8);
+        two[0] = codes_of<T>(w[0], w[1], s);
+        two[1] = codes_of<T>(w[2], w[3], s);
+      } else {
+        *(int*)(to + (((l >> 2) ^ (r >> 1 & 7)) << 4) + (l & 3) * 4) = codes_of(w[0], w[1], w[2], w[3], s);
+      }
+      if (l == 0) scales[r * ks + kb] = (unsigned char)s;
+    };
+    if (whole) {
+      intx4 next[GROUPS];
+#pragma unroll
+      for (int q = 0; q < GROUPS; ++q) next[q] = load_vec(p[q] + l * V);
+      for (int kb = 0; kb < whole; ++kb) {
+        uint32_t w[GROUPS][4];
+        const int then = kb + 1 < whole ? kb + 1 : kb;
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q) {
+          __builtin_memcpy(w[q], &next[q], 16);
+          next[q] = load_vec(p[q] + then * BLOCK8 + l * V);
+        }
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q) put_codes(q, kb, w[q]);
+      }
+    }
+    if (whole < blocks) {
+      const int left = a.k - whole * BLOCK8 - l * V, n = left > 0 ? left : 0;
+#pragma unroll
+      for (int q = 0; q < GROUPS; ++q) {
+        float v[V];
+        uint32_t w[4];
+        load_some(p[q] + (n ? whole * BLOCK8 + l * V : 0), n, v);
+        const intx4 raw = pack<T>(v);
+        __builtin_memcpy(w, &raw, 16);
+        put_codes(q, whole, w);
+      }
+    }
+  }
+  __syncthreads();
+  const int wm = wave / WN, wn = wave % WN, r16 = lane & 15, g = lane >> 4;
+  const int line = (wm * TM * 16 + r16) * LINE, piece0 = ((2 * g) ^ (r16 >> 1)) << 4, piece1 = ((2 * g + 1) ^ (r16 >> 1)) << 4;
+  constexpr int STRIP = TN * 16;
+  const int first = blockIdx.y * columns, last = first + columns < a.n ? first + columns : a.n;
+  intx4 lo[TN], hi[TN];
+  int sb[TN];
+  const auto fetch = [&](int n1, int kb) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int row = n1 + j * 16 + r16 < a.n ? n1 + j * 16 + r16 : a.n - 1;
+      const intx4* c = (const intx4*)((const char*)a.b + row * kp + kb * BLOCK8 + 32 * g);
+      lo[j] = c[0];
+      hi[j] = c[1];
+      sb[j] = ((const unsigned char*)a.b_scales)[(int64_t)row * ks + kb];
+    }
+  };
+  int n1 = first + wn * STRIP;
+  if (n1 >= last) return;
+  fetch(n1, 0);
+  for (; n1 < last; n1 += WN * STRIP) {
+    float bias[TN][4];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bias[j][i] = bias_at<T>(a, n1 + j * 16 + 4 * g + i);
+    floatx4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int kb = 0; kb < blocks; ++kb) {
+      Operand<EXACT> fb[TN];
+      int s[TN], eb[TN][4];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        fb[j].set(lo[j], hi[j]);
+        s[j] = sb[j];
+        if (EXACT)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) eb[j][i] = __shfl(s[j], 4 * g + i);
+      }
+      const bool more = kb + 1 < blocks;
+      fetch(more ? n1 : n1 + WN * STRIP, more ? kb + 1 : 0);  // past the last column its rows again
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const char* p = lds + kb * SHORT_ROWS * LINE + line + i * 16 * LINE;
+        Operand<EXACT> fa;
+        fa.set(*(const intx4*)(p + piece0), *(const intx4*)(p + piece1));
+        const int sa = scales[(wm * TM * 16 + i * 16 + r16) * ks + kb];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) multiply<0>(acc[i][j], fb[j], fa, s[j], sa, eb[j]);
+      }
+    }
+    const int m1 = m0 + wm * TM * 16;
+    if constexpr (EXACT) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int m = m1 + i * 16 + r16, n = n1 + j * 16 + 4 * g;
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = activate<T>(acc[i][j][e] + bias[j][e], a.act);
+          if (m < a.m && n < a.n) store_four<T>((T*)a.out + (int64_t)m * a.n + n, v, a.n - n);
+        }
+    } else {
+      char* mine = results + wave * store_bytes(TN);
+      if (a.act == KAD_ACT_SILU) store_tile<T, TM, TN, KAD_ACT_SILU>(a, acc, bias, mine, lane, m1, n1);
+      else if (a.act == KAD_ACT_RELU) store_tile<T, TM, TN, KAD_ACT_RELU>(a, acc, bias, mine, lane, m1, n1);
+      else store_tile<T, TM, TN, KAD_ACT_NONE>(a, acc, bias, mine, lane, m1, n1);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------- host
 constexpr int CUS = 256;
 
@@ -677,6 +819,22 @@ Plan plan_of(const kad_gemm8_args& a) {
 
 bool few(const kad_gemm8_args& a) { return a.m <= KAD_GEMM8_FEW; }
 
+// Whether rows of a that are values are brought to 8 bits by the product's own blocks, against a launch before it.  A wave
+// reads b's codes 16 bytes a lane, one row a lane, which takes 4 times what copies of whole lines do, so b has to be short,
+// us in one launch and in two, fp16:
+//   [40000, 64] x [64, 64]     8.5 against 14.4    [40000, 512] x [64, 512]   16.0 against 21.9
+//   [40000, 256] x [128, 256] 14.5 against 19.2    [40000, 256] x [256, 256] (20000 rows) 12.0 against 15.3
+//   [40000, 512] x [256, 512] 28.2 against 27.3    [40000, 512] x [512, 512]  42.8 against 34.9
+// or blocks so few that each has a CU for itself: [300, 512] x [512, 512] 7.6 against 10.0, [4000, 512] x [512, 512] 13.4
+// against 10.3.
+bool few_columns(const kad_gemm8_args& a) {
+  return a.n <= 128 || (int64_t)ceil_div(a.m, SHORT_ROWS) * ceil_div(a.n, 64) <= CUS;
+}
+bool takes_values(const kad_gemm8_args& a) {
+  const bool known = a.a_dtype == KAD_F32 || a.a_dtype == KAD_F16 || a.a_dtype == KAD_BF16;
+  return known && (few(a) || (a.a_dtype == a.dtype && a.k <= SHORT_MOST && (few_columns(a) || (a.n <= 256 && a.k <= 256))));
+}
+
 template <typename T, typename X, int MT>
 void launch_few(const kad_gemm8_args& a, hipStream_t st) {
   gemm8_few_kernel<T, X, MT, sizeof(T) == 4><<<ceil_div(a.n, 16), 64 * FEW_WAVES, 0, st>>>(a);
@@ -686,6 +844,17 @@ template <typename T, typename X>
 void launch_few(const kad_gemm8_args& a, hipStream_t st) {
   if (a.m <= 16) launch_few<T, X, 1>(a, st);
   else launch_few<T, X, 2>(a, st);
+}
+
+template <typename T, int WM, int TN>
+void launch_short(const kad_gemm8_args& a, hipStream_t st) {
+  constexpr int COLUMNS = 4 / WM * TN * 16;  // that a block's waves take at a time
+  const int tm = ceil_div(a.m, SHORT_ROWS), most = ceil_div(a.n, COLUMNS), blocks = ceil_div(a.k, BLOCK8);
+  int parts = tm >= 2 * CUS ? 1 : 2 * CUS / tm;
+  if (parts > most) parts = most;
+  const int columns = round_up(ceil_div(a.n, parts), COLUMNS);
+  const size_t bytes = blocks * SHORT_ROWS * LINE + SHORT_ROWS * round_up(blocks, 4) + (sizeof(T) == 2 ? 4 * store_bytes(TN) : 0);
+  gemm8_short_kernel<T, WM, TN><<<dim3(tm, ceil_div(a.n, columns)), 256, bytes, st>>>(a, columns);
 }
 
 template <typename T, int BM, int BN, int WM, int WN>
@@ -702,6 +871,11 @@ void launch(const kad_gemm8_args& a, hipStream_t st) {
     else if (a.a_dtype == KAD_F32) launch_few<T, float>(a, st);
     else if (a.a_dtype == KAD_F16) launch_few<T, half_t>(a, st);
     else launch_few<T, bf16_t>(a, st);
+    return;
+  }
+  if (!a.a_scales) {
+    if (few_columns(a)) launch_short<T, 2, 2>(a, st);
+    else launch_short<T, 1, 4>(a, st);
     return;
   }
   const Plan p = plan_of(a);
@@ -724,8 +898,7 @@ int check_args(const kad_gemm8_args* a, const char* what) {
   KAD_CHECK_ARG((int64_t)ceil_div(a->m, 64) * ceil_div(a->n, 64) < 1 << 24, "%s: fewer than 2^24 tiles of 64 x 64 results expected", what);
   KAD_CHECK_ARG(!few(*a) || a->n < 1 << 26, "%s: up to %d rows: fewer than 2^26 columns expected", what, KAD_GEMM8_FEW);
   KAD_CHECK_ARG(a->act == KAD_ACT_NONE || a->act == KAD_ACT_RELU || a->act == KAD_ACT_SILU, "%s: unknown activation", what);
-  KAD_CHECK_ARG(a->a_scales || (is_dtype(a->a_dtype) && few(*a)), "%s: a as values: of a known dtype, and at most %d rows", what,
-                KAD_GEMM8_FEW);
+  KAD_CHECK_ARG(a->a_scales || takes_values(*a), "%s: a as values is not taken at these sizes and types", what);
   KAD_CHECK_ARG(!a->bias || is_dtype(a->bias_dtype), "%s: bad bias_dtype", what);
   return KAD_OK;
 }
@@ -737,9 +910,13 @@ using namespace kad;
 
 extern "C" int64_t kad_gemm8_work_elems(const kad_gemm8_args* a) {
   if (int rc = check_args(a, "kad_gemm8_work_elems")) return rc;
-  if (few(*a)) return 0;
+  if (few(*a) || !a->a_scales) return 0;
   const Plan p = plan_of(*a);
   return p.o.splits > 1 ? (int64_t)p.o.splits * a->m * a->n : 0;
+}
+
+extern "C" int kad_gemm8_takes_values(const kad_gemm8_args* a) {
+  return a && takes_values(*a);
 }
 
 extern "C" int kad_gemm8(const kad_gemm8_args* a, void* stream) {

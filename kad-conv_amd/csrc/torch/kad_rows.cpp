@@ -577,14 +577,10 @@ void quantize(const Rows& r, const Held8& along, const Held8& across, const Tens
   check(kad_quant8(&a, stream_of(x)), "kad_quant8");
 }
 
-// out = act(a b^T + bias), a in 8 bits or, where it has no scales, as values of a_dtype in rows a_rs apart.
-void product(const void* a, const void* a_scales, int64_t a_rs, int a_dtype, const Held8& b, int64_t m, int64_t n, int64_t k,
-             const Tensor& bias, int act, const Tensor& out) {
+// out = act(a b^T + bias), but for a.
+kad_gemm8_args product_args(const Held8& b, int64_t m, int64_t n, int64_t k, const Tensor& bias, int act, const Tensor& out) {
   TORCH_CHECK_VALUE(m <= INT32_MAX - 255 && n <= INT32_MAX - 255, "too many rows: ", m, " and ", n);
   kad_gemm8_args g{};
-  g.a = a;
-  g.a_scales = a_scales;
-  g.a_rs = a_rs;
   g.b = b.codes;
   g.b_scales = b.scales;
   g.bias = pointer(bias);
@@ -594,8 +590,11 @@ void product(const void* a, const void* a_scales, int64_t a_rs, int a_dtype, con
   g.k = (int)k;
   g.act = act;
   g.dtype = dtype_of(out);
-  g.a_dtype = a_dtype;
   g.bias_dtype = bias.defined() ? dtype_of(bias) : KAD_F32;
+  return g;
+}
+
+void launch_product(kad_gemm8_args& g, const Tensor& out) {
   const int64_t elems = kad_gemm8_work_elems(&g);
   if (elems < 0) check((int)elems, "kad_gemm8_work_elems");
   const Tensor work = elems ? floats(out, {elems}) : Tensor();
@@ -604,18 +603,26 @@ void product(const void* a, const void* a_scales, int64_t a_rs, int a_dtype, con
 }
 
 void product(const Held8& a, const Held8& b, int64_t m, int64_t n, int64_t k, const Tensor& bias, int act, const Tensor& out) {
-  product(a.codes, a.scales, 0, KAD_F32, b, m, n, k, bias, act, out);
-}
-void product(const Rows& a, const Held8& b, int64_t n, const Tensor& bias, int act, const Tensor& out) {
-  product(a.held.const_data_ptr(), nullptr, a.rs, dtype_of(a.held), b, a.count, n, a.c, bias, act, out);
+  kad_gemm8_args g = product_args(b, m, n, k, bias, act, out);
+  g.a = a.codes;
+  g.a_scales = a.scales;
+  launch_product(g, out);
 }
 
-// Of values: by way of 8 bits along k, in memory where they are many.
+// Of values: by way of 8 bits along k, in memory where the product does not bring them there itself.
 void product_of_values(const Rows& r, const Held8& b, int64_t n, const Tensor& bias, int act, const Tensor& out) {
-  if (r.count <= KAD_GEMM8_FEW) return product(r, b, n, bias, act, out);
-  const Held8 h = new_held(r.held, r.count, r.c);
-  quantize(r, h, {}, Tensor(), r.held);
-  product(h, b, r.count, n, r.c, bias, act, out);
+  kad_gemm8_args g = product_args(b, r.count, n, r.c, bias, act, out);
+  g.a = r.held.const_data_ptr();
+  g.a_rs = r.rs;
+  g.a_dtype = dtype_of(r.held);
+  Held8 h;
+  if (!kad_gemm8_takes_values(&g)) {
+    h = new_held(r.held, r.count, r.c);
+    quantize(r, h, {}, Tensor(), r.held);
+    g.a = h.codes;
+    g.a_scales = h.scales;
+  }
+  launch_product(g, out);
 }
 
 void check_quantized(const Tensor& x, int64_t k) {
@@ -740,7 +747,7 @@ Tensor linear8_run(const Tensor& x, bool map, const Tensor& weight, const Tensor
     product_of_values(r, wh, n, b, act, y);
   } else if (m <= KAD_GEMM8_FEW) {
     quantize(r, {}, across.x, Tensor(), x);
-    product(r, wh, n, b, act, y);
+    product_of_values(r, wh, n, b, act, y);
   } else {
     const Held8 h = new_held(x, m, k);
     quantize(r, h, across.x, Tensor(), x);
@@ -773,7 +780,7 @@ std::tuple<Tensor, Tensor, Tensor> linear8_gradients(const Tensor& dy, bool map,
   if (need_weight) down = new_held(dy, o.n, o.m);
   if (in_memory || need_weight || need_bias) quantize(r, along, down, db, dy);
   if (in_memory) product(along, across.w, o.m, o.k, o.n, Tensor(), KAD_ACT_NONE, dx);
-  else if (need_x) product(r, across.w, o.k, Tensor(), KAD_ACT_NONE, dx);
+  else if (need_x) product_of_values(r, across.w, o.k, Tensor(), KAD_ACT_NONE, dx);
   if (need_weight) product(down, across.x, o.n, o.k, o.m, Tensor(), KAD_ACT_NONE, dw);
   return {dx, dw, db};
 }

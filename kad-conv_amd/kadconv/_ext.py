@@ -238,6 +238,7 @@ SIGNATURES = {
     'kad_quant8_work_elems': (c_i64, [ctypes.POINTER(Quant8Args)]),
     'kad_quant8': (c_int, [ctypes.POINTER(Quant8Args), c_vp]),
     'kad_gemm8_work_elems': (c_i64, [ctypes.POINTER(Gemm8Args)]),
+    'kad_gemm8_takes_values': (c_int, [ctypes.POINTER(Gemm8Args)]),
     'kad_gemm8': (c_int, [ctypes.POINTER(Gemm8Args), c_vp]),
     'kad_adamw_chunks': (c_i64, [c_vp, c_vp, c_vp, c_int, c_int, c_vp, ctypes.POINTER(c_i64)]),
     'kad_adamw_step': (c_int, [ctypes.POINTER(AdamwArgs), c_vp]),

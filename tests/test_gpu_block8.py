@@ -169,6 +169,26 @@ def test_activations_and_bias(m, act, dtype):
             assert torch.equal(kadconv.matmul8(kadconv.quantize8(x), kept, b, act, dtype), kadconv.linear8(x, kept, b, act))
 
 
+@DTYPES
+@pytest.mark.parametrize('shape', [(33, 1, 1), (64, 64, 128), (65, 63, 127), (100, 65, 129), (129, 128, 512), (700, 300, 500), (2000, 129, 256),
+                                   (20000, 200, 255), (16500, 256, 130), (40, 16300, 7), (8241, 43, 86), (16400, 100, 384)], ids=str)
+def test_short_rows_in_one_launch(shape, dtype):
+    """Values of short rows that the product brings to 8 bits itself: as those that another launch brings there, to the bit
+    (the sums of a result are taken in one order in both, but for 16-bit tiles of 256, which these sizes do not take)."""
+    m, n, k = shape
+    x, w, b = make(m, k, dtype, 1, spread=3.0), kadconv.quantize8(make(n, k, dtype, 2)), make(1, n, dtype, 3)[0]
+    x[m // 2, k // 2] = float('nan')
+    x[m // 3] = 0
+    x[-1, 0] = float('inf')
+    for act in (None, 'silu'):
+        want = kadconv.matmul8(kadconv.quantize8(x), w, b, act, dtype)
+        got = kadconv.linear8(x, w, b, act)
+        assert torch.equal(got.nan_to_num(123.0), want.nan_to_num(123.0)) and torch.equal(got.isnan(), want.isnan())
+        apart = torch.full((m, k + 3), float('nan'), device=DEV, dtype=dtype)[:, 2:-1]  # at odd places, other values around
+        apart.copy_(x)
+        assert torch.equal(kadconv.linear8(apart, w, b, act).nan_to_num(123.0), got.nan_to_num(123.0))
+
+
 def check_gradients(x, w, b, dy, dim=-1):
     rows = x.detach().movedim(dim, -1).reshape(-1, x.shape[dim])
     drows = dy.movedim(dim, -1).reshape(-1, dy.shape[dim])
