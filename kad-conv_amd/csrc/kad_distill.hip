@@ -8,9 +8,13 @@
 // Memory bounds it: forward reads z once (the largest value and the sum in one pass), backward reads z and writes dz;
 // what the classes of the entries are is looked up in z, a few values a row.
 //
-// Two forms.  Up to MOST_SMALL classes a row stays in the registers of up to 64 lanes (kad_rows.h), many rows a wave;
-// beyond, a block walks a row, or a part of one where rows are few: forward these parts are joined in a second launch,
-// backward each writes its own classes.
+// Two forms.  Up to 1024 classes a row stays in the registers of up to 64 lanes (kad_rows.h), many rows a wave; beyond, a
+// wave or a block walks a row, or a block a part of one where rows are few: forward these parts are joined in a second
+// launch, backward each writes its own classes.
+//
+// 4096 rows of 32768 classes, bf16, 32 entries: forward 53 us (5.1 TB/s), backward 112 (4.8), 158 one after the other, with
+// gradients written past the cache that holds the logits (183 through it).  537600 rows of 16 classes, fp16, 16 entries:
+// 24 us (3.1 TB/s) and 29 (3.2).
 //
 // An index may come twice: its p add up, in no order that could change them: of small rows in LDS as whole numbers of
 // 2^-62 (a p of 2^-38 and more keeps its 24 bits; of what is smaller, no more than 2^-62 of the row's weight is lost),
@@ -20,7 +24,7 @@
 namespace kad {
 namespace {
 
-constexpr int MOST_SMALL = 1024;
+constexpr int MOST_WAVE = KAD_DISTILL_MOST / 4;  // entries of a row that is a wave's
 constexpr int MOST_BLOCKS = 1 << 20;  // a grid has at most 2^32 threads
 constexpr float INF = __builtin_inff();
 
@@ -372,32 +376,53 @@ struct Soft {
   }
 };
 
-// Joined over a block of 256 threads.
-__device__ __forceinline__ Soft join_block(Soft v, float c2, float* red) {
+// A row's threads are WAVES waves of a block of four: its own place in shared memory, its threads' order.
+template <int WAVES> __device__ __forceinline__ int row_lane() { return threadIdx.x & (64 * WAVES - 1); }
+template <int WAVES> __device__ __forceinline__ int row_of_block() { return threadIdx.x / (64 * WAVES); }
+template <int WAVES> __device__ __forceinline__ void row_barrier() {
+  if constexpr (WAVES > 1) __syncthreads();
+  else wave_order();
+}
+
+// Joined over a row's threads.
+template <int WAVES>
+__device__ __forceinline__ Soft join_row(Soft v, float c2) {
+  __shared__ float red[8];
   const float m = lanes_max(v.m, 64), b = Soft::base(m);
-  float s = lanes_sum(v.s * exp2_((v.m - b) * c2), 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    red[2 * (threadIdx.x >> 6)] = m;
-    red[2 * (threadIdx.x >> 6) + 1] = s;
-  }
-  __syncthreads();
+  const float s = lanes_sum(v.s * exp2_((v.m - b) * c2), 64);
   Soft r;
-  r.m = red[0];
-  r.s = red[1];
-  for (int w = 1; w < 4; ++w) r.join(red[2 * w], red[2 * w + 1], c2);
+  r.m = m;
+  r.s = s;
+  if constexpr (WAVES > 1) {
+    static_assert(WAVES == 4, "a row has one wave or a block");
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+      red[2 * (threadIdx.x >> 6)] = m;
+      red[2 * (threadIdx.x >> 6) + 1] = s;
+    }
+    __syncthreads();
+    r.m = red[0];
+    r.s = red[1];
+    for (int w = 1; w < 4; ++w) r.join(red[2 * w], red[2 * w + 1], c2);
+  }
   return r;
 }
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
+template <int WAVES>
+__device__ __forceinline__ float sum_of_row(float v) {
+  __shared__ float red[4];
   v = lanes_sum(v, 64);
+  if constexpr (WAVES == 1) return v;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   return red[0] + red[1] + red[2] + red[3];
 }
-__device__ __forceinline__ float block_max(float v, float* red) {
+template <int WAVES>
+__device__ __forceinline__ float max_of_row(float v) {
+  __shared__ float red[4];
   v = lanes_max(v, 64);
+  if constexpr (WAVES == 1) return v;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -410,14 +435,13 @@ struct Teacher {
   float s, d, zr;
   bool counts;
 };
-template <typename T>
+template <typename T, int WAVES>
 __device__ __forceinline__ Teacher teacher_of(const kad_distill_args& a, const Entries& en, const T* z, const Scales& c) {
-  constexpr int MOST = KAD_DISTILL_MOST / 256;
-  __shared__ float red[3][4];
+  constexpr int MOST = KAD_DISTILL_MOST / 256;  // a wave's rows have MOST_WAVE entries at most
   float t[MOST], zi[MOST], tm = -INF, zr = -INF, any = 0.f;
 #pragma unroll
   for (int i = 0; i < MOST; ++i) {
-    const int e = threadIdx.x + 256 * i;
+    const int e = row_lane<WAVES>() + 64 * WAVES * i;
     t[i] = -INF;
     zi[i] = 0.f;
     int at;
@@ -430,78 +454,58 @@ __device__ __forceinline__ Teacher teacher_of(const kad_distill_args& a, const E
       any = 1.f;
     }
   }
-  const int wave = threadIdx.x >> 6;
-  tm = lanes_max(tm, 64);
-  zr = lanes_max(zr, 64);
-  any = lanes_max(any, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    red[0][wave] = tm;
-    red[1][wave] = zr;
-    red[2][wave] = any;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    tm = fmaxf(tm, red[0][w]);
-    zr = fmaxf(zr, red[1][w]);
-    any = fmaxf(any, red[2][w]);
-  }
+  tm = max_of_row<WAVES>(tm);
+  zr = max_of_row<WAVES>(zr);
+  any = max_of_row<WAVES>(any);
   if (zr == -INF) zr = 0.f;  // no entry's class has weight: d is infinite
   Teacher r{0.f, 0.f, zr, any != 0.f};
 #pragma unroll
   for (int i = 0; i < MOST; ++i)
     if (t[i] != -INF) add_entry(t[i], tm, zi[i], zr, c.c2, r.s, r.d);
-  r.s = lanes_sum(r.s, 64);
-  r.d = lanes_sum(r.d, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    red[0][wave] = r.s;
-    red[1][wave] = r.d;
-  }
-  __syncthreads();
-  r.s = red[0][0] + red[0][1] + red[0][2] + red[0][3];
-  r.d = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  r.s = sum_of_row<WAVES>(r.s);
+  r.d = sum_of_row<WAVES>(r.d);
   return r;
 }
 __device__ __forceinline__ float large_loss(const kad_distill_args& a, const Teacher& t, const Soft& soft, const Scales& c) {
   return t.counts ? row_loss(a.temperature, t.s, t.d + t.s * (soft.m - t.zr), soft.s, c) : 0.f;
 }
 
-// The Soft of values [begin, end), which are VEC<T> at least: the next vectors are on their way while some are added.
-template <typename T>
-__device__ __forceinline__ Soft soft_of(const T* z, int begin, int end, float c2) {
-  constexpr int V = VEC<T>, AT_ONCE = 4;
-  Soft r;
-  const int n = (end - begin + V - 1) / V;
+// A thread's share of values [begin, end), which are VEC<T> at least: the next vectors are on their way while some are added,
+// the first ones from the start.
+template <typename T, int WAVES>
+struct Stream {
+  static constexpr int V = VEC<T>, AT_ONCE = 4, N = 64 * WAVES;
+  const T* z;
+  int begin, end;
   intx4 next[AT_ONCE];
-  const auto fetch = [&](int j) {
+  __device__ __forceinline__ Stream(const T* p, int from, int to) : z(p), begin(from), end(to) { fetch(row_lane<WAVES>()); }
+  __device__ __forceinline__ void fetch(int j) {
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
-      const int i = begin + (j + u * 256) * V;
+      const int i = begin + (j + u * N) * V;
       next[u] = load_vec(z + (i < end - V ? i : end - V));
     }
-  };
-  fetch(threadIdx.x);
-  for (int j = threadIdx.x; j - (int)threadIdx.x < n; j += AT_ONCE * 256) {
-    intx4 raw[AT_ONCE];
-#pragma unroll
-    for (int u = 0; u < AT_ONCE; ++u) raw[u] = next[u];
-    fetch(j + AT_ONCE * 256);
-#pragma unroll
-    for (int u = 0; u < AT_ONCE; ++u) {
-      const int i = begin + (j + u * 256) * V;
-      float v[V];
-      unpack<T>(raw[u], v);
-      if (i > end - V) {  // moved back to end with the row: its first values are another thread's, or all are
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = e >= i - (end - V) ? v[e] : -INF;
-      }
-      r.add<V>(v, c2);
-    }
   }
-  return r;
-}
+  __device__ __forceinline__ Soft soft(float c2) {
+    Soft r;
+    const int l = row_lane<WAVES>(), n = (end - begin + V - 1) / V;
+    for (int j = l; j - l < n; j += AT_ONCE * N) {
+      float v[AT_ONCE][V];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = begin + (j + u * N) * V;
+        unpack<T>(next[u], v[u]);
+        if (i > end - V) {  // moved back to end with the row: its first values are another thread's, or all are
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[u][e] = e >= i - (end - V) ? v[u][e] : -INF;
+        }
+      }
+      fetch(j + AT_ONCE * N);
+      r.add<AT_ONCE * V>(v[0], c2);
+    }
+    return r;
+  }
+};
 
 // sum and largest of no values, or of -inf alone: the softmax is not defined
 __device__ __forceinline__ Soft settled(Soft v) {
@@ -509,17 +513,18 @@ __device__ __forceinline__ Soft settled(Soft v) {
   return v;
 }
 
-template <typename T>
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void distill_large_fwd_kernel(kad_distill_args a) {
-  __shared__ float red[8];
+  constexpr int ROWS = 4 / WAVES;
   const Scales c(a.temperature);
   float total = 0.f;
   unsigned count = 0;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + row_of_block<WAVES>(); row < a.rows; row += (int64_t)gridDim.x * ROWS) {
     const T* z = (const T*)a.logits + row * a.z_rs;
-    const Teacher teacher = teacher_of(a, Entries(a, row), z, c);
-    const Soft soft = settled(join_block(soft_of(z, 0, a.v, c.c2), c.c2, red));
-    if (threadIdx.x == 0) {
+    Stream<T, WAVES> stream(z, 0, a.v);
+    const Teacher teacher = teacher_of<T, WAVES>(a, Entries(a, row), z, c);
+    const Soft soft = settled(join_row<WAVES>(stream.soft(c.c2), c.c2));
+    if (row_lane<WAVES>() == 0) {
       const float loss = large_loss(a, teacher, soft, c);
       leave_row(a, row, teacher.counts, soft.m, soft.s, loss);
       total += loss;
@@ -532,18 +537,16 @@ __global__ __launch_bounds__(256) void distill_large_fwd_kernel(kad_distill_args
 // Where rows are few: a part of one a block, [rows][parts][2] behind the blocks' losses in work.
 template <typename T>
 __global__ __launch_bounds__(256) void distill_part_kernel(kad_distill_args a, int part, float* softs) {
-  __shared__ float red[8];
   const Scales c(a.temperature);
   const int64_t row = blockIdx.x;
   const int begin = blockIdx.y * part, end = begin + part < a.v ? begin + part : a.v;
-  const Soft soft = join_block(soft_of((const T*)a.logits + row * a.z_rs, begin, end, c.c2), c.c2, red);
+  const Soft soft = join_row<4>(Stream<T, 4>((const T*)a.logits + row * a.z_rs, begin, end).soft(c.c2), c.c2);
   if (threadIdx.x) return;
   softs[2 * (row * gridDim.y + blockIdx.y)] = soft.m;
   softs[2 * (row * gridDim.y + blockIdx.y) + 1] = soft.s;
 }
 template <typename T>
 __global__ __launch_bounds__(256) void distill_parts_fwd_kernel(kad_distill_args a, int parts, const float* softs) {
-  __shared__ float red[8];
   const Scales c(a.temperature);
   const int64_t row = blockIdx.x;
   Soft mine;
@@ -551,23 +554,25 @@ __global__ __launch_bounds__(256) void distill_parts_fwd_kernel(kad_distill_args
     mine.m = softs[2 * (row * parts + threadIdx.x)];
     mine.s = softs[2 * (row * parts + threadIdx.x) + 1];
   }
-  const Soft soft = settled(join_block(mine, c.c2, red));
-  const Teacher teacher = teacher_of(a, Entries(a, row), (const T*)a.logits + row * a.z_rs, c);
+  const Soft soft = settled(join_row<4>(mine, c.c2));
+  const Teacher teacher = teacher_of<T, 4>(a, Entries(a, row), (const T*)a.logits + row * a.z_rs, c);
   const float loss = large_loss(a, teacher, soft, c);
   if (threadIdx.x == 0) leave_row(a, row, teacher.counts, soft.m, soft.s, loss);
   leave_part(a, threadIdx.x ? 0.f : loss, threadIdx.x == 0 && teacher.counts);
 }
 
 // Rows from the last to the first: the forward pass left the last ones in the memory-side cache.
-template <typename T>
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void distill_large_bwd_kernel(kad_distill_args a, int part) {
-  constexpr int V = VEC<T>, AT_ONCE = 4;
-  __shared__ float red[8];
-  __shared__ int at_of[KAD_DISTILL_MOST];
-  __shared__ float p_of[KAD_DISTILL_MOST];
+  constexpr int V = VEC<T>, AT_ONCE = 4, N = 64 * WAVES, ROWS = 4 / WAVES;
+  __shared__ int at_of_rows[KAD_DISTILL_MOST];
+  __shared__ float p_of_rows[KAD_DISTILL_MOST];
+  const int l = row_lane<WAVES>();
+  int* at_of = at_of_rows + row_of_block<WAVES>() * (KAD_DISTILL_MOST / ROWS);
+  float* p_of = p_of_rows + row_of_block<WAVES>() * (KAD_DISTILL_MOST / ROWS);
   const Scales c(a.temperature);
   const int begin = blockIdx.y * part, end = begin + part < a.v ? begin + part : a.v, n = (end - begin + V - 1) / V;
-  for (int64_t turn = blockIdx.x; turn < a.rows; turn += gridDim.x) {
+  for (int64_t turn = (int64_t)blockIdx.x * ROWS + row_of_block<WAVES>(); turn < a.rows; turn += (int64_t)gridDim.x * ROWS) {
     const int64_t row = a.rows - 1 - turn;
     const T* z = (const T*)a.logits + row * a.z_rs;
     T* dz = (T*)a.dlogits + row * a.v;
@@ -575,40 +580,41 @@ __global__ __launch_bounds__(256) void distill_large_bwd_kernel(kad_distill_args
     const Entries en(a, row);
     float tm = -INF, s = 0.f, t;
     int at;
-    for (int e = threadIdx.x; e < a.k; e += 256)
+    for (int e = l; e < a.k; e += N)
       if (en.get(e, at, t)) tm = fmaxf(tm, t);
-    tm = block_max(tm, red);
-    for (int e = threadIdx.x; e < a.k; e += 256) {
+    tm = max_of_row<WAVES>(tm);
+    row_barrier<WAVES>();  // the row before is done with its entries
+    for (int e = l; e < a.k; e += N) {
       const bool counts = en.get(e, at, t);
       const float w = counts ? exp2_((t - tm) * c.c2) : 0.f;
       at_of[e] = counts ? at : -1;
       p_of[e] = w;
       s += w;
     }
-    s = block_sum(s, red);  // NaN, or a row that counts: 1 at least
+    s = sum_of_row<WAVES>(s);  // NaN, or a row that counts: 1 at least
     const float norm = 1.0f / s, scale = s == s ? f * inv : s;
-    for (int j = threadIdx.x; j < n; j += AT_ONCE * 256) {
+    for (int j = l; j < n; j += AT_ONCE * N) {
       intx4 raw[AT_ONCE];
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < AT_ONCE; ++u) {
-        const int i = begin + (j + u * 256) * V;
+        const int i = begin + (j + u * N) * V;
         raw[u] = load_vec(z + (i < end - V ? i : end - V));
       }
-  #pragma unroll
+#pragma unroll
       for (int u = 0; u < AT_ONCE; ++u) {
-        const int i = begin + (j + u * 256) * V;
+        const int i = begin + (j + u * N) * V;
         float v[V];
         unpack<T>(raw[u], v);
-  #pragma unroll
+#pragma unroll
         for (int e = 0; e < V; ++e) v[e] = inv == 0.f ? 0.f : scale * exp2_((v[e] - zm) * c.c2);
-        if (i < end) store_vec(dz + (i < end - V ? i : end - V), v);
+        if (i < end) stream_vec(dz + (i < end - V ? i : end - V), v);
       }
     }
     if (inv == 0.f) continue;
-    // The entries' classes again, once all of the block's stores are done.
+    // The entries' classes again, once all of the row's stores are done.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int e = threadIdx.x; e < a.k; e += 256) {
+    row_barrier<WAVES>();
+    for (int e = l; e < a.k; e += N) {
       const int mine = at_of[e];
       if (mine < begin || mine >= end) continue;
       float p = 0.f;
@@ -627,13 +633,17 @@ __global__ __launch_bounds__(256) void distill_large_bwd_kernel(kad_distill_args
 struct Shape {
   int vv, u, G;
   int64_t blocks;  // whose losses are joined
+  bool wave_rows;  // large rows: a wave each
   int part, parts; // large rows: classes of a block, blocks of a row
 };
 
 Shape shape_of(const kad_distill_args& a, bool backward) {
   Shape s{};
   const int v = 16 / dtype_size(a.dtype);
-  if (a.v <= MOST_SMALL) {
+  // Rows in registers or not, us, 131072 rows of 1024 classes, 32 entries: forward bf16 134 and 134, fp32 140 and 129,
+  // backward fp32 208 and 303, but bf16 244 and 173 (and 266 against 274 at 512 classes, twice the rows).
+  const int most_small = backward && dtype_size(a.dtype) == 2 ? 512 : 1024;
+  if (a.v <= most_small) {
     s.vv = a.v >= v ? v : 1;
     const int vecs = ceil_div(a.v, s.vv);
     s.u = 1;
@@ -644,7 +654,11 @@ Shape shape_of(const kad_distill_args& a, bool backward) {
     s.blocks = turns < 2048 ? turns : 2048;
     return s;
   }
-  s.blocks = a.rows < 2048 || backward ? a.rows : 2048;
+  // A row a wave, or a block, us: forward, bf16, 65536 rows of 2048 classes 76 against 263, 16384 of 8192 54 against 77;
+  // backward 150 against 204 at 2048, 126 against 123 at 4096, where a block's loads reach further ahead.
+  s.wave_rows = a.rows >= 1024 && a.k <= MOST_WAVE && (backward ? a.v * dtype_size(a.dtype) <= 6144 : a.v <= 8192);
+  const int64_t turns = s.wave_rows ? (a.rows + 3) / 4 : a.rows, most_blocks = backward ? MOST_BLOCKS : 2048;
+  s.blocks = turns < most_blocks ? turns : most_blocks;
   s.parts = 1;
   s.part = a.v;
   const int64_t wanted = backward ? 2048 : 1024;
@@ -687,10 +701,12 @@ int check_call(const kad_distill_args* a, bool backward, const char* what) {
 
 template <typename T, int VV, int U, bool RAGGED, bool IN_REGS>
 void launch_small(const kad_distill_args& a, const Shape& s, bool backward, hipStream_t st) {
-  if (backward)
-    distill_small_bwd_kernel<T, VV, U, RAGGED, IN_REGS><<<s.blocks, 256, (256 / s.G) * a.v * sizeof(unsigned long long), st>>>(a, s.G);
-  else
-    distill_small_fwd_kernel<T, VV, U, RAGGED, IN_REGS><<<s.blocks, 256, 0, st>>>(a, s.G);
+  if (backward) {
+    if constexpr (sizeof(T) == 4 || U == 1)  // others have too many classes
+      distill_small_bwd_kernel<T, VV, U, RAGGED, IN_REGS><<<s.blocks, 256, (256 / s.G) * a.v * sizeof(unsigned long long), st>>>(a, s.G);
+    return;
+  }
+  distill_small_fwd_kernel<T, VV, U, RAGGED, IN_REGS><<<s.blocks, 256, 0, st>>>(a, s.G);
 }
 
 template <typename T, int VV, int U, bool RAGGED>
@@ -714,13 +730,15 @@ void launch(const kad_distill_args& a, bool backward, hipStream_t st) {
     else if (s.u == 2) launch_small<T, 2>(a, s, backward, st);
     else if constexpr (sizeof(T) == 4) launch_small<T, 4>(a, s, backward, st);
   } else if (backward) {
-    distill_large_bwd_kernel<T><<<dim3(a.rows < MOST_BLOCKS ? a.rows : MOST_BLOCKS, s.parts), 256, 0, st>>>(a, s.part);
+    if (s.wave_rows) distill_large_bwd_kernel<T, 1><<<s.blocks, 256, 0, st>>>(a, s.part);
+    else distill_large_bwd_kernel<T, 4><<<dim3(s.blocks, s.parts), 256, 0, st>>>(a, s.part);
   } else if (s.parts > 1) {
     float* softs = a.work + 2 * s.blocks;
     distill_part_kernel<T><<<dim3(a.rows, s.parts), 256, 0, st>>>(a, s.part, softs);
     distill_parts_fwd_kernel<T><<<a.rows, 256, 0, st>>>(a, s.parts, softs);
   } else {
-    distill_large_fwd_kernel<T><<<s.blocks, 256, 0, st>>>(a);
+    if (s.wave_rows) distill_large_fwd_kernel<T, 1><<<s.blocks, 256, 0, st>>>(a);
+    else distill_large_fwd_kernel<T, 4><<<s.blocks, 256, 0, st>>>(a);
   }
   if (!backward && a.reduction != KAD_REDUCE_NONE) distill_join_kernel<<<1, 1024, 0, st>>>(a, (int)s.blocks);
 }

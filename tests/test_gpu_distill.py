@@ -76,6 +76,34 @@ def test_loss_and_gradient(shape, dtype):
 
 
 @DTYPES
+@pytest.mark.parametrize('shape', [(1024, 1025, 3), (1025, 2047, 64), (1101, 3000, 256), (1030, 8192, 20), (1027, 1500, 257),
+                                   (1024, 8193, 30), (1500, 513, 12), (1026, 1024, 40), (1024, 600, 900)], ids=lambda s: 'x'.join(map(str, s)))
+def test_many_rows(shape, dtype):
+    """Rows of a wave each, and at the borders of that form, with rows that are unlike each other side by side."""
+    rows, v, k = shape
+    z, t, i = make(rows, v, k, dtype, seed=v)
+    i[0] = -1
+    i[1] = i[1].max()
+    t[2] = -INF
+    i[5, k // 2:] = i[5, 0]
+    i[-1, 1:] = v
+    z[6, ::3] = torch.where(torch.isin(torch.arange(0, v, 3, device=DEV), i[6]), z[6, ::3], -INF)
+    check(z, t, i, 1.5)
+    bad = z.clone()
+    bad[7, 11], bad[8, -1], bad[9] = NAN, INF, -INF
+    some = [r for r in range(rows) if r not in (7, 8, 9)]
+    for zs in (z, bad):
+        zs.requires_grad_(True)
+        loss = kadconv.distill_loss(zs, t, i, 1.5, 'none')
+        dz, = torch.autograd.grad(loss, zs, torch.ones_like(loss))
+        if zs is z:
+            want, want_dz = loss.detach(), dz
+    assert torch.equal(loss[some], want[some]) and torch.equal(dz[some], want_dz[some])
+    counts = ((i[7:10] >= 0) & (i[7:10] < v)).any(1)
+    assert torch.equal(loss[7:10].isnan(), counts) and torch.equal(dz[7:10].isnan().all(1), counts)
+
+
+@DTYPES
 @pytest.mark.parametrize('layout', ['cl', 'nchw', 'slice'])
 @pytest.mark.parametrize('shape', [(2, 20, 5, 7, 4), (1, 16, 20, 20, 16), (3, 9, 1, 4, 2), (2, 1100, 3, 2, 10), (2, 6, 4, 1, 3)],
                          ids=lambda s: 'x'.join(map(str, s)))
