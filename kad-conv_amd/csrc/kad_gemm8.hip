@@ -127,7 +127,9 @@ __device__ __forceinline__ bool tile_of(const Tiles& o, int& m, int& n, int& spl
   return true;
 }
 
-// A wave's 16-bit results: two rows of fragments at a time by way of its part of LDS, so that whole lines are written.
+// A wave's 16-bit results: two rows of fragments at a time by way of its part of LDS, so that whole lines are written, and past
+// the caches that hold the operands ([40000, 512] x [512, 512] fp16: 19.7 us, 22.4 through them; of tiles of 256, whose products
+// take long, it makes no difference).
 constexpr int store_bytes(int tn) { return 32 * (tn * 32 + 16); }
 template <typename T, int TM, int TN, int ACT>
 __device__ __forceinline__ void store_tile(const kad_gemm8_args& a, const floatx4 (&acc)[TM][TN], const float (&bias)[TN][4], char* lds,
@@ -157,7 +159,7 @@ __device__ __forceinline__ void store_tile(const kad_gemm8_args& a, const floatx
       if (m >= a.m || left <= 0) continue;
       T* to = (T*)a.out + (int64_t)m * a.n + n;
       if (left >= 8) {
-        __builtin_memcpy(to, &v[r], 16);
+        __builtin_nontemporal_store(v[r], (loose<T>*)to);
       } else {
         T t[8];
         __builtin_memcpy(t, &v[r], 16);
