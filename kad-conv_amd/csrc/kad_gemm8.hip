@@ -22,8 +22,6 @@
 namespace kad {
 namespace {
 
-typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
-
 constexpr int LINE = BLOCK8;        // bytes of a row in a stage: one block of codes
 constexpr int KB_GROUP = 4;         // scales are read by fours
 
@@ -803,10 +801,13 @@ Plan plan_of(const kad_gemm8_args& a) {
   const int blocks = ceil_div(a.k, BLOCK8);
   const bool exact = a.dtype == KAD_F32;
   const auto count = [&](int bm, int bn) { return (int64_t)ceil_div(a.m, bm) * ceil_div(a.n, bn); };
-  // A round of 256 x 256 tiles (one a CU) takes 3.1 / 4 of the time that their 128 x 128 ones take, two a CU at a time:
-  // [8192, 4096] x [4096, 4096] 126 us against 167; where it leaves CUs idle, [40000, 512] x [512, 512] 26.3 against 22.7.
-  const auto rounds = [](int64_t tiles, int at_once) { return (tiles + at_once - 1) / at_once; };
-  p.bm = p.bn = !exact && rounds(count(WIDE, WIDE), CUS) * 3.1 < rounds(count(128, 128), 2 * CUS) * 2 ? WIDE
+  // A round of 256 x 256 tiles, one a CU, takes 22 us and 12.5 for each 1000 of k; one of 128 x 128 tiles, two a CU and half
+  // the results, 7.9 and 9.2 (fits of 4096 x 4096 results at k of 4096 and 8192).  us with tiles of 256 and of 128:
+  //   [8192, 4096] x [4096, 4096] 148 and 193     [4096, 8192] x [4096, 8192] 124 and 166
+  //   [6000, 1000] x [6000, 1000]  57 and 52      [40000, 512] x [512, 512]  26.3 and 18.6
+  const auto rounds = [&](int tile, int at_once) { return (double)((count(tile, tile) + at_once - 1) / at_once); };
+  const double k = a.k * 1e-3;
+  p.bm = p.bn = !exact && rounds(WIDE, CUS) * (22 + 12.5 * k) < rounds(128, 2 * CUS) * (7.9 + 9.2 * k) ? WIDE
                 : count(128, 128) >= CUS ? 128 : 64;
   p.o.tm = ceil_div(a.m, p.bm);
   p.o.tn = ceil_div(a.n, p.bn);

@@ -5,6 +5,8 @@
 // block of 8-bit numbers in either direction, so that neither scale needs more than the tile; what goes transposed takes
 // its way through LDS, 8 or 16 rows of a column at a time.  The tile's column sums, of which a bias' gradient is made,
 // are left in work and joined by a second launch, in an order that the sizes alone decide.
+//
+// [8192, 4096] bf16 along its rows 18.6 us (5.4 TB/s), both ways 35 (3.9: every tile's way through LDS, and its two barriers).
 #include "kad_block8.h"
 
 namespace kad {

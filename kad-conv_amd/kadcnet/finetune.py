@@ -144,8 +144,8 @@ def main(argv=None):
     a = ap.parse_args(argv)
     if a.steps < 1 or a.batch < 1 or a.size < 128 or a.size % 32:
         ap.error('steps and batch must be positive, size a multiple of 32 from 128 on')
-    if a.distill < 0 or not a.temperature > 0:
-        ap.error('distill must not be negative, and temperature positive')
+    if a.distill < 0 or not 1e-6 <= a.temperature <= 1e6:
+        ap.error('distill must not be negative, and temperature lie in 1e-6 to 1e6')
     from .synthetic import build_kadcnet_s
     device, dtype = torch.device('cuda'), DTYPES[a.dtype]
     model = build_kadcnet_s(seed=a.seed).fuse().to(device, dtype)

@@ -6,9 +6,11 @@ Added here: ``deform_conv2d`` (torchvision-compatible DCNv2 on the GPU), the
 fused blocks ``Conv1x1SiLU``, ``SqueezeExcitation`` and ``KADDown``, for
 training ``group_norm_act`` / ``GroupNormAct`` (group norm and an activation on
 channels-last maps, with its gradients) and ``AdamW`` / ``AdamWPlan`` (the step
-over a network's tensors in one launch, states in 32 or 8 bits), and the typed
-custom operators ``torch.ops.kadconv.deform_conv2d`` / ``layer_fwd`` /
-``group_norm_act`` (kadconv.library).
+over a network's tensors in one launch, states in 32 or 8 bits), for a head that
+is trained by a teacher and served ``layer_norm`` / ``LayerNorm``, ``quantize8`` /
+``matmul8`` / ``linear8`` / ``Linear8`` (products in 8 bits) and ``distill_loss``,
+and the typed custom operators ``torch.ops.kadconv.deform_conv2d`` /
+``layer_fwd`` / ``group_norm_act`` and their like (kadconv.library).
 """
 from . import library  # registers the kadconv:: custom operators
 from .block8 import Block8, linear8, matmul8, quantize8

@@ -130,7 +130,8 @@ def test_products(shape, dtype):
             assert_within(kadconv.matmul8(kadconv.quantize8(x), kept, dtype=out), z.cpu(), rounded(z, t, out).cpu(), 'matmul8')
 
 
-@pytest.mark.parametrize('shape', [(2100, 4100, 300), (8200, 2048, 1024), (4096, 4096, 640)], ids=lambda s: 'x'.join(map(str, s)))
+@pytest.mark.parametrize('shape', [(2100, 4100, 300), (8200, 2048, 1024), (4096, 4096, 640), (2100, 4100, 1100), (4000, 4090, 1207),
+                                   (3000, 5100, 1500), (4096, 4096, 1300), (8192, 4096, 1152), (4003, 4096, 2048)], ids=lambda s: 'x'.join(map(str, s)))
 def test_large_tiles(shape):
     """Results in 16 bits next to those in 32, whose sums are exact: off by the cut of the products and two roundings.
     The cut is bounded by 7 * 2^-13 of the sum of magnitudes."""
