@@ -742,7 +742,7 @@ int kad_quant8(const kad_quant8_args *a, void *stream);
 
 /* out = act(a b^T + bias): a [m][k] and b [n][k] in 8 bits along k (as kad_quant8 writes them), or a as values
  * (a_scales NULL), which are brought to 8 bits on the way where kad_gemm8_takes_values says 1: with m up to
- * KAD_GEMM8_FEW, and with short rows of dtype and few columns.
+ * KAD_GEMM8_FEW, and with short rows of dtype.
  * Sums are 32-bit.  Those of 32-bit results are taken from exact products; for 16-bit results the 8-bit matrix instruction
  * cuts the products of eight consecutive k to 2^-13 of the largest of them. */
 typedef struct kad_gemm8_args {

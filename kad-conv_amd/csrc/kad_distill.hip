@@ -271,12 +271,6 @@ __device__ __forceinline__ void add_weight(unsigned long long* sum, float weight
 __device__ __forceinline__ float weight_of(unsigned long long sum) {
   return __builtin_fmaf((float)(uint32_t)(sum >> 32), 0x1p-30f, (float)(uint32_t)sum * 0x1p-62f);
 }
-// Orders a wave's accesses to LDS: the unit takes them in turn, so it is the compiler alone that has to.
-__device__ __forceinline__ void wave_order() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 template <typename T, int VV, int U, bool RAGGED, bool IN_REGS>
 __global__ __launch_bounds__(256) void distill_small_bwd_kernel(kad_distill_args a, int G) {
   extern __shared__ unsigned long long sums[];  // [rows of the block][v]; a row's are its own wave's

@@ -14,7 +14,7 @@
 // its waves take every eighth 128 columns and join in LDS.  a as values is brought to 8 bits in those registers, by each
 // block for itself: a launch less, and a is small (at 48 rows and [8192, 4096] it is not: 48 us against 33).
 //
-// Many rows, short ones, and few columns: a block brings its rows of values to 8 bits once and keeps them in LDS.
+// Many rows, short ones: a block brings its rows of values to 8 bits once and keeps them in LDS.
 //
 // The instruction computes b a^T: a lane then holds four results of one row of out that follow each other.
 #include "kad_block8.h"
@@ -650,9 +650,12 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void gemm8_few_kernel(kad_gemm8_arg
 
 // ---------------------------------------------------------------------------- many short rows
 // a as values of the result's type: a block brings 64 rows to 8 bits, keeps their codes in LDS, and meets them with all of
-// b's rows, or a part, whose codes go straight into the instruction's operands.  So a is read once, and its codes take no
-// way through memory.
+// b's rows, or a part.  So a is read once, and its codes take no way through memory.  A wave reads b's codes in whole lines, the
+// next block's while it multiplies, and turns them into operands by way of its own part of LDS: read as operands, 16 bytes a
+// lane and one row a lane, they came at a quarter of the rate.
 constexpr int SHORT_ROWS = 64, SHORT_MOST = 512;  // rows of a block, their values
+constexpr int short_bytes(int tn) { return tn * 16 * LINE; }
+static_assert(short_bytes(2) >= store_bytes(2) && short_bytes(4) >= store_bytes(4), "results take the place of codes");
 
 template <typename T, int WM, int TN>
 __global__ __launch_bounds__(256) void gemm8_short_kernel(kad_gemm8_args a, int columns) {
@@ -663,7 +666,7 @@ __global__ __launch_bounds__(256) void gemm8_short_kernel(kad_gemm8_args a, int 
   const int whole = a.k / BLOCK8, blocks = (a.k + BLOCK8 - 1) / BLOCK8, ks = (blocks + 3) / 4 * 4;
   const int64_t kp = (int64_t)blocks * BLOCK8;
   unsigned char* scales = (unsigned char*)lds + blocks * SHORT_ROWS * LINE;
-  char* results = (char*)scales + SHORT_ROWS * ks;
+  char* mine = (char*)scales + SHORT_ROWS * ks + (t >> 6) * short_bytes(TN);  // of the wave: b's codes, then results
   {
     const int l = lane % L, sub = lane / L;
     const T* p[GROUPS];
@@ -718,15 +721,17 @@ __global__ __launch_bounds__(256) void gemm8_short_kernel(kad_gemm8_args a, int 
   const int line = (wm * TM * 16 + r16) * LINE, piece0 = ((2 * g) ^ (r16 >> 1)) << 4, piece1 = ((2 * g + 1) ^ (r16 >> 1)) << 4;
   constexpr int STRIP = TN * 16;
   const int first = blockIdx.y * columns, last = first + columns < a.n ? first + columns : a.n;
-  intx4 lo[TN], hi[TN];
+  intx4 raw[2 * TN];
   int sb[TN];
   const auto fetch = [&](int n1, int kb) {
 #pragma unroll
+    for (int i = 0; i < 2 * TN; ++i) {
+      const int at = n1 + i * 8 + (lane >> 3), row = at < a.n ? at : a.n - 1;
+      raw[i] = *(const intx4*)((const char*)a.b + row * kp + kb * BLOCK8 + (lane & 7) * 16);
+    }
+#pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int row = n1 + j * 16 + r16 < a.n ? n1 + j * 16 + r16 : a.n - 1;
-      const intx4* c = (const intx4*)((const char*)a.b + row * kp + kb * BLOCK8 + 32 * g);
-      lo[j] = c[0];
-      hi[j] = c[1];
+      const int at = n1 + j * 16 + r16, row = at < a.n ? at : a.n - 1;
       sb[j] = ((const unsigned char*)a.b_scales)[(int64_t)row * ks + kb];
     }
   };
@@ -747,9 +752,14 @@ __global__ __launch_bounds__(256) void gemm8_short_kernel(kad_gemm8_args a, int 
     for (int kb = 0; kb < blocks; ++kb) {
       Operand<EXACT> fb[TN];
       int s[TN], eb[TN][4];
+      wave_order();
+#pragma unroll
+      for (int i = 0; i < 2 * TN; ++i) {
+        const int r = i * 8 + (lane >> 3);
+        *(intx4*)(mine + r * LINE + (((lane & 7) ^ (r >> 1 & 7)) << 4)) = raw[i];
+      }
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        fb[j].set(lo[j], hi[j]);
         s[j] = sb[j];
         if (EXACT)
 #pragma unroll
@@ -757,6 +767,12 @@ __global__ __launch_bounds__(256) void gemm8_short_kernel(kad_gemm8_args a, int 
       }
       const bool more = kb + 1 < blocks;
       fetch(more ? n1 : n1 + WN * STRIP, more ? kb + 1 : 0);  // past the last column its rows again
+      wave_order();
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const char* p = mine + (j * 16 + r16) * LINE;
+        fb[j].set(*(const intx4*)(p + piece0), *(const intx4*)(p + piece1));
+      }
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const char* p = lds + kb * SHORT_ROWS * LINE + line + i * 16 * LINE;
@@ -780,7 +796,7 @@ __global__ __launch_bounds__(256) void gemm8_short_kernel(kad_gemm8_args a, int 
           if (m < a.m && n < a.n) store_four<T>((T*)a.out + (int64_t)m * a.n + n, v, a.n - n);
         }
     } else {
-      char* mine = results + wave * store_bytes(TN);
+      wave_order();
       if (a.act == KAD_ACT_SILU) store_tile<T, TM, TN, KAD_ACT_SILU>(a, acc, bias, mine, lane, m1, n1);
       else if (a.act == KAD_ACT_RELU) store_tile<T, TM, TN, KAD_ACT_RELU>(a, acc, bias, mine, lane, m1, n1);
       else store_tile<T, TM, TN, KAD_ACT_NONE>(a, acc, bias, mine, lane, m1, n1);
@@ -822,20 +838,22 @@ Plan plan_of(const kad_gemm8_args& a) {
 
 bool few(const kad_gemm8_args& a) { return a.m <= KAD_GEMM8_FEW; }
 
-// Whether rows of a that are values are brought to 8 bits by the product's own blocks, against a launch before it.  A wave
-// reads b's codes 16 bytes a lane, one row a lane, which takes 4 times what copies of whole lines do, so b has to be short,
-// us in one launch and in two, fp16:
-//   [40000, 64] x [64, 64]     8.5 against 14.4    [40000, 512] x [64, 512]   16.0 against 21.9
-//   [40000, 256] x [128, 256] 14.5 against 19.2    [40000, 256] x [256, 256] (20000 rows) 12.0 against 15.3
-//   [40000, 512] x [256, 512] 28.2 against 27.3    [40000, 512] x [512, 512]  42.8 against 34.9
-// or blocks so few that each has a CU for itself: [300, 512] x [512, 512] 7.6 against 10.0, [4000, 512] x [512, 512] 13.4
-// against 10.3.
-bool few_columns(const kad_gemm8_args& a) {
-  return a.n <= 128 || (int64_t)ceil_div(a.m, SHORT_ROWS) * ceil_div(a.n, 64) <= CUS;
+// Whether rows of a that are values are brought to 8 bits by the product's own blocks, against a launch before it, and by
+// which blocks: of 64 columns at a time, which many find a place on a CU, or of 256, for which more of a block's loads are a's.
+// us in one launch (64 and 256) and in two:
+//   fp16 [40000, 64] x [64, 64]     7.7,  9.3 and 14.4     [40000, 512] x [64, 512]    13.5,  18.9 and 22.0
+//        [40000, 256] x [128, 256] 11.6, 14.2 and 18.5     [20000, 256] x [256, 256]   11.8,   9.4 and 14.8
+//        [300, 512] x [512, 512]    6.7,  9.1 and 9.9      [40000, 512] x [512, 512]   38.4,  32.4 and 34.4
+//        [8000, 256] x [8000, 256] 59.4, 40.2 and 48.4     [40000, 512] x [2048, 512] 115,    86   and 82
+//   fp32 [40000, 64] x [64, 64]    12.8, 32.3 and 23.2     [40000, 512] x [512, 512]   83.1, 100   and 75.0
+//        [300, 512] x [512, 512]   10.8, 19.1 and 13.1     [40000, 512] x [256, 512]   51.8,  61.4 and 56.5
+bool narrow(const kad_gemm8_args& a) {
+  return a.n <= (a.dtype == KAD_F32 ? 256 : 128) || (int64_t)ceil_div(a.m, SHORT_ROWS) * ceil_div(a.n, 64) <= CUS;
 }
 bool takes_values(const kad_gemm8_args& a) {
   const bool known = a.a_dtype == KAD_F32 || a.a_dtype == KAD_F16 || a.a_dtype == KAD_BF16;
-  return known && (few(a) || (a.a_dtype == a.dtype && a.k <= SHORT_MOST && (few_columns(a) || (a.n <= 256 && a.k <= 256))));
+  return known && (few(a) || (a.a_dtype == a.dtype && a.k <= SHORT_MOST &&
+                              (narrow(a) || (a.dtype != KAD_F32 && (a.n <= 1024 || a.k <= 256)))));
 }
 
 template <typename T, typename X, int MT>
@@ -856,7 +874,7 @@ void launch_short(const kad_gemm8_args& a, hipStream_t st) {
   int parts = tm >= 2 * CUS ? 1 : 2 * CUS / tm;
   if (parts > most) parts = most;
   const int columns = round_up(ceil_div(a.n, parts), COLUMNS);
-  const size_t bytes = blocks * SHORT_ROWS * LINE + SHORT_ROWS * round_up(blocks, 4) + (sizeof(T) == 2 ? 4 * store_bytes(TN) : 0);
+  const size_t bytes = blocks * SHORT_ROWS * LINE + SHORT_ROWS * round_up(blocks, 4) + 4 * short_bytes(TN);
   gemm8_short_kernel<T, WM, TN><<<dim3(tm, ceil_div(a.n, columns)), 256, bytes, st>>>(a, columns);
 }
 
@@ -877,8 +895,8 @@ void launch(const kad_gemm8_args& a, hipStream_t st) {
     return;
   }
   if (!a.a_scales) {
-    if (few_columns(a)) launch_short<T, 2, 2>(a, st);
-    else launch_short<T, 1, 4>(a, st);
+    if (narrow(a)) launch_short<T, 2, 2>(a, st);
+    else if constexpr (sizeof(T) == 2) launch_short<T, 1, 4>(a, st);
     return;
   }
   const Plan p = plan_of(a);

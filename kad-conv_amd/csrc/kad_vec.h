@@ -71,4 +71,10 @@ __device__ __forceinline__ void store_some(T* p, int n, const float v[VEC<T>]) {
     if (i < n) p[i] = from_f32<T>(v[i]);
 }
 
+// Orders a wave's accesses to LDS: the unit takes them in turn, so it is the compiler alone that has to.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 }  // namespace kad

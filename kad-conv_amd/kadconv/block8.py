@@ -219,7 +219,7 @@ def linear8(input, weight, bias=None, act=None, dim=-1):
     seen.  The gradient of W takes up to 2^22 rows.
 
     GPU tensors (fp32, fp16, bf16) run the gfx950 HIP kernels; rows that lie a fixed distance apart are read where they
-    are.  Up to 32 rows, and short ones with few columns, take one launch, their numbers brought to 8 bits by the product's
+    are.  Up to 32 rows, and short ones (up to 512 values), take one launch, their numbers brought to 8 bits by the product's
     own threads.  The result is
     dense (a map's: channels-last).  CPU tensors run the plain composition."""
     kept = isinstance(weight, Block8)

@@ -172,7 +172,8 @@ def test_activations_and_bias(m, act, dtype):
 
 @DTYPES
 @pytest.mark.parametrize('shape', [(33, 1, 1), (64, 64, 128), (65, 63, 127), (100, 65, 129), (129, 128, 512), (700, 300, 500), (2000, 129, 256),
-                                   (20000, 200, 255), (16500, 256, 130), (40, 16300, 7), (8241, 43, 86), (16400, 100, 384)], ids=str)
+                                   (20000, 200, 255), (16500, 256, 130), (40, 16300, 7), (8241, 43, 86), (16400, 100, 384), (5000, 1024, 500),
+                                   (4100, 1000, 257), (3001, 5003, 256), (90, 30001, 65)], ids=str)
 def test_short_rows_in_one_launch(shape, dtype):
     """Values of short rows that the product brings to 8 bits itself: as those that another launch brings there, to the bit
     (the sums of a result are taken in one order in both, but for 16-bit tiles of 256, which these sizes do not take)."""

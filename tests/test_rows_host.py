@@ -323,8 +323,11 @@ def test_gemm8_takes_values():
     lib = _ext.load()
     takes = lambda **kw: lib.kad_gemm8_takes_values(ctypes.byref(_gemm_args(**{**dict(m=1000, n=64, k=300, a_dtype=1), **kw})))
     assert lib.kad_gemm8_takes_values(None) == 0
-    assert takes() == takes(n=128, k=512) == takes(m=1 << 24) == takes(n=256, k=256) == takes(m=64, n=10000) == 1
-    assert takes(a_dtype=0) == takes(k=513) == takes(m=40000, n=257) == takes(m=40000, n=200, k=257) == takes(a_dtype=9, m=3) == 0
+    assert takes() == takes(n=128, k=512) == takes(m=1 << 24) == takes(n=1024, k=512) == takes(m=64, n=10000) == takes(n=1 << 20, k=256) == 1
+    assert takes(a_dtype=0) == takes(k=513) == takes(m=40000, n=1025) == takes(a_dtype=9, m=3) == 0
+    f32 = dict(dtype=0, a_dtype=0)
+    assert takes(**f32) == takes(m=40000, n=256, k=512, **f32) == takes(n=1024, **f32) == 1
+    assert takes(m=40000, n=257, **f32) == takes(k=513, **f32) == 0
     assert takes(m=32, n=1 << 20, k=1 << 20, a_dtype=0) == 1
 
 
