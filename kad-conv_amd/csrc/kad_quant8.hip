@@ -6,21 +6,26 @@
 // its way through LDS, 8 or 16 rows of a column at a time.  The tile's column sums, of which a bias' gradient is made,
 // are left in work and joined by a second launch, in an order that the sizes alone decide.
 //
-// [8192, 4096] bf16 along its rows 18.6 us (5.4 TB/s), both ways 35 (3.9: every tile's way through LDS, and its two barriers).
+// [8192, 4096] bf16 along its rows 18.6 us (5.4 TB/s), both ways 32.7 (4.2: every tile's way through LDS, and its two
+// barriers; 35 with 30 KB of LDS and columns that met in a few banks).
 #include "kad_block8.h"
 
 namespace kad {
 namespace {
 
 template <typename T> constexpr int DEEP = LANES<T> / 2;       // rows of a thread
-constexpr int PITCH = BLOCK8 + 16;                             // bytes from column to column in LDS
+
+// Where 16-byte piece p of a column of codes lies in LDS: so that neither the threads that write some rows of many columns nor
+// those that read whole columns meet in a few banks.
+__device__ __forceinline__ int piece_of(int c, int p) { return (c ^ (c >> 3 & 1)) * BLOCK8 + ((p ^ (c >> 4 & 3) << 1) << 4); }
 
 template <typename T>
 __global__ __launch_bounds__(256) void quant8_kernel(kad_quant8_args a) {
   constexpr int V = VEC<T>, L = LANES<T>, D = DEEP<T>, SUBS = 256 / L;  // SUBS threads share a column
-  __shared__ float column_sums[SUBS][BLOCK8];
-  __shared__ uint32_t most[SUBS][L * 4];                                // of a thread's columns, as its words hold them
-  __shared__ __attribute__((aligned(16))) unsigned char flat[BLOCK8 * PITCH];
+  // 20 KB in all, of which a CU holds eight
+  __shared__ uint32_t most[SUBS][L * 4];  // of a thread's columns, as its words hold them
+  __shared__ __attribute__((aligned(16))) unsigned char flat[BLOCK8 * BLOCK8];
+  float(*column_sums)[BLOCK8] = (float(*)[BLOCK8])flat;  // before the codes
   const int t = threadIdx.x, l = t % L, sub = t / L;
   const int tiles = (a.c + BLOCK8 - 1) / BLOCK8;
   const int64_t band = blockIdx.x / tiles;
@@ -111,7 +116,7 @@ __global__ __launch_bounds__(256) void quant8_kernel(kad_quant8_args a) {
 #pragma unroll
     for (int h = 0; h < PER; ++h) {
       const int s = scale_of<T>(PER == 1 ? m : h ? m >> 16 : m & 0xFFFFu), c = l * V + i * PER + h;
-      int* to = (int*)(flat + c * PITCH + sub * D);
+      int* to = (int*)(flat + piece_of(c, sub * D / 16) + sub * D % 16);
 #pragma unroll
       for (int r = 0; r < D; r += 4) {
         if constexpr (PER == 1) {
@@ -134,7 +139,7 @@ __global__ __launch_bounds__(256) void quant8_kernel(kad_quant8_args a) {
   for (int i = t; i < BLOCK8 * 8; i += 256) {  // 16 bytes each
     const int c = i / 8, at = i % 8 * 16;
     if (tile * BLOCK8 + c < a.c)
-      *(intx4*)((unsigned char*)a.t_codes + (tile * BLOCK8 + c) * mp + band * BLOCK8 + at) = *(const intx4*)(flat + c * PITCH + at);
+      *(intx4*)((unsigned char*)a.t_codes + (tile * BLOCK8 + c) * mp + band * BLOCK8 + at) = *(const intx4*)(flat + piece_of(c, at / 16));
   }
 }
 
