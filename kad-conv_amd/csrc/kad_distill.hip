@@ -25,6 +25,7 @@ namespace kad {
 namespace {
 
 constexpr int MOST_WAVE = KAD_DISTILL_MOST / 4;  // entries of a row that is a wave's
+constexpr int MOST_HELD = 8;  // entries of a lane in registers
 constexpr int MOST_BLOCKS = 1 << 20;  // a grid has at most 2^32 threads
 constexpr float INF = __builtin_inff();
 
@@ -136,9 +137,9 @@ __device__ __forceinline__ float row_factor(const kad_distill_args& a, int64_t r
 }
 
 // ---------------------------------------------------------------------------- rows in registers
-constexpr int HELD = 8;  // entries of a lane that stay in registers too
 
-// A lane's entries: `chunk` that follow each other, at most HELD; those that do not count have class -1.
+// A lane's entries: `chunk` that follow each other, at most HELD (1 or 8); those that do not count have class -1.
+template <int HELD>
 struct Own {
   int at[HELD];
   float t[HELD];
@@ -153,6 +154,12 @@ struct Own {
   __device__ __forceinline__ void load(const Entries& en, int l) {
     const kad_distill_args& a = en.a;
     const int e = l * chunk;
+    if (HELD == 1) {
+      t[0] = 0.f;
+      at[0] = -1;
+      if (l < a.k && !en.get(l, at[0], t[0])) at[0] = -1;
+      return;
+    }
     if (chunk == HELD && e + HELD <= a.k && a.t_sk == 1 && a.i_sk == 1) {
       if (a.index_bits == 32) {
         const int32_t* p = (const int32_t*)a.index + en.i0 + e;
@@ -191,14 +198,15 @@ struct Own {
   }
 };
 
-// IN_REGS: a row's entries are at most HELD G; otherwise they are read again for each use.
-template <typename T, int VV, int U, bool RAGGED, bool IN_REGS>
+// HELD: entries of a lane that stay in registers too, where a row has HELD G at most (1 or 8); 0: they are read again for each
+// use.
+template <typename T, int VV, int U, bool RAGGED, int HELD>
 __global__ __launch_bounds__(256) void distill_small_fwd_kernel(kad_distill_args a, int G) {
   const int sub = threadIdx.x / G, l = threadIdx.x & (G - 1), per = 256 / G;
   const Place<VV, U, RAGGED> o(l, G, a.v);
   const Scales c(a.temperature);
   const int64_t step = (int64_t)gridDim.x * per, last = a.rows - 1;
-  Own own((a.k + G - 1) / G);
+  Own<HELD> own(HELD == 1 ? 1 : (a.k + G - 1) / G);
   float total = 0.f;
   unsigned count = 0;
   for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows; base += step) {
@@ -211,8 +219,8 @@ __global__ __launch_bounds__(256) void distill_small_fwd_kernel(kad_distill_args
     const Entries en(a, row);
     float tm = -INF, any = 0.f, t;
     int at;
-    float zi[HELD];
-    if (IN_REGS) {
+    float zi[HELD ? HELD : 1];
+    if constexpr (HELD > 0) {
       own.load(en, l);
 #pragma unroll
       for (int i = 0; i < HELD; ++i) zi[i] = i < own.chunk && own.at[i] >= 0 ? to_f32(z[own.at[i]]) : 0.f;
@@ -243,7 +251,7 @@ __global__ __launch_bounds__(256) void distill_small_fwd_kernel(kad_distill_args
     }
     zsum = lanes_sum(zsum, G);
     float s = 0.f, d = 0.f;
-    if (IN_REGS) {
+    if constexpr (HELD > 0) {
 #pragma unroll
       for (int i = 0; i < HELD; ++i)
         if (i < own.chunk && own.at[i] >= 0) add_entry(own.t[i], tm, zi[i], zm, c.c2, s, d);
@@ -271,14 +279,14 @@ __device__ __forceinline__ void add_weight(unsigned long long* sum, float weight
 __device__ __forceinline__ float weight_of(unsigned long long sum) {
   return __builtin_fmaf((float)(uint32_t)(sum >> 32), 0x1p-30f, (float)(uint32_t)sum * 0x1p-62f);
 }
-template <typename T, int VV, int U, bool RAGGED, bool IN_REGS>
+template <typename T, int VV, int U, bool RAGGED, int HELD>
 __global__ __launch_bounds__(256) void distill_small_bwd_kernel(kad_distill_args a, int G) {
   extern __shared__ unsigned long long sums[];  // [rows of the block][v]; a row's are its own wave's
   const int sub = threadIdx.x / G, l = threadIdx.x & (G - 1), per = 256 / G;
   const Place<VV, U, RAGGED> o(l, G, a.v);
   const Scales c(a.temperature);
   const int64_t step = (int64_t)gridDim.x * per, last = a.rows - 1;
-  Own own((a.k + G - 1) / G);
+  Own<HELD> own(HELD == 1 ? 1 : (a.k + G - 1) / G);
   unsigned long long* mine = sums + sub * a.v;
   for (int i = threadIdx.x; i < per * a.v; i += 256) sums[i] = 0;
   __syncthreads();
@@ -293,7 +301,7 @@ __global__ __launch_bounds__(256) void distill_small_bwd_kernel(kad_distill_args
     const Entries en(a, row);
     float tm = -INF, s = 0.f, t;
     int at;
-    if (IN_REGS) {
+    if constexpr (HELD > 0) {
       own.load(en, l);
       tm = lanes_max(own.largest(), G);
 #pragma unroll
@@ -312,7 +320,7 @@ __global__ __launch_bounds__(256) void distill_small_bwd_kernel(kad_distill_args
     s = lanes_sum(s, G);
     const float unit = 0x1p62f / s;
     if (s == s) {
-      if (IN_REGS) {
+      if constexpr (HELD > 0) {
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
           if (i < own.chunk && own.at[i] >= 0) add_weight(mine + own.at[i], own.t[i], unit);
@@ -643,7 +651,7 @@ Shape shape_of(const kad_distill_args& a, bool backward) {
     s.u = 1;
     while (vecs > 64 * s.u) s.u *= 2;
     s.G = 1;
-    while (s.G * s.u < vecs || (s.G < 64 && s.G * HELD < a.k)) s.G *= 2;
+    while (s.G * s.u < vecs || (s.G < 64 && s.G * MOST_HELD < a.k)) s.G *= 2;
     const int64_t turns = (a.rows + 256 / s.G - 1) / (256 / s.G);
     s.blocks = turns < 2048 ? turns : 2048;
     return s;
@@ -693,20 +701,21 @@ int check_call(const kad_distill_args* a, bool backward, const char* what) {
   return KAD_OK;
 }
 
-template <typename T, int VV, int U, bool RAGGED, bool IN_REGS>
+template <typename T, int VV, int U, bool RAGGED, int HELD>
 void launch_small(const kad_distill_args& a, const Shape& s, bool backward, hipStream_t st) {
   if (backward) {
     if constexpr (sizeof(T) == 4 || U == 1)  // others have too many classes
-      distill_small_bwd_kernel<T, VV, U, RAGGED, IN_REGS><<<s.blocks, 256, (256 / s.G) * a.v * sizeof(unsigned long long), st>>>(a, s.G);
+      distill_small_bwd_kernel<T, VV, U, RAGGED, HELD><<<s.blocks, 256, (256 / s.G) * a.v * sizeof(unsigned long long), st>>>(a, s.G);
     return;
   }
-  distill_small_fwd_kernel<T, VV, U, RAGGED, IN_REGS><<<s.blocks, 256, 0, st>>>(a, s.G);
+  distill_small_fwd_kernel<T, VV, U, RAGGED, HELD><<<s.blocks, 256, 0, st>>>(a, s.G);
 }
 
 template <typename T, int VV, int U, bool RAGGED>
 void launch_small(const kad_distill_args& a, const Shape& s, bool backward, hipStream_t st) {
-  if (a.k <= HELD * s.G) launch_small<T, VV, U, RAGGED, true>(a, s, backward, st);
-  else launch_small<T, VV, U, RAGGED, false>(a, s, backward, st);
+  if (a.k <= s.G) launch_small<T, VV, U, RAGGED, 1>(a, s, backward, st);
+  else if (a.k <= MOST_HELD * s.G) launch_small<T, VV, U, RAGGED, MOST_HELD>(a, s, backward, st);
+  else launch_small<T, VV, U, RAGGED, 0>(a, s, backward, st);
 }
 
 template <typename T, int U>
