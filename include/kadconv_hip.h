@@ -700,7 +700,7 @@ typedef struct kad_distill_args {
   int64_t rows;           /* 1 .. 2^31 - 1 */
   int64_t z_rs;           /* elements from row to row (any, at least v; at most 2^31 - 1) */
   int64_t inner;          /* >= 1 */
-  int64_t t_sn, t_sp, t_sk, i_sn, i_sp, i_sk;  /* >= 0 */
+  int64_t t_sn, t_sp, t_sk, i_sn, i_sp, i_sk;  /* >= 0; _sp and _sk below 2^32 */
   int v, k;               /* v: 1 .. 2^30, k: 1 .. KAD_DISTILL_MOST */
   float temperature;      /* 1e-6 .. 1e6 */
   int reduction;

@@ -31,22 +31,26 @@ constexpr float INF = __builtin_inff();
 
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 
+// One 32-bit multiplication: what both are at most is checked.
+__device__ __forceinline__ int64_t product(uint32_t n, int64_t stride) { return (int64_t)((uint64_t)n * (uint32_t)stride); }
+
 // A row's entries.
 struct Entries {
   const kad_distill_args& a;
   int64_t t0, i0;
-  __device__ __forceinline__ Entries(const kad_distill_args& args, int64_t row) : a(args) {
-    int64_t n = 0, p = row;
+  __device__ __forceinline__ Entries(const kad_distill_args& args, uint32_t row) : a(args) {
     if (a.inner < a.rows) {
-      n = (uint32_t)row / (uint32_t)a.inner;
-      p = row - n * a.inner;
+      const uint32_t n = row / (uint32_t)a.inner, p = row - n * (uint32_t)a.inner;
+      t0 = (int64_t)n * a.t_sn + product(p, a.t_sp);
+      i0 = (int64_t)n * a.i_sn + product(p, a.i_sp);
+    } else {
+      t0 = product(row, a.t_sp);
+      i0 = product(row, a.i_sp);
     }
-    t0 = n * a.t_sn + p * a.t_sp;
-    i0 = n * a.i_sn + p * a.i_sp;
   }
   // Whether entry e counts; its class and logit.
   __device__ __forceinline__ bool get(int e, int& at, float& t) const {
-    const int64_t i = i0 + e * a.i_sk, ti = t0 + e * a.t_sk;
+    const int64_t i = i0 + product(e, a.i_sk), ti = t0 + product(e, a.t_sk);
     const int64_t c = a.index_bits == 32 ? (int64_t)((const int32_t*)a.index)[i] : ((const int64_t*)a.index)[i];
     t = a.teacher_dtype == KAD_F32 ? ((const float*)a.teacher)[ti]
         : a.teacher_dtype == KAD_F16 ? (float)((const half_t*)a.teacher)[ti] : (float)((const bf16_t*)a.teacher)[ti];
@@ -205,14 +209,14 @@ __global__ __launch_bounds__(256) void distill_small_fwd_kernel(kad_distill_args
   const int sub = threadIdx.x / G, l = threadIdx.x & (G - 1), per = 256 / G;
   const Place<VV, U, RAGGED> o(l, G, a.v);
   const Scales c(a.temperature);
-  const int64_t step = (int64_t)gridDim.x * per, last = a.rows - 1;
+  const uint32_t step = gridDim.x * per, rows = (uint32_t)a.rows, last = rows - 1;  // rows + step < 2^32
   Own<HELD> own(HELD == 1 ? 1 : (a.k + G - 1) / G);
   float total = 0.f;
   unsigned count = 0;
-  for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows; base += step) {
+  for (uint32_t base = blockIdx.x * per; base < rows; base += step) {
     const bool live = base + sub <= last;
-    const int64_t row = live ? base + sub : last;
-    const T* z = (const T*)a.logits + row * a.z_rs;
+    const uint32_t row = live ? base + sub : last;
+    const T* z = (const T*)a.logits + product(row, a.z_rs);
     Piece<T, VV> raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u].load(z + o.at[u]);
@@ -285,19 +289,20 @@ __global__ __launch_bounds__(256) void distill_small_bwd_kernel(kad_distill_args
   const int sub = threadIdx.x / G, l = threadIdx.x & (G - 1), per = 256 / G;
   const Place<VV, U, RAGGED> o(l, G, a.v);
   const Scales c(a.temperature);
-  const int64_t step = (int64_t)gridDim.x * per, last = a.rows - 1;
+  const uint32_t step = gridDim.x * per, rows = (uint32_t)a.rows, last = rows - 1;  // rows + step < 2^32
   Own<HELD> own(HELD == 1 ? 1 : (a.k + G - 1) / G);
   unsigned long long* mine = sums + sub * a.v;
   for (int i = threadIdx.x; i < per * a.v; i += 256) sums[i] = 0;
   __syncthreads();
-  for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows; base += step) {
+  for (uint32_t base = blockIdx.x * per; base < rows; base += step) {
     const bool live = base + sub <= last;
-    const int64_t row = live ? base + sub : last;
-    const T* z = (const T*)a.logits + row * a.z_rs;
+    const uint32_t row = live ? base + sub : last;
+    const T* z = (const T*)a.logits + product(row, a.z_rs);
     Piece<T, VV> raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u].load(z + o.at[u]);
-    const float zm = a.stats[2 * row], inv = a.stats[2 * row + 1], f = row_factor(a, row);
+    const float2 stats = ((const float2*)a.stats)[row];
+    const float zm = stats.x, inv = stats.y, f = row_factor(a, row);
     const Entries en(a, row);
     float tm = -INF, s = 0.f, t;
     int at;
@@ -346,7 +351,7 @@ __global__ __launch_bounds__(256) void distill_small_bwd_kernel(kad_distill_args
       if (!o.on[u]) continue;
 #pragma unroll
       for (int e = 0; e < VV; ++e) mine[o.at[u] + e] = 0;
-      if (live) put<T, VV>((T*)a.dlogits + row * a.v + o.at[u], x[u]);
+      if (live) put<T, VV>((T*)a.dlogits + product(row, a.v) + o.at[u], x[u]);
     }
     wave_order();
   }
@@ -696,6 +701,8 @@ int check_call(const kad_distill_args* a, bool backward, const char* what) {
   KAD_CHECK_ARG(backward || a->work || kad_distill_work_elems(a) == 0, "%s: work is missing", what);
   KAD_CHECK_ARG(a->z_rs >= a->v && a->z_rs <= INT32_MAX, "%s: z_rs does not fit v", what);
   KAD_CHECK_ARG(a->inner >= 1, "%s: inner must be at least 1", what);
+  KAD_CHECK_ARG(a->t_sp <= UINT32_MAX && a->t_sk <= UINT32_MAX && a->i_sp <= UINT32_MAX && a->i_sk <= UINT32_MAX,
+                "%s: strides from pixel to pixel and entry to entry must be below 2^32", what);
   KAD_CHECK_ARG(a->t_sn >= 0 && a->t_sp >= 0 && a->t_sk >= 0 && a->i_sn >= 0 && a->i_sp >= 0 && a->i_sk >= 0,
                 "%s: strides must not be negative", what);
   return KAD_OK;

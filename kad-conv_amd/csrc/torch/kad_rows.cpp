@@ -324,19 +324,20 @@ Strided entries_of(const Tensor& t, bool map) {
   if (map) {
     const int64_t h = t.size(2), w = t.size(3);
     Strided r{t, t.stride(0), w > 1 ? t.stride(3) : t.stride(2), t.stride(1)};
-    if (h > 1 && w > 1 && t.stride(2) != w * t.stride(3)) {
+    if ((h > 1 && w > 1 && t.stride(2) != w * t.stride(3)) || r.sp > UINT32_MAX || r.sk > UINT32_MAX) {
       r.held = t.contiguous();
       r.sn = t.size(1) * h * w, r.sp = 1, r.sk = h * w;
     }
     return r;
   }
   Strided r{t, 0, t.size(-1), t.stride(-1)};
+  if (r.sk > UINT32_MAX) return {t.contiguous(), 0, t.size(-1), 1};
   bool first = true;
   int64_t expected = 0;
   for (int64_t i = t.dim() - 2; i >= 0; --i) {
     if (t.size(i) == 1) continue;
     if (first) r.sp = expected = t.stride(i), first = false;
-    if (t.stride(i) != expected) {
+    if (t.stride(i) != expected || r.sp > UINT32_MAX) {
       r.held = t.contiguous();
       r.sp = t.size(-1), r.sk = 1;
       return r;

@@ -160,7 +160,7 @@ def _distill_args(**kw):
 
 @pytest.mark.parametrize('kw', [dict(logits=None), dict(teacher=None), dict(index=None), dict(loss=None), dict(work=None), dict(rows=0),
                                 dict(rows=1 << 31), dict(v=0), dict(v=(1 << 30) + 1), dict(k=0), dict(k=1025), dict(z_rs=7),
-                                dict(z_rs=1 << 31), dict(inner=0), dict(t_sk=-1), dict(i_sn=-1), dict(temperature=0.0), dict(temperature=1e7), dict(reduction=3),
+                                dict(z_rs=1 << 31), dict(inner=0), dict(t_sk=-1), dict(i_sn=-1), dict(t_sp=1 << 32), dict(i_sk=1 << 32), dict(temperature=0.0), dict(temperature=1e7), dict(reduction=3),
                                 dict(dtype=9), dict(teacher_dtype=-1), dict(index_bits=16)], ids=str)
 def test_distill_c_refuses(kw):
     lib = _ext.load()
