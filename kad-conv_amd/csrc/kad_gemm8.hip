@@ -10,9 +10,10 @@
 // hold them exactly, the fp16 instruction sums a block in 32 bits (1e-7), and the scales are applied to its sum.
 //
 // Three forms.  Many rows: tiles of BM x BN results, both operands' codes copied to LDS past the registers, ahead of their use.
-// Few rows (KAD_GEMM8_FEW): b's codes are read once, straight into the instruction's operands; a block takes 16 rows of b,
-// its waves take every eighth 128 columns and join in LDS.  a as values is brought to 8 bits in those registers, by each
-// block for itself: a launch less, and a is small (at 48 rows and [8192, 4096] it is not: 48 us against 33).
+//
+// Few rows (KAD_GEMM8_FEW): b's codes are read once, in whole lines that a wave turns into operands by way of its part of LDS;
+// a block takes 16 rows of b, its waves take every eighth 128 columns and join in LDS.  a as values is brought to 8 bits in
+// registers, by each block for itself: a launch less, and a is small (at 48 rows and [8192, 4096] it is not: 48 us against 33).
 //
 // Many rows, short ones: a block brings its rows of values to 8 bits once and keeps them in LDS.
 //
@@ -581,16 +582,25 @@ template <> struct Numbers<unsigned char> {
 
 // X: a's type as values, or unsigned char: a in 8 bits.  A wave has the loads of AT_ONCE blocks under way: they are made for
 // the last block again where there are fewer, since the compiler waits for all loads where branches around some meet
-// ([1, 4096] x [8192, 4096] bf16, weights from memory: 17.6 us with such branches, 12.7 without).
+// ([1, 4096] x [8192, 4096] bf16, weights from memory: 17.6 us with such branches, 12.7 without; 11.4 with b in whole lines, of
+// which 3 are a's way into 8 bits: 8.2 where it is there already).
 template <typename T, typename X, int MT, bool EXACT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void gemm8_few_kernel(kad_gemm8_args a) {
   constexpr int AT_ONCE = 4 / MT;
   __shared__ floatx4 red[FEW_WAVES][MT][64];
+  __shared__ __attribute__((aligned(128))) char lines[FEW_WAVES][16 * LINE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16, row_b = n0 + r16 < a.n ? n0 + r16 : a.n - 1;
   const int blocks = (a.k + BLOCK8 - 1) / BLOCK8, whole = Numbers<X>::whole(a);
   const int64_t kp = (int64_t)blocks * BLOCK8, ks = (blocks + 3) / 4 * 4;
-  const char* codes_b = (const char*)a.b + row_b * kp + 32 * g;
+  // eight rows' lines at a time
+  const int line = n0 + (lane >> 3);
+  const char* codes_b[2] = {(const char*)a.b + (line < a.n ? line : a.n - 1) * kp + (lane & 7) * 16,
+                            (const char*)a.b + (line + 8 < a.n ? line + 8 : a.n - 1) * kp + (lane & 7) * 16};
+  char* mine = lines[wave];
+  const int to = (lane >> 3) * LINE + (((lane & 7) ^ (lane >> 4)) << 4);
+  const int to8 = (8 + (lane >> 3)) * LINE + (((lane & 7) ^ (4 + (lane >> 4))) << 4);
+  const int piece0 = r16 * LINE + (((2 * g) ^ (r16 >> 1)) << 4), piece1 = r16 * LINE + (((2 * g + 1) ^ (r16 >> 1)) << 4);
   const unsigned char* scales_b = (const unsigned char*)a.b_scales + row_b * ks;
   int row[MT];
   floatx4 acc[MT];
@@ -601,7 +611,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void gemm8_few_kernel(kad_gemm8_arg
   }
   const auto add = [&](intx4 lo, intx4 hi, int sb, const Numbers<X> (&x)[MT]) {
     Operand<EXACT> fb, fa;
-    fb.set(lo, hi);
+    wave_order();
+    *(intx4*)(mine + to) = lo;
+    *(intx4*)(mine + to8) = hi;
+    wave_order();
+    fb.set(*(const intx4*)(mine + piece0), *(const intx4*)(mine + piece1));
     int eb[4];
     if (EXACT)
 #pragma unroll
@@ -621,8 +635,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void gemm8_few_kernel(kad_gemm8_arg
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
       const int kb = first + u * FEW_WAVES < whole ? first + u * FEW_WAVES : whole - 1;
-      lo[u] = *(const intx4*)(codes_b + kb * BLOCK8);
-      hi[u] = *(const intx4*)(codes_b + kb * BLOCK8 + 16);
+      lo[u] = *(const intx4*)(codes_b[0] + kb * BLOCK8);
+      hi[u] = *(const intx4*)(codes_b[1] + kb * BLOCK8);
       sb[u] = scales_b[kb];
 #pragma unroll
       for (int i = 0; i < MT; ++i) x[u][i].load(a, kp, ks, row[i], kb, g);
@@ -635,7 +649,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void gemm8_few_kernel(kad_gemm8_arg
     Numbers<X> x[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) x[i].load_end(a, row[i], whole, g);
-    add(*(const intx4*)(codes_b + whole * BLOCK8), *(const intx4*)(codes_b + whole * BLOCK8 + 16), scales_b[whole], x);
+    add(*(const intx4*)(codes_b[0] + whole * BLOCK8), *(const intx4*)(codes_b[1] + whole * BLOCK8), scales_b[whole], x);
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) red[wave][i][lane] = acc[i];
