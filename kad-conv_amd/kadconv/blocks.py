@@ -239,7 +239,8 @@ class Linear8(nn.Module):
             return {'relu': F.relu, 'silu': F.silu}[self.act](block8.linear8(x, self.weight, self.bias, None, self.dim))
         # the other calls: with gradients, traced, on fake tensors, captured
         keep = not (grad or self.training or torch.compiler.is_compiling()) and x.is_cuda and \
-            type(self.weight) is nn.Parameter and not torch.cuda.is_current_stream_capturing()
+            type(self.weight) is nn.Parameter and not _ext.native().observed(x, self.weight) and \
+            not torch.cuda.is_current_stream_capturing()
         return block8.linear8(x, self._weight8() if keep else self.weight, self.bias, self.act, self.dim)
 
     def extra_repr(self):
