@@ -924,7 +924,7 @@ Tensor linear8_kept_forward(const Tensor& x, const Tensor& codes, const Tensor& 
 }  // namespace
 
 void kad_torch::bind_rows(py::module_& m) {
-  // for the modules: whether a call is
+  // a call of these two, for the modules
   m.def("observed", [](const Tensor& a, const Tensor& b) { return observed({&a, &b}); });
   m.def("layer_norm", &layer_norm);
   m.def("layer_norm_forward", &layer_norm_forward);

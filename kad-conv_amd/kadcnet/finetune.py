@@ -11,7 +11,7 @@ runs it on synthetic images: a cell's class is the largest of fixed random proje
 
 goes on with a smaller head that learns from the first one's 4 best logits of each cell alone (``kadconv.distill_loss``):
 1 x 1 convolutions whose products are in 8 bits (``kadconv.Linear8``), with ``kadconv.LayerNorm`` over each cell's channels.
-In eval mode it serves with its weights kept in 8 bits.
+``StudentHead.serve`` keeps its weights in 8 bits.
 """
 import argparse
 import time
@@ -55,6 +55,14 @@ class StudentHead(nn.Module):
 
     def forward(self, maps):
         return [scale(m) for scale, m in zip(self.scales, maps)]
+
+    def serve(self):
+        """In eval mode, the weights kept in 8 bits; until ``train()``."""
+        self.eval()
+        for m in self.modules():
+            if isinstance(m, kadconv.Linear8):
+                m.keep()
+        return self
 
 
 def neck_maps(model, images):
@@ -194,7 +202,7 @@ def distill(a, teacher, channels, maps):
     ms = (time.perf_counter() - start) * 1e3 / a.steps
     tenth = max(1, a.steps // 10)
     print(f'student: {a.steps} steps by {a.distill} entries a cell: {ms:.1f} ms a step, loss {sum(losses[:tenth]) / tenth:.4f} -> '
-          f'{sum(losses[-tenth:]) / tenth:.4f}, served in 8 bits it agrees on {agreement(student.eval(), teacher, maps()):.3f} of the cells')
+          f'{sum(losses[-tenth:]) / tenth:.4f}, served in 8 bits it agrees on {agreement(student.serve(), teacher, maps()):.3f} of the cells')
     return losses
 
 

@@ -198,10 +198,12 @@ class Linear8(nn.Module):
     """x W^T + b along the last axis or, with ``dim=1``, of each pixel of a map [N, C, H, W] (a 1 x 1 convolution), the
     products in 8 bits (``kadconv.linear8``); parameters as torch.nn.Linear's, so its state dicts load.
 
-    In eval mode, where nothing is differentiated, W is kept in 8 bits and laid out anew when it has changed (seen by its
-    version: a write through ``.data`` is not), and ``act`` is applied in the same launch.  Other calls go by W itself, and
-    so does one that is captured into a graph: its replays follow W.  (For a graph that reads W in 8 bits only, capture
-    ``kadconv.linear8`` with ``kadconv.quantize8(W)``.)"""
+    Every call brings W to 8 bits as it is then.  A program that serves spares that: ``keep()`` makes a copy in 8 bits, by which
+    the calls go that follow in eval mode, where nothing is differentiated; ``act`` is part of such a call's launch.  The
+    copy is dropped where W is seen to have changed (another tensor or version of it, ``train()``); writes that no version
+    tells, through ``.data`` or by the replay of a graph, need another ``keep()``.  Traced calls, and ones that are captured into
+    a graph, go by W itself, and so do their replays.  (For a graph that reads W in 8 bits only, capture ``kadconv.linear8``
+    with ``kadconv.quantize8(W)``.)"""
 
     def __init__(self, in_features, out_features, bias=True, act=None, dim=-1):
         super().__init__()
@@ -214,34 +216,61 @@ class Linear8(nn.Module):
         self.in_features, self.out_features, self.act, self.dim = in_features, out_features, act, dim
         like = nn.Linear(in_features, out_features, bias)
         self.weight, self.bias = like.weight, like.bias
-        self._kept = None  # (weight, its version, the weight in 8 bits, the stream that it was laid out on, and when)
+        self._kept = None  # (W, what it is known by, the copy, the stream that it was made on, and when)
 
     def __getstate__(self):
-        return {**self.__dict__, '_kept': None}  # a copy of the module lays out its own
+        return {**self.__dict__, '_kept': None}  # a copy of the module makes its own
+
+    def train(self, mode=True):
+        if mode:
+            self._kept = None
+        return super().train(mode)
+
+    def _known_by(self):
+        w = self.weight
+        return w.data_ptr(), w.shape, w.stride(), w.dtype, 0 if w.is_inference() else w._version
+
+    def keep(self, on=True):
+        """Makes the copy of W in 8 bits that calls in eval mode go by (on=False: drops it); returns the module."""
+        self._kept = None
+        if not on:
+            return self
+        w = self.weight.detach()  # held, so that its address is no other's
+        if self.training or not w.is_cuda or type(self.weight) is not nn.Parameter:
+            raise RuntimeError('keep() is for eval mode and a parameter on a GPU')
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('keep() cannot be captured into a graph')
+        stream = torch.cuda.current_stream(w.device)
+        copy = block8.quantize8(w)
+        self._kept = w, self._known_by(), copy, stream, stream.record_event()
+        return self
 
     def _weight8(self):
-        w, kept = self.weight.detach(), self._kept
-        if w.is_inference():
-            return block8.quantize8(w)
-        # the weight that was laid out is held, so that its address is no other's
+        """The copy, for the current stream; None where there is none of W as it is."""
+        if self._kept is None:
+            return None
+        w, known_by, copy, made_on, made = self._kept
+        if known_by != self._known_by():
+            self._kept = None
+            return None
         stream = torch.cuda.current_stream(w.device)
-        if kept is None or kept[0].data_ptr() != w.data_ptr() or (kept[0].dtype, kept[1]) != (w.dtype, self.weight._version):
-            kept = self._kept = w, self.weight._version, block8.quantize8(w), stream, stream.record_event()
-        if stream != kept[3]:  # laid out on another one
-            stream.wait_event(kept[4])
-            kept[2].codes.record_stream(stream)
-            kept[2].scales.record_stream(stream)
-        return kept[2]
+        if stream != made_on:
+            stream.wait_event(made)
+            copy.codes.record_stream(stream)
+            copy.scales.record_stream(stream)
+        return copy
 
     def forward(self, x):
         grad = torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters()))
         if grad and self.act is not None:
             return {'relu': F.relu, 'silu': F.silu}[self.act](block8.linear8(x, self.weight, self.bias, None, self.dim))
-        # the other calls: with gradients, traced, on fake tensors, captured
-        keep = not (grad or self.training or torch.compiler.is_compiling()) and x.is_cuda and \
-            type(self.weight) is nn.Parameter and not _ext.native().observed(x, self.weight) and \
-            not torch.cuda.is_current_stream_capturing()
-        return block8.linear8(x, self._weight8() if keep else self.weight, self.bias, self.act, self.dim)
+        weight = self.weight
+        if not (grad or self.training or torch.compiler.is_compiling()) and self._kept is not None and x.is_cuda and \
+                type(weight) is nn.Parameter and not _ext.native().observed(x, weight) and \
+                not torch.cuda.is_current_stream_capturing():
+            copy = self._weight8()
+            weight = weight if copy is None else copy
+        return block8.linear8(x, weight, self.bias, self.act, self.dim)
 
     def extra_repr(self):
         return f'{self.in_features}, {self.out_features}, bias={self.bias is not None}, act={self.act!r}, dim={self.dim}'
