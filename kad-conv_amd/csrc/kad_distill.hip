@@ -8,7 +8,7 @@
 // Memory bounds it: forward reads z once (the largest value and the sum in one pass), backward reads z and writes dz;
 // what the classes of the entries are is looked up in z, a few values a row.
 //
-// Two forms.  Up to 1024 classes a row stays in the registers of up to 64 lanes (kad_rows.h), many rows a wave; beyond, a
+// Two forms, and one in 64 bits for high temperatures (below).  Up to 1024 classes a row stays in the registers of up to 64 lanes (kad_rows.h), many rows a wave; beyond, a
 // wave or a block walks a row, or a block a part of one where rows are few: forward these parts are joined in a second
 // launch, backward each writes its own classes.
 //
@@ -636,8 +636,161 @@ __global__ __launch_bounds__(256) void distill_large_bwd_kernel(kad_distill_args
   }
 }
 
+// ---------------------------------------------------------------------------- high temperatures
+// Loss and gradient are T^2 and T times what is left of logarithms and weights of order 1 that agree in all but 1 / T^2 and 1 / T
+// of themselves, where the entries have nearly all of the row's weight.  So 32 bits are off by T^2 2^-24 and T 2^-24 times a
+// row's sums' own errors (16 classes, all of them entries, losses of 0.04: 2e-5 of a loss at T of 4, 7e-5 at 8, 1e-2 at 100, all
+// of it at 1000): up to MOST_32 that is the arithmetic above, beyond it is in 64 bits.  There too the logarithms' own size is kept
+// out of the loss:
+//   log(Z / S) = log1p((Z - S) / S),  Z - S from exponentials less 1, which are of the arguments' size, 1 / T:
+// T 2^-53 is what the loss is off by, 1e-10 at T of 10^6.
+//
+// One row to 16, 64 or 256 lanes, a value at a time, z read twice in either direction.  64-bit exponentials bound it: 4096 rows of
+// 32768 classes, bf16, 64 entries, forward 614 us (49 in 32 bits) and backward 474 (106); 537600 of 16, fp16, 16 entries, 175 (31)
+// and 147 (29).
+constexpr float MOST_32 = 8.f;
+
+template <int G>
+__device__ __forceinline__ float max_of_lanes(float v) {
+  if constexpr (G > 64) return max_of_row<G / 64>(v);
+  else return lanes_max(v, G);
+}
+template <int G>
+__device__ __forceinline__ double sum_of_lanes(double v) {
+#pragma unroll
+  for (int m = 1; m < (G < 64 ? G : 64); m <<= 1) v += __shfl_xor(v, m);
+  if constexpr (G > 64) {
+    __shared__ double red[G / 64];
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+    for (int i = 1; i < G / 64; ++i) v += red[i];
+  }
+  return v;
+}
+
+// A sum of exponentials of x <= 0: how many x are above -1, the sum of e^x - 1 over these, and that of the others' e^x.
+struct Mass {
+  double near = 0., less = 0., far = 0.;
+  __device__ __forceinline__ void add(double x) {
+    if (x > -1.) {
+      near += 1.;
+      less += expm1(x);
+    } else {
+      far += exp(x);
+    }
+  }
+  template <int G>
+  __device__ __forceinline__ void join() {
+    near = sum_of_lanes<G>(near);
+    less = sum_of_lanes<G>(less);
+    far = sum_of_lanes<G>(far);
+  }
+  __device__ __forceinline__ double whole() const { return near + far + less; }
+  __device__ __forceinline__ double over(const Mass& o) const { return (near - o.near) + (far - o.far) + (less - o.less); }
+};
+
+template <typename T, int G>
+__global__ __launch_bounds__(256) void distill_high_fwd_kernel(kad_distill_args a) {
+  constexpr int ROWS = 256 / G;
+  const int l = threadIdx.x & (G - 1);
+  const double heat = a.temperature, c = 1. / heat;
+  float total = 0.f;
+  unsigned count = 0;
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
+    const T* z = (const T*)a.logits + row * a.z_rs;
+    const Entries en(a, row);
+    float tm = -INF, zm = -INF, any = 0.f, t;
+    int at;
+    for (int e = l; e < a.k; e += G)
+      if (en.get(e, at, t)) {
+        any = 1.f;
+        tm = fmaxf(tm, t);
+      }
+    for (int j = l; j < a.v; j += G) zm = fmaxf(zm, to_f32(z[j]));
+    any = max_of_lanes<G>(any);
+    tm = max_of_lanes<G>(tm);
+    zm = max_of_lanes<G>(zm);
+    Mass of_z, of_t;
+    double d = 0.;
+    for (int j = l; j < a.v; j += G) of_z.add(((double)to_f32(z[j]) - zm) * c);
+    for (int e = l; e < a.k; e += G)
+      if (en.get(e, at, t)) {
+        const double y = ((double)t - tm) * c, w = exp(y);
+        of_t.add(y);
+        d += w == 0. ? 0. : w * (y - ((double)to_f32(z[at]) - zm) * c);  // as in add_entry
+      }
+    of_z.join<G>();
+    of_t.join<G>();
+    d = sum_of_lanes<G>(d);
+    if (l == 0) {
+      const double s = of_t.whole();
+      const float loss = any != 0.f ? (float)(heat * heat * (d / s + log1p(of_z.over(of_t) / s))) : 0.f;
+      leave_row(a, row, any != 0.f, zm, (float)of_z.whole(), loss);
+      total += loss;
+      count += any != 0.f;
+    }
+  }
+  leave_part(a, total, count);
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(256) void distill_high_bwd_kernel(kad_distill_args a) {
+  constexpr int ROWS = 256 / G;
+  __shared__ int at_of_rows[KAD_DISTILL_MOST];
+  __shared__ double p_of_rows[KAD_DISTILL_MOST];
+  const int l = threadIdx.x & (G - 1), sub = threadIdx.x / G;
+  int* at_of = at_of_rows + sub * (KAD_DISTILL_MOST / ROWS);
+  double* p_of = p_of_rows + sub * (KAD_DISTILL_MOST / ROWS);
+  const double heat = a.temperature, c = 1. / heat;
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + sub; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
+    const T* z = (const T*)a.logits + row * a.z_rs;
+    T* dz = (T*)a.dlogits + row * a.v;
+    const float zm = a.stats[2 * row];
+    const bool live = a.stats[2 * row + 1] != 0.f;
+    const double f = a.dloss[a.reduction == KAD_REDUCE_NONE ? row : 0] * heat * (a.reduction == KAD_REDUCE_MEAN ? *a.share : 1.f);
+    const Entries en(a, row);
+    float tm = -INF, t;
+    int at;
+    for (int e = l; e < a.k; e += G)
+      if (en.get(e, at, t)) tm = fmaxf(tm, t);
+    tm = max_of_lanes<G>(tm);
+    row_barrier<(G > 64 ? G / 64 : 1)>();  // the row before is done with its entries
+    double s = 0., zsum = 0.;
+    for (int e = l; e < a.k; e += G) {
+      const bool counts = en.get(e, at, t);
+      const double w = counts ? exp(((double)t - tm) * c) : 0.;
+      at_of[e] = counts ? at : -1;
+      p_of[e] = w;
+      s += w;
+    }
+    for (int j = l; j < a.v; j += G) zsum += exp(((double)to_f32(z[j]) - zm) * c);
+    s = sum_of_lanes<G>(s);
+    zsum = sum_of_lanes<G>(zsum);
+    const double inv = 1. / zsum, norm = 1. / s, scale = s == s ? f * inv : s;
+    for (int j = l; j < a.v; j += G) dz[j] = from_f32<T>(live ? (float)(scale * exp(((double)to_f32(z[j]) - zm) * c)) : 0.f);
+    // The entries' classes again, once all of the row's stores are done.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    row_barrier<(G > 64 ? G / 64 : 1)>();
+    for (int e = l; e < a.k; e += G) {
+      const int mine = at_of[e];
+      if (mine < 0 || !live) continue;
+      double p = 0.;
+      bool again = false;
+      for (int i = 0; i < a.k; ++i) {
+        const bool same = at_of[i] == mine;
+        p += same ? p_of[i] : 0.;
+        again |= same && i < e;
+      }
+      if (!again) dz[mine] = from_f32<T>((float)(f * (exp(((double)to_f32(z[mine]) - zm) * c) * inv - p * norm)));
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------- host
 struct Shape {
+  int lanes;       // of a row, at high temperatures; else 0
   int vv, u, G;
   int64_t blocks;  // whose losses are joined
   bool wave_rows;  // large rows: a wave each
@@ -646,6 +799,12 @@ struct Shape {
 
 Shape shape_of(const kad_distill_args& a, bool backward) {
   Shape s{};
+  if (a.temperature > MOST_32) {  // a block's rows have KAD_DISTILL_MOST entries
+    s.lanes = a.v <= 256 && a.k <= 64 ? 16 : a.v <= 4096 && a.k <= 256 ? 64 : 256;
+    const int64_t turns = (a.rows + 256 / s.lanes - 1) / (256 / s.lanes), most = backward ? MOST_BLOCKS : 2048;
+    s.blocks = turns < most ? turns : most;
+    return s;
+  }
   const int v = 16 / dtype_size(a.dtype);
   // Rows in registers or not, us, 131072 rows of 1024 classes, 32 entries: forward bf16 134 and 134, fp32 140 and 129,
   // backward fp32 208 and 303, but bf16 244 and 173 (and 266 against 274 at 512 classes, twice the rows).
@@ -731,10 +890,20 @@ void launch_small(const kad_distill_args& a, const Shape& s, bool backward, hipS
   else launch_small<T, VEC<T>, U, false>(a, s, backward, st);
 }
 
+template <typename T, int G>
+void launch_high(const kad_distill_args& a, const Shape& s, bool backward, hipStream_t st) {
+  if (backward) distill_high_bwd_kernel<T, G><<<s.blocks, 256, 0, st>>>(a);
+  else distill_high_fwd_kernel<T, G><<<s.blocks, 256, 0, st>>>(a);
+}
+
 template <typename T>
 void launch(const kad_distill_args& a, bool backward, hipStream_t st) {
   const Shape s = shape_of(a, backward);
-  if (s.G) {
+  if (s.lanes) {
+    if (s.lanes == 16) launch_high<T, 16>(a, s, backward, st);
+    else if (s.lanes == 64) launch_high<T, 64>(a, s, backward, st);
+    else launch_high<T, 256>(a, s, backward, st);
+  } else if (s.G) {
     if (s.vv == 1) launch_small<T, 1, 1, false>(a, s, backward, st);
     else if (s.u == 1) launch_small<T, 1>(a, s, backward, st);
     else if (s.u == 2) launch_small<T, 2>(a, s, backward, st);

@@ -388,26 +388,37 @@ def _distill_check(x, t, index, temperature, reduction, dim):
             raise TypeError(f'logits must be floating-point numbers, got {v.dtype}')
 
 
+def _exponentials(x):
+    """A sum of exponentials of x <= 0: how many x are above -1, the sum of e^x - 1 over these, and that of the others' e^x."""
+    near = x > -1
+    zero = torch.zeros_like(x)
+    return near.sum(-1), torch.where(near, torch.expm1(x), zero).sum(-1), torch.where(near, zero, torch.exp(x)).sum(-1)
+
+
 def _distill_cpu(x, t, index, temperature, reduction, dim):
+    """In 64 bits, and with log(Z / S) from a difference of sums that keeps its digits where T is large."""
     axis = _row_axis(x, dim)
-    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
-    z = x.to(wide).movedim(axis, -1) / temperature
-    t = t.detach().to(wide).movedim(axis, -1) / temperature
-    index = index.movedim(axis, -1).long()
+    z, t, index = x.double().movedim(axis, -1), t.detach().double().movedim(axis, -1), index.movedim(axis, -1).long()
     counts = (index >= 0) & (index < z.shape[-1]) & (t != -float('inf'))
     live = counts.any(-1)
     t = torch.where(counts, t, torch.full_like(t, -float('inf'))).masked_fill(~live[..., None], 0.0)
-    log_p = F.log_softmax(t, -1)
-    p = log_p.exp()
     z = torch.where(live[..., None], z, torch.zeros_like(z))  # a row without entries: 0, whatever its logits are
-    log_q = F.log_softmax(z, -1).gather(-1, index.clamp(0, z.shape[-1] - 1))
-    weighs = live[..., None] & (p != 0)
-    terms = p * (log_p - torch.where(weighs, log_q, torch.zeros_like(log_q)))
-    loss = temperature ** 2 * torch.where(weighs, terms, torch.zeros_like(p)).sum(-1)
-    if reduction == 'none':
-        return loss.to(torch.promote_types(torch.float32, x.dtype))
-    loss = loss.sum()
-    return loss / live.sum().clamp(min=1) if reduction == 'mean' else loss
+    b = (t - t.amax(-1, keepdim=True)) / temperature
+    a = (z - z.detach().amax(-1, keepdim=True)) / temperature
+    e = b.exp()
+    total = e.sum(-1)
+    zero = torch.zeros_like(e)
+    weighs = e != 0
+    at = a.gather(-1, index.clamp(0, z.shape[-1] - 1))
+    terms = e * (torch.where(weighs, b, zero) - torch.where(weighs, at, zero))
+    (near_z, less_z, far_z), (near_t, less_t, far_t) = _exponentials(a), _exponentials(b)
+    ratio = torch.log1p(((near_z - near_t) + (far_z - far_t) + (less_z - less_t)) / total)
+    loss = temperature ** 2 * torch.where(live, terms.sum(-1) / total + ratio, torch.zeros_like(ratio))
+    if reduction != 'none':
+        loss = loss.sum()
+    if reduction == 'mean':
+        loss = loss / live.sum().clamp(min=1)
+    return loss.to(torch.promote_types(torch.float32, x.dtype))
 
 
 def distill_loss_forward(logits, teacher_logits, teacher_index, temperature, reduction, dim):
@@ -434,7 +445,8 @@ def distill_loss(logits, teacher_logits, teacher_index, temperature=1.0, reducti
     row that has some, but logits of -infinity alone, is NaN.
 
     ``reduction``: 'none' (a row's loss each, float32), 'sum', or 'mean' over the rows that have entries (0 if none has).
-    Sums are taken in 32 bits and in an order that the sizes decide.  The teacher's tensors are constants.
+    Sums are taken in 32 bits, at temperatures above 8 (where T^2
+    times their errors would show) and on the CPU in 64, in an order that the sizes decide.  The teacher's tensors are constants.
 
     GPU tensors (fp32, fp16, bf16; up to 1024 entries) run the gfx950 HIP kernels, forward and backward (once
     differentiable); logits are read where they are if their rows lie a fixed distance apart.  The gradient is dense (a
