@@ -173,21 +173,24 @@ def _(x, weight, bias, eps, dim):
     return _rows_empty(x, dim), mean, torch.empty_like(mean)
 
 
+def _or_empty(like, *grads):
+    """Gradients as an operator's results: of what is not needed or has no tensor an empty one."""
+    return tuple(like.new_empty(0) if g is None else g for g in grads)
+
+
 @torch.library.custom_op('kadconv::layer_norm_backward', mutates_args=())
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None,
-                        mean: torch.Tensor, rstd: torch.Tensor, eps: float,
-                        dim: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                        mean: torch.Tensor, rstd: torch.Tensor, eps: float, dim: int, need_x: bool = True, need_weight: bool = True,
+                        need_bias: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     from . import ops
-    dx, dw, db = ops.layer_norm_backward(dy, x, weight, bias, mean, rstd, eps, dim)
-    none = mean.new_empty(0)
-    return dx, none if dw is None else dw, none.clone() if db is None else db
+    return _or_empty(mean, *ops.layer_norm_backward(dy, x, weight, bias, mean, rstd, eps, dim, need_x, need_weight, need_bias))
 
 
 @layer_norm_backward.register_fake
-def _(dy, x, weight, bias, mean, rstd, eps, dim):
-    def like(p):
-        return mean.new_empty(0) if p is None else torch.empty_like(p, memory_format=torch.contiguous_format)
-    return _rows_empty(x, dim), like(weight), like(bias)
+def _(dy, x, weight, bias, mean, rstd, eps, dim, need_x=True, need_weight=True, need_bias=True):
+    def like(need, p):
+        return torch.empty_like(p, memory_format=torch.contiguous_format) if need and p is not None else None
+    return _or_empty(mean, _rows_empty(x, dim) if need_x else None, like(need_weight, weight), like(need_bias, bias))
 
 
 def _layer_norm_context(ctx, inputs, output):
@@ -199,8 +202,9 @@ def _layer_norm_context(ctx, inputs, output):
 
 def _layer_norm_grad(ctx, dy, _mean, _rstd):
     x, weight, bias, mean, rstd = ctx.saved_tensors
-    dx, dw, db = torch.ops.kadconv.layer_norm_backward(dy, x, weight, bias, mean, rstd, *ctx.rest)
-    return dx, None if weight is None else dw, None if bias is None else db, None, None
+    need = ctx.needs_input_grad[:3]
+    grads = torch.ops.kadconv.layer_norm_backward(dy, x, weight, bias, mean, rstd, *ctx.rest, *need)
+    return *(g if n else None for g, n in zip(grads, need)), None, None
 
 
 layer_norm.register_autograd(_layer_norm_grad, setup_context=_layer_norm_context)
@@ -292,17 +296,17 @@ def _(x, weight, bias, act, dim):
 
 
 @torch.library.custom_op('kadconv::linear8_backward', mutates_args=())
-def linear8_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
-                     dim: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def linear8_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, dim: int, need_x: bool = True,
+                     need_weight: bool = True, need_bias: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     from . import block8
-    dx, dw, db = block8.linear8_backward(dy, x, weight, bias, dim)
-    return dx, dw, dw.new_empty(0) if db is None else db
+    return _or_empty(weight, *block8.linear8_backward(dy, x, weight, bias, dim, need_x, need_weight, need_bias))
 
 
 @linear8_backward.register_fake
-def _(dy, x, weight, bias, dim):
-    dw = torch.empty_like(weight, memory_format=torch.contiguous_format)
-    return _rows_empty(x, dim), dw, dw.new_empty(0) if bias is None else torch.empty_like(bias, memory_format=torch.contiguous_format)
+def _(dy, x, weight, bias, dim, need_x=True, need_weight=True, need_bias=True):
+    def like(need, p):
+        return torch.empty_like(p, memory_format=torch.contiguous_format) if need and p is not None else None
+    return _or_empty(weight, _rows_empty(x, dim) if need_x else None, like(need_weight, weight), like(need_bias, bias))
 
 
 def _linear8_context(ctx, inputs, output):
@@ -315,8 +319,9 @@ def _linear8_context(ctx, inputs, output):
 
 def _linear8_grad(ctx, dy):
     x, weight, bias = ctx.saved_tensors
-    dx, dw, db = torch.ops.kadconv.linear8_backward(dy, x, weight, bias, ctx.dim)
-    return dx, dw, None if bias is None else db, None, None
+    need = ctx.needs_input_grad[:3]
+    grads = torch.ops.kadconv.linear8_backward(dy, x, weight, bias, ctx.dim, *need)
+    return *(g if n else None for g, n in zip(grads, need)), None, None
 
 
 linear8.register_autograd(_linear8_grad, setup_context=_linear8_context)
