@@ -724,9 +724,13 @@ struct Across {
   Held8 x, w;
 };
 
-// The gradient of a weight is a product over the rows.
-void check_many(int64_t rows) {
-  TORCH_CHECK_VALUE(rows <= KAD_GEMM8_MOST, "a weight has a gradient of up to ", KAD_GEMM8_MOST, " rows, got ", rows);
+// The gradient of a weight is a product over the rows, that of the input one over the outputs; for all but the input's of few
+// rows the gradient of y is brought to 8 bits in memory.  The checks of kadconv.block8._gradient_check.
+void check_gradients8(int64_t rows, int64_t outputs, bool need_x, bool need_weight, bool need_bias) {
+  TORCH_CHECK_VALUE(!need_weight || rows <= KAD_GEMM8_MOST, "a weight has a gradient of up to ", KAD_GEMM8_MOST, " rows, got ", rows);
+  const bool in_memory = need_weight || need_bias || (need_x && rows > KAD_GEMM8_FEW);
+  const int64_t most = in_memory ? KAD_QUANT8_MOST : need_x ? KAD_GEMM8_MOST : outputs;
+  TORCH_CHECK_VALUE(!rows || outputs <= most, "gradients of up to ", most, " outputs expected, got ", outputs);
 }
 
 // y of values and a weight, which are brought to 8 bits; `across`: where wanted, along the columns in the same reads.
@@ -735,7 +739,6 @@ Tensor linear8_run(const Tensor& x, bool map, const Tensor& weight, const Tensor
   const int64_t n = weight.size(0), k = weight.size(1);
   Tensor y = result_like(x, map, n);
   const int64_t m = row_count(x, map);
-  if (across_x) check_many(m);
   const Rows w = rows_of(weight, false);
   const Held8 wh = new_held(x, n, k);
   if (across_w) across.w = new_held(x, k, n);
@@ -836,7 +839,10 @@ OptTensor linear8(const Tensor& x, const Tensor& weight, const OptTensor& bias, 
   std::shared_ptr<Linear8Backward> node;
   Tensor y;
   Across across;
-  if (grad) node = new_node<Linear8Backward>(torch::autograd::collect_next_edges(x, weight, b));
+  if (grad) {
+    check_gradients8(row_count(x, map), weight.size(0), x.requires_grad(), weight.requires_grad(), b.defined() && b.requires_grad());
+    node = new_node<Linear8Backward>(torch::autograd::collect_next_edges(x, weight, b));
+  }
   {
     at::AutoDispatchBelowADInplaceOrView below;
     const c10::DeviceGuard guard(x.device());
@@ -879,7 +885,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear8_backward(const Tensor& dy, c
   at::AutoDispatchBelowADInplaceOrView below;
   const c10::DeviceGuard guard(x.device());
   Across across;
-  if (need_weight) check_many(o.m);
+  check_gradients8(o.m, o.n, need_x, need_weight, need_bias && b.defined());
   if (need_weight && o.m) {
     across.x = new_held(x, o.k, o.m);
     quantize(rows_of(x, map), {}, across.x, Tensor(), x);

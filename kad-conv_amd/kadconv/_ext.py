@@ -154,6 +154,8 @@ ADAMW_SEG = 256          # KAD_ADAMW_SEG
 LAYER_NORM_MOST = 16384  # KAD_LAYER_NORM_MOST
 DISTILL_MOST = 1024      # KAD_DISTILL_MOST
 QUANT8_MOST = 1 << 20    # KAD_QUANT8_MOST
+GEMM8_MOST = 1 << 22     # KAD_GEMM8_MOST
+GEMM8_FEW = 32           # KAD_GEMM8_FEW
 ADAMW_SCALARS = 4        # 4-byte words of kad_adamw_scalars
 
 

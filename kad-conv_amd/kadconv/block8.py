@@ -133,6 +133,16 @@ def matmul8(a, b, bias=None, act=None, dtype=torch.bfloat16):
     return _act_cpu(z, act).to(dtype)
 
 
+def _gradient_check(rows, outputs, need_x, need_weight, need_bias):
+    """The limits of gradients on the GPU: sums over the rows, and over the outputs."""
+    if need_weight and rows > _ext.GEMM8_MOST:
+        raise ValueError(f'a weight has a gradient of up to {_ext.GEMM8_MOST} rows, got {rows}')
+    in_memory = need_weight or need_bias or (need_x and rows > _ext.GEMM8_FEW)
+    most = _ext.QUANT8_MOST if in_memory else _ext.GEMM8_MOST if need_x else outputs
+    if rows and outputs > most:
+        raise ValueError(f'gradients of up to {most} outputs expected, got {outputs}')
+
+
 def _linear8_check(x, weight, bias, act, dim):
     axis = _quantize_check(x, dim)
     kept = isinstance(weight, Block8)
@@ -152,6 +162,9 @@ def _linear8_check(x, weight, bias, act, dim):
             raise NotImplementedError('kadconv.linear8 with a weight in 8 bits has no gradient')
         if act is not None and not kept and (grad or weight.requires_grad):
             raise NotImplementedError('kadconv.linear8 with an activation has no gradient')
+        if x.is_cuda and not kept:
+            _gradient_check(x.numel() // x.shape[axis], weight.shape[0], x.requires_grad, weight.requires_grad,
+                            bias is not None and bias.requires_grad)
     return axis
 
 
@@ -216,7 +229,8 @@ def linear8(input, weight, bias=None, act=None, dim=-1):
     With numbers as weight and no ``act`` it is differentiable once.  Gradients pass the rounding as if it were not there,
     and are products in 8 bits themselves: that of x is dy W, both along N, that of W is dy^T x, both along the rows; that
     of the bias is the sum of dy.  For them x and W are kept in 8 bits, not as they are: later changes of either are not
-    seen.  The gradient of W takes up to 2^22 rows.
+    seen.  On the GPU the gradient of W takes up to 2^22 rows, and gradients up to 2^20 outputs N (that of x alone, of up to 32
+    rows, 2^22).
 
     GPU tensors (fp32, fp16, bf16) run the gfx950 HIP kernels; rows that lie a fixed distance apart are read where they
     are.  Up to 32 rows, and short ones (up to 512 values), take one launch, their numbers brought to 8 bits by the product's

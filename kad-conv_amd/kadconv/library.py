@@ -310,9 +310,11 @@ def _(dy, x, weight, bias, dim, need_x=True, need_weight=True, need_bias=True):
 
 
 def _linear8_context(ctx, inputs, output):
+    from . import block8
     x, weight, bias, act, dim = inputs
     if act is not None:
         raise NotImplementedError('kadconv.linear8 with an activation has no gradient')
+    block8._gradient_check(x.numel() // weight.shape[1], weight.shape[0], *ctx.needs_input_grad[:3])
     ctx.save_for_backward(x, weight, bias)
     ctx.dim = dim
 
