@@ -889,6 +889,7 @@ void launch_short(const kad_gemm8_args& a, hipStream_t st) {
   if (parts > most) parts = most;
   const int columns = round_up(ceil_div(a.n, parts), COLUMNS);
   const size_t bytes = blocks * SHORT_ROWS * LINE + SHORT_ROWS * round_up(blocks, 4) + 4 * short_bytes(TN);
+  allow_lds(gemm8_short_kernel<T, WM, TN>, bytes);
   gemm8_short_kernel<T, WM, TN><<<dim3(tm, ceil_div(a.n, columns)), 256, bytes, st>>>(a, columns);
 }
 
