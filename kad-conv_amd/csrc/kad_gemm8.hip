@@ -147,11 +147,11 @@ __device__ __forceinline__ void store_tile(const kad_gemm8_args& a, const floatx
         for (int e = 0; e < 4; ++e) t[e] = from_f32<T>(activate<T>(acc[i + h][j][e] + bias[j][e], ACT));
         __builtin_memcpy(lds + (h * 16 + r16) * PITCH + (j * 16 + 4 * g) * 2, t, 8);
       }
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
     intx4 v[32 / ROWS];
 #pragma unroll
     for (int r = 0; r < 32 / ROWS; ++r) v[r] = *(const intx4*)(lds + (r * ROWS + row) * PITCH + piece * 16);
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
 #pragma unroll
     for (int r = 0; r < 32 / ROWS; ++r) {
       const int m = m1 + i * 16 + r * ROWS + row;
@@ -345,11 +345,11 @@ __device__ __forceinline__ void store_wide(const kad_gemm8_args& a, const floatx
         for (int e = 0; e < 4; ++e) t[e] = from_f32<T>(activate<T>(acc[i][j][4 * q + e] + bias[j][4 * q + e], ACT));
         __builtin_memcpy(lds + r32 * PITCH + (j * 32 + 8 * q + 4 * h) * 2, t, 8);
       }
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
     intx4 v[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = *(const intx4*)(lds + (r * 8 + row) * PITCH + piece * 16);
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int m = m1 + i * 32 + r * 8 + row;
