@@ -303,8 +303,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm8_tile_kernel(kad_gemm8_args
 // time (4900 cycles, of which the instructions take 2048).
 //
 // The copies are written as assembly: of ones that it knows the compiler waits for more than a step needs before it reads
-// LDS (it does not tell all stages apart), which ends the run ahead.  They write no register but m0, which nothing else
-// here uses, and every wait for them is one of KAD_STEP's.  Scales go the same way, two groups of four blocks in turn.
+// LDS (it does not tell all stages apart), which ends the run ahead.  They write no register but m0, and name it, and
+// every wait for them is one of KAD_STEP's.  Scales go the same way, two groups of four blocks in turn.
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ uint32_t lds_address(const char* p) {
@@ -319,11 +319,11 @@ __device__ __forceinline__ intx4 resource(const void* base, uint32_t bytes) {
 // there before a wait for vmcnt.
 __device__ __forceinline__ void copy16(intx4 r, uint32_t lds, uint32_t off, uint32_t at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(r), "s"(at)
-               : "memory");
+               : "m0", "memory");
 }
 __device__ __forceinline__ void copy4(intx4 r, uint32_t lds, uint32_t off, uint32_t at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(r), "s"(at)
-               : "memory");
+               : "m0", "memory");
 }
 
 constexpr int WIDE = 256, HALF = 64;  // rows of a tile, bytes of a row in a stage
