@@ -688,6 +688,7 @@ OptTensor matmul8(const Tensor& a, const Tensor& a_scales, const Tensor& b, cons
                   const std::optional<std::string_view>& act, at::ScalarType dtype) {
   const Tensor bi = defined(bias);
   if (observed({&a, &a_scales, &b, &b_scales, &bi})) return std::nullopt;
+  check_no_forward_grad({&bi}, "kadconv.matmul8");
   return matmul8_forward(a, a_scales, b, b_scales, k, bias, act, dtype);
 }
 
