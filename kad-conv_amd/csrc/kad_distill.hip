@@ -12,9 +12,9 @@
 // wave or a block walks a row, or a block a part of one where rows are few: forward these parts are joined in a second
 // launch, backward each writes its own classes.
 //
-// 4096 rows of 32768 classes, bf16, 32 entries: forward 53 us (5.1 TB/s), backward 112 (4.8), 158 one after the other, with
-// gradients written past the cache that holds the logits (183 through it).  537600 rows of 16 classes, fp16, 16 entries:
-// 24 us (3.1 TB/s) and 29 (3.2).
+// 4096 rows of 32768 classes, bf16, 64 entries: 159 us a pass, 58 forward (4.7 TB/s), 5 for the join and 98 backward (5.8, part of z
+// from the cache that holds the logits, past which gradients are written: 183 a pass through it).  537600 rows of 16 classes,
+// fp16, 16 entries: 25 us (3.0 TB/s) and 29 (3.1).
 //
 // An index may come twice: its p add up, in no order that could change them: of small rows in LDS as whole numbers of
 // 2^-62 (a p of 2^-38 and more keeps its 24 bits; of what is smaller, no more than 2^-62 of the row's weight is lost),

@@ -5,15 +5,17 @@
 // The scales are powers of two, so the scaled matrix instruction takes them as they are: one of 16 x 16 x 128 meets one
 // block of each of its rows, and the sums need no arithmetic beside it.  Every 8-bit matrix instruction cuts the products
 // of eight consecutive k to 2^-13 of the largest of them (found by giving it single products: 2^3 next to 2^16 is kept,
-// 2^2 is not) before it adds them up in 32 bits.  Of normally distributed numbers that is 1.3e-5 of a result, of codes with
-// all bits random 5e-5: under the rounding of a 16-bit result.  For 32-bit results (EXACT) codes become fp16 numbers, which
+// 2^2 is not) before it adds them up in 32 bits.  Of normally distributed numbers that is 1.3e-5 of a result, of channels of unlike
+// sizes 4e-5, of codes with all bits random 5e-5: under the rounding of a 16-bit result (2.1e-4 in fp16, 1.7e-3 in bf16).  For 32-bit results (EXACT) codes become fp16 numbers, which
 // hold them exactly, the fp16 instruction sums a block in 32 bits (1e-7), and the scales are applied to its sum.
 //
-// Three forms.  Many rows: tiles of BM x BN results, both operands' codes copied to LDS past the registers, ahead of their use.
+// Three forms.  Many rows: tiles of BM x BN results, both operands' codes copied to LDS past the registers, ahead of their use, in
+// two kernels: a stage ahead for tiles of 64 and 128, three for those of 256.
 //
 // Few rows (KAD_GEMM8_FEW): b's codes are read once, in whole lines that a wave turns into operands by way of its part of LDS;
 // a block takes 16 rows of b, its waves take every eighth 128 columns and join in LDS.  a as values is brought to 8 bits in
-// registers, by each block for itself: a launch less, and a is small (at 48 rows and [8192, 4096] it is not: 48 us against 33).
+// registers, by each block for itself: a launch less, and a is small (at 48 rows and [8192, 4096], b from memory, it was not: 48 us
+// against 33).
 //
 // Many rows, short ones: a block brings its rows of values to 8 bits once and keeps them in LDS.
 //
@@ -831,10 +833,17 @@ Plan plan_of(const kad_gemm8_args& a) {
   const int blocks = ceil_div(a.k, BLOCK8);
   const bool exact = a.dtype == KAD_F32;
   const auto count = [&](int bm, int bn) { return (int64_t)ceil_div(a.m, bm) * ceil_div(a.n, bn); };
-  // A round of 256 x 256 tiles, one a CU, takes 22 us and 12.5 for each 1000 of k; one of 128 x 128 tiles, two a CU and half
-  // the results, 7.9 and 9.2 (fits of 4096 x 4096 results at k of 4096 and 8192).  us with tiles of 256 and of 128:
-  //   [8192, 4096] x [4096, 4096] 148 and 193     [4096, 8192] x [4096, 8192] 124 and 166
-  //   [6000, 1000] x [6000, 1000]  57 and 52      [40000, 512] x [512, 512]  26.3 and 18.6
+  // A round of 256 x 256 tiles, one a CU, is taken to be 22 us and 12.5 for each 1000 of k; one of 128 x 128 tiles, two a CU and
+  // half the results, 7.9 and 9.2: a fit of 4096 x 4096 results at k of 4096 and 8192, where both are met to a tenth.  At smaller k
+  // launches overlap what the fit counts as a round's ends, and only the order of the two is meant.  us with tiles of 256 and of
+  // 128 (by the rule):
+  //   [8192, 4096] x [4096, 4096] 146 (146) and 188 (182)     [8192, 2048] x [8192, 2048] 135 (190) and 151 (214)
+  //   [4096, 8192] x [4096, 8192] 126 (124) and 168 (167)     [6000, 2000] x [6000, 2000]  92 (141) and  89 (132)
+  //   [4096, 4096] x [4096, 4096]  65 (73)  and  86 (91)      [6000, 1000] x [6000, 1000]  56 (104) and  52 (86)
+  //   [4096, 2048] x [4096, 2048]  36 (48)  and  41 (54)      [8192, 1024] x [8192, 1024]  82 (139) and  85 (139)
+  //   [4096, 1024] x [4096, 1024]  23 (35)  and  23 (35)      [40000, 512] x [512, 512]    26 (57)  and  18 (38)
+  // Not met: where 256 x 256 tiles are fewer than the CUs, k is cut and its parts joined, which the rule leaves out ([3000, 4096] x
+  // [3000, 4096]: 111 and 70, and it takes 256).
   const auto rounds = [&](int tile, int at_once) { return (double)((count(tile, tile) + at_once - 1) / at_once); };
   const double k = a.k * 1e-3;
   p.bm = p.bn = !exact && rounds(WIDE, CUS) * (22 + 12.5 * k) < rounds(128, 2 * CUS) * (7.9 + 9.2 * k) ? WIDE

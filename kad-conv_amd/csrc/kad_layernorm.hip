@@ -9,8 +9,8 @@
 //
 // Layout.  A row belongs to G threads (1 .. 1024), each with U vectors (kad_rows.h).  A block walks rows with its
 // parameters (and, backward, its share of dw and db) in registers, the next row's values on their way while it computes.
-// [16384, 4096] bf16: forward 52 us (5.1 TB/s), backward 66 (6.3, part of x still in the memory-side cache) and 5 for the join;
-// the map [8, 256, 100, 100] 15 us (5.5); a copy reaches 5.1.  [3, 86, 67, 41] fp32: 4.6 + 5.8 + 4.8, latencies.
+// [16384, 4096] bf16: forward 54 us (5.0 TB/s), backward 67 (6.3, part of x still in the memory-side cache) and 5 for the join;
+// the map [8, 256, 100, 100] 15 us (5.5); a copy reaches 5.1.  [3, 86, 67, 41] fp32: 4.6 + 5.9 + 4.8, latencies.
 //
 // Sums.  The variance is that of the differences to the mean, in 32 bits, whose own mean corrects both: a row of one value
 // repeated is 0 everywhere.  All sums are joined in an order that the sizes alone decide: dw and db first over a block's

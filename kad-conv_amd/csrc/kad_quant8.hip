@@ -6,8 +6,8 @@
 // its way through LDS, 8 or 16 rows of a column at a time.  The tile's column sums, of which a bias' gradient is made,
 // are left in work and joined by a second launch, in an order that the sizes alone decide.
 //
-// [8192, 4096] bf16 along its rows 18.6 us (5.4 TB/s), both ways 32.7 (4.2: every tile's way through LDS, and its two
-// barriers; 35 with 30 KB of LDS and columns that met in a few banks).
+// [8192, 4096] bf16 along its rows 20.1 us (5.0 TB/s; 17.4 where the matrix is still in the memory-side cache), both ways 32.7 (4.2:
+// every tile's way through LDS, and its two barriers; 35 with 30 KB of LDS and columns that met in a few banks).
 #include "kad_block8.h"
 
 namespace kad {

@@ -110,7 +110,7 @@ def matmul8(a, b, bias=None, act=None, dtype=torch.bfloat16):
     """act(a b^T + bias) for a ``Block8`` a [..., K] and b [N, K]: [..., N] of ``dtype`` (fp32, fp16 or bf16).
 
     Sums are 32-bit.  A result in fp32 is a sum of exact products; for one in 16 bits the matrix instruction cuts the
-    products of eight consecutive k to 2^-13 of the largest of them, which for ordinary numbers is 1e-5 of the result.
+    products of eight consecutive k to 2^-13 of the largest of them, which comes to 1e-5 to 5e-5 of the result.
     Inference only."""
     if not isinstance(a, Block8) or not isinstance(b, Block8):
         raise TypeError('a and b must be Block8')
