@@ -103,3 +103,22 @@ def test_long_rows(shape):
             z[torch.ones(z.shape, dtype=torch.bool).scatter_(1, i, False)] = -float('inf')
         for temperature in (9.0, 1e3, 1e6):
             check(z, t, i, temperature, 'cuda')
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('temperature', [1.0, 20.0])
+def test_not_finite_stays_in_its_row(temperature, device):
+    nan, inf = float('nan'), float('inf')
+    z, t, i = make(8, 12, 4, torch.float32, 7)
+    z[1, 11], z[2], t[3, 1], z[4, 0] = nan, -inf, nan, inf
+    i[5] = -1
+    z[5] = nan
+    z[6, i[6, 2]] = -inf
+    zs = z.to(device).requires_grad_(True)
+    loss = kadconv.distill_loss(zs, t.to(device), i.to(device), temperature, 'none')
+    dz, = torch.autograd.grad(loss, zs, torch.ones_like(loss))
+    loss, dz = loss.detach().cpu(), dz.cpu()
+    assert torch.isfinite(loss[[0, 7]]).all() and torch.isfinite(dz[[0, 7]]).all()
+    assert torch.isnan(loss[1:5]).all() and torch.isnan(dz[1:5]).any(1).all()
+    assert loss[5] == 0 and not dz[5].any()
+    assert loss[6] == inf and torch.isfinite(dz[6]).all() and dz[6, i[6, 2]] < 0
