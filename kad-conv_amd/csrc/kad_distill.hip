@@ -8,9 +8,9 @@
 // Memory bounds it: forward reads z once (the largest value and the sum in one pass), backward reads z and writes dz;
 // what the classes of the entries are is looked up in z, a few values a row.
 //
-// Two forms, and one in 64 bits for high temperatures (below).  Up to 1024 classes a row stays in the registers of up to 64 lanes (kad_rows.h), many rows a wave; beyond, a
-// wave or a block walks a row, or a block a part of one where rows are few: forward these parts are joined in a second
-// launch, backward each writes its own classes.
+// Two forms, and one in 64 bits for high temperatures (below).  Up to 1024 classes a row stays in the registers of up to 64
+// lanes (kad_rows.h), many rows a wave; beyond, a wave or a block walks a row, or a block a part of one where rows are few:
+// forward these parts are joined in a second launch, backward each writes its own classes.
 //
 // 4096 rows of 32768 classes, bf16, 64 entries: 159 us a pass, 58 forward (4.7 TB/s), 5 for the join and 98 backward (5.8, part of z
 // from the cache that holds the logits, past which gradients are written: 183 a pass through it).  537600 rows of 16 classes,
@@ -647,7 +647,8 @@ __global__ __launch_bounds__(256) void distill_large_bwd_kernel(kad_distill_args
 //
 // One row to 16, 64 or 256 lanes, z read twice in either direction.  64-bit exponentials and one row's loads after another bound it:
 // 4096 rows of 32768 classes, bf16, 64 entries, forward 356 us (614 a value at a time; 49 in 32 bits) and backward 381 (474; 106);
-// 537600 of 16, fp16, 16 entries, 177 (31) and 162 (29).  A series for e^x - 1 in (-1, 0] took 395 and 427.
+// 537600 of 16, fp16, 16 entries, 177 (31) and 162 (29); of few long rows each is one block's: 4 of 150000, bf16, 201 (12) and 171
+// (9).  A series for e^x - 1 in (-1, 0] took 395 and 427.
 constexpr float MOST_32 = 8.f;
 
 template <int G>

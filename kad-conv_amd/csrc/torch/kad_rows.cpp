@@ -931,7 +931,7 @@ Tensor linear8_kept_forward(const Tensor& x, const Tensor& codes, const Tensor& 
 }  // namespace
 
 void kad_torch::bind_rows(py::module_& m) {
-  // a call of these two, for the modules
+  // whether a call with these two is, for the modules
   m.def("observed", [](const Tensor& a, const Tensor& b) { return observed({&a, &b}); });
   m.def("layer_norm", &layer_norm);
   m.def("layer_norm_forward", &layer_norm_forward);

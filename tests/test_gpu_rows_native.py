@@ -234,3 +234,19 @@ def test_served_products_in_traces():
         for f in (served, product):
             for traced in (torch.jit.trace(f, a), make_fx(f)(a)):
                 assert torch.equal(traced(a), f(a)) and torch.equal(traced(c), f(c))
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
+def test_short_rows_of_the_most_values_in_a_graph(dtype):
+    """Rows of 500 values take more LDS than a launch has by default: what it asks for is asked for in captures too."""
+    x, kept = randn(2100, 500).to(dtype), kadconv.quantize8(randn(600, 500, seed=1))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = kadconv.linear8(x, kept, act='silu')
+    for k in range(3):
+        x.copy_(randn(2100, 500, seed=5 + k))
+        graph.replay()
+        want = kadconv.linear8(x, kept, act='silu')
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and y.any(), k
